@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import os
 from pathlib import Path
+from typing import NamedTuple
 
 import torch
 
@@ -26,7 +27,7 @@ INT8, UINT8, INT4, INT32, F16, BF16, F32, U64, FP8_E4M3, FP8_E5M2, FP4_E2M1, E8M
 # ascq_round_mode
 ROUND_NONE, ROUND_RINT, ROUND_FLOOR, ROUND_CEIL, ROUND_ROUND, ROUND_TRUNC = range(6)
 # ascq_policy
-ACT_NONE, ACT_FASTER_GELU = 0, 1
+ACT_NONE, ACT_FASTER_GELU, ACT_RELU, ACT_GELU, ACT_SILU = range(5)
 PER_TENSOR, PER_CHANNEL, PER_TOKEN, PER_GROUP = range(4)
 # IterateAll enAtomic (matmul_config_utils.h:53-55)
 ATOMIC_NONE, ATOMIC_ADD, ATOMIC_MAX, ATOMIC_MIN = range(4)
@@ -78,6 +79,29 @@ class _QuantizeParam(ctypes.Structure):
     _fields_ = [("policy", ctypes.c_int32), ("has_offset", ctypes.c_int32), ("round_mode", ctypes.c_int32),
                 ("kdim", ctypes.c_int32), ("m", ctypes.c_uint32), ("n", ctypes.c_uint32),
                 ("group_size", ctypes.c_uint32)]
+
+
+class _NormQuantParam(ctypes.Structure):
+    _fields_ = [("m", ctypes.c_int64), ("n", ctypes.c_int64), ("ld_x", ctypes.c_int64),
+                ("ld_residual", ctypes.c_int64), ("ld_h", ctypes.c_int64), ("src_type", ctypes.c_int32),
+                ("dst_type", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class _LinearParam(ctypes.Structure):
+    _fields_ = [("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64), ("ld_x", ctypes.c_int64),
+                ("ld_w", ctypes.c_int64), ("ld_residual", ctypes.c_int64), ("ld_y", ctypes.c_int64),
+                ("operand_type", ctypes.c_int32), ("out_type", ctypes.c_int32), ("w_trans", ctypes.c_int32),
+                ("activation", ctypes.c_int32)]
+
+
+class _RouteParam(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("experts", ctypes.c_int64), ("ld_logits", ctypes.c_int64),
+                ("logits_type", ctypes.c_int32), ("top_k", ctypes.c_int32), ("renormalize", ctypes.c_int32)]
+
+
+class _RowsParam(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("n", ctypes.c_int64), ("ld_x", ctypes.c_int64), ("type", ctypes.c_int32),
+                ("top_k", ctypes.c_int32)]
 
 
 class _MatmulTypes(ctypes.Structure):
@@ -157,6 +181,15 @@ SIGNATURES = {
     "ascq_weight_pack": (_I32, [_P, _P, _I32, _I64, _I64, _I32, _P]),
     "ascq_antiquant_matmul": (_I32, [_P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _I64, _P]),
     "ascq_quant_group_matmul": (_I32, [_P, _I32, _P, _P, _P, _I32, _P, _P, _I32, _I64, _I64, _I64, _I64, _I32, _P]),
+    "ascq_add_rms_norm_quant": (_I32, [_P] * 7 + [ctypes.POINTER(_NormQuantParam), _P]),
+    "ascq_quant_linear_workspace_size": (_I32, [_P, _P, ctypes.POINTER(_LinearParam), ctypes.POINTER(ctypes.c_size_t)]),
+    "ascq_quant_linear": (_I32, [_P] * 7 + [ctypes.POINTER(_LinearParam), _P, ctypes.c_size_t, _P]),
+    "ascq_moe_route_workspace_size": (_I32, [ctypes.POINTER(_RouteParam), ctypes.POINTER(ctypes.c_size_t)]),
+    "ascq_moe_route": (_I32, [_P] * 8 + [ctypes.POINTER(_RouteParam), _P, ctypes.c_size_t, _P]),
+    "ascq_moe_route_grad": (_I32, [_P, _I64] + [_P] * 7 + [ctypes.POINTER(_RouteParam), _P]),
+    "ascq_moe_dispatch": (_I32, [_P] * 6 + [ctypes.POINTER(_RowsParam), _P]),
+    "ascq_moe_combine": (_I32, [_P] * 5 + [ctypes.POINTER(_RowsParam), _P]),
+    "ascq_moe_combine_grad": (_I32, [_P] * 7 + [ctypes.POINTER(_RowsParam), _P]),
     "ascq_nz_size": (ctypes.c_size_t, [_I32, _I64, _I64, _I64]),
     "ascq_nz_to_nd": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _I32, _P]),
     "ascq_nd_to_nz": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _P]),
@@ -487,6 +520,297 @@ def quant_group_matmul(x: torch.Tensor, per_token_scale: torch.Tensor, w: torch.
                                         _stream(stream)),
           "quant_group_matmul")
     return y
+
+
+# ------------------------------------------------------------------------------------------
+# a transformer block's operators around its products: norm, linear, routing, rows by expert
+# ------------------------------------------------------------------------------------------
+_CODE_TYPE = {torch.int8: INT8, torch.float8_e4m3fn: FP8_E4M3}
+_CODE_DTYPE = {INT8: torch.int8, FP8_E4M3: torch.float8_e4m3fn}
+
+
+def _refuse(what: str, message: str):
+    raise AscqError(E_INVALID_ARG, f"{what}: {message}")
+
+
+def _typed(what: str, name: str, t: torch.Tensor, table: dict) -> int:
+    """the ascq_dtype of t; a type outside the table is refused"""
+    code = table.get(t.dtype)
+    if code is None:
+        raise AscqError(E_UNSUPPORTED, f"{what}: {name} of type {t.dtype}")
+    return code
+
+
+def _pitch(what: str, name: str, t: torch.Tensor, shape: tuple, dtype) -> int:
+    """The row pitch of t [rows, n], whose rows are contiguous (pitch at least n)."""
+    if t.shape != shape or t.dtype is not dtype:
+        _refuse(what, f"{name} must be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+    rows, n = shape
+    ld, unit = t.stride()
+    if (unit != 1 and n > 1) or (ld < n and rows > 1):
+        _refuse(what, f"{name}: the elements of a row must be contiguous")
+    return max(ld, n)  # (torch gives rows of a single one any stride)
+
+
+def _dense(what: str, name: str, t: torch.Tensor, shape: tuple, dtype) -> None:
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
+        _refuse(what, f"{name} must be a contiguous {tuple(shape)} tensor of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+
+
+def _same_device(what: str, *tensors) -> None:
+    device = tensors[0].device
+    if device.type != "cuda":
+        _refuse(what, f"tensors on {device}: there is no CPU path")
+    for t in tensors:
+        if t is not None and t.device != device:
+            _refuse(what, f"tensors on {device} and {t.device}")
+
+
+def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, dst_type: int = INT8, residual=None,
+                       residual_out=None, norm_out=None, out=None, scale_out=None, stream=None):
+    """h = x + residual, RMS norm of h by gamma, 8-bit codes with one fp32 scale per row: returns (codes, scale, h), the
+    codes int8 (INT8) or float8_e4m3fn (FP8_E4M3).  x [m, n] and residual f16 / bf16 / f32, rows contiguous at any pitch;
+    residual_out may be x or residual (in place; without it h is a new tensor, and without a residual h is x);
+    norm_out takes the unquantised norm."""
+    what = "add_rms_norm_quant"
+    if x.dim() != 2:
+        _refuse(what, "x must be [m, n]")
+    shape, dt = x.shape, x.dtype
+    m, n = shape
+    src_type = _typed(what, "x", x, _FLOAT_CODE)
+    if dst_type not in _CODE_DTYPE:
+        raise AscqError(E_UNSUPPORTED, f"{what}: dst_type {dst_type}")
+    ldx, ldr, ldh = _pitch(what, "x", x, shape, dt), 0, 0
+    _dense(what, "gamma", gamma, (n,), dt)
+    h = x
+    if residual is not None:
+        ldr = _pitch(what, "residual", residual, shape, dt)
+        h = residual_out if residual_out is not None else torch.empty((m, n), dtype=dt, device=x.device)
+        ldh = _pitch(what, "residual_out", h, shape, dt)
+    elif residual_out is not None:
+        _refuse(what, "residual_out needs a residual")
+    if norm_out is not None:
+        _dense(what, "norm_out", norm_out, shape, dt)
+    q = out if out is not None else torch.empty((m, n), dtype=_CODE_DTYPE[dst_type], device=x.device)
+    _dense(what, "out", q, shape, _CODE_DTYPE[dst_type])
+    s = scale_out if scale_out is not None else torch.empty((m,), dtype=torch.float32, device=x.device)
+    _dense(what, "scale_out", s, (m,), torch.float32)
+    _same_device(what, x, gamma, residual, h, norm_out, q, s)
+    p = _NormQuantParam(m, n, ldx, ldr, ldh, src_type, dst_type, eps)
+    check(lib().ascq_add_rms_norm_quant(_ptr(q), _ptr(s), _ptr(h) if residual is not None else None, _ptr(norm_out), _ptr(x),
+                                        _ptr(residual), _ptr(gamma), ctypes.byref(p), _stream(stream)), what)
+    return q, s, h
+
+
+def quant_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias=None,
+                 activation: int = ACT_NONE, residual=None, w_trans: bool = True, out_dtype=torch.bfloat16, out=None,
+                 workspace=None, stream=None):
+    """y = cast(act((x @ W) * w_scale * x_scale[:, None] + bias) + residual) of int8 or float8_e4m3fn codes: x [m, k] with a
+    scale per token (fp32 [m]), w [n, k] (w_trans) or [k, n] with a scale per channel (fp32 [n]), bias fp32 [n]; y f16,
+    bf16 or f32 and residual of its type; rows at any pitch.  out may be the residual.  workspace: a uint8 tensor of
+    quant_linear_workspace_size bytes; without one the call takes what it needs from torch's allocator."""
+    what = "quant_linear"
+    if x.dim() != 2 or w.dim() != 2:
+        _refuse(what, "x and w must be matrices")
+    m, k = x.shape
+    n = w.shape[0] if w_trans else w.shape[1]
+    code = _typed(what, "x", x, _CODE_TYPE)
+    ldx, ldr = _pitch(what, "x", x, (m, k), x.dtype), 0
+    ldw = _pitch(what, "w", w, (n, k) if w_trans else (k, n), x.dtype)
+    y = out if out is not None else torch.empty((m, n), dtype=out_dtype, device=x.device)
+    out_type = _typed(what, "out", y, _FLOAT_CODE)
+    ldy = _pitch(what, "out", y, (m, n), y.dtype)
+    _dense(what, "x_scale", x_scale, (m,), torch.float32)
+    _dense(what, "w_scale", w_scale, (n,), torch.float32)
+    if bias is not None:
+        _dense(what, "bias", bias, (n,), torch.float32)
+    if residual is not None:
+        ldr = _pitch(what, "residual", residual, (m, n), y.dtype)
+    _same_device(what, x, x_scale, w, w_scale, bias, residual, y, workspace)
+    p = _LinearParam(m, n, k, ldx, ldw, ldr, ldy, code, out_type, int(w_trans), activation)
+    if workspace is None:
+        need = ctypes.c_size_t(0)
+        check(lib().ascq_quant_linear_workspace_size(_ptr(x), _ptr(w), ctypes.byref(p), ctypes.byref(need)), what)
+        if need.value:
+            workspace = torch.empty((need.value,), dtype=torch.uint8, device=x.device)
+            if stream is not None:
+                workspace.record_stream(_torch_stream(stream))
+    check(lib().ascq_quant_linear(_ptr(y), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(residual),
+                                  ctypes.byref(p), _ptr(workspace), _room(workspace), _stream(stream)), what)
+    return y
+
+
+def _room(workspace) -> int:
+    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def _torch_stream(stream):
+    return torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
+
+
+def quant_linear_workspace_size(x: torch.Tensor, w: torch.Tensor, w_trans: bool = True, out_dtype=torch.bfloat16) -> int:
+    """Bytes of the workspace that quant_linear uses for these operands (0: none)"""
+    what = "quant_linear_workspace_size"
+    m, k = x.shape
+    n = w.shape[0] if w_trans else w.shape[1]
+    p = _LinearParam(m, n, k, _pitch(what, "x", x, (m, k), x.dtype),
+                     _pitch(what, "w", w, (n, k) if w_trans else (k, n), x.dtype), 0, 0, _typed(what, "x", x, _CODE_TYPE),
+                     _FLOAT_CODE[out_dtype], int(w_trans), ACT_NONE)
+    need = ctypes.c_size_t(0)
+    check(lib().ascq_quant_linear_workspace_size(_ptr(x), _ptr(w), ctypes.byref(p), ctypes.byref(need)), what)
+    return need.value
+
+
+class MoeRouting(NamedTuple):
+    """What moe_route gives for tokens [T] of k choices among E experts."""
+    weights: torch.Tensor  # f32 [T, k]
+    experts: torch.Tensor  # int32 [T, k], -1: no choice
+    slots: torch.Tensor    # int32 [T, k]: the choice's row, ordered by expert, then token; -1: none
+    tokens: torch.Tensor   # int32 [T * k]: the token of each row; -1 behind the last
+    counts: torch.Tensor   # int64 [E]: rows per expert, quant_group_matmul's group_list of list_type 1
+    routed: torch.Tensor   # int64 [1]: tokens with a choice
+    loss: torch.Tensor     # f32 [1]: the balance loss
+
+
+def _check_routing(what: str, r: MoeRouting, t: int, e: int, k: int) -> None:
+    for name, shape, dt in (("weights", (t, k), torch.float32), ("experts", (t, k), torch.int32),
+                            ("slots", (t, k), torch.int32), ("tokens", (t * k,), torch.int32),
+                            ("counts", (e,), torch.int64), ("routed", (1,), torch.int64), ("loss", (1,), torch.float32)):
+        _dense(what, name, getattr(r, name), shape, dt)
+
+
+def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True, out=None, workspace=None,
+              stream=None) -> MoeRouting:
+    """The top_k experts of each token by its logits [T, E] (f16 / bf16 / f32; -inf or NaN: masked), their softmax weights,
+    the rows' order by expert, the rows per expert and the balance loss (see ascq_moe_route)."""
+    what = "moe_route"
+    if logits.dim() != 2:
+        _refuse(what, "logits must be [tokens, experts]")
+    t, e = logits.shape
+    p = _RouteParam(t, e, _pitch(what, "logits", logits, (t, e), logits.dtype), _typed(what, "logits", logits, _FLOAT_CODE),
+                    top_k, int(renormalize))
+    need = ctypes.c_size_t(0)
+    check(lib().ascq_moe_route_workspace_size(ctypes.byref(p), ctypes.byref(need)), what)
+    r = out
+    if r is None:
+        new = lambda shape, dt: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
+        r = MoeRouting(new((t, top_k), torch.float32), new((t, top_k), torch.int32), new((t, top_k), torch.int32),
+                       new((t * top_k,), torch.int32), new((e,), torch.int64), new((1,), torch.int64),
+                       new((1,), torch.float32))
+    _check_routing(what, r, t, e, top_k)
+    _same_device(what, logits, *r, workspace)
+    if workspace is None and need.value:
+        workspace = torch.empty((need.value,), dtype=torch.uint8, device=logits.device)
+        if stream is not None:
+            workspace.record_stream(_torch_stream(stream))
+    check(lib().ascq_moe_route(*map(_ptr, r), _ptr(logits), ctypes.byref(p), _ptr(workspace), _room(workspace),
+                               _stream(stream)), what)
+    return r
+
+
+def moe_route_grad(logits: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, counts: torch.Tensor,
+                   routed: torch.Tensor, grad_weights=None, grad_loss=None, renormalize: bool = True, out=None, stream=None):
+    """d / d logits of grad_loss * loss + (grad_weights * weights).sum(), with moe_route's outputs of the same logits;
+    grad_weights f32 [T, k], grad_loss f32 [1].  Returns a tensor of the logits' type."""
+    what = "moe_route_grad"
+    if logits.dim() != 2 or weights.dim() != 2:
+        _refuse(what, "logits must be [tokens, experts], weights [tokens, top_k]")
+    t, e = logits.shape
+    k = weights.shape[1]
+    ld = _pitch(what, "logits", logits, (t, e), logits.dtype)
+    _dense(what, "weights", weights, (t, k), torch.float32)
+    _dense(what, "experts", experts, (t, k), torch.int32)
+    _dense(what, "counts", counts, (e,), torch.int64)
+    _dense(what, "routed", routed, (1,), torch.int64)
+    if grad_weights is not None:
+        _dense(what, "grad_weights", grad_weights, (t, k), torch.float32)
+    if grad_loss is not None:
+        _dense(what, "grad_loss", grad_loss, (1,), torch.float32)
+    g = out if out is not None else torch.empty((t, e), dtype=logits.dtype, device=logits.device)
+    ldg = _pitch(what, "out", g, (t, e), logits.dtype)
+    _same_device(what, logits, weights, experts, counts, routed, grad_weights, grad_loss, g)
+    p = _RouteParam(t, e, ld, _typed(what, "logits", logits, _FLOAT_CODE), k, int(renormalize))
+    check(lib().ascq_moe_route_grad(_ptr(g), ldg, _ptr(logits), _ptr(weights), _ptr(experts), _ptr(counts), _ptr(routed),
+                                    _ptr(grad_weights), _ptr(grad_loss), ctypes.byref(p), _stream(stream)), what)
+    return g
+
+
+def moe_dispatch(x: torch.Tensor, x_scale, slots: torch.Tensor, tokens: torch.Tensor, out=None, scale_out=None,
+                 stream=None):
+    """Rows of x [T, n] (int8, float8_e4m3fn, f16, bf16 or f32) and their scales (fp32 [T] or None) in the experts' order of
+    a MoeRouting's slots and tokens: returns (rows [T * k, n], scales [T * k] or None); rows of no token are 0."""
+    what = "moe_dispatch"
+    if x.dim() != 2 or slots.dim() != 2:
+        _refuse(what, "x must be [tokens, n], slots [tokens, top_k]")
+    t, n = x.shape
+    k = slots.shape[1]
+    code = _typed(what, "x", x, {**_CODE_TYPE, **_FLOAT_CODE})
+    ldx = _pitch(what, "x", x, (t, n), x.dtype)
+    _dense(what, "slots", slots, (t, k), torch.int32)
+    _dense(what, "tokens", tokens, (t * k,), torch.int32)
+    rows = out if out is not None else torch.empty((t * k, n), dtype=x.dtype, device=x.device)
+    _dense(what, "out", rows, (t * k, n), x.dtype)
+    s = None
+    if x_scale is not None:
+        _dense(what, "x_scale", x_scale, (t,), torch.float32)
+        s = scale_out if scale_out is not None else torch.empty((t * k,), dtype=torch.float32, device=x.device)
+        _dense(what, "scale_out", s, (t * k,), torch.float32)
+    elif scale_out is not None:
+        _refuse(what, "scale_out needs x_scale")
+    _same_device(what, x, x_scale, slots, tokens, rows, s)
+    p = _RowsParam(t, n, ldx, code, k)
+    check(lib().ascq_moe_dispatch(_ptr(rows), _ptr(s), _ptr(x), _ptr(x_scale), _ptr(slots), _ptr(tokens), ctypes.byref(p),
+                                  _stream(stream)), what)
+    return rows, s
+
+
+def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual=None, out=None, stream=None):
+    """out[t] = sum_j weights[t, j] y[slots[t, j]] + residual[t], of y [T * k, n] f16 / bf16 / f32; out may be the residual"""
+    what = "moe_combine"
+    if y.dim() != 2 or slots.dim() != 2:
+        _refuse(what, "y must be [tokens * top_k, n], slots [tokens, top_k]")
+    t, k = slots.shape
+    n = y.shape[1]
+    code = _typed(what, "y", y, _FLOAT_CODE)
+    _dense(what, "y", y, (t * k, n), y.dtype)
+    _dense(what, "slots", slots, (t, k), torch.int32)
+    _dense(what, "weights", weights, (t, k), torch.float32)
+    if residual is not None:
+        _dense(what, "residual", residual, (t, n), y.dtype)
+    r = out if out is not None else torch.empty((t, n), dtype=y.dtype, device=y.device)
+    _dense(what, "out", r, (t, n), y.dtype)
+    _same_device(what, y, slots, weights, residual, r)
+    p = _RowsParam(t, n, 0, code, k)
+    check(lib().ascq_moe_combine(_ptr(r), _ptr(y), _ptr(slots), _ptr(weights), _ptr(residual), ctypes.byref(p),
+                                 _stream(stream)), what)
+    return r
+
+
+def moe_combine_grad(grad_out: torch.Tensor, y: torch.Tensor, slots: torch.Tensor, tokens: torch.Tensor,
+                     weights: torch.Tensor, need_grad_y: bool = True, out=None, grad_y_out=None, stream=None):
+    """moe_combine's gradients: (grad_weights f32 [T, k], grad_y [T * k, n] of y's type, or None without need_grad_y)"""
+    what = "moe_combine_grad"
+    if y.dim() != 2 or slots.dim() != 2:
+        _refuse(what, "y must be [tokens * top_k, n], slots [tokens, top_k]")
+    t, k = slots.shape
+    n = y.shape[1]
+    code = _typed(what, "y", y, _FLOAT_CODE)
+    _dense(what, "y", y, (t * k, n), y.dtype)
+    _dense(what, "grad_out", grad_out, (t, n), y.dtype)
+    _dense(what, "slots", slots, (t, k), torch.int32)
+    _dense(what, "tokens", tokens, (t * k,), torch.int32)
+    _dense(what, "weights", weights, (t, k), torch.float32)
+    dw = out if out is not None else torch.empty((t, k), dtype=torch.float32, device=y.device)
+    _dense(what, "out", dw, (t, k), torch.float32)
+    dy = None
+    if need_grad_y:
+        dy = grad_y_out if grad_y_out is not None else torch.empty_like(y)
+        _dense(what, "grad_y_out", dy, (t * k, n), y.dtype)
+    _same_device(what, y, grad_out, slots, tokens, weights, dw, dy)
+    p = _RowsParam(t, n, 0, code, k)
+    check(lib().ascq_moe_combine_grad(_ptr(dw), _ptr(dy), _ptr(grad_out), _ptr(y), _ptr(slots), _ptr(tokens), _ptr(weights),
+                                      ctypes.byref(p), _stream(stream)), what)
+    return dw, dy
 
 
 # ------------------------------------------------------------------------------------------

@@ -1663,6 +1663,318 @@ ascq_status ascq_quant_group_matmul(void* y, int32_t out_type, const int8_t* x, 
 }
 
 // ------------------------------------------------------------------------------------------------
+// a transformer block's operators around its products: norm, linear, routing, rows by expert
+// ------------------------------------------------------------------------------------------------
+namespace {
+bool float_type(int32_t t) { return t == ASCQ_DT_F16 || t == ASCQ_DT_BF16 || t == ASCQ_DT_F32; }
+size_t float_bytes(int32_t t) { return t == ASCQ_DT_F32 ? 4 : 2; }
+// a row pitch: dense when 0, else at least the row
+bool pitch(int64_t& ld, int64_t n)
+{
+    if (ld == 0) ld = n;
+    return ld >= n;
+}
+// rows * ld elements of at most 16 bytes are addressed with 64-bit products
+bool addressable(int64_t rows, int64_t ld) { return rows == 0 || ld <= (1ll << 58) / rows; }
+}  // namespace
+
+ascq_status ascq_add_rms_norm_quant(void* q, float* scale, void* h_out, void* norm_out, const void* x,
+                                    const void* residual, const void* gamma, const ascq_norm_quant_param* p, void* stream)
+{
+    CallScope scope;
+    if (!p) return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: null params");
+    if (!float_type(p->src_type)) return fail(ASCQ_E_UNSUPPORTED, "add_rms_norm_quant: src must be f16, bf16 or f32");
+    if (p->dst_type != ASCQ_DT_INT8 && p->dst_type != ASCQ_DT_FP8_E4M3)
+        return fail(ASCQ_E_UNSUPPORTED, "add_rms_norm_quant: dst must be int8 or fp8_e4m3");
+    if (p->m < 0 || p->n < 0) return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: negative shape");
+    if (p->m > INT32_MAX || p->n > INT32_MAX) return fail(ASCQ_E_UNSUPPORTED, "add_rms_norm_quant: rows and columns below 2^31");
+    if (!(p->eps >= 0.0f) || p->eps > 3.4e38f) return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: eps must be finite, not negative");
+    int64_t ldx = p->ld_x, ldr = p->ld_residual, ldh = p->ld_h;
+    if (!pitch(ldx, p->n) || !pitch(ldr, p->n) || !pitch(ldh, p->n))
+        return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: a row pitch is smaller than the row");
+    if (!addressable(p->m, ldx) || !addressable(p->m, ldr) || !addressable(p->m, ldh))
+        return fail(ASCQ_E_UNSUPPORTED, "add_rms_norm_quant: tensor too large");
+    if (h_out && !residual) return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: h_out needs a residual");
+    if (p->m == 0 || p->n == 0) return ASCQ_OK;
+    if (!q || !scale || !x || !gamma) return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: null argument");
+    if ((h_out == x && ldh != ldx) || (h_out && h_out == residual && ldh != ldr))
+        return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: h_out in place of an input needs its row pitch");
+    const size_t es = float_bytes(p->src_type);
+    if (!aligned(x, es) || !aligned(residual, es) || !aligned(gamma, es) || !aligned(h_out, es) || !aligned(norm_out, es) ||
+        !aligned(scale, 4))
+        return fail(ASCQ_E_INVALID_ARG, "add_rms_norm_quant: a pointer is not aligned to its element type");
+    trace("add_rms_norm_quant: src %d dst %d, m %lld n %lld, residual %d", p->src_type, p->dst_type, (long long)p->m,
+          (long long)p->n, residual ? 1 : 0);
+    const ascq::NormQuantArgs a{q,        scale,       h_out, norm_out, x,   residual, gamma, p->src_type,
+                                p->dst_type, p->m, p->n,  ldx,      ldr, ldh,      p->eps};
+    return hip_status(ascq::launch_norm_quant(a, S(stream)), "add_rms_norm_quant");
+}
+
+namespace {
+ascq_status linear_args(const char* what, const ascq_linear_param* p, ascq::LinearArgs& a)
+{
+    if (!p) return fail(ASCQ_E_INVALID_ARG, "%s: null params", what);
+    if (p->operand_type != ASCQ_DT_INT8 && p->operand_type != ASCQ_DT_FP8_E4M3)
+        return fail(ASCQ_E_UNSUPPORTED, "%s: operands must be int8 or fp8_e4m3", what);
+    if (!float_type(p->out_type)) return fail(ASCQ_E_UNSUPPORTED, "%s: output must be f16, bf16 or f32", what);
+    if (p->w_trans != 0 && p->w_trans != 1) return fail(ASCQ_E_INVALID_ARG, "%s: w_trans must be 0 or 1", what);
+    if (p->activation < ASCQ_ACT_NONE || p->activation > ASCQ_ACT_SILU)
+        return fail(ASCQ_E_INVALID_ARG, "%s: unknown activation %d", what, p->activation);
+    if (p->m < 0 || p->n < 0 || p->k < 0) return fail(ASCQ_E_INVALID_ARG, "%s: negative shape", what);
+    if (p->m > INT32_MAX || p->n > INT32_MAX || p->k > INT32_MAX) return fail(ASCQ_E_UNSUPPORTED, "%s: sizes below 2^31", what);
+    if (p->operand_type == ASCQ_DT_INT8 && p->k >= (1 << 17))
+        return fail(ASCQ_E_UNSUPPORTED, "%s: int8 sums of 2^17 products may pass int32", what);
+    a.ldx = p->ld_x;
+    a.ldw = p->ld_w;
+    a.ldr = p->ld_residual;
+    a.ldy = p->ld_y;
+    if (!pitch(a.ldx, p->k) || !pitch(a.ldw, p->w_trans ? p->k : p->n) || !pitch(a.ldr, p->n) || !pitch(a.ldy, p->n))
+        return fail(ASCQ_E_INVALID_ARG, "%s: a row pitch is smaller than the row", what);
+    if (!addressable(p->m, a.ldx) || !addressable(p->w_trans ? p->n : p->k, a.ldw) || !addressable(p->m, a.ldr) ||
+        !addressable(p->m, a.ldy))
+        return fail(ASCQ_E_UNSUPPORTED, "%s: tensor too large", what);
+    if (((p->m + 63) / 64) * ((p->n + 63) / 64) > INT32_MAX) return fail(ASCQ_E_UNSUPPORTED, "%s: output too large", what);
+    a.M = p->m;
+    a.N = p->n;
+    a.K = p->k;
+    a.f8 = p->operand_type == ASCQ_DT_FP8_E4M3;
+    a.w_trans = p->w_trans;
+    a.act = p->activation;
+    a.out_type = p->out_type;
+    return ASCQ_OK;
+}
+}  // namespace
+
+ascq_status ascq_quant_linear_workspace_size(const void* x, const void* w, const ascq_linear_param* p, size_t* bytes)
+{
+    if (!bytes) return fail(ASCQ_E_INVALID_ARG, "quant_linear_workspace_size: null argument");
+    ascq::LinearArgs a{};
+    const ascq_status s = linear_args("quant_linear_workspace_size", p, a);
+    if (s != ASCQ_OK) return s;
+    *bytes = 0;
+    return ASCQ_OK;
+}
+
+ascq_status ascq_quant_linear(void* y, const void* x, const float* x_scale, const void* w, const float* w_scale,
+                              const float* bias, const void* residual, const ascq_linear_param* p, void* workspace,
+                              size_t workspace_bytes, void* stream)
+{
+    CallScope scope;
+    ascq::LinearArgs a{};
+    const ascq_status s = linear_args("quant_linear", p, a);
+    if (s != ASCQ_OK) return s;
+    if (a.M == 0 || a.N == 0) return ASCQ_OK;
+    if (!y || !x_scale || !w_scale || (a.K > 0 && (!x || !w))) return fail(ASCQ_E_INVALID_ARG, "quant_linear: null argument");
+    if (residual == y && a.ldr != a.ldy)
+        return fail(ASCQ_E_INVALID_ARG, "quant_linear: y in place of the residual needs its row pitch");
+    const size_t es = float_bytes(a.out_type);
+    if (!aligned(y, es) || !aligned(residual, es) || !aligned(x_scale, 4) || !aligned(w_scale, 4) || !aligned(bias, 4))
+        return fail(ASCQ_E_INVALID_ARG, "quant_linear: a pointer is not aligned to its element type");
+    a.y = y;
+    a.x = (const uint8_t*)x;
+    a.w = (const uint8_t*)w;
+    a.x_scale = x_scale;
+    a.w_scale = w_scale;
+    a.bias = bias;
+    a.residual = residual;
+    trace("quant_linear: operands %d out %d, M %lld N %lld K %lld, w_trans %d, act %d, bias %d, residual %d", p->operand_type,
+          a.out_type, (long long)a.M, (long long)a.N, (long long)a.K, a.w_trans, a.act, bias ? 1 : 0, residual ? 1 : 0);
+    return hip_status(ascq::launch_linear(a, S(stream)), "quant_linear");
+}
+
+namespace {
+ascq_status route_check(const char* what, const ascq_route_param* p, int64_t* ld)
+{
+    if (!p) return fail(ASCQ_E_INVALID_ARG, "%s: null params", what);
+    if (!float_type(p->logits_type)) return fail(ASCQ_E_UNSUPPORTED, "%s: logits must be f16, bf16 or f32", what);
+    if (p->tokens < 0 || p->experts < 1) return fail(ASCQ_E_INVALID_ARG, "%s: bad shape", what);
+    if (p->experts > 1024) return fail(ASCQ_E_UNSUPPORTED, "%s: at most 1024 experts", what);
+    if (p->top_k < 1 || p->top_k > 16 || p->top_k > p->experts)
+        return fail(ASCQ_E_INVALID_ARG, "%s: top_k must be 1 .. 16 and at most the experts", what);
+    if (p->tokens > INT32_MAX / p->top_k) return fail(ASCQ_E_UNSUPPORTED, "%s: tokens * top_k must stay below 2^31", what);
+    *ld = p->ld_logits;
+    if (!pitch(*ld, p->experts)) return fail(ASCQ_E_INVALID_ARG, "%s: a row pitch is smaller than the row", what);
+    if (!addressable(p->tokens, *ld)) return fail(ASCQ_E_UNSUPPORTED, "%s: tensor too large", what);
+    return ASCQ_OK;
+}
+}  // namespace
+
+ascq_status ascq_moe_route_workspace_size(const ascq_route_param* p, size_t* bytes)
+{
+    if (!bytes) return fail(ASCQ_E_INVALID_ARG, "moe_route_workspace_size: null argument");
+    int64_t ld;
+    const ascq_status s = route_check("moe_route_workspace_size", p, &ld);
+    if (s != ASCQ_OK) return s;
+    *bytes = ascq::moe_route_ws_bytes(p->tokens, p->experts);
+    return ASCQ_OK;
+}
+
+ascq_status ascq_moe_route(float* weights, int32_t* experts, int32_t* slots, int32_t* row_tokens, int64_t* counts,
+                           int64_t* routed, float* loss, const void* logits, const ascq_route_param* p, void* workspace,
+                           size_t workspace_bytes, void* stream)
+{
+    CallScope scope;
+    int64_t ld;
+    const ascq_status s = route_check("moe_route", p, &ld);
+    if (s != ASCQ_OK) return s;
+    if (!counts || !routed || !loss || (p->tokens > 0 && (!weights || !experts || !slots || !row_tokens || !logits)))
+        return fail(ASCQ_E_INVALID_ARG, "moe_route: null argument");
+    const size_t need = ascq::moe_route_ws_bytes(p->tokens, p->experts);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return fail(ASCQ_E_INVALID_ARG, "moe_route: the workspace must be 16-byte aligned and hold %zu bytes", need);
+    if (!aligned(weights, 4) || !aligned(experts, 4) || !aligned(slots, 4) || !aligned(row_tokens, 4) || !aligned(counts, 8) ||
+        !aligned(routed, 8) || !aligned(loss, 4) || !aligned(logits, float_bytes(p->logits_type)))
+        return fail(ASCQ_E_INVALID_ARG, "moe_route: a pointer is not aligned to its element type");
+    ascq::MoeRouteArgs a{};
+    a.weights = weights;
+    a.experts = experts;
+    a.slots = slots;
+    a.row_tokens = row_tokens;
+    a.counts = counts;
+    a.routed = routed;
+    a.loss = loss;
+    a.logits = logits;
+    a.type = p->logits_type;
+    a.T = p->tokens;
+    a.E = p->experts;
+    a.ld = ld;
+    a.k = p->top_k;
+    a.renormalize = p->renormalize ? 1 : 0;
+    trace("moe_route: logits %d, T %lld E %lld k %d", a.type, (long long)a.T, (long long)a.E, a.k);
+    return hip_status(ascq::launch_moe_route(a, workspace, S(stream)), "moe_route");
+}
+
+ascq_status ascq_moe_route_grad(void* grad_logits, int64_t ld_grad, const void* logits, const float* weights,
+                                const int32_t* experts, const int64_t* counts, const int64_t* routed,
+                                const float* grad_weights, const float* grad_loss, const ascq_route_param* p, void* stream)
+{
+    CallScope scope;
+    int64_t ld;
+    const ascq_status s = route_check("moe_route_grad", p, &ld);
+    if (s != ASCQ_OK) return s;
+    if (!pitch(ld_grad, p->experts)) return fail(ASCQ_E_INVALID_ARG, "moe_route_grad: a row pitch is smaller than the row");
+    if (!addressable(p->tokens, ld_grad)) return fail(ASCQ_E_UNSUPPORTED, "moe_route_grad: tensor too large");
+    if (p->tokens == 0) return ASCQ_OK;
+    if (!grad_logits || !logits || (grad_weights && (!weights || !experts)) || (grad_loss && (!counts || !routed)))
+        return fail(ASCQ_E_INVALID_ARG, "moe_route_grad: null argument");
+    if (grad_logits == logits && ld != ld_grad)
+        return fail(ASCQ_E_INVALID_ARG, "moe_route_grad: gradients in place of the logits need their row pitch");
+    const size_t es = float_bytes(p->logits_type);
+    if (!aligned(grad_logits, es) || !aligned(logits, es) || !aligned(weights, 4) || !aligned(experts, 4) ||
+        !aligned(counts, 8) || !aligned(routed, 8) || !aligned(grad_weights, 4) || !aligned(grad_loss, 4))
+        return fail(ASCQ_E_INVALID_ARG, "moe_route_grad: a pointer is not aligned to its element type");
+    const ascq::MoeRouteGradArgs a{grad_logits, logits,       p->logits_type, weights,   experts,    counts, routed,
+                                   grad_weights, grad_loss,   p->tokens,      p->experts, ld,        ld_grad, p->top_k,
+                                   p->renormalize ? 1 : 0};
+    trace("moe_route_grad: logits %d, T %lld E %lld k %d", a.type, (long long)a.T, (long long)a.E, a.k);
+    return hip_status(ascq::launch_moe_route_grad(a, S(stream)), "moe_route_grad");
+}
+
+namespace {
+ascq_status rows_check(const char* what, const ascq_rows_param* p, bool codes)
+{
+    if (!p) return fail(ASCQ_E_INVALID_ARG, "%s: null params", what);
+    if (!float_type(p->type) && !(codes && (p->type == ASCQ_DT_INT8 || p->type == ASCQ_DT_FP8_E4M3)))
+        return fail(ASCQ_E_UNSUPPORTED, "%s: unsupported element type %d", what, p->type);
+    if (p->tokens < 0 || p->n < 0) return fail(ASCQ_E_INVALID_ARG, "%s: negative shape", what);
+    if (p->top_k < 1 || p->top_k > 16) return fail(ASCQ_E_INVALID_ARG, "%s: top_k must be 1 .. 16", what);
+    if (p->tokens > INT32_MAX / p->top_k || p->n > INT32_MAX / 4)
+        return fail(ASCQ_E_UNSUPPORTED, "%s: tokens * top_k must stay below 2^31, rows below 2^29 elements", what);
+    return ASCQ_OK;
+}
+}  // namespace
+
+ascq_status ascq_moe_dispatch(void* rows, float* row_scale, const void* x, const float* x_scale, const int32_t* slots,
+                              const int32_t* row_tokens, const ascq_rows_param* p, void* stream)
+{
+    CallScope scope;
+    const ascq_status s = rows_check("moe_dispatch", p, true);
+    if (s != ASCQ_OK) return s;
+    int64_t ldx = p->ld_x;
+    if (!pitch(ldx, p->n)) return fail(ASCQ_E_INVALID_ARG, "moe_dispatch: a row pitch is smaller than the row");
+    if (!addressable(p->tokens, ldx)) return fail(ASCQ_E_UNSUPPORTED, "moe_dispatch: tensor too large");
+    if ((row_scale == nullptr) != (x_scale == nullptr))
+        return fail(ASCQ_E_INVALID_ARG, "moe_dispatch: row_scale and x_scale go together");
+    if (p->tokens == 0 || p->n == 0) return ASCQ_OK;
+    if (!rows || !x || !slots || !row_tokens) return fail(ASCQ_E_INVALID_ARG, "moe_dispatch: null argument");
+    const size_t es = float_type(p->type) ? float_bytes(p->type) : 1;
+    if (!aligned(rows, es) || !aligned(x, es) || !aligned(row_scale, 4) || !aligned(x_scale, 4) || !aligned(slots, 4) ||
+        !aligned(row_tokens, 4))
+        return fail(ASCQ_E_INVALID_ARG, "moe_dispatch: a pointer is not aligned to its element type");
+    ascq::MoeRowsArgs a{};
+    a.out = rows;
+    a.scale_out = row_scale;
+    a.x = x;
+    a.scale = x_scale;
+    a.slots = slots;
+    a.row_tokens = row_tokens;
+    a.type = p->type;
+    a.k = p->top_k;
+    a.T = p->tokens;
+    a.n = p->n;
+    a.row_bytes = p->n * (int64_t)es;
+    a.ldx = ldx * (int64_t)es;
+    trace("moe_dispatch: type %d, T %lld n %lld k %d", a.type, (long long)a.T, (long long)a.n, a.k);
+    return hip_status(ascq::launch_moe_dispatch(a, S(stream)), "moe_dispatch");
+}
+
+ascq_status ascq_moe_combine(void* out, const void* y, const int32_t* slots, const float* weights, const void* residual,
+                             const ascq_rows_param* p, void* stream)
+{
+    CallScope scope;
+    const ascq_status s = rows_check("moe_combine", p, false);
+    if (s != ASCQ_OK) return s;
+    if (p->tokens == 0 || p->n == 0) return ASCQ_OK;
+    if (!out || !y || !slots || !weights) return fail(ASCQ_E_INVALID_ARG, "moe_combine: null argument");
+    const size_t es = float_bytes(p->type);
+    if (!aligned(out, es) || !aligned(y, es) || !aligned(residual, es) || !aligned(slots, 4) || !aligned(weights, 4))
+        return fail(ASCQ_E_INVALID_ARG, "moe_combine: a pointer is not aligned to its element type");
+    ascq::MoeRowsArgs a{};
+    a.out = out;
+    a.y = y;
+    a.slots = slots;
+    a.weights = weights;
+    a.residual = residual;
+    a.type = p->type;
+    a.k = p->top_k;
+    a.T = p->tokens;
+    a.n = p->n;
+    trace("moe_combine: type %d, T %lld n %lld k %d, residual %d", a.type, (long long)a.T, (long long)a.n, a.k, residual ? 1 : 0);
+    return hip_status(ascq::launch_moe_combine(a, S(stream)), "moe_combine");
+}
+
+ascq_status ascq_moe_combine_grad(float* grad_weights, void* grad_y, const void* grad_out, const void* y,
+                                  const int32_t* slots, const int32_t* row_tokens, const float* weights,
+                                  const ascq_rows_param* p, void* stream)
+{
+    CallScope scope;
+    const ascq_status s = rows_check("moe_combine_grad", p, false);
+    if (s != ASCQ_OK) return s;
+    if (p->tokens == 0) return ASCQ_OK;
+    if (!grad_weights && !grad_y) return ASCQ_OK;
+    if (!slots || (p->n > 0 && !grad_out) || (grad_weights && p->n > 0 && !y) || (grad_y && (!row_tokens || !weights)))
+        return fail(ASCQ_E_INVALID_ARG, "moe_combine_grad: null argument");
+    const size_t es = float_bytes(p->type);
+    if (!aligned(grad_weights, 4) || !aligned(grad_y, es) || !aligned(grad_out, es) || !aligned(y, es) || !aligned(slots, 4) ||
+        !aligned(row_tokens, 4) || !aligned(weights, 4))
+        return fail(ASCQ_E_INVALID_ARG, "moe_combine_grad: a pointer is not aligned to its element type");
+    ascq::MoeRowsArgs a{};
+    a.out = grad_y;
+    a.grad_weights = grad_weights;
+    a.x = grad_out;
+    a.y = y;
+    a.slots = slots;
+    a.row_tokens = row_tokens;
+    a.weights = weights;
+    a.type = p->type;
+    a.k = p->top_k;
+    a.T = p->tokens;
+    a.n = p->n;
+    trace("moe_combine_grad: type %d, T %lld n %lld k %d", a.type, (long long)a.T, (long long)a.n, a.k);
+    return hip_status(ascq::launch_moe_combine_grad(a, S(stream)), "moe_combine_grad");
+}
+
+// ------------------------------------------------------------------------------------------------
 // NZ fractal <-> ND
 // ------------------------------------------------------------------------------------------------
 namespace {

@@ -248,4 +248,75 @@ hipError_t launch_unpack_int4(int8_t* dst, const uint8_t* src, int64_t bytes, hi
 // transpose a [K, N] packed fp4 matrix (two per byte along N) into [N, K] (two per byte along K)
 hipError_t launch_fp4_transpose(uint8_t* dst, const uint8_t* src, int64_t K, int64_t N, hipStream_t st);
 
+// norm.hip: residual addition, RMS norm, 8-bit codes with a scale per row (any n, strides in elements, any alignment)
+struct NormQuantArgs {
+    void* q;                // [m, n] int8 / fp8 e4m3 codes
+    float* scale_out;       // [m]
+    void* h_out;            // x + residual [m, ldh], or null; may be x or residual (same stride)
+    void* norm_out;         // the norm itself [m, n], or null
+    const void *x, *residual, *gamma;  // [m, ldx], [m, ldr] or null, [n]
+    int src_type, dst_type;
+    int64_t m, n, ldx, ldr, ldh;
+    float eps;
+};
+hipError_t launch_norm_quant(const NormQuantArgs& a, hipStream_t st);
+
+// linear.hip: y = cast(act(sum_k x w * w_scale[n] * x_scale[m] + bias[n]) + residual)
+enum : int { ACT_NONE = 0, ACT_FASTER_GELU = 1, ACT_RELU = 2, ACT_GELU = 3, ACT_SILU = 4 };
+struct LinearArgs {
+    void* y;                // [M, ldy]
+    const uint8_t *x, *w;   // [M, ldx]; [N, ldw] (w_trans) or [K, ldw]; int8 or fp8 e4m3
+    const float *x_scale, *w_scale, *bias;  // [M], [N], [N] or null
+    const void* residual;   // [M, ldr] of the output type, or null; may be y (same stride)
+    int64_t M, N, K, ldx, ldw, ldr, ldy;
+    int f8, w_trans, act, out_type;
+};
+hipError_t launch_linear(const LinearArgs& a, hipStream_t st);
+
+// moe.hip
+struct MoeRouteArgs {
+    float* weights;         // [T, k]
+    int *experts, *slots;   // [T, k], -1: none
+    int* row_tokens;        // [T k], -1 behind the routed rows
+    int64_t *counts, *routed;  // [E], [1]
+    float* loss;            // [1]
+    const void* logits;     // [T, ld]
+    int type;
+    int64_t T, E, ld;
+    int k, renormalize;
+    int* block_counts;      // (set by the launcher, in the workspace) [blocks][E]
+    float* block_sums;      // [blocks][E]
+    int* block_live;        // [blocks]
+};
+size_t moe_route_ws_bytes(int64_t T, int64_t E);
+hipError_t launch_moe_route(MoeRouteArgs a, void* ws, hipStream_t st);
+struct MoeRouteGradArgs {
+    void* grad_logits;      // [T, ld_grad] of the logits' type
+    const void* logits;     // [T, ld]
+    int type;
+    const float* weights;
+    const int* experts;
+    const int64_t *counts, *routed;
+    const float *grad_weights, *grad_loss;  // [T, k] or null, [1] or null
+    int64_t T, E, ld, ld_grad;
+    int k, renormalize;
+};
+hipError_t launch_moe_route_grad(const MoeRouteGradArgs& a, hipStream_t st);
+// rows between the tokens' order and the experts': T tokens of k choices, T k rows
+struct MoeRowsArgs {
+    void* out;              // dispatch: rows [T k]; combine: [T, n]; combine_grad: grad of the rows [T k, n] or null
+    float* scale_out;       // dispatch: [T k] or null
+    float* grad_weights;    // combine_grad: [T, k] or null
+    const void* x;          // dispatch: tokens of row_bytes, ldx bytes apart; combine_grad: grad of the output [T, n]
+    const float* scale;     // dispatch: [T] or null
+    const void *y, *residual;  // combine: the experts' rows [T k, n]; [T, n] or null
+    const int *slots, *row_tokens;
+    const float* weights;
+    int type, k;
+    int64_t T, n, row_bytes, ldx;
+};
+hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st);
+hipError_t launch_moe_combine(const MoeRowsArgs& a, hipStream_t st);
+hipError_t launch_moe_combine_grad(const MoeRowsArgs& a, hipStream_t st);
+
 }  // namespace ascq

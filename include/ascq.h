@@ -541,9 +541,16 @@ ascq_status ascq_antiquant_matmul(uint16_t* y, const uint16_t* x, const void* w_
 /* ------------------------------------------------------------------------------------------
  * Quantized group matmul (MoE)
  * ------------------------------------------------------------------------------------------ */
-/* Activation of the group-matmul epilogue: none, or the sample's FasterGelu x / (1 + exp(-1.702 x)) in fp32
- * (quant_group_matmul_custom.asc:442-445; impl/adv_api/detail/activation/gelu/gelu_3510_impl.h:113-122). */
-typedef enum { ASCQ_ACT_NONE = 0, ASCQ_ACT_FASTER_GELU = 1 } ascq_activation;
+/* Activation of an epilogue, in fp32: none, the sample's FasterGelu x / (1 + exp(-1.702 x))
+ * (quant_group_matmul_custom.asc:442-445; impl/adv_api/detail/activation/gelu/gelu_3510_impl.h:113-122), and for
+ * ascq_quant_linear also ReLU, GELU (x Phi(x), the error-function form) and SiLU (x / (1 + exp(-x))). */
+typedef enum {
+    ASCQ_ACT_NONE = 0,
+    ASCQ_ACT_FASTER_GELU = 1,
+    ASCQ_ACT_RELU = 2,
+    ASCQ_ACT_GELU = 3,
+    ASCQ_ACT_SILU = 4
+} ascq_activation;
 
 /* ------------------------------------------------------------------------------------------
  * Replaces quant_group_matmul_custom (examples/01_simd_cpp_api/05_best_practices/03_fusion_compute/
@@ -558,6 +565,108 @@ ascq_status ascq_quant_group_matmul(void* y, int32_t out_type, const int8_t* x, 
                                     const int8_t* w, int32_t w_trans, const float* scale,
                                     const int64_t* group_list, int32_t list_type, int64_t num_groups, int64_t m,
                                     int64_t k, int64_t n, int32_t activation, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The operators of a quantised transformer block around its matrix products: no counterpart in the reference's
+ * hot path.  Strides (ld*) are row pitches in elements, 0 for dense rows; the elements of a row are contiguous.
+ * Pointers are aligned to their element type; 16-byte-aligned rows take the fast kernels.  Tensors may pass 2^32
+ * elements where nothing else is said.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+    int64_t m, n;
+    int64_t ld_x, ld_residual, ld_h;
+    int32_t src_type; /* F16, BF16, F32: x, residual, gamma, h_out, norm_out */
+    int32_t dst_type; /* INT8 or FP8_E4M3 */
+    float eps;
+} ascq_norm_quant_param;
+
+/* Residual addition, RMS norm and an 8-bit output with one scale per token, in one pass (no counterpart in the reference):
+ *   h = rnd(x + residual) (rounded to src_type, saturating; without residual h = x), stored to h_out when given
+ *   t_c = h_c gamma_c,  rstd = 1 / sqrt(mean_c h_c^2 + eps),  a = max_c |t_c|,  Q = 127 (int8) or 448 (e4m3)
+ *   q_c = rint(t_c (Q (1 / a))),  scale[row] = a rstd / Q, so that q scale is the norm h rstd gamma
+ *   norm_out (optional): rnd(t_c rstd), the unquantised norm.
+ * q and norm_out are dense [m, n].  h_out may be x or residual itself (with its stride); it needs a residual.  A row of
+ * zeros gives codes and scale 0.  A row with a NaN or an infinity in h or t, or whose sum of squares passes fp32's range,
+ * gives codes 0 and scale (and norm_out) NaN.  eps >= 0. */
+ascq_status ascq_add_rms_norm_quant(void* q, float* scale, void* h_out, void* norm_out, const void* x,
+                                    const void* residual, const void* gamma, const ascq_norm_quant_param* p,
+                                    void* stream);
+
+typedef struct {
+    int64_t m, n, k;
+    int64_t ld_x, ld_w, ld_residual, ld_y;
+    int32_t operand_type; /* INT8 or FP8_E4M3: x and w */
+    int32_t out_type;     /* F16, BF16, F32: y and residual */
+    int32_t w_trans;      /* 1: w [n, k]; 0: w [k, n] */
+    int32_t activation;   /* ascq_activation */
+} ascq_linear_param;
+
+/* The quantised linear (no counterpart in the reference):
+ * y = cast(act((sum_k x[m, k] w[k, n]) w_scale[n] x_scale[m] + bias[n]) + residual[m, n]), fp32 in this order, one
+ * rounding at the end (nearest even, saturating).  int8 sums are exact int32 (k below 2^17); fp8 sums are those of the fp8
+ * Matmul.  x_scale f32 [m], w_scale f32 [n]; bias f32 [n] or NULL; residual [m, n] or NULL (it may be y itself, with its
+ * stride).  k = 0 gives act(bias) + residual.
+ * workspace: optional, 16-byte aligned, ascq_quant_linear_workspace_size bytes (0 for many calls): room for the partial
+ * sums of few rows and for operands whose rows are off 16 bytes; a call with less of it, or none, takes kernels that
+ * need none and returns the same int8 results. */
+ascq_status ascq_quant_linear_workspace_size(const void* x, const void* w, const ascq_linear_param* p, size_t* bytes);
+ascq_status ascq_quant_linear(void* y, const void* x, const float* x_scale, const void* w, const float* w_scale,
+                              const float* bias, const void* residual, const ascq_linear_param* p, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+typedef struct {
+    int64_t tokens, experts; /* experts <= 1024 */
+    int64_t ld_logits;
+    int32_t logits_type;     /* F16, BF16, F32 */
+    int32_t top_k;           /* 1 <= top_k <= 16, <= experts */
+    int32_t renormalize;     /* 1: a token's weights are divided by their sum */
+} ascq_route_param;
+
+/* Expert routing (no counterpart in the reference).  logits [tokens, experts]; a logit of -inf or NaN counts nothing (its expert is masked for the token),
+ * +inf counts as the largest finite number.  p = softmax over what counts; a token's choices are its top_k largest logits
+ * in falling order, of equal ones the lowest expert; a token with fewer that count has fewer choices, a token of none
+ * (padding) has none.
+ *   weights  f32 [tokens, top_k]: p of the choice (renormalize: divided by their sum); 0 where there is none
+ *   experts  int32 [tokens, top_k]: the choice, -1 where there is none
+ *   slots    int32 [tokens, top_k]: the choice's row when rows are ordered by expert, then by token; -1 for none
+ *   row_tokens int32 [tokens * top_k]: the token of each row; -1 for the rows behind the last
+ *   counts   int64 [experts]: rows per expert -- ascq_quant_group_matmul's group list of list_type 1
+ *   routed   int64 [1]: tokens with a choice
+ *   loss     f32 [1]: the balance loss experts sum_e (counts_e / sum counts) (sum_t p_te / routed); 0 without a choice
+ * tokens * top_k < 2^31.  Equal inputs give equal bits: no order depends on timing.
+ * workspace (no counterpart in the reference): ascq_moe_route_workspace_size bytes, 16-byte aligned (NULL when 0). */
+ascq_status ascq_moe_route_workspace_size(const ascq_route_param* p, size_t* bytes);
+ascq_status ascq_moe_route(float* weights, int32_t* experts, int32_t* slots, int32_t* row_tokens, int64_t* counts,
+                           int64_t* routed, float* loss, const void* logits, const ascq_route_param* p, void* workspace,
+                           size_t workspace_bytes, void* stream);
+/* (no counterpart in the reference) The gradient with respect to the logits of grad_loss loss + sum_tj grad_weights_tj weights_tj (counts and choices taken
+ * as constants): grad_logits [tokens, ld_grad] of the logits' type; weights, experts, counts and routed as
+ * ascq_moe_route left them; grad_weights f32 [tokens, top_k] and grad_loss f32 [1], on the device, either may be NULL. */
+ascq_status ascq_moe_route_grad(void* grad_logits, int64_t ld_grad, const void* logits, const float* weights,
+                                const int32_t* experts, const int64_t* counts, const int64_t* routed,
+                                const float* grad_weights, const float* grad_loss, const ascq_route_param* p,
+                                void* stream);
+
+/* Rows between the tokens' order and the experts', by the slots and row_tokens of ascq_moe_route.  A slot outside
+ * [0, tokens * top_k) counts as none. */
+typedef struct {
+    int64_t tokens, n;
+    int64_t ld_x;   /* dispatch: x */
+    int32_t type;   /* dispatch: INT8, FP8_E4M3, F16, BF16 or F32; combine, combine_grad: F16, BF16, F32 */
+    int32_t top_k;  /* 1 .. 16 */
+} ascq_rows_param;
+/* (no counterpart in the reference) rows[slots[t, j]] = x[t], row_scale[slots[t, j]] = x_scale[t] (both NULL without scales); rows of no token are 0 */
+ascq_status ascq_moe_dispatch(void* rows, float* row_scale, const void* x, const float* x_scale, const int32_t* slots,
+                              const int32_t* row_tokens, const ascq_rows_param* p, void* stream);
+/* (no counterpart in the reference) out[t] = sum_j weights[t, j] y[slots[t, j]] + residual[t]: fp32, in the order of j, one rounding.  residual may be
+ * NULL, or out itself. */
+ascq_status ascq_moe_combine(void* out, const void* y, const int32_t* slots, const float* weights, const void* residual,
+                             const ascq_rows_param* p, void* stream);
+/* (no counterpart in the reference) grad_weights[t, j] = <grad_out[t], y[slots[t, j]]> (f32, 0 where there is no row) and grad_y[slots[t, j]] =
+ * weights[t, j] grad_out[t] (rows of no token are 0); either may be NULL.  The residual's gradient is grad_out. */
+ascq_status ascq_moe_combine_grad(float* grad_weights, void* grad_y, const void* grad_out, const void* y,
+                                  const int32_t* slots, const int32_t* row_tokens, const float* weights,
+                                  const ascq_rows_param* p, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * NZ fractal <-> ND layout converters
