@@ -70,6 +70,145 @@ __device__ __forceinline__ void block_reduce(float& ss, uint32_t& top)
     }
 }
 
+// A unit is 8 elements of a row: 16 bytes of a 16-bit type, 32 of f32.
+template <int T>
+struct Unit {
+    static constexpr int W = T == DT_F32 ? 2 : 1;  // 16-byte words
+    u32x4 w[W];
+    __device__ __forceinline__ float get(int e) const
+    {
+        if constexpr (T == DT_F32) return __uint_as_float(w[e / 4][e % 4]);
+        const uint32_t d = w[0][e / 2];
+        const uint16_t b = (uint16_t)(e & 1 ? d >> 16 : d);
+        return T == DT_F16 ? f16_to_f32(b) : bf16_to_f32(b);
+    }
+    // the unit of eight floats, rounded (16-bit types: nearest even, saturating)
+    __device__ __forceinline__ void set(const float (&f)[8])
+    {
+        if constexpr (T == DT_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e / 4][e % 4] = __float_as_uint(f[e]);
+        } else {
+            us2_t top = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[0][e] = cvt_pair<T == DT_BF16>(f[2 * e], f[2 * e + 1], top);
+            if (__builtin_expect(cvt_special<T == DT_BF16>(top), 0)) {
+                auto one = [](float x) { return (uint32_t)(T == DT_BF16 ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[0][e] = one(f[2 * e]) | (one(f[2 * e + 1]) << 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const void* row, uint32_t unit)
+    {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = __builtin_nontemporal_load((const u32x4*)row + unit * W + i);
+    }
+    __device__ __forceinline__ void store(void* row, uint32_t unit) const
+    {
+#pragma unroll
+        for (int i = 0; i < W; ++i) __builtin_nontemporal_store(w[i], (u32x4*)row + unit * W + i);
+    }
+};
+
+// Eight codes of values within the largest code (up to the fp32 roundings in front, which stay below the next one).
+// int8: adding 1.5 x 2^23 leaves the nearest integer, ties to even, in the low bits.
+__device__ __forceinline__ u32x2 codes8(const float (&v)[8], bool int8)
+{
+    u32x2 o;
+    if (int8) {
+        uint32_t b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(v[e] + 12582912.0f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t lo = __builtin_amdgcn_perm(b[4 * h + 1], b[4 * h], 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(b[4 * h + 3], b[4 * h + 2], 0x04000c0cu);
+            o[h] = lo | hi;
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            int d = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h], v[4 * h + 1], 0, false);
+            o[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2], v[4 * h + 3], d, true);
+        }
+    }
+    return o;
+}
+
+// Rows of whole units, aligned: one workgroup of NT threads per row, U units per thread, which hold the row (and gamma) in
+// registers between the reduction and the codes, so every byte moves once.  All loads of a thread are issued in front of
+// its first wait: units past the row repeat its last one (the maximum is not changed; they add nothing to the sum).
+template <int T, int NT, int U, bool RES>
+__global__ __launch_bounds__(NT) void norm_quant_row_kernel(NormQuantArgs a)
+{
+    const int64_t row = blockIdx.x;
+    const uint32_t units = (uint32_t)(a.n / 8), last = units - 1;
+    constexpr int ES = T == DT_F32 ? 4 : 2;
+    const uint8_t* x = (const uint8_t*)a.x + row * a.ldx * ES;
+    const uint8_t* r = (const uint8_t*)a.residual + (RES ? row * a.ldr * ES : 0);
+    Unit<T> h[U], g[U], add[RES ? U : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t c = threadIdx.x + u * NT;
+        h[u].load(x, c < units ? c : last);
+        if constexpr (RES) add[u].load(r, c < units ? c : last);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t c = threadIdx.x + u * NT;
+#pragma unroll
+        for (int i = 0; i < Unit<T>::W; ++i) g[u].w[i] = ((const u32x4*)a.gamma)[(c < units ? c : last) * Unit<T>::W + i];
+    }
+    float ss = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t c = threadIdx.x + u * NT;
+        if constexpr (RES) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = h[u].get(e) + add[u].get(e);
+            h[u].set(f);
+            if (a.h_out && c < units) h[u].store((uint8_t*)a.h_out + row * a.ldh * ES, c);
+        }
+        float part = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = h[u].get(e);
+            part = fmaf(v, v, part);
+            const uint32_t t = __float_as_uint(v * g[u].get(e)) & 0x7fffffffu;
+            top = t > top ? t : top;
+        }
+        ss += c < units ? part : 0.0f;
+    }
+    block_reduce<NT / 64>(ss, top);
+    const bool int8 = a.dst_type == DT_INT8;
+    const RowScale s = row_scale(ss, top, 1.0f / (float)a.n, a.eps, int8 ? 127.0f : 448.0f);
+    if (threadIdx.x == 0) a.scale_out[row] = s.scale;
+    u32x2* q = (u32x2*)((uint8_t*)a.q + row * a.n);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t c = threadIdx.x + u * NT;
+        if (c >= units) break;
+        float t[8], v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            t[e] = h[u].get(e) * g[u].get(e);
+            // (mult 0: a row of zeros, or one without an answer, whose products with 0 may be NaN)
+            v[e] = s.mult == 0.0f ? 0.0f : t[e] * s.mult;
+        }
+        __builtin_nontemporal_store(codes8(v, int8), q + c);
+        if (a.norm_out) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] *= s.rstd;
+            Unit<T> o;
+            o.set(t);
+            o.store((uint8_t*)a.norm_out + row * a.n * ES, c);
+        }
+    }
+}
+
 // Any n, strides and alignment: one workgroup per row, element by element, the row read twice (the second time from the
 // caches).  h is taken from h_out the second time: it may lie where x or the residual lay.
 __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
@@ -105,8 +244,42 @@ __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
 
 }  // namespace
 
+// The workgroup of a row: one wave up to 1024 elements, four up to 16384 (f32: 8192), sixteen up to 65536 (f32: 32768).
+template <int T, bool RES>
+static bool launch_row(const NormQuantArgs& a, hipStream_t st)
+{
+    const int64_t units = a.n / 8;
+    const dim3 grid((unsigned)a.m);
+#define ASCQ_NORM(NT, U)                                                                   \
+    if (units <= NT * U) {                                                                 \
+        launch_k((norm_quant_row_kernel<T, NT, U, RES>), grid, dim3(NT), 0u, st, a);       \
+        return true;                                                                       \
+    }
+    ASCQ_NORM(64, 1)
+    ASCQ_NORM(64, 2)
+    ASCQ_NORM(256, 1)
+    ASCQ_NORM(256, 2)
+    ASCQ_NORM(256, 4)
+    if constexpr (T != DT_F32) ASCQ_NORM(256, 8)
+    ASCQ_NORM(1024, 4)
+    if constexpr (T != DT_F32) ASCQ_NORM(1024, 8)
+#undef ASCQ_NORM
+    return false;
+}
+
 hipError_t launch_norm_quant(const NormQuantArgs& a, hipStream_t st)
 {
+    const int64_t es = a.src_type == DT_F32 ? 4 : 2;
+    const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.h_out | (uintptr_t)a.norm_out |
+                           (uintptr_t)a.gamma | (uintptr_t)(a.ldx * es) | (uintptr_t)(a.residual ? a.ldr * es : 0) |
+                           (uintptr_t)(a.h_out ? a.ldh * es : 0);
+    if (bits % 16 == 0 && (uintptr_t)a.q % 8 == 0 && a.n % 8 == 0) {
+        bool done;
+        if (a.src_type == DT_F16) done = a.residual ? launch_row<DT_F16, true>(a, st) : launch_row<DT_F16, false>(a, st);
+        else if (a.src_type == DT_BF16) done = a.residual ? launch_row<DT_BF16, true>(a, st) : launch_row<DT_BF16, false>(a, st);
+        else done = a.residual ? launch_row<DT_F32, true>(a, st) : launch_row<DT_F32, false>(a, st);
+        if (done) return hipGetLastError();
+    }
     launch_k(norm_quant_any_kernel, dim3((unsigned)a.m), dim3(256), 0u, st, a);
     return hipGetLastError();
 }
