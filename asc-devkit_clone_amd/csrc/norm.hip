@@ -9,6 +9,8 @@
 // stored stream's type), the codes' and norm's.
 // A row of zeros has codes and scale 0.  A row with a NaN, an infinity, or squares that pass fp32's range has codes 0 and
 // scale NaN, so that its products are NaN and not some number.
+#include <type_traits>
+
 #include "common.h"
 #include "launch.h"
 
@@ -70,6 +72,10 @@ __device__ __forceinline__ void block_reduce(float& ss, uint32_t& top)
     }
 }
 
+// 16 (8) bytes at any element's (byte's) address: the memory pipeline takes wide accesses of any alignment
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+
 // A unit is 8 elements of a row: 16 bytes of a 16-bit type, 32 of f32.
 template <int T>
 struct Unit {
@@ -99,15 +105,39 @@ struct Unit {
             }
         }
     }
+    template <bool ANY>
     __device__ __forceinline__ void load(const void* row, uint32_t unit)
     {
+        typedef typename std::conditional<ANY, u32x4_any, u32x4>::type word_t;
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = __builtin_nontemporal_load((const u32x4*)row + unit * W + i);
+        for (int i = 0; i < W; ++i) w[i] = __builtin_nontemporal_load((const word_t*)row + unit * W + i);
     }
+    template <bool ANY>
     __device__ __forceinline__ void store(void* row, uint32_t unit) const
     {
+        typedef typename std::conditional<ANY, u32x4_any, u32x4>::type word_t;
 #pragma unroll
-        for (int i = 0; i < W; ++i) __builtin_nontemporal_store(w[i], (u32x4*)row + unit * W + i);
+        for (int i = 0; i < W; ++i) __builtin_nontemporal_store(w[i], (word_t*)row + unit * W + i);
+    }
+    // the first `count` elements, zeros behind
+    __device__ __forceinline__ void load_part(const void* row, uint32_t unit, int count)
+    {
+        w[0] = w[W - 1] = (u32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e >= count) continue;
+            if constexpr (T == DT_F32) w[e / 4][e % 4] = ((const uint32_t*)row)[unit * 8 + e];
+            else w[0][e / 2] |= (uint32_t)((const uint16_t*)row)[unit * 8 + e] << (16 * (e & 1));
+        }
+    }
+    __device__ __forceinline__ void store_part(void* row, uint32_t unit, int count) const
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e >= count) continue;
+            if constexpr (T == DT_F32) ((uint32_t*)row)[unit * 8 + e] = w[e / 4][e % 4];
+            else ((uint16_t*)row)[unit * 8 + e] = (uint16_t)(w[0][e / 2] >> (16 * (e & 1)));
+        }
     }
 };
 
@@ -136,57 +166,75 @@ __device__ __forceinline__ u32x2 codes8(const float (&v)[8], bool int8)
     return o;
 }
 
-// Rows of whole units, aligned: one workgroup of NT threads per row, U units per thread, which hold the row (and gamma) in
-// registers between the reduction and the codes, so every byte moves once.  All loads of a thread are issued in front of
-// its first wait: units past the row repeat its last one (the maximum is not changed; they add nothing to the sum).
-template <int T, int NT, int U, bool RES>
+// One workgroup of NT threads per row, U units per thread, which hold the row (and gamma) in registers between the reduction
+// and the codes, so every byte moves once.  All loads of a thread are issued in front of its first wait: units past the
+// row read its last whole one and are dropped (in place, another thread may have stored it by then).
+// ANY: rows that start at any element, whose last unit may be a part of one.
+template <int T, int NT, int U, bool RES, bool ANY>
 __global__ __launch_bounds__(NT) void norm_quant_row_kernel(NormQuantArgs a)
 {
     const int64_t row = blockIdx.x;
-    const uint32_t units = (uint32_t)(a.n / 8), last = units - 1;
+    const uint32_t whole = (uint32_t)(a.n / 8), units = ANY ? (uint32_t)((a.n + 7) / 8) : whole;
+    const int part = ANY ? (int)(a.n % 8) : 0;
     constexpr int ES = T == DT_F32 ? 4 : 2;
     const uint8_t* x = (const uint8_t*)a.x + row * a.ldx * ES;
     const uint8_t* r = (const uint8_t*)a.residual + (RES ? row * a.ldr * ES : 0);
     Unit<T> h[U], g[U], add[RES ? U : 1];
+    if (!ANY || whole > 0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t c = threadIdx.x + u * NT;
-        h[u].load(x, c < units ? c : last);
-        if constexpr (RES) add[u].load(r, c < units ? c : last);
-    }
+        for (int u = 0; u < U; ++u) {
+            const uint32_t c = threadIdx.x + u * NT, k = c < whole ? c : whole - 1;
+            h[u].template load<ANY>(x, k);
+            if constexpr (RES) add[u].template load<ANY>(r, k);
+        }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t c = threadIdx.x + u * NT;
+        for (int u = 0; u < U; ++u) {
+            typedef typename std::conditional<ANY, u32x4_any, u32x4>::type word_t;
+            const uint32_t c = threadIdx.x + u * NT, k = c < whole ? c : whole - 1;
 #pragma unroll
-        for (int i = 0; i < Unit<T>::W; ++i) g[u].w[i] = ((const u32x4*)a.gamma)[(c < units ? c : last) * Unit<T>::W + i];
+            for (int i = 0; i < Unit<T>::W; ++i) g[u].w[i] = ((const word_t*)a.gamma)[k * Unit<T>::W + i];
+        }
     }
     float ss = 0.0f;
     uint32_t top = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t c = threadIdx.x + u * NT;
+        if (ANY && c == whole && part) {
+            h[u].load_part(x, c, part);
+            if constexpr (RES) add[u].load_part(r, c, part);
+            g[u].load_part(a.gamma, c, part);
+        }
         if constexpr (RES) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = h[u].get(e) + add[u].get(e);
             h[u].set(f);
-            if (a.h_out && c < units) h[u].store((uint8_t*)a.h_out + row * a.ldh * ES, c);
+            if (a.h_out) {
+                uint8_t* to = (uint8_t*)a.h_out + row * a.ldh * ES;
+                if (c < whole) h[u].template store<ANY>(to, c);
+                else if (ANY && c == whole) h[u].store_part(to, c, part);
+            }
         }
-        float part = 0.0f;
+        float sum = 0.0f;
+        uint32_t most = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float v = h[u].get(e);
-            part = fmaf(v, v, part);
+            sum = fmaf(v, v, sum);
             const uint32_t t = __float_as_uint(v * g[u].get(e)) & 0x7fffffffu;
-            top = t > top ? t : top;
+            most = t > most ? t : most;
         }
-        ss += c < units ? part : 0.0f;
+        if (c < units) {
+            ss += sum;
+            top = most > top ? most : top;
+        }
     }
     block_reduce<NT / 64>(ss, top);
     const bool int8 = a.dst_type == DT_INT8;
     const RowScale s = row_scale(ss, top, 1.0f / (float)a.n, a.eps, int8 ? 127.0f : 448.0f);
     if (threadIdx.x == 0) a.scale_out[row] = s.scale;
-    u32x2* q = (u32x2*)((uint8_t*)a.q + row * a.n);
+    uint8_t* q = (uint8_t*)a.q + row * a.n;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t c = threadIdx.x + u * NT;
@@ -198,18 +246,28 @@ __global__ __launch_bounds__(NT) void norm_quant_row_kernel(NormQuantArgs a)
             // (mult 0: a row of zeros, or one without an answer, whose products with 0 may be NaN)
             v[e] = s.mult == 0.0f ? 0.0f : t[e] * s.mult;
         }
-        __builtin_nontemporal_store(codes8(v, int8), q + c);
+        const u32x2 codes = codes8(v, int8);
+        if (!ANY || c < whole) {
+            typedef typename std::conditional<ANY, u32x2_any, u32x2>::type codes_t;
+            __builtin_nontemporal_store(codes, (codes_t*)q + c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < part) q[c * 8 + e] = (uint8_t)(codes[e / 4] >> (8 * (e % 4)));
+        }
         if (a.norm_out) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] *= s.rstd;
             Unit<T> o;
             o.set(t);
-            o.store((uint8_t*)a.norm_out + row * a.n * ES, c);
+            uint8_t* to = (uint8_t*)a.norm_out + row * a.n * ES;
+            if (!ANY || c < whole) o.template store<ANY>(to, c);
+            else o.store_part(to, c, part);
         }
     }
 }
 
-// Any n, strides and alignment: one workgroup per row, element by element, the row read twice (the second time from the
+// Rows too long for registers: one workgroup per row, element by element, the row read twice (the second time from the
 // caches).  h is taken from h_out the second time: it may lie where x or the residual lay.
 __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
 {
@@ -244,27 +302,39 @@ __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
 
 }  // namespace
 
-// The workgroup of a row: one wave up to 1024 elements, four up to 16384 (f32: 8192), sixteen up to 65536 (f32: 32768).
-template <int T, bool RES>
+// The workgroup of a row: a thread holds up to 8 units (f32: 4)
+template <int T, bool RES, bool ANY>
 static bool launch_row(const NormQuantArgs& a, hipStream_t st)
 {
-    const int64_t units = a.n / 8;
+    const int64_t units = (a.n + 7) / 8;
     const dim3 grid((unsigned)a.m);
 #define ASCQ_NORM(NT, U)                                                                   \
     if (units <= NT * U) {                                                                 \
-        launch_k((norm_quant_row_kernel<T, NT, U, RES>), grid, dim3(NT), 0u, st, a);       \
+        launch_k((norm_quant_row_kernel<T, NT, U, RES, ANY>), grid, dim3(NT), 0u, st, a);  \
         return true;                                                                       \
     }
     ASCQ_NORM(64, 1)
     ASCQ_NORM(64, 2)
     ASCQ_NORM(256, 1)
     ASCQ_NORM(256, 2)
-    ASCQ_NORM(256, 4)
-    if constexpr (T != DT_F32) ASCQ_NORM(256, 8)
-    ASCQ_NORM(1024, 4)
-    if constexpr (T != DT_F32) ASCQ_NORM(1024, 8)
+    if constexpr (T == DT_F32) {
+        ASCQ_NORM(512, 2)
+        ASCQ_NORM(1024, 2)
+        ASCQ_NORM(1024, 4)
+    } else {
+        ASCQ_NORM(256, 4)
+        ASCQ_NORM(256, 8)
+        ASCQ_NORM(1024, 4)
+        ASCQ_NORM(1024, 8)
+    }
 #undef ASCQ_NORM
     return false;
+}
+template <int T>
+static bool launch_row_of(const NormQuantArgs& a, bool any, hipStream_t st)
+{
+    if (any) return a.residual ? launch_row<T, true, true>(a, st) : launch_row<T, false, true>(a, st);
+    return a.residual ? launch_row<T, true, false>(a, st) : launch_row<T, false, false>(a, st);
 }
 
 hipError_t launch_norm_quant(const NormQuantArgs& a, hipStream_t st)
@@ -273,14 +343,11 @@ hipError_t launch_norm_quant(const NormQuantArgs& a, hipStream_t st)
     const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.h_out | (uintptr_t)a.norm_out |
                            (uintptr_t)a.gamma | (uintptr_t)(a.ldx * es) | (uintptr_t)(a.residual ? a.ldr * es : 0) |
                            (uintptr_t)(a.h_out ? a.ldh * es : 0);
-    if (bits % 16 == 0 && (uintptr_t)a.q % 8 == 0 && a.n % 8 == 0) {
-        bool done;
-        if (a.src_type == DT_F16) done = a.residual ? launch_row<DT_F16, true>(a, st) : launch_row<DT_F16, false>(a, st);
-        else if (a.src_type == DT_BF16) done = a.residual ? launch_row<DT_BF16, true>(a, st) : launch_row<DT_BF16, false>(a, st);
-        else done = a.residual ? launch_row<DT_F32, true>(a, st) : launch_row<DT_F32, false>(a, st);
-        if (done) return hipGetLastError();
-    }
-    launch_k(norm_quant_any_kernel, dim3((unsigned)a.m), dim3(256), 0u, st, a);
+    const bool any = bits % 16 != 0 || (uintptr_t)a.q % 8 != 0 || a.n % 8 != 0;
+    const bool done = a.src_type == DT_F16    ? launch_row_of<DT_F16>(a, any, st)
+                      : a.src_type == DT_BF16 ? launch_row_of<DT_BF16>(a, any, st)
+                                              : launch_row_of<DT_F32>(a, any, st);
+    if (!done) launch_k(norm_quant_any_kernel, dim3((unsigned)a.m), dim3(256), 0u, st, a);
     return hipGetLastError();
 }
 

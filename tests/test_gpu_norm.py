@@ -97,10 +97,12 @@ def test_strides_and_alignment(ascq_gpu, n, pad, shift, dt):
     assert torch.equal(bh[untouched], before[untouched])
 
 
-@pytest.mark.parametrize("n", [257, 4096, 30000])
+@pytest.mark.parametrize("n", [8, 72, 257, 1000, 3001, 4096, 5120, 11008, 20000, 30000, 66000])
 @pytest.mark.parametrize("into", ["x", "residual"])
 def test_in_place(ascq_gpu, n, into):
-    x, r, gamma = _data(4, n, "bf16", n)
+    """threads whose share of a row is not whole read its last elements too: they must not count once they are stored over"""
+    x, r, gamma = _data(40, n, "bf16", n)
+    r[:, -8:] *= 30  # (the last elements' second sum would be the largest)
     gx, gr = x.cuda(), r.cuda()
     q, s, h = ascq_gpu.add_rms_norm_quant(gx, gamma.cuda(), EPS, residual=gr, residual_out=gx if into == "x" else gr)
     _check(x, gamma, r, "int8", q.cpu(), s.cpu(), h.cpu())
