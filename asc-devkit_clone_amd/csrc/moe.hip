@@ -10,9 +10,12 @@
 //   loss = E sum_e (counts_e / sum counts) (sum_t p_te / routed).
 // Every order is fixed -- no atomic decides a row or the order of a sum -- so equal inputs give equal bits.
 //
-// A block of ROUTE_TOKENS tokens notes the tokens that chose an expert as one 64-bit mask per expert: the rank of a token
-// among them is a population count, and so is the block's count.  Blocks meet through a workspace: their counts and their
-// sums of p; a second launch turns the counts before a block into its rows' offsets.
+// A chunk of 64 tokens notes those that chose an expert as one 64-bit mask per expert: the rank of a token among them is a
+// population count, and so is the chunk's count.  Blocks of chunks meet through a workspace: their counts and their sums
+// of p; the second launch turns the counts before a block into its rows' offsets.  Up to 64 tokens are one block, which does it all.
+// What bounds it is latency: a chain of k maxima over a token's experts, and two launches.
+#include <type_traits>
+
 #include "common.h"
 #include "group_tile.h"
 #include "launch.h"
@@ -21,7 +24,9 @@ namespace ascq {
 
 namespace {
 
-constexpr int ROUTE_TOKENS = 64;
+constexpr int CHUNK = 64;        // tokens of a mask
+constexpr int MAX_BLOCKS = 512;  // (each block of the second launch reads the counts of all)
+constexpr int MAX_K = 16;
 
 __device__ __forceinline__ float load_logit(const void* p, int64_t i, int dtype)
 {
@@ -29,29 +34,6 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i, int dtype)
     return v != v ? -__builtin_inff() : fminf(v, 3.402823466e38f);
 }
 
-// One wave per token, lane l holding experts l, l + 64, ...: the largest remaining logit and its expert (the lowest of
-// equals), in every lane; expert -1 when nothing is left that counts
-template <int V>
-__device__ __forceinline__ void wave_best(const float (&v)[V], int lane, float& best, int& expert)
-{
-    best = -__builtin_inff();
-    expert = -1;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (v[i] > best) {
-            best = v[i];
-            expert = lane + 64 * i;
-        }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const float ov = __shfl_xor(best, o, 64);
-        const int oe = __shfl_xor(expert, o, 64);
-        if (ov > best || (ov == best && (uint32_t)oe < (uint32_t)expert)) {
-            best = ov;
-            expert = oe;
-        }
-    }
-}
 __device__ __forceinline__ float wave_sum(float v)
 {
 #pragma unroll
@@ -59,133 +41,299 @@ __device__ __forceinline__ float wave_sum(float v)
     return v;
 }
 
-__device__ __forceinline__ uint64_t below(int t) { return t >= 64 ? ~0ull : (1ull << t) - 1ull; }
+// The value of the lane that step S (1, 2, 4, 8) of a butterfly within 16 lanes meets: quad permutations, then mirrors,
+// which reach the other half because the lanes of a half already agree.
+template <int S>
+__device__ __forceinline__ int meet(int v)
+{
+    constexpr int ctrl = S == 1 ? 0xB1 : S == 2 ? 0x4E : S == 4 ? 0x141 : 0x140;
+    return __builtin_amdgcn_update_dpp(0, v, ctrl, 0xf, 0xf, true);
+}
+// (beyond 16 lanes: through the cross-lane network)
+template <int S>
+__device__ __forceinline__ int meet_any(int v)
+{
+    if constexpr (S < 16) return meet<S>(v);
+    else return __shfl_xor(v, S, 64);
+}
+template <int S>
+__device__ __forceinline__ float meet_any(float v) { return __int_as_float(meet_any<S>(__float_as_int(v))); }
+// f(step) for the steps of a butterfly over G lanes
+template <int G, class F>
+__device__ __forceinline__ void butterfly(F f)
+{
+    if constexpr (G > 1) f(std::integral_constant<int, 1>{});
+    if constexpr (G > 2) f(std::integral_constant<int, 2>{});
+    if constexpr (G > 4) f(std::integral_constant<int, 4>{});
+    if constexpr (G > 8) f(std::integral_constant<int, 8>{});
+    if constexpr (G > 16) f(std::integral_constant<int, 16>{});
+    if constexpr (G > 32) f(std::integral_constant<int, 32>{});
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v)
+{
+    butterfly<G>([&](auto s) { v += meet_any<decltype(s)::value>(v); });
+    return v;
+}
+
+// logits e0 .. e0 + V - 1 of a row (past E: -inf); vec: the row's V are one aligned run
+template <int V>
+__device__ __forceinline__ void load_logits(const void* row, int type, int e0, int E, bool vec, float (&v)[V])
+{
+    if (vec && e0 + V <= E) {
+        if (type == DT_F32) {
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+                const u32x4 w = ((const u32x4*)((const float*)row + e0))[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * i + j] = __uint_as_float(w[j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 8; ++i) {
+                const u32x4 w = ((const u32x4*)((const uint16_t*)row + e0))[i];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint16_t h = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+                    v[8 * i + j] = type == DT_F16 ? f16_to_f32(h) : bf16_to_f32(h);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = e0 + i < E ? load_f32_of(row, e0 + i, type) : -__builtin_inff();
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = v[i] != v[i] ? -__builtin_inff() : fminf(v[i], 3.402823466e38f);
+}
 
 }  // namespace
 
-// one workgroup of 4 waves per ROUTE_TOKENS tokens
-template <int V>
-__global__ __launch_bounds__(256) void moe_route_kernel(MoeRouteArgs a)
+// G lanes per token, each with V neighbouring experts; a chunk at a time, all of its tokens at once up to 16 lanes.
+// SINGLE: one block has all tokens.
+template <int G>
+constexpr int route_threads = G < 16 ? 64 * G : 1024;
+template <int G, int V, bool SINGLE>
+__global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArgs a)
 {
-    extern __shared__ uint64_t masks[];          // [E] tokens of this block that chose the expert
-    float* sums = (float*)(masks + a.E);         // [4][E]
-    __shared__ uint64_t live;                    // tokens of this block with a choice
-    const int E = (int)a.E, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int e = threadIdx.x; e < E; e += 256) masks[e] = 0;
-    if (threadIdx.x == 0) live = 0;
-    __syncthreads();
-    const int64_t t0 = (int64_t)blockIdx.x * ROUTE_TOKENS;
+    constexpr int NT = route_threads<G>, NW = NT / 64, TOK = NT / G;  // TOK tokens at once
+    extern __shared__ __attribute__((aligned(8))) uint8_t lds[];
+    const int E = (int)a.E, k = a.k;
+    uint64_t* masks = (uint64_t*)lds;           // [E] tokens of the chunk that chose the expert
+    float* sums = (float*)(masks + E);          // [waves][E] sums of p
+    int* first = (int*)(sums + NW * E);         // [E] the block's choices of the expert in the chunks before
+    __shared__ float s_w[CHUNK * MAX_K], s_f[CHUNK];
+    __shared__ int s_e[CHUNK * MAX_K];
+    __shared__ int s_live[NW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e0 = tid % G * V;
+    const int64_t chunks = (a.T + CHUNK - 1) / CHUNK;
+    const int64_t c0 = chunks * blockIdx.x / gridDim.x, c1 = chunks * (blockIdx.x + 1) / gridDim.x;
+    const bool vec = ((uintptr_t)a.logits | (uintptr_t)(a.ld * (a.type == DT_F32 ? 4 : 2))) % 16 == 0;
+    const int64_t row_bytes = a.ld * (a.type == DT_F32 ? 4 : 2);
+    if (tid < E) first[tid] = 0;
     float psum[V] = {};
-    for (int i = wave; i < ROUTE_TOKENS; i += 4) {
-        const int64_t t = t0 + i;
-        if (t >= a.T) break;
-        float v[V], p[V];
+    int live = 0;
+    for (int64_t c = c0; c < c1; ++c) {
+        if (tid < E) masks[tid] = 0;
+        __syncthreads();
+        for (int token = tid / G; token < CHUNK; token += TOK) {
+            const int64_t t = c * CHUNK + token;
+            const bool here = t < a.T;
+            float v[V], p[V];
+            if (here) load_logits<V>((const uint8_t*)a.logits + t * row_bytes, a.type, e0, E, vec, v);
+            else {
 #pragma unroll
-        for (int u = 0; u < V; ++u) {
-            const int e = lane + 64 * u;
-            p[u] = v[u] = e < E ? load_logit(a.logits, t * a.ld + e, a.type) : -__builtin_inff();
-        }
-        float top = 0.0f, sum = 0.0f, wsum = 0.0f, w = 0.0f;
-        int choice = -1;
-        for (int j = 0; j < a.k; ++j) {
-            float best;
-            int e;
-            wave_best<V>(v, lane, best, e);
-            if (j == 0) {
-                top = best;
-#pragma unroll
-                for (int u = 0; u < V; ++u) p[u] = e >= 0 && p[u] > -__builtin_inff() ? expf(p[u] - top) : 0.0f;
-#pragma unroll
-                for (int u = 0; u < V; ++u) sum += p[u];
-                sum = wave_sum(sum);
-                if (e < 0) sum = 1.0f;
-                if (lane == 0 && e >= 0) atomicOr((unsigned long long*)&live, 1ull << i);
+                for (int i = 0; i < V; ++i) v[i] = -__builtin_inff();
             }
-            const float q = e >= 0 ? expf(best - top) / sum : 0.0f;
-            wsum += q;
-            if (lane == j) {
-                w = q;
-                choice = e;
-            }
-            if (e >= 0) {
-                if (lane == (e & 63)) {
 #pragma unroll
-                    for (int u = 0; u < V; ++u)
-                        if (u == e >> 6) v[u] = -__builtin_inff();
+            for (int i = 0; i < V; ++i) p[i] = v[i];
+            float top = 0.0f, inv = 0.0f, wsum = 0.0f;
+            for (int j = 0; j < k; ++j) {
+                // the largest logit left and its expert, the lowest of equals; -1 when nothing is left that counts
+                float best = -__builtin_inff();
+                int e = -1;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (v[i] > best) {
+                        best = v[i];
+                        e = e0 + i;
+                    }
+                butterfly<G>([&](auto s) {
+                    const float ob = meet_any<decltype(s)::value>(best);
+                        const int oe = meet_any<decltype(s)::value>(e);
+                    if (ob > best || (ob == best && (uint32_t)oe < (uint32_t)e)) {
+                        best = ob;
+                        e = oe;
+                    }
+                });
+                if (j == 0) {
+                    top = e >= 0 ? best : 0.0f;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        p[i] = expf(p[i] - top);
+                        sum += p[i];
+                    }
+                    sum = group_sum<G>(sum);
+                    inv = e >= 0 ? 1.0f / sum : 0.0f;
+                    live += e >= 0;
                 }
-                if (lane == 0) atomicOr((unsigned long long*)&masks[e], 1ull << i);
+                const float q = e >= 0 ? expf(best - top) * inv : 0.0f;
+                wsum += q;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (e == e0 + i) v[i] = -__builtin_inff();
+                if (e0 == 0 && here) {
+                    s_w[token * k + j] = q;
+                    s_e[token * k + j] = e;
+                    if (e >= 0) atomicOr((unsigned long long*)&masks[e], 1ull << token);
+                }
             }
-        }
-        if (lane < a.k) {
-            if (a.renormalize) w = wsum > 0.0f ? w / wsum : 0.0f;
-            a.weights[t * a.k + lane] = w;
-            a.experts[t * a.k + lane] = choice;
-        }
+            if (e0 == 0) s_f[token] = !a.renormalize ? 1.0f : (wsum > 0.0f ? 1.0f / wsum : 0.0f);
 #pragma unroll
-        for (int u = 0; u < V; ++u) psum[u] += p[u] / sum;
+            for (int i = 0; i < V; ++i) psum[i] += p[i] * inv;
+        }
+        __syncthreads();
+        // the choices leave in order; a choice's rank among those of its expert in this block
+        const int64_t left = (a.T - c * CHUNK) * k, n = left < CHUNK * k ? left : CHUNK * k;
+        for (int i = tid; i < n; i += NT) {
+            const int e = s_e[i], tk = i / k;
+            const int64_t at = c * CHUNK * k + i;
+            a.weights[at] = s_w[i] * s_f[tk];
+            a.experts[at] = e;
+            const int rank = e < 0 ? -1 : first[e] + __popcll(masks[e] & ((1ull << tk) - 1ull));
+            if constexpr (!SINGLE) a.slots[at] = rank;
+            else s_w[i] = __int_as_float(rank);
+        }
+        __syncthreads();
+        if (tid < E) first[tid] += __popcll(masks[tid]);
     }
+    // sums over the block's tokens: the wave's, then the waves' in order
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-        const int e = lane + 64 * u;
-        if (e < E) sums[wave * E + e] = psum[u];
+    for (int o = G; o < 64; o <<= 1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) psum[i] += __shfl_xor(psum[i], o, 64);
+        live += __shfl_xor(live, o, 64);
+    }
+    if (lane < G) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (e0 + i < E) sums[wave * E + e0 + i] = psum[i];
+        if (lane == 0) s_live[wave] = live;
     }
     __syncthreads();
-    // rank of each choice among the block's choices of its expert; the block's counts and sums of p
-    for (int i = threadIdx.x; i < ROUTE_TOKENS * a.k; i += 256) {
-        const int64_t at = t0 * a.k + i;
-        if (at >= a.T * a.k) break;
-        const int e = a.experts[at];
-        a.slots[at] = e < 0 ? -1 : __popcll(masks[e] & below(i / a.k));
+    float p = 0.0f;
+    int routed = 0;
+    for (int w = 0; w < NW; ++w) {
+        if (tid < E) p += sums[w * E + tid];
+        routed += s_live[w];
     }
-    for (int e = threadIdx.x; e < E; e += 256) {
-        a.block_counts[(int64_t)blockIdx.x * E + e] = __popcll(masks[e]);
-        a.block_sums[(int64_t)blockIdx.x * E + e] = (sums[e] + sums[E + e]) + (sums[2 * E + e] + sums[3 * E + e]);
+    if constexpr (!SINGLE) {
+        if (tid < E) {
+            a.block_counts[(int64_t)blockIdx.x * E + tid] = first[tid];
+            a.block_sums[(int64_t)blockIdx.x * E + tid] = p;
+        }
+        if (tid == 0) a.block_live[blockIdx.x] = routed;
+    } else {
+        __shared__ int64_t wtot[NW];
+        __shared__ float s_loss[NW];
+        int64_t total;
+        const int mine = tid < E ? first[tid] : 0;
+        const int64_t before = block_exclusive_scan<NT>(mine, wtot, &total);
+        if (tid < E) {
+            first[tid] = (int)before;
+            a.counts[tid] = mine;
+        }
+        const float part = wave_sum((float)mine * p);
+        if (lane == 0) s_loss[wave] = part;
+        __syncthreads();
+        const int n = (int)a.T * k;
+        for (int i = tid; i < n; i += NT) {
+            const int rank = __float_as_int(s_w[i]), e = s_e[i];
+            const int slot = rank < 0 ? -1 : first[e] + rank;
+            a.slots[i] = slot;
+            if (slot >= 0) a.row_tokens[slot] = i / k;
+            if (i >= total) a.row_tokens[i] = -1;
+        }
+        if (tid == 0) {
+            float sum = 0.0f;
+            for (int w = 0; w < NW; ++w) sum += s_loss[w];
+            *a.routed = routed;
+            *a.loss = total > 0 ? (float)E * (sum / ((float)total * (float)routed)) : 0.0f;
+        }
     }
-    if (threadIdx.x == 0) a.block_live[blockIdx.x] = __popcll(live);
 }
 
-// offsets of every block's rows: those of the experts before, then of the blocks before within the expert
-__global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a)
+// Offsets of a block's rows: those of the experts before, then of the blocks before within the expert.  A thread adds up
+// one expert's counts over every P-th block.
+__global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int blocks)
 {
     extern __shared__ int base[];  // [E]
     __shared__ int64_t wtot[16];
     __shared__ float s_loss[16];
-    const int E = (int)a.E, e = threadIdx.x;
-    const int64_t blocks = (a.T + ROUTE_TOKENS - 1) / ROUTE_TOKENS;
-    int64_t before = 0, all = 0, total;
+    __shared__ int s_all[1024], s_before[1024];
+    __shared__ float s_p[1024];
+    const int E = (int)a.E, k = a.k, tid = threadIdx.x, b0 = blockIdx.x;
+    const int P = 1024 / E, e = tid % E, part = tid / E;
+    int before = 0, all = 0;
     float p = 0.0f;
-    if (e < E)
-        for (int64_t b = 0; b < blocks; ++b) {
+    if (part < P) {
+#pragma unroll 4
+        for (int b = part; b < blocks; b += P) {
             const int c = a.block_counts[b * E + e];
-            if (b < (int64_t)blockIdx.x) before += c;
             all += c;
-            p += a.block_sums[b * E + e];
+            before += b < b0 ? c : 0;
         }
-    const int64_t first = block_exclusive_scan<1024>(all, wtot, &total);
-    if (e < E) base[e] = (int)(first + before);
+        if (b0 == 0)
+#pragma unroll 4
+            for (int b = part; b < blocks; b += P) p += a.block_sums[b * E + e];
+    }
+    s_all[tid] = all;
+    s_before[tid] = before;
+    s_p[tid] = p;
     __syncthreads();
-    const int64_t t0 = (int64_t)blockIdx.x * ROUTE_TOKENS;
-    for (int i = threadIdx.x; i < ROUTE_TOKENS * a.k; i += 1024) {
-        const int64_t at = t0 * a.k + i;
-        if (at >= a.T * a.k) break;
+    all = before = 0;
+    p = 0.0f;
+    if (tid < E)
+        for (int i = 0; i < P; ++i) {
+            all += s_all[i * E + tid];
+            before += s_before[i * E + tid];
+            p += s_p[i * E + tid];
+        }
+    int64_t total;
+    const int64_t start = block_exclusive_scan<1024>(all, wtot, &total);
+    if (tid < E) base[tid] = (int)start + before;
+    __syncthreads();
+    const int64_t chunks = (a.T + CHUNK - 1) / CHUNK;
+    const int64_t c0 = chunks * b0 / blocks, c1 = chunks * (b0 + 1) / blocks;
+    const int64_t end = c1 * CHUNK < a.T ? c1 * CHUNK * k : a.T * k;
+    for (int64_t at = c0 * CHUNK * k + tid; at < end; at += 1024) {
         if (at >= total) a.row_tokens[at] = -1;
         const int x = a.experts[at];
         if (x < 0) continue;
         const int slot = base[x] + a.slots[at];
         a.slots[at] = slot;
-        a.row_tokens[slot] = (int)(at / a.k);
+        a.row_tokens[slot] = (int)(at / k);
     }
-    if (blockIdx.x != 0) return;
-    int64_t live = 0;
-    for (int64_t b = 0; b < blocks; ++b) live += a.block_live[b];
-    if (e < E) a.counts[e] = all;
-    float part = e < E ? (float)all * p : 0.0f;
-    part = wave_sum(part);
-    if ((threadIdx.x & 63) == 0) s_loss[threadIdx.x >> 6] = part;
+    if (b0 != 0) return;
+    int live = 0;
+    for (int b = tid; b < blocks; b += 1024) live += a.block_live[b];
+    if (tid < E) a.counts[tid] = all;
+    const float loss = wave_sum(tid < E ? (float)all * p : 0.0f);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) live += __shfl_xor(live, o, 64);
+    if ((tid & 63) == 0) {
+        s_loss[tid >> 6] = loss;
+        s_all[tid >> 6] = live;
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         float sum = 0.0f;
-        for (int w = 0; w < 16; ++w) sum += s_loss[w];
+        live = 0;
+        for (int w = 0; w < 16; ++w) {
+            sum += s_loss[w];
+            live += s_all[w];
+        }
         *a.routed = live;
         *a.loss = total > 0 ? (float)E * (sum / ((float)total * (float)live)) : 0.0f;
     }
@@ -259,98 +407,262 @@ __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
     }
 }
 
-// Rows to the experts' order: one workgroup per token reads its row once and writes it to its k slots; it also clears the
-// rows t k .. t k + k - 1 where no token has them (they lie behind the routed ones).
+namespace {
+
+// 16 bytes at an address of any alignment
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+template <bool ANY>
+using row_word = typename std::conditional<ANY, u32x4_any, u32x4>::type;
+
+// 8 elements of a row of T, at element 8 u; `count` of them where the row ends inside
+template <int T, bool ANY>
+struct Eight {
+    static constexpr int W = T == DT_F32 ? 2 : 1;
+    u32x4 w[W];
+    __device__ __forceinline__ float get(int e) const
+    {
+        if constexpr (T == DT_F32) return __uint_as_float(w[e / 4][e % 4]);
+        const uint16_t b = (uint16_t)(w[0][e / 2] >> (16 * (e & 1)));
+        return T == DT_F16 ? f16_to_f32(b) : bf16_to_f32(b);
+    }
+    __device__ __forceinline__ void load(const void* row, int64_t u, int count)
+    {
+        if (!ANY || count >= 8) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = ((const row_word<ANY>*)row)[u * W + i];
+            return;
+        }
+        w[0] = w[W - 1] = (u32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e >= count) continue;
+            if constexpr (T == DT_F32) w[e / 4][e % 4] = ((const uint32_t*)row)[u * 8 + e];
+            else w[0][e / 2] |= (uint32_t)((const uint16_t*)row)[u * 8 + e] << (16 * (e & 1));
+        }
+    }
+    __device__ __forceinline__ static void store(void* row, int64_t u, int count, const float (&f)[8])
+    {
+        uint32_t d[8];
+        if constexpr (T == DT_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = __float_as_uint(f[e]);
+        } else {
+            us2_t top = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = cvt_pair<T == DT_BF16>(f[2 * e], f[2 * e + 1], top);
+            if (__builtin_expect(cvt_special<T == DT_BF16>(top), 0)) {
+                auto one = [](float x) { return (uint32_t)(T == DT_BF16 ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] = one(f[2 * e]) | (one(f[2 * e + 1]) << 16);
+            }
+        }
+        if (!ANY || count >= 8) {
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                __builtin_nontemporal_store((u32x4){d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]},
+                                            (row_word<ANY>*)row + u * W + i);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e >= count) continue;
+            if constexpr (T == DT_F32) ((uint32_t*)row)[u * 8 + e] = d[e];
+            else ((uint16_t*)row)[u * 8 + e] = (uint16_t)(d[e / 2] >> (16 * (e & 1)));
+        }
+    }
+};
+
+// a token's slot j, or -1 when it is none of the rows
+__device__ __forceinline__ int64_t row_of(const MoeRowsArgs& a, int64_t t, int j)
+{
+    const int64_t slot = a.slots[t * a.k + j];
+    return slot >= 0 && slot < a.T * a.k ? slot : -1;
+}
+
+}  // namespace
+
+// Rows to the experts' order: one workgroup per token reads its row once and writes it to its k slots, so nothing is read
+// twice; it also clears the rows t k .. t k + k - 1 where no token has them (they lie behind the routed ones).  Bound by
+// memory.
+template <bool ANY>
 __global__ __launch_bounds__(256) void moe_dispatch_kernel(MoeRowsArgs a)
 {
-    const int64_t t = blockIdx.x;
+    const int64_t t = blockIdx.x, words = a.row_bytes / 16;
+    const int rest = ANY ? (int)(a.row_bytes % 16) : 0;
     const uint8_t* src = (const uint8_t*)a.x + t * a.ldx;
-    const int64_t rows = a.T * a.k;
-    for (int j = 0; j < a.k; ++j) {
-        const int64_t slot = a.slots[t * a.k + j];
-        if (slot >= 0 && slot < rows) {
-            uint8_t* dst = (uint8_t*)a.out + slot * a.row_bytes;
-            for (int64_t c = threadIdx.x; c < a.row_bytes; c += 256) dst[c] = src[c];
-            if (threadIdx.x == 0 && a.scale_out) a.scale_out[slot] = a.scale[t];
+    uint8_t* out = (uint8_t*)a.out;
+    for (int64_t c = threadIdx.x; c < words; c += 256) {
+        const u32x4 w = ((const row_word<ANY>*)src)[c];
+        for (int j = 0; j < a.k; ++j) {
+            const int64_t slot = row_of(a, t, j), r = t * a.k + j;
+            if (slot >= 0) __builtin_nontemporal_store(w, (row_word<ANY>*)(out + slot * a.row_bytes) + c);
+            if (a.row_tokens[r] < 0)
+                __builtin_nontemporal_store((u32x4){0, 0, 0, 0}, (row_word<ANY>*)(out + r * a.row_bytes) + c);
         }
-        const int64_t r = t * a.k + j;
-        if (a.row_tokens[r] < 0) {
-            uint8_t* dst = (uint8_t*)a.out + r * a.row_bytes;
-            for (int64_t c = threadIdx.x; c < a.row_bytes; c += 256) dst[c] = 0;
-            if (threadIdx.x == 0 && a.scale_out) a.scale_out[r] = 0.0f;
+    }
+    // the bytes behind the last whole word, and the scales
+    const int i = threadIdx.x;
+    if (i < rest || (i == 16 && a.scale_out)) {
+        const int64_t at = words * 16 + i;
+        const uint8_t b = i < rest ? src[at] : 0;
+        const float s = i == 16 ? a.scale[t] : 0.0f;
+        for (int j = 0; j < a.k; ++j) {
+            const int64_t slot = row_of(a, t, j), r = t * a.k + j;
+            const bool clear = a.row_tokens[r] < 0;
+            if (i == 16) {
+                if (slot >= 0) a.scale_out[slot] = s;
+                if (clear) a.scale_out[r] = 0.0f;
+            } else {
+                if (slot >= 0) out[slot * a.row_bytes + at] = b;
+                if (clear) out[r * a.row_bytes + at] = 0;
+            }
         }
     }
 }
 
-// out_t = residual_t + sum_j w_tj y[slot_tj]: fp32, in the order of j, one rounding
+// out_t = sum_j w_tj y[slot_tj] + residual_t: fp32, in the order of j, one rounding.  One workgroup per token; four rows'
+// loads of a thread are in flight together (a choice of no row reads row 0 and is dropped).  Bound by memory.
+template <int T, bool ANY>
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a)
 {
-    const int64_t t = blockIdx.x, rows = a.T * a.k;
-    for (int64_t c = threadIdx.x; c < a.n; c += 256) {
-        float v = 0.0f;
-        for (int j = 0; j < a.k; ++j) {
-            const int64_t slot = a.slots[t * a.k + j];
-            if (slot >= 0 && slot < rows) v += a.weights[t * a.k + j] * load_f32_of(a.y, slot * a.n + c, a.type);
+    constexpr int ES = T == DT_F32 ? 4 : 2;
+    const int64_t t = blockIdx.x, pitch = a.n * ES;
+    for (int64_t u = threadIdx.x; u * 8 < a.n; u += 256) {
+        const int count = ANY && a.n - u * 8 < 8 ? (int)(a.n - u * 8) : 8;
+        float v[8] = {};
+        Eight<T, ANY> r;
+        if (a.residual) r.load((const uint8_t*)a.residual + t * pitch, u, count);
+        for (int j0 = 0; j0 < a.k; j0 += 4) {
+            Eight<T, ANY> y[4];
+            bool ok[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j0 + j >= a.k) continue;
+                const int64_t slot = row_of(a, t, j0 + j);
+                ok[j] = slot >= 0;
+                y[j].load((const uint8_t*)a.y + (ok[j] ? slot : 0) * pitch, u, count);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j0 + j >= a.k) continue;
+                const float w = a.weights[t * a.k + j0 + j];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += ok[j] ? w * y[j].get(e) : 0.0f;
+            }
         }
-        if (a.residual) v += load_f32_of(a.residual, t * a.n + c, a.type);
-        store_cast(a.out, t * a.n + c, v, a.type);
+        if (a.residual) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r.get(e);
+        }
+        Eight<T, ANY>::store((uint8_t*)a.out + t * pitch, u, count, v);
     }
 }
 
-// dw_tj = <dout_t, y[slot_tj]>, dy[slot_tj] = w_tj dout_t; rows of no token get 0
+// dw_tj = <dout_t, y[slot_tj]>, dy[slot_tj] = w_tj dout_t; rows of no token get 0.  One workgroup per token, four choices at
+// a time; the token's gradient is read once for them.  Bound by memory.
+template <int T, bool ANY>
 __global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a)
 {
-    __shared__ float red[4];
-    const int64_t t = blockIdx.x, rows = a.T * a.k;
-    for (int j = 0; j < a.k; ++j) {
-        const int64_t slot = a.slots[t * a.k + j], r = t * a.k + j;
-        const bool ok = slot >= 0 && slot < rows;
-        const float w = a.out ? a.weights[r] : 0.0f;
-        float dot = 0.0f;
-        if (ok)
-            for (int64_t c = threadIdx.x; c < a.n; c += 256) {
-                const float d = load_f32_of(a.x, t * a.n + c, a.type);
-                if (a.grad_weights) dot += d * load_f32_of(a.y, slot * a.n + c, a.type);
-                if (a.out) store_cast(a.out, slot * a.n + c, w * d, a.type);
+    constexpr int ES = T == DT_F32 ? 4 : 2;
+    __shared__ float red[4][4];
+    const int64_t t = blockIdx.x, pitch = a.n * ES;
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+        float dot[4] = {};
+        for (int64_t u = threadIdx.x; u * 8 < a.n; u += 256) {
+            const int count = ANY && a.n - u * 8 < 8 ? (int)(a.n - u * 8) : 8;
+            Eight<T, ANY> d, y[4];
+            int64_t slot[4];
+            d.load((const uint8_t*)a.x + t * pitch, u, count);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                slot[j] = j0 + j < a.k ? row_of(a, t, j0 + j) : -1;
+                if (j0 + j < a.k && a.grad_weights) y[j].load((const uint8_t*)a.y + (slot[j] >= 0 ? slot[j] : 0) * pitch, u, count);
             }
-        if (a.grad_weights) {
-            dot = wave_sum(dot);
-            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = dot;
-            __syncthreads();
-            if (threadIdx.x == 0) a.grad_weights[r] = (red[0] + red[1]) + (red[2] + red[3]);
-            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j0 + j >= a.k) continue;
+                const int64_t r = t * a.k + j0 + j;
+                if (a.grad_weights && slot[j] >= 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dot[j] = fmaf(d.get(e), y[j].get(e), dot[j]);
+                }
+                if (a.out) {
+                    float f[8];
+                    if (slot[j] >= 0) {
+                        const float w = a.weights[r];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = w * d.get(e);
+                        Eight<T, ANY>::store((uint8_t*)a.out + slot[j] * pitch, u, count, f);
+                    }
+                    if (a.row_tokens[r] < 0) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+                        Eight<T, ANY>::store((uint8_t*)a.out + r * pitch, u, count, f);
+                    }
+                }
+            }
         }
-        if (a.out && a.row_tokens[r] < 0)
-            for (int64_t c = threadIdx.x; c < a.n; c += 256) store_cast(a.out, r * a.n + c, 0.0f, a.type);
+        if (!a.grad_weights) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dot[j] = wave_sum(dot[j]);
+        __syncthreads();  // (the sums of the choices before are read)
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) red[threadIdx.x >> 6][j] = dot[j];
+        }
+        __syncthreads();
+        const int j = threadIdx.x;
+        if (j < 4 && j0 + j < a.k) a.grad_weights[t * a.k + j0 + j] = (red[0][j] + red[1][j]) + (red[2][j] + red[3][j]);
     }
 }
 
 namespace {
-int64_t route_blocks(int64_t T) { return (T + ROUTE_TOKENS - 1) / ROUTE_TOKENS; }
+int64_t route_blocks(int64_t T)
+{
+    const int64_t chunks = (T + CHUNK - 1) / CHUNK;
+    return chunks < MAX_BLOCKS ? chunks : MAX_BLOCKS;
+}
+
+template <int G, int V, bool SINGLE>
+hipError_t launch_route(const MoeRouteArgs& a, int blocks, hipStream_t st)
+{
+    constexpr auto kern = moe_route_kernel<G, V, SINGLE>;
+    constexpr uint32_t per = 8 + 4 * (route_threads<G> / 64) + 4;  // bytes of LDS per expert
+    const hipError_t e = ensure_dynamic_lds<kern>(G * V * per);
+    if (e != hipSuccess) return e;
+    launch_k(kern, dim3((unsigned)blocks), dim3(route_threads<G>), (uint32_t)a.E * per, st, a);
+    return hipGetLastError();
+}
+template <bool SINGLE>
+hipError_t launch_route_experts(const MoeRouteArgs& a, int blocks, hipStream_t st)
+{
+    if (a.E <= 8) return launch_route<1, 8, SINGLE>(a, blocks, st);
+    if (a.E <= 16) return launch_route<2, 8, SINGLE>(a, blocks, st);
+    if (a.E <= 32) return launch_route<4, 8, SINGLE>(a, blocks, st);
+    if (a.E <= 64) return launch_route<8, 8, SINGLE>(a, blocks, st);
+    if (a.E <= 128) return launch_route<16, 8, SINGLE>(a, blocks, st);
+    if (a.E <= 256) return launch_route<16, 16, SINGLE>(a, blocks, st);
+    if (a.E <= 512) return launch_route<32, 16, SINGLE>(a, blocks, st);
+    return launch_route<64, 16, SINGLE>(a, blocks, st);
+}
 }  // namespace
 
 size_t moe_route_ws_bytes(int64_t T, int64_t E)
 {
-    return (size_t)route_blocks(T) * ((size_t)E * 8 + 4);
+    const int64_t blocks = route_blocks(T);
+    return blocks <= 1 ? 0 : (size_t)blocks * ((size_t)E * 8 + 4);
 }
 
 hipError_t launch_moe_route(MoeRouteArgs a, void* ws, hipStream_t st)
 {
-    const int64_t blocks = route_blocks(a.T);
+    const int blocks = (int)route_blocks(a.T);
+    if (blocks <= 1) return launch_route_experts<true>(a, 1, st);
     a.block_counts = (int*)ws;
-    a.block_sums = (float*)(a.block_counts + blocks * a.E);
-    a.block_live = (int*)(a.block_sums + blocks * a.E);
-    if (blocks > 0) {
-        const uint32_t lds = (uint32_t)a.E * 24;
-        const dim3 grid((unsigned)blocks), block(256);
-        if (a.E <= 64) launch_k(moe_route_kernel<1>, grid, block, lds, st, a);
-        else if (a.E <= 128) launch_k(moe_route_kernel<2>, grid, block, lds, st, a);
-        else if (a.E <= 256) launch_k(moe_route_kernel<4>, grid, block, lds, st, a);
-        else launch_k(moe_route_kernel<16>, grid, block, lds, st, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    launch_k(moe_rows_kernel, dim3((unsigned)(blocks > 0 ? blocks : 1)), dim3(1024), (uint32_t)a.E * 4, st, a);
+    a.block_sums = (float*)(a.block_counts + (int64_t)blocks * a.E);
+    a.block_live = (int*)(a.block_sums + (int64_t)blocks * a.E);
+    const hipError_t e = launch_route_experts<false>(a, blocks, st);
+    if (e != hipSuccess) return e;
+    launch_k(moe_rows_kernel, dim3((unsigned)blocks), dim3(1024), (uint32_t)a.E * 4, st, a, blocks);
     return hipGetLastError();
 }
 
@@ -366,17 +678,47 @@ hipError_t launch_moe_route_grad(const MoeRouteGradArgs& a, hipStream_t st)
 
 hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st)
 {
-    launch_k(moe_dispatch_kernel, dim3((unsigned)a.T), dim3(256), 0u, st, a);
+    const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.ldx | (uintptr_t)a.row_bytes;
+    const dim3 grid((unsigned)a.T), block(256);
+    if (bits % 16 == 0) launch_k(moe_dispatch_kernel<false>, grid, block, 0u, st, a);
+    else launch_k(moe_dispatch_kernel<true>, grid, block, 0u, st, a);
     return hipGetLastError();
 }
+
+namespace {
+// rows of whole 16-byte words (f32: of 8 elements), all of them aligned
+bool rows_aligned(const MoeRowsArgs& a)
+{
+    const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.y | (uintptr_t)a.residual;
+    return bits % 16 == 0 && a.n % 8 == 0;
+}
+}  // namespace
+
 hipError_t launch_moe_combine(const MoeRowsArgs& a, hipStream_t st)
 {
-    launch_k(moe_combine_kernel, dim3((unsigned)a.T), dim3(256), 0u, st, a);
+    const dim3 grid((unsigned)a.T), block(256);
+    auto go = [&](auto any) {
+        constexpr bool ANY = decltype(any)::value;
+        if (a.type == DT_F16) launch_k((moe_combine_kernel<DT_F16, ANY>), grid, block, 0u, st, a);
+        else if (a.type == DT_BF16) launch_k((moe_combine_kernel<DT_BF16, ANY>), grid, block, 0u, st, a);
+        else launch_k((moe_combine_kernel<DT_F32, ANY>), grid, block, 0u, st, a);
+    };
+    if (rows_aligned(a)) go(std::false_type{});
+    else go(std::true_type{});
     return hipGetLastError();
 }
+
 hipError_t launch_moe_combine_grad(const MoeRowsArgs& a, hipStream_t st)
 {
-    launch_k(moe_combine_grad_kernel, dim3((unsigned)a.T), dim3(256), 0u, st, a);
+    const dim3 grid((unsigned)a.T), block(256);
+    auto go = [&](auto any) {
+        constexpr bool ANY = decltype(any)::value;
+        if (a.type == DT_F16) launch_k((moe_combine_grad_kernel<DT_F16, ANY>), grid, block, 0u, st, a);
+        else if (a.type == DT_BF16) launch_k((moe_combine_grad_kernel<DT_BF16, ANY>), grid, block, 0u, st, a);
+        else launch_k((moe_combine_grad_kernel<DT_F32, ANY>), grid, block, 0u, st, a);
+    };
+    if (rows_aligned(a)) go(std::false_type{});
+    else go(std::true_type{});
     return hipGetLastError();
 }
 
