@@ -1751,7 +1751,9 @@ ascq_status ascq_quant_linear_workspace_size(const void* x, const void* w, const
     ascq::LinearArgs a{};
     const ascq_status s = linear_args("quant_linear_workspace_size", p, a);
     if (s != ASCQ_OK) return s;
-    *bytes = 0;
+    a.x = (const uint8_t*)x;
+    a.w = (const uint8_t*)w;
+    *bytes = ascq::linear_ws_bytes(a);
     return ASCQ_OK;
 }
 
@@ -1779,7 +1781,9 @@ ascq_status ascq_quant_linear(void* y, const void* x, const float* x_scale, cons
     a.residual = residual;
     trace("quant_linear: operands %d out %d, M %lld N %lld K %lld, w_trans %d, act %d, bias %d, residual %d", p->operand_type,
           a.out_type, (long long)a.M, (long long)a.N, (long long)a.K, a.w_trans, a.act, bias ? 1 : 0, residual ? 1 : 0);
-    return hip_status(ascq::launch_linear(a, S(stream)), "quant_linear");
+    // (a workspace off its alignment is none)
+    uint8_t* ws = workspace && aligned(workspace, 16) ? (uint8_t*)workspace : nullptr;
+    return hip_status(ascq::launch_linear(a, ws, ws ? workspace_bytes : 0, S(stream)), "quant_linear");
 }
 
 namespace {

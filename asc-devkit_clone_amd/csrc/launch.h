@@ -271,7 +271,13 @@ struct LinearArgs {
     int64_t M, N, K, ldx, ldw, ldr, ldy;
     int f8, w_trans, act, out_type;
 };
-hipError_t launch_linear(const LinearArgs& a, hipStream_t st);
+// workspace (16-byte aligned, or null): linear_ws_bytes(a) bytes, room for copies of operands off their alignment
+size_t linear_ws_bytes(const LinearArgs& a);
+hipError_t launch_linear(const LinearArgs& a, uint8_t* ws, size_t ws_bytes, hipStream_t st);
+// linear_pipe_i8.hip, linear_pipe_f8.hip: x [M, K] with 16-byte-aligned rows and w [N, K] the same, K a multiple of 16, or w
+// [K, N] with 4-byte-aligned rows (int8: any K, x's bytes past K within a 16-byte chunk meet zeros); operands below 2^31 bytes
+hipError_t launch_linear_pipe_i8(const LinearArgs& a, hipStream_t st);
+hipError_t launch_linear_pipe_f8(const LinearArgs& a, hipStream_t st);
 
 // moe.hip
 struct MoeRouteArgs {

@@ -36,4 +36,84 @@ __device__ __forceinline__ float activate(float v, int act)
     }
 }
 
+// Eight neighbouring outputs of a row: the scaled sums with their bias, activated, plus the residual's eight, stored.  Rows
+// may start at any element; a run that the row ends in goes element by element.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+template <int OUT>
+struct OutRun {
+    static constexpr int W = OUT == DT_F32 ? 2 : 1, ES = OUT == DT_F32 ? 4 : 2;
+    u32x4 w[W];
+    __device__ __forceinline__ void load(const void* row, int64_t col, int count)
+    {
+        const uint8_t* p = (const uint8_t*)row + col * ES;
+        if (count >= 8) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = ((const u32x4_any*)p)[i];
+            return;
+        }
+        w[0] = w[W - 1] = (u32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e >= count) continue;
+            if constexpr (OUT == DT_F32) w[e / 4][e % 4] = ((const uint32_t*)p)[e];
+            else w[0][e / 2] |= (uint32_t)((const uint16_t*)p)[e] << (16 * (e & 1));
+        }
+    }
+    __device__ __forceinline__ float get(int e) const
+    {
+        if constexpr (OUT == DT_F32) return __uint_as_float(w[e / 4][e % 4]);
+        const uint16_t b = (uint16_t)(w[0][e / 2] >> (16 * (e & 1)));
+        return OUT == DT_F16 ? f16_to_f32(b) : bf16_to_f32(b);
+    }
+    __device__ __forceinline__ static void store(void* row, int64_t col, int count, const float (&f)[8])
+    {
+        uint8_t* p = (uint8_t*)row + col * ES;
+        uint32_t d[8];
+        if constexpr (OUT == DT_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = __float_as_uint(f[e]);
+        } else {
+            us2_t top = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = cvt_pair<OUT == DT_BF16>(f[2 * e], f[2 * e + 1], top);
+            if (__builtin_expect(cvt_special<OUT == DT_BF16>(top), 0)) {
+                auto one = [](float x) { return (uint32_t)(OUT == DT_BF16 ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] = one(f[2 * e]) | (one(f[2 * e + 1]) << 16);
+            }
+        }
+        if (count >= 8) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) ((u32x4_any*)p)[i] = (u32x4){d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]};
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e >= count) continue;
+            if constexpr (OUT == DT_F32) ((uint32_t*)p)[e] = d[e];
+            else ((uint16_t*)p)[e] = (uint16_t)(d[e / 2] >> (16 * (e & 1)));
+        }
+    }
+};
+
+// sums -> z = sum w_scale x_scale + bias (-0.0f for none: adding it changes nothing) -> act(z), eight at a time: one branch
+// on the activation for all of them
+template <class A>
+__device__ __forceinline__ void activate8(const A (&acc)[8], const float (&ws)[8], float xs, const float (&bias)[8], int act,
+                                          float (&v)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)acc[e] * ws[e] * xs + bias[e];
+    auto all = [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
+    };
+    if (act == ACT_NONE) return;
+    if (act == ACT_FASTER_GELU) all([](float x) { return faster_gelu(x); });
+    else if (act == ACT_RELU) all([](float x) { return activate(x, ACT_RELU); });
+    else if (act == ACT_GELU) all([](float x) { return gelu_erf(x); });
+    else all([](float x) { return silu(x); });
+}
+
 }  // namespace ascq

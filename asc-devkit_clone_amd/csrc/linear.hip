@@ -86,12 +86,81 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a)
 
 }  // namespace
 
-hipError_t launch_linear(const LinearArgs& a, hipStream_t st)
+namespace {
+
+constexpr int64_t SPAN = (1ll << 31) - 16;  // bytes of an operand that the tiles address
+
+// Which operands of a call the tiles cannot take as they lie, and the pitch of their copies (rows of zero-padded 16-byte
+// words).  K-contiguous operands whose K is no multiple of 16 need zeros behind K in one of them -- the smaller, x, as
+// long as the other's rows are aligned and what lies behind its K within a 16-byte word cannot be a NaN (int8).
+struct PackPlan {
+    bool x, w;
+    int64_t kp, ldx, ldw;
+    size_t x_bytes, w_bytes;
+};
+PackPlan pack_plan(const LinearArgs& a)
+{
+    const bool x_ok = ((uintptr_t)a.x | (uintptr_t)a.ldx) % 16 == 0;
+    const bool w_ok = ((uintptr_t)a.w | (uintptr_t)a.ldw) % (a.w_trans ? 16 : 4) == 0;
+    const bool ragged = a.K % 16 != 0 && (a.w_trans || a.f8);
+    PackPlan p{};
+    p.x = !x_ok || ragged;
+    p.w = !w_ok || (a.w_trans && ragged && a.f8);
+    p.kp = (a.K + 15) / 16 * 16;
+    p.ldx = p.kp;
+    p.ldw = a.w_trans ? p.kp : (a.N + 15) / 16 * 16;
+    p.x_bytes = p.x ? (size_t)(a.M * p.ldx) : 0;
+    p.w_bytes = p.w ? (size_t)((a.w_trans ? a.N : a.K) * p.ldw) : 0;
+    return p;
+}
+// spans that neither the tiles nor the copying launch take
+bool too_large(const LinearArgs& a)
+{
+    const int64_t kp = (a.K + 15) / 16 * 16;
+    return a.ldx * (a.M - 1) + kp > SPAN || a.M * kp > SPAN || (a.w_trans ? a.ldw * (a.N - 1) + kp : a.ldw * (a.K - 1) + a.N + 3) > SPAN ||
+           (a.w_trans ? a.N * kp : a.K * ((a.N + 15) / 16 * 16)) > SPAN;
+}
+
+hipError_t launch_any(const LinearArgs& a, hipStream_t st)
 {
     const dim3 grid((unsigned)(((a.M + 63) / 64) * ((a.N + 63) / 64)));
     if (a.f8) launch_k(linear_any_kernel<true>, grid, dim3(256), 0u, st, a);
     else launch_k(linear_any_kernel<false>, grid, dim3(256), 0u, st, a);
     return hipGetLastError();
+}
+
+}  // namespace
+
+size_t linear_ws_bytes(const LinearArgs& a)
+{
+    if (a.M == 0 || a.N == 0 || a.K == 0 || too_large(a)) return 0;
+    const PackPlan p = pack_plan(a);
+    return p.x_bytes + p.w_bytes;
+}
+
+hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hipStream_t st)
+{
+    LinearArgs a = in;
+    if (a.K == 0 || too_large(a)) return launch_any(a, st);
+    const PackPlan p = pack_plan(a);
+    if (p.x || p.w) {
+        if (p.x_bytes + p.w_bytes > ws_bytes) return launch_any(a, st);
+        uint8_t* px = p.x ? ws : nullptr;
+        uint8_t* pw = p.w ? ws + p.x_bytes : nullptr;
+        const hipError_t e = launch_pack_rows(PackRows{px, a.x, a.M, a.K, a.ldx},
+                                              a.w_trans ? PackRows{pw, a.w, a.N, a.K, a.ldw} : PackRows{pw, a.w, a.K, a.N, a.ldw}, st);
+        if (e != hipSuccess) return e;
+        if (p.x) {
+            a.x = px;
+            a.ldx = p.ldx;
+        }
+        if (p.w) {
+            a.w = pw;
+            a.ldw = p.ldw;
+        }
+        if (a.w_trans) a.K = p.kp;  // (zeros behind K in one operand at least)
+    }
+    return a.f8 ? launch_linear_pipe_f8(a, st) : launch_linear_pipe_i8(a, st);
 }
 
 }  // namespace ascq
