@@ -20,18 +20,18 @@ __device__ __forceinline__ float gelu_erf(float x)
     const float tail = 0.5f * ax * poly * __expf(-z * z);
     return x >= 0.0f ? x - tail : (x < 0.0f ? -tail : x);
 }
-// x / (1 + exp(-x)): -0 as x -> -inf
-__device__ __forceinline__ float silu(float x)
+// x / (1 + exp(-b x)): -0 as x -> -inf (SiLU: b = 1, FasterGelu: 1.702)
+__device__ __forceinline__ float swish(float x, float b)
 {
-    return fmaxf(x, -200.0f) * __builtin_amdgcn_rcpf(1.0f + __expf(-x));
+    return fmaxf(x, -200.0f) * __builtin_amdgcn_rcpf(1.0f + __expf(-b * x));
 }
 __device__ __forceinline__ float activate(float v, int act)
 {
     switch (act) {
-    case ACT_FASTER_GELU: return faster_gelu(v);
+    case ACT_FASTER_GELU: return swish(v, 1.702f);
     case ACT_RELU: return v > 0.0f || v != v ? v : 0.0f;
     case ACT_GELU: return gelu_erf(v);
-    case ACT_SILU: return silu(v);
+    case ACT_SILU: return swish(v, 1.0f);
     default: return v;
     }
 }
@@ -97,23 +97,30 @@ struct OutRun {
     }
 };
 
-// sums -> z = sum w_scale x_scale + bias (-0.0f for none: adding it changes nothing) -> act(z), eight at a time: one branch
-// on the activation for all of them
+// f(activation) once, whatever the activation: the branch is taken for many elements together
+template <class F>
+__device__ __forceinline__ void activation(int act, F f)
+{
+    if (act == ACT_NONE) return;
+    if (act == ACT_RELU) f([](float x) { return activate(x, ACT_RELU); });
+    else if (act == ACT_GELU) f([](float x) { return gelu_erf(x); });
+    else {
+        const float b = act == ACT_SILU ? 1.0f : 1.702f;
+        f([b](float x) { return swish(x, b); });
+    }
+}
+
+// sums -> z = sum w_scale x_scale + bias (-0.0f for none: adding it changes nothing) -> act(z), eight at a time
 template <class A>
 __device__ __forceinline__ void activate8(const A (&acc)[8], const float (&ws)[8], float xs, const float (&bias)[8], int act,
                                           float (&v)[8])
 {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (float)acc[e] * ws[e] * xs + bias[e];
-    auto all = [&](auto f) {
+    activation(act, [&](auto f) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = f(v[e]);
-    };
-    if (act == ACT_NONE) return;
-    if (act == ACT_FASTER_GELU) all([](float x) { return faster_gelu(x); });
-    else if (act == ACT_RELU) all([](float x) { return activate(x, ACT_RELU); });
-    else if (act == ACT_GELU) all([](float x) { return gelu_erf(x); });
-    else all([](float x) { return silu(x); });
+    });
 }
 
 }  // namespace ascq

@@ -113,10 +113,12 @@ PackPlan pack_plan(const LinearArgs& a)
     p.w_bytes = p.w ? (size_t)((a.w_trans ? a.N : a.K) * p.ldw) : 0;
     return p;
 }
-// spans that neither the tiles nor the copying launch take
+// spans and pitches that the tiles or the copying launch do not take
 bool too_large(const LinearArgs& a)
 {
     const int64_t kp = (a.K + 15) / 16 * 16;
+    // (the epilogue addresses 16 rows with 32-bit offsets)
+    if (a.ldy > (1ll << 24) || (a.residual && a.ldr > (1ll << 24))) return true;
     return a.ldx * (a.M - 1) + kp > SPAN || a.M * kp > SPAN || (a.w_trans ? a.ldw * (a.N - 1) + kp : a.ldw * (a.K - 1) + a.N + 3) > SPAN ||
            (a.w_trans ? a.N * kp : a.K * ((a.N + 15) / 16 * 16)) > SPAN;
 }
