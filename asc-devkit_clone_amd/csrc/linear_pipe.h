@@ -5,7 +5,9 @@
 // The epilogue of 16-bit outputs works on the accumulators where they are, a step at a time: R fragment rows of two
 // neighbouring fragment columns.  v_permlane16_swap trades halves of the two, after which a lane owns eight columns of a
 // row; they are scaled, biased, activated (one branch for the step), joined by the residual, rounded and stored in one
-// 16-byte piece.  The residual of a step is requested one step ahead.
+// 16-byte piece.  The residual is requested whole in front of the first step, into the registers that the main loop's operands
+// have left (one step ahead instead: 443 us against 439, bf16 out; a word of each of its lines read in front of the main loop as
+// well: 448).  What it costs is its bytes: all CUs come to their epilogues together and read at memory's rate.
 // f32 outputs, and tiles whose columns end inside a piece, go through LDS, which the main loop has left: chunks of fragment
 // rows are parked there, then each thread takes runs of eight columns in a rolled loop, so the element-wise code for a row's
 // end is there once per chunk and not once per piece.  That form for all (8192^3 int8, bf16 out): 447 us against 417, 490 against
@@ -37,20 +39,23 @@ struct LinearEpilogue {
             return (uint8_t*)base + ((m0 + T::block_row(wm, i)) * ld + n0) * 2;
         };
         auto inside = [&](int i, int c) { return T::ct_row(wm, i, lane) < rows && c < cols; };
-        u32x4 res[2][R];
-        auto request = [&](int s, u32x4 (&r)[R]) {
-            const int c = col_of(s);
-#pragma unroll
-            for (int q = 0; q < R; ++q) {
-                const int i = s / PAIRS * R + q;
-                if (inside(i, c)) r[q] = *(const u32x4_any*)(base_of(p.residual, p.ldr, i) + (uint64_t)(lr + (uint32_t)(c * 2)));
-            }
-        };
+        u32x4 res[STEPS][R];
         const bool has = p.residual != nullptr;
-        if (has) request(0, res[0]);
+        if (has) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int c = col_of(s);
+#pragma unroll
+                for (int q = 0; q < R; ++q) {
+                    const int i = s / PAIRS * R + q;
+                    if (inside(i, c))
+                        res[s][q] = *(const u32x4_any*)(base_of(p.residual, p.ldr, i) + (uint64_t)(lr + (uint32_t)(c * 2)));
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            if (has && s + 1 < STEPS) request(s + 1, res[(s + 1) & 1]);
             const int c = col_of(s), j = s % PAIRS * 2;
             float v[R][8];
             {
@@ -83,7 +88,7 @@ struct LinearEpilogue {
                 for (int q = 0; q < R; ++q)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const uint16_t h = (uint16_t)(res[s & 1][q][e / 2] >> (16 * (e & 1)));
+                        const uint16_t h = (uint16_t)(res[s][q][e / 2] >> (16 * (e & 1)));
                         v[q][e] += BF ? bf16_to_f32(h) : f16_to_f32(h);
                     }
             }
