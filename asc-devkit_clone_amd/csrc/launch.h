@@ -271,13 +271,18 @@ struct LinearArgs {
     int64_t M, N, K, ldx, ldw, ldr, ldy;
     int f8, w_trans, act, out_type;
 };
-// workspace (16-byte aligned, or null): linear_ws_bytes(a) bytes, room for copies of operands off their alignment
+// workspace (16-byte aligned, or null): linear_ws_bytes(a) bytes, room for copies of operands off their
+// alignment and for the sums of a split K
 size_t linear_ws_bytes(const LinearArgs& a);
 hipError_t launch_linear(const LinearArgs& a, uint8_t* ws, size_t ws_bytes, hipStream_t st);
 // linear_pipe_i8.hip, linear_pipe_f8.hip: x [M, K] with 16-byte-aligned rows and w [N, K] the same, K a multiple of 16, or w
 // [K, N] with 4-byte-aligned rows (int8: any K, x's bytes past K within a 16-byte chunk meet zeros); operands below 2^31 bytes
 hipError_t launch_linear_pipe_i8(const LinearArgs& a, hipStream_t st);
 hipError_t launch_linear_pipe_f8(const LinearArgs& a, hipStream_t st);
+// linear_decode.hip: x [M <= 64, K] and w [N, K] with 16-byte-aligned rows, K a multiple of 16; `part`: linear_decode_ws_bytes
+// bytes for the sums of a split K (0: not split)
+size_t linear_decode_ws_bytes(int64_t M, int64_t N, int64_t K);
+hipError_t launch_linear_decode(const LinearArgs& a, void* part, hipStream_t st);
 
 // moe.hip
 struct MoeRouteArgs {

@@ -133,11 +133,19 @@ hipError_t launch_any(const LinearArgs& a, hipStream_t st)
 
 }  // namespace
 
+namespace {
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+bool decode_rows(const LinearArgs& a) { return a.w_trans && a.M <= 64; }
+
+}  // namespace
+
 size_t linear_ws_bytes(const LinearArgs& a)
 {
     if (a.M == 0 || a.N == 0 || a.K == 0 || too_large(a)) return 0;
     const PackPlan p = pack_plan(a);
-    return p.x_bytes + p.w_bytes;
+    const size_t pack = p.x_bytes + p.w_bytes, part = decode_rows(a) ? linear_decode_ws_bytes(a.M, a.N, p.kp) : 0;
+    return part ? align256(pack) + part : pack;
 }
 
 hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hipStream_t st)
@@ -145,8 +153,9 @@ hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hip
     LinearArgs a = in;
     if (a.K == 0 || too_large(a)) return launch_any(a, st);
     const PackPlan p = pack_plan(a);
-    if (p.x || p.w) {
-        if (p.x_bytes + p.w_bytes > ws_bytes) return launch_any(a, st);
+    const size_t pack = p.x_bytes + p.w_bytes;
+    if (pack) {
+        if (pack > ws_bytes) return launch_any(a, st);
         uint8_t* px = p.x ? ws : nullptr;
         uint8_t* pw = p.w ? ws + p.x_bytes : nullptr;
         const hipError_t e = launch_pack_rows(PackRows{px, a.x, a.M, a.K, a.ldx},
@@ -161,6 +170,10 @@ hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hip
             a.ldw = p.ldw;
         }
         if (a.w_trans) a.K = p.kp;  // (zeros behind K in one operand at least)
+    }
+    if (decode_rows(a)) {
+        const size_t part = linear_decode_ws_bytes(a.M, a.N, a.K);
+        if (part == 0 || align256(pack) + part <= ws_bytes) return launch_linear_decode(a, ws + align256(pack), st);
     }
     return a.f8 ? launch_linear_pipe_f8(a, st) : launch_linear_pipe_i8(a, st);
 }
