@@ -558,12 +558,16 @@ def _dense(what: str, name: str, t: torch.Tensor, shape: tuple, dtype) -> None:
 
 
 def _same_device(what: str, *tensors) -> None:
-    device = tensors[0].device
-    if device.type != "cuda":
-        _refuse(what, f"tensors on {device}: there is no CPU path")
+    device = tensors[0].get_device()
+    if device < 0:
+        _refuse(what, "tensors on the CPU: there is no CPU path")
     for t in tensors:
-        if t is not None and t.device != device:
-            _refuse(what, f"tensors on {device} and {t.device}")
+        if t is not None and t.get_device() != device:
+            _refuse(what, f"tensors on {tensors[0].device} and {t.device}")
+
+
+def _at(t) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, dst_type: int = INT8, residual=None,
@@ -597,8 +601,8 @@ def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, 
     _dense(what, "scale_out", s, (m,), torch.float32)
     _same_device(what, x, gamma, residual, h, norm_out, q, s)
     p = _NormQuantParam(m, n, ldx, ldr, ldh, src_type, dst_type, eps)
-    check(lib().ascq_add_rms_norm_quant(_ptr(q), _ptr(s), _ptr(h) if residual is not None else None, _ptr(norm_out), _ptr(x),
-                                        _ptr(residual), _ptr(gamma), ctypes.byref(p), _stream(stream)), what)
+    check(lib().ascq_add_rms_norm_quant(_at(q), _at(s), _at(h) if residual is not None else None, _at(norm_out), _at(x),
+                                        _at(residual), _at(gamma), ctypes.byref(p), _stream(stream)), what)
     return q, s, h
 
 
@@ -630,13 +634,13 @@ def quant_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     p = _LinearParam(m, n, k, ldx, ldw, ldr, ldy, code, out_type, int(w_trans), activation)
     if workspace is None:
         need = ctypes.c_size_t(0)
-        check(lib().ascq_quant_linear_workspace_size(_ptr(x), _ptr(w), ctypes.byref(p), ctypes.byref(need)), what)
+        check(lib().ascq_quant_linear_workspace_size(_at(x), _at(w), ctypes.byref(p), ctypes.byref(need)), what)
         if need.value:
             workspace = torch.empty((need.value,), dtype=torch.uint8, device=x.device)
             if stream is not None:
                 workspace.record_stream(_torch_stream(stream))
-    check(lib().ascq_quant_linear(_ptr(y), _ptr(x), _ptr(x_scale), _ptr(w), _ptr(w_scale), _ptr(bias), _ptr(residual),
-                                  ctypes.byref(p), _ptr(workspace), _room(workspace), _stream(stream)), what)
+    check(lib().ascq_quant_linear(_at(y), _at(x), _at(x_scale), _at(w), _at(w_scale), _at(bias), _at(residual),
+                                  ctypes.byref(p), _at(workspace), _room(workspace), _stream(stream)), what)
     return y
 
 
@@ -657,7 +661,7 @@ def quant_linear_workspace_size(x: torch.Tensor, w: torch.Tensor, w_trans: bool 
                      _pitch(what, "w", w, (n, k) if w_trans else (k, n), x.dtype), 0, 0, _typed(what, "x", x, _CODE_TYPE),
                      _FLOAT_CODE[out_dtype], int(w_trans), ACT_NONE)
     need = ctypes.c_size_t(0)
-    check(lib().ascq_quant_linear_workspace_size(_ptr(x), _ptr(w), ctypes.byref(p), ctypes.byref(need)), what)
+    check(lib().ascq_quant_linear_workspace_size(_at(x), _at(w), ctypes.byref(p), ctypes.byref(need)), what)
     return need.value
 
 
@@ -673,10 +677,13 @@ class MoeRouting(NamedTuple):
 
 
 def _check_routing(what: str, r: MoeRouting, t: int, e: int, k: int) -> None:
-    for name, shape, dt in (("weights", (t, k), torch.float32), ("experts", (t, k), torch.int32),
-                            ("slots", (t, k), torch.int32), ("tokens", (t * k,), torch.int32),
-                            ("counts", (e,), torch.int64), ("routed", (1,), torch.int64), ("loss", (1,), torch.float32)):
-        _dense(what, name, getattr(r, name), shape, dt)
+    _dense(what, "weights", r.weights, (t, k), torch.float32)
+    _dense(what, "experts", r.experts, (t, k), torch.int32)
+    _dense(what, "slots", r.slots, (t, k), torch.int32)
+    _dense(what, "tokens", r.tokens, (t * k,), torch.int32)
+    _dense(what, "counts", r.counts, (e,), torch.int64)
+    _dense(what, "routed", r.routed, (1,), torch.int64)
+    _dense(what, "loss", r.loss, (1,), torch.float32)
 
 
 def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True, out=None, workspace=None,
@@ -703,7 +710,7 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True, out=No
         workspace = torch.empty((need.value,), dtype=torch.uint8, device=logits.device)
         if stream is not None:
             workspace.record_stream(_torch_stream(stream))
-    check(lib().ascq_moe_route(*map(_ptr, r), _ptr(logits), ctypes.byref(p), _ptr(workspace), _room(workspace),
+    check(lib().ascq_moe_route(*map(_at, r), _at(logits), ctypes.byref(p), _at(workspace), _room(workspace),
                                _stream(stream)), what)
     return r
 
@@ -730,8 +737,8 @@ def moe_route_grad(logits: torch.Tensor, weights: torch.Tensor, experts: torch.T
     ldg = _pitch(what, "out", g, (t, e), logits.dtype)
     _same_device(what, logits, weights, experts, counts, routed, grad_weights, grad_loss, g)
     p = _RouteParam(t, e, ld, _typed(what, "logits", logits, _FLOAT_CODE), k, int(renormalize))
-    check(lib().ascq_moe_route_grad(_ptr(g), ldg, _ptr(logits), _ptr(weights), _ptr(experts), _ptr(counts), _ptr(routed),
-                                    _ptr(grad_weights), _ptr(grad_loss), ctypes.byref(p), _stream(stream)), what)
+    check(lib().ascq_moe_route_grad(_at(g), ldg, _at(logits), _at(weights), _at(experts), _at(counts), _at(routed),
+                                    _at(grad_weights), _at(grad_loss), ctypes.byref(p), _stream(stream)), what)
     return g
 
 
@@ -759,7 +766,7 @@ def moe_dispatch(x: torch.Tensor, x_scale, slots: torch.Tensor, tokens: torch.Te
         _refuse(what, "scale_out needs x_scale")
     _same_device(what, x, x_scale, slots, tokens, rows, s)
     p = _RowsParam(t, n, ldx, code, k)
-    check(lib().ascq_moe_dispatch(_ptr(rows), _ptr(s), _ptr(x), _ptr(x_scale), _ptr(slots), _ptr(tokens), ctypes.byref(p),
+    check(lib().ascq_moe_dispatch(_at(rows), _at(s), _at(x), _at(x_scale), _at(slots), _at(tokens), ctypes.byref(p),
                                   _stream(stream)), what)
     return rows, s
 
@@ -781,7 +788,7 @@ def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, res
     _dense(what, "out", r, (t, n), y.dtype)
     _same_device(what, y, slots, weights, residual, r)
     p = _RowsParam(t, n, 0, code, k)
-    check(lib().ascq_moe_combine(_ptr(r), _ptr(y), _ptr(slots), _ptr(weights), _ptr(residual), ctypes.byref(p),
+    check(lib().ascq_moe_combine(_at(r), _at(y), _at(slots), _at(weights), _at(residual), ctypes.byref(p),
                                  _stream(stream)), what)
     return r
 
@@ -808,7 +815,7 @@ def moe_combine_grad(grad_out: torch.Tensor, y: torch.Tensor, slots: torch.Tenso
         _dense(what, "grad_y_out", dy, (t * k, n), y.dtype)
     _same_device(what, y, grad_out, slots, tokens, weights, dw, dy)
     p = _RowsParam(t, n, 0, code, k)
-    check(lib().ascq_moe_combine_grad(_ptr(dw), _ptr(dy), _ptr(grad_out), _ptr(y), _ptr(slots), _ptr(tokens), _ptr(weights),
+    check(lib().ascq_moe_combine_grad(_at(dw), _at(dy), _at(grad_out), _at(y), _at(slots), _at(tokens), _at(weights),
                                       ctypes.byref(p), _stream(stream)), what)
     return dw, dy
 
