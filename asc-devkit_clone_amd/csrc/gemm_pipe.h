@@ -580,8 +580,9 @@ struct GemmPipe {
 // element: at short K the stores of all rounds are what a call takes (M = 4096, N = 11008, K = 256: 256 x 256 in 31 us,
 // 192 x 256 33).
 enum PipeTile { PIPE_256x256, PIPE_192x256, PIPE_256x192, PIPE_128x256, PIPE_128x192, PIPE_128x128, PIPE_64x128, PIPE_TILES };
+// about what a call takes on tile shape t, in microseconds; `parts`: workgroups that share a tile's K, `kbytes` each.
 // groups: of a group matmul, whose M rows fall into groups of sizes the host does not know: half a row tile more each.
-inline PipeTile pick_pipe_tile(int64_t M, int64_t N, int64_t kbytes, int64_t groups = 0)
+inline float pipe_tile_us(int t, int64_t M, int64_t N, int64_t kbytes, int64_t groups = 0, int64_t parts = 1)
 {
     static const struct {
         int bm, bn;
@@ -590,12 +591,16 @@ inline PipeTile pick_pipe_tile(int64_t M, int64_t N, int64_t kbytes, int64_t gro
                        {128, 256, 0.59f, 0.90f, 4.0f}, {128, 192, 0.50f, 0.67f, 3.5f}, {128, 128, 0.375f, 0.47f, 1.9f},
                        {64, 128, 0.25f, 0.30f, 0.65f}};
     const float stages = (float)((kbytes + 127) / 128);
+    const int64_t tiles = ((M + T[t].bm - 1) / T[t].bm + groups / 2) * ((N + T[t].bn - 1) / T[t].bn) * parts;
+    const float c = (float)((tiles + 255) / 256), fill = (float)tiles / (256.0f * c);
+    return c * ((T[t].solo + (T[t].full - T[t].solo) * fill) * stages + T[t].tail * fill);
+}
+inline PipeTile pick_pipe_tile(int64_t M, int64_t N, int64_t kbytes, int64_t groups = 0)
+{
     PipeTile best = PIPE_256x256;
     float least = 0.0f;
     for (int t = 0; t < PIPE_TILES; ++t) {
-        const int64_t tiles = ((M + T[t].bm - 1) / T[t].bm + groups / 2) * ((N + T[t].bn - 1) / T[t].bn);
-        const float c = (float)((tiles + 255) / 256), fill = (float)tiles / (256.0f * c);
-        const float cost = c * ((T[t].solo + (T[t].full - T[t].solo) * fill) * stages + T[t].tail * fill);
+        const float cost = pipe_tile_us(t, M, N, kbytes, groups);
         if (t == 0 || cost < least) {
             best = (PipeTile)t;
             least = cost;

@@ -270,6 +270,11 @@ struct LinearArgs {
     const void* residual;   // [M, ldr] of the output type, or null; may be y (same stride)
     int64_t M, N, K, ldx, ldw, ldr, ldy;
     int f8, w_trans, act, out_type;
+    // (set by the launcher) the tile shape; workgroups that share a tile's K, and where they leave their sums:
+    // [splits][M][part_pitch], fp32 or int32
+    int tile, splits;
+    void* part;
+    int64_t part_pitch;
 };
 // workspace (16-byte aligned, or null): linear_ws_bytes(a) bytes, room for copies of operands off their
 // alignment and for the sums of a split K
@@ -279,10 +284,12 @@ hipError_t launch_linear(const LinearArgs& a, uint8_t* ws, size_t ws_bytes, hipS
 // [K, N] with 4-byte-aligned rows (int8: any K, x's bytes past K within a 16-byte chunk meet zeros); operands below 2^31 bytes
 hipError_t launch_linear_pipe_i8(const LinearArgs& a, hipStream_t st);
 hipError_t launch_linear_pipe_f8(const LinearArgs& a, hipStream_t st);
-// linear_decode.hip: x [M <= 64, K] and w [N, K] with 16-byte-aligned rows, K a multiple of 16; `part`: linear_decode_ws_bytes
-// bytes for the sums of a split K (0: not split)
-size_t linear_decode_ws_bytes(int64_t M, int64_t N, int64_t K);
-hipError_t launch_linear_decode(const LinearArgs& a, void* part, hipStream_t st);
+// linear_decode.hip: x [M <= 64, K] and w [N, K] with 16-byte-aligned rows, K a multiple of 16; K is split a.splits =
+// linear_decode_splits ways
+int linear_decode_splits(int64_t M, int64_t K);
+hipError_t launch_linear_decode(const LinearArgs& a, hipStream_t st);
+// adds the sums that the workgroups of a split K left, in order, and runs the epilogue
+hipError_t launch_linear_slices(const LinearArgs& a, hipStream_t st);
 
 // moe.hip
 struct MoeRouteArgs {

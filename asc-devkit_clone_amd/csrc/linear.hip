@@ -3,7 +3,7 @@
 // fp32.
 #include "linear.h"
 
-#include "gemm_core.h"
+#include "gemm_pipe.h"
 
 namespace ascq {
 
@@ -136,7 +136,33 @@ hipError_t launch_any(const LinearArgs& a, hipStream_t st)
 namespace {
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
-bool decode_rows(const LinearArgs& a) { return a.w_trans && a.M <= 64; }
+
+// How an aligned call runs: the weight-streaming kernel for few rows, or tiles, whose K may be shared by several workgroups
+struct Plan {
+    bool decode;
+    int tile, splits;
+};
+Plan plan_of(int64_t M, int64_t N, int64_t K, bool w_trans)
+{
+    if (w_trans && M <= 64) return {true, 0, linear_decode_splits(M, K)};
+    Plan best{false, (int)pick_pipe_tile(M, N, K), 1};
+    float least = pipe_tile_us(best.tile, M, N, K);
+    for (int tile : {PIPE_128x128, PIPE_64x128})
+        for (int s = 2; s <= 16; ++s) {
+            const int64_t stages = (K + 127) / 128, per = (stages + s - 1) / s;
+            if (per < 4) break;
+            // the sums' way through memory and the second launch
+            const float extra = 3.0f + (float)(M * N) * (4.0f * s) * 5e-7f;
+            const float us = pipe_tile_us(tile, M, N, per * 128, 0, s) + extra;
+            if (us < least) {
+                best = {false, tile, s};
+                least = us;
+            }
+        }
+    return best;
+}
+int64_t part_pitch(int64_t N) { return (N + 7) / 8 * 8; }
+size_t part_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? (size_t)splits * (size_t)(M * part_pitch(N)) * 4 : 0; }
 
 }  // namespace
 
@@ -144,7 +170,8 @@ size_t linear_ws_bytes(const LinearArgs& a)
 {
     if (a.M == 0 || a.N == 0 || a.K == 0 || too_large(a)) return 0;
     const PackPlan p = pack_plan(a);
-    const size_t pack = p.x_bytes + p.w_bytes, part = decode_rows(a) ? linear_decode_ws_bytes(a.M, a.N, p.kp) : 0;
+    const size_t pack = p.x_bytes + p.w_bytes;
+    const size_t part = part_bytes(a.M, a.N, plan_of(a.M, a.N, a.w_trans ? p.kp : a.K, a.w_trans).splits);
     return part ? align256(pack) + part : pack;
 }
 
@@ -171,11 +198,16 @@ hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hip
         }
         if (a.w_trans) a.K = p.kp;  // (zeros behind K in one operand at least)
     }
-    if (decode_rows(a)) {
-        const size_t part = linear_decode_ws_bytes(a.M, a.N, a.K);
-        if (part == 0 || align256(pack) + part <= ws_bytes) return launch_linear_decode(a, ws + align256(pack), st);
+    Plan plan = plan_of(a.M, a.N, a.K, a.w_trans);
+    if (plan.splits > 1) {
+        if (align256(pack) + part_bytes(a.M, a.N, plan.splits) > ws_bytes) plan = {false, (int)pick_pipe_tile(a.M, a.N, a.K), 1};
+        a.part = ws + align256(pack);
+        a.part_pitch = part_pitch(a.N);
     }
-    return a.f8 ? launch_linear_pipe_f8(a, st) : launch_linear_pipe_i8(a, st);
+    a.tile = plan.tile;
+    a.splits = plan.splits;
+    const hipError_t e = plan.decode ? launch_linear_decode(a, st) : a.f8 ? launch_linear_pipe_f8(a, st) : launch_linear_pipe_i8(a, st);
+    return e != hipSuccess || a.splits == 1 ? e : launch_linear_slices(a, st);
 }
 
 }  // namespace ascq

@@ -20,20 +20,10 @@ namespace {
 __device__ __forceinline__ float scaled(float v) { return v; }
 __device__ __forceinline__ float scaled(int v) { return (float)v; }
 
-// one output: the sum, scaled, biased, activated, plus the residual
-template <class A>
-__device__ __forceinline__ void put(const LinearArgs& p, int64_t m, int64_t n, A sum, float ws, float b)
-{
-    float v = scaled(sum) * ws * p.x_scale[m] + b;
-    v = activate(v, p.act);
-    if (p.residual) v += load_f32_of(p.residual, m * p.ldr + n, p.out_type);
-    store_cast(p.y, m * p.ldy + n, v, p.out_type);
-}
-
 constexpr int BLOCKS = 64;  // blocks of 16 channels that a workgroup keeps the scales of
 
 template <bool F8, int MB, int KW, int U, int D>
-__global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p, int slices, void* part)
+__global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
 {
     typedef typename std::conditional<F8, v4f, v4i>::type acc_t;
     typedef typename std::conditional<F8, float, int>::type sum_t;
@@ -42,6 +32,7 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p, in
     float* s_ws = (float*)(smem + KW * D * 2048 + 2 * sizeof(acc_t) * KW * MB * 64);
     float* s_b = s_ws + BLOCKS * 16;
     float* s_xs = s_b + BLOCKS * 16;  // [16 MB]
+    const int slices = p.splits;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const int slice = (int)blockIdx.x % slices, b0 = (int)blockIdx.x / slices, step = (int)gridDim.x / slices;
@@ -145,7 +136,7 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p, in
             const int64_t col = (int64_t)b * 16 + n;
             if (m >= p.M || col >= p.N) continue;
             if (slices > 1) {
-                ((sum_t*)part)[((int64_t)slice * p.M + m) * p.N + col] = s;
+                ((sum_t*)p.part)[((int64_t)slice * p.M + m) * p.part_pitch + col] = s;
                 continue;
             }
             float y = scaled(s) * s_ws[i * 16 + n] * s_xs[m] + s_b[i * 16 + n];
@@ -157,21 +148,45 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p, in
     wait_vmcnt<0>();  // no copy may still target LDS when the wave ends
 }
 
-// the slices' sums, in order
-template <bool F8>
-__global__ __launch_bounds__(256) void linear_slices_kernel(LinearArgs p, int slices, const void* part)
+// the sums of a split K, in order, eight columns per thread
+template <bool F8, int OUT>
+__global__ __launch_bounds__(256) void linear_slices_kernel(LinearArgs p)
 {
     typedef typename std::conditional<F8, float, int>::type sum_t;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, total = p.M * p.N;
-    if (id >= total) return;
-    const int64_t m = id / p.N, n = id % p.N;
-    sum_t s = ((const sum_t*)part)[id];
-    for (int v = 1; v < slices; ++v) s += ((const sum_t*)part)[v * total + id];
-    put(p, m, n, s, p.w_scale[n], p.bias ? p.bias[n] : -0.0f);
+    typedef typename std::conditional<F8, v4f, v4i>::type sum4_t;
+    constexpr int ES = OUT == DT_F32 ? 4 : 2;
+    const int64_t runs = p.part_pitch / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= p.M * runs) return;
+    const int64_t m = id / runs, n = id % runs * 8;
+    const int count = p.N - n < 8 ? (int)(p.N - n) : 8;
+    OutRun<OUT> res;
+    if (p.residual) res.load((const uint8_t*)p.residual + m * p.ldr * ES, n, count);
+    const sum_t* at = (const sum_t*)p.part + m * p.part_pitch + n;
+    sum4_t s[2] = {((const sum4_t*)at)[0], ((const sum4_t*)at)[1]};
+    for (int v = 1; v < p.splits; ++v) {
+        at += p.M * p.part_pitch;
+        s[0] += ((const sum4_t*)at)[0];
+        s[1] += ((const sum4_t*)at)[1];
+    }
+    sum_t sum[8];
+    float ws[8], b[8], y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int64_t c = e < count ? n + e : n;
+        sum[e] = s[e / 4][e % 4];
+        ws[e] = p.w_scale[c];
+        b[e] = p.bias ? p.bias[c] : -0.0f;
+    }
+    activate8(sum, ws, p.x_scale[m], b, p.act, y);
+    if (p.residual) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] += res.get(e);
+    }
+    OutRun<OUT>::store((uint8_t*)p.y + m * p.ldy * ES, n, count, y);
 }
 
 template <bool F8, int MB, int KW, int U, int D>
-hipError_t go(const LinearArgs& a, int slices, void* part, hipStream_t st)
+hipError_t go(const LinearArgs& a, hipStream_t st)
 {
     constexpr auto kern = linear_decode_kernel<F8, MB, KW, U, D>;
     constexpr int LDS = KW * D * 2048 + 2 * 16 * KW * MB * 64 + (2 * BLOCKS * 16 + 16 * MB) * 4;
@@ -180,10 +195,10 @@ hipError_t go(const LinearArgs& a, int slices, void* part, hipStream_t st)
     const hipError_t e = ensure_dynamic_lds<kern>(LDS);
     if (e != hipSuccess) return e;
     const int nblocks = (int)((a.N + 15) / 16);
-    int per = 256 / slices;  // workgroups of a slice
+    int per = 256 / a.splits;  // workgroups of a slice
     if (per * BLOCKS < nblocks) per = (nblocks + BLOCKS - 1) / BLOCKS;
     if (per > nblocks) per = nblocks;
-    launch_k(kern, dim3((unsigned)(per * slices)), dim3(64 * KW), (uint32_t)LDS, st, a, slices, part);
+    launch_k(kern, dim3((unsigned)(per * a.splits)), dim3(64 * KW), (uint32_t)LDS, st, a);
     return hipGetLastError();
 }
 
@@ -206,41 +221,46 @@ DecodePlan decode_plan(int64_t M, int64_t K)
 }
 
 template <bool F8>
-hipError_t launch_plan(const LinearArgs& a, const DecodePlan& d, void* part, hipStream_t st)
+hipError_t launch_plan(const LinearArgs& a, const DecodePlan& d, hipStream_t st)
 {
     if (d.mb == 1) {
-        if (d.u == 2) return go<F8, 1, 16, 2, 3>(a, d.slices, part, st);
-        if (d.u == 4) return go<F8, 1, 16, 4, 3>(a, d.slices, part, st);
-        if (d.u == 6) return go<F8, 1, 16, 6, 3>(a, d.slices, part, st);
-        return go<F8, 1, 16, 8, 3>(a, d.slices, part, st);
+        if (d.u == 2) return go<F8, 1, 16, 2, 3>(a, st);
+        if (d.u == 4) return go<F8, 1, 16, 4, 3>(a, st);
+        if (d.u == 6) return go<F8, 1, 16, 6, 3>(a, st);
+        return go<F8, 1, 16, 8, 3>(a, st);
     }
     if (d.mb == 2) {
-        if (d.u == 2) return go<F8, 2, 8, 2, 6>(a, d.slices, part, st);
-        if (d.u == 4) return go<F8, 2, 8, 4, 6>(a, d.slices, part, st);
-        if (d.u == 6) return go<F8, 2, 8, 6, 6>(a, d.slices, part, st);
-        if (d.u == 8) return go<F8, 2, 8, 8, 6>(a, d.slices, part, st);
-        return go<F8, 2, 8, 10, 6>(a, d.slices, part, st);
+        if (d.u == 2) return go<F8, 2, 8, 2, 6>(a, st);
+        if (d.u == 4) return go<F8, 2, 8, 4, 6>(a, st);
+        if (d.u == 6) return go<F8, 2, 8, 6, 6>(a, st);
+        if (d.u == 8) return go<F8, 2, 8, 8, 6>(a, st);
+        return go<F8, 2, 8, 10, 6>(a, st);
     }
-    if (d.u == 2) return go<F8, 4, 8, 2, 5>(a, d.slices, part, st);
-    return go<F8, 4, 8, 4, 5>(a, d.slices, part, st);
+    if (d.u == 2) return go<F8, 4, 8, 2, 5>(a, st);
+    return go<F8, 4, 8, 4, 5>(a, st);
 }
 
 }  // namespace
 
-size_t linear_decode_ws_bytes(int64_t M, int64_t N, int64_t K)
-{
-    const DecodePlan d = decode_plan(M, K);
-    return d.slices > 1 ? (size_t)d.slices * (size_t)M * (size_t)N * 4 : 0;
-}
+int linear_decode_splits(int64_t M, int64_t K) { return decode_plan(M, K).slices; }
 
-hipError_t launch_linear_decode(const LinearArgs& a, void* part, hipStream_t st)
+hipError_t launch_linear_decode(const LinearArgs& a, hipStream_t st)
 {
     const DecodePlan d = decode_plan(a.M, a.K);
-    hipError_t e = a.f8 ? launch_plan<true>(a, d, part, st) : launch_plan<false>(a, d, part, st);
-    if (e != hipSuccess || d.slices == 1) return e;
-    const dim3 grid((unsigned)((a.M * a.N + 255) / 256));
-    if (a.f8) launch_k(linear_slices_kernel<true>, grid, dim3(256), 0u, st, a, d.slices, (const void*)part);
-    else launch_k(linear_slices_kernel<false>, grid, dim3(256), 0u, st, a, d.slices, (const void*)part);
+    return a.f8 ? launch_plan<true>(a, d, st) : launch_plan<false>(a, d, st);
+}
+
+hipError_t launch_linear_slices(const LinearArgs& a, hipStream_t st)
+{
+    const dim3 grid((unsigned)((a.M * (a.part_pitch / 8) + 255) / 256)), block(256);
+    auto go_out = [&](auto f8) {
+        constexpr bool F8 = decltype(f8)::value;
+        if (a.out_type == DT_F16) launch_k((linear_slices_kernel<F8, DT_F16>), grid, block, 0u, st, a);
+        else if (a.out_type == DT_BF16) launch_k((linear_slices_kernel<F8, DT_BF16>), grid, block, 0u, st, a);
+        else launch_k((linear_slices_kernel<F8, DT_F32>), grid, block, 0u, st, a);
+    };
+    if (a.f8) go_out(std::true_type{});
+    else go_out(std::false_type{});
     return hipGetLastError();
 }
 

@@ -172,13 +172,17 @@ private:
     }
 };
 
-template <int BM, int BN, int WM, int WN, int OP, bool BTR>
+// SPLIT: few tiles of a long K, each shared by p.splits workgroups, which leave their sums (fp32 / int32) in p.part,
+// [split][M][part_pitch]; linear_slices_kernel adds them and runs the epilogue.
+template <int BM, int BN, int WM, int WN, int OP, bool BTR, bool SPLIT>
 __global__ __launch_bounds__(WM * WN * 64, 2) void linear_pipe_kernel(LinearArgs p)
 {
     using T = GemmPipe<BM, BN, WM, WN, OP, 0, BTR>;  // (e4m3 x e4m3)
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     int tm, tn;
-    pipe_tile((int)blockIdx.x, (int)((p.M + BM - 1) / BM), (int)((p.N + BN - 1) / BN), tm, tn);
+    const int tiles_m = (int)((p.M + BM - 1) / BM), tiles_n = (int)((p.N + BN - 1) / BN);
+    const int split = SPLIT ? (int)blockIdx.x / (tiles_m * tiles_n) : 0;
+    pipe_tile(SPLIT ? (int)blockIdx.x % (tiles_m * tiles_n) : (int)blockIdx.x, tiles_m, tiles_n, tm, tn);
     const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
     const int rows = (int)(p.M - m0 < BM ? p.M - m0 : BM), cols = (int)(p.N - n0 < BN ? p.N - n0 : BN);
     PipeArgs c{};
@@ -189,6 +193,26 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_pipe_kernel(LinearArgs
     c.a0 = (uint32_t)(m0 * p.ldx);
     c.b0 = (uint32_t)(BTR ? n0 : n0 * p.ldw);
     c.kbytes = (int32_t)p.K;
+    if constexpr (SPLIT) {  // whole stages each, shared out evenly
+        const int64_t stages = (p.K + 127) / 128, k0 = stages * split / p.splits * 128, k1 = stages * (split + 1) / p.splits * 128;
+        c.a0 += (uint32_t)k0;
+        c.b0 += (uint32_t)(BTR ? k0 * p.ldw : k0);
+        c.kbytes = (int32_t)((k1 < p.K ? k1 : p.K) - k0);
+        typename T::acc_t acc[T::FM][T::FN];
+        T::run(c, smem, acc);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+        uint8_t* part = (uint8_t*)p.part + ((split * p.M + m0) * p.part_pitch + n0) * 4;
+#pragma unroll
+        for (int j = 0; j < T::FN; ++j) {
+            const int col = T::ct_col(wn, j, lane);  // (the pitch is a multiple of 8)
+#pragma unroll
+            for (int i = 0; i < T::FM; ++i) {
+                const int row = T::ct_row(wm, i, lane);
+                if (row < rows && col < cols) *(typename T::acc_t*)(part + (row * p.part_pitch + col) * 4) = acc[i][j];
+            }
+        }
+        return;
+    }
     // the epilogue's vectors go to LDS now: older than the main loop's copies, whose first wait covers them.  What lies past
     // the tile's rows and columns reads 0.
     float* s_xs = (float*)(smem + T::LDS_BYTES);
@@ -213,22 +237,25 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_pipe_kernel(LinearArgs
     }
 }
 
-template <int BM, int BN, int WM, int WN, int OP, bool BTR>
+template <int BM, int BN, int WM, int WN, int OP, bool BTR, bool SPLIT = false>
 static hipError_t launch_linear_tile(const LinearArgs& a, hipStream_t st)
 {
     using T = GemmPipe<BM, BN, WM, WN, OP, 0, BTR>;
-    constexpr int LDS = (int)T::LDS_BYTES + 3072;  // the ring, the vectors
-    const int tiles = (int)(((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN));
-    const hipError_t e = ensure_dynamic_lds<linear_pipe_kernel<BM, BN, WM, WN, OP, BTR>>(LDS);
+    constexpr int LDS = (int)T::LDS_BYTES + (SPLIT ? 0 : 3072);  // the ring, the vectors
+    const int tiles = (int)(((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN)) * (SPLIT ? a.splits : 1);
+    const hipError_t e = ensure_dynamic_lds<linear_pipe_kernel<BM, BN, WM, WN, OP, BTR, SPLIT>>(LDS);
     if (e != hipSuccess) return e;
-    launch_k((linear_pipe_kernel<BM, BN, WM, WN, OP, BTR>), dim3(tiles), dim3(T::NT), (uint32_t)LDS, st, a);
+    launch_k((linear_pipe_kernel<BM, BN, WM, WN, OP, BTR, SPLIT>), dim3(tiles), dim3(T::NT), (uint32_t)LDS, st, a);
     return hipGetLastError();
 }
 
 template <int OP, bool BTR>
 static hipError_t launch_linear_layout(const LinearArgs& a, hipStream_t st)
 {
-    switch (pick_pipe_tile(a.M, a.N, a.K)) {
+    if (a.splits > 1)
+        return a.tile == PIPE_128x128 ? launch_linear_tile<128, 128, 2, 2, OP, BTR, true>(a, st)
+                                      : launch_linear_tile<64, 128, 2, 2, OP, BTR, true>(a, st);
+    switch (a.tile) {
     case PIPE_256x256: return launch_linear_tile<256, 256, 2, 4, OP, BTR>(a, st);
     case PIPE_192x256: return launch_linear_tile<192, 256, 2, 4, OP, BTR>(a, st);
     case PIPE_256x192: return launch_linear_tile<256, 192, 4, 2, OP, BTR>(a, st);
