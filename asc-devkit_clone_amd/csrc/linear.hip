@@ -146,7 +146,11 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, bool w_trans)
 {
     if (w_trans && M <= 64) return {true, 0, linear_decode_splits(M, K)};
     Plan best{false, (int)pick_pipe_tile(M, N, K), 1};
+    // (up to 256 rows the weight comes from memory, not from a cache that other tiles filled, and few workgroups wait for it:
+    // 128 x 4096 x 4096, 64 tiles, takes 17.7 us against the table's 8.6, w [K, N] 24.7; 256 x 11008 x 4096, 172 tiles, 23.8
+    // against 15.3 but split in two 40)
     float least = pipe_tile_us(best.tile, M, N, K);
+    if (M <= 256 && ((M + 63) / 64) * ((N + 127) / 128) <= (w_trans ? 96 : 128)) least *= w_trans ? 1.6f : 2.2f;
     for (int tile : {PIPE_128x128, PIPE_64x128})
         for (int s = 2; s <= 16; ++s) {
             const int64_t stages = (K + 127) / 128, per = (stages + s - 1) / s;

@@ -278,15 +278,24 @@ __global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int bloc
     int before = 0, all = 0;
     float p = 0.0f;
     if (part < P) {
-#pragma unroll 4
-        for (int b = part; b < blocks; b += P) {
-            const int c = a.block_counts[b * E + e];
-            all += c;
-            before += b < b0 ? c : 0;
+        for (int b = part; b < blocks; b += 8 * P) {  // eight loads in flight
+            int c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = b + i * P < blocks ? a.block_counts[(b + i * P) * E + e] : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                all += c[i];
+                before += b + i * P < b0 ? c[i] : 0;
+            }
         }
         if (b0 == 0)
-#pragma unroll 4
-            for (int b = part; b < blocks; b += P) p += a.block_sums[b * E + e];
+            for (int b = part; b < blocks; b += 8 * P) {
+                float c[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[i] = b + i * P < blocks ? a.block_sums[(b + i * P) * E + e] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p += c[i];
+            }
     }
     s_all[tid] = all;
     s_before[tid] = before;
@@ -339,71 +348,83 @@ __global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int bloc
     }
 }
 
-// d loss / d l and d w / d l: one wave per token
+// d loss / d l and d w / d l: G lanes per token, each with V neighbouring experts
 //   g_e = dL E counts_e / (sum counts x routed)  (+ dw_j at choice j without renormalisation),  dl_e = p_e (g_e - sum p g)
 //   renormalised: + w_j (dw_j - sum_i dw_i w_i) at choice j
-template <int V>
+// Bound by latency up to some ten thousand tokens, then by memory.
+template <int G, int V>
 __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
 {
-    const int E = (int)a.E, lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= a.T) return;
+    const int E = (int)a.E, e0 = (int)threadIdx.x % G * V;
+    const int64_t t = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool here = t < a.T;  // (the lanes of a wave go through the butterflies together)
+    const int64_t es = a.type == DT_F32 ? 4 : 2;
+    const bool vec = ((uintptr_t)a.logits | (uintptr_t)(a.ld * es)) % 16 == 0;
     float p[V], g[V], d[V];
+    if (here) load_logits<V>((const uint8_t*)a.logits + t * a.ld * es, a.type, e0, E, vec, p);
     float top = -__builtin_inff(), cnt = 0.0f;
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-        const int e = lane + 64 * u;
-        p[u] = e < E ? load_logit(a.logits, t * a.ld + e, a.type) : -__builtin_inff();
-        g[u] = e < E && a.grad_loss ? (float)a.counts[e] : 0.0f;
-        d[u] = 0.0f;
-        top = fmaxf(top, p[u]);
-        cnt += g[u];
+    for (int i = 0; i < V; ++i) {
+        if (!here) p[i] = -__builtin_inff();
+        g[i] = e0 + i < E && a.grad_loss ? (float)a.counts[e0 + i] : 0.0f;
+        d[i] = 0.0f;
+        top = fmaxf(top, p[i]);
+        cnt += g[i];
     }
-    top = wave_max(top);
+    butterfly<G>([&](auto s) { top = fmaxf(top, meet_any<decltype(s)::value>(top)); });
     const bool none = !(top > -__builtin_inff());  // nothing counts: no gradient
     float sum = 0.0f;
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-        p[u] = none ? 0.0f : expf(p[u] - top);
-        sum += p[u];
+    for (int i = 0; i < V; ++i) {
+        p[i] = none ? 0.0f : expf(p[i] - top);
+        sum += p[i];
     }
-    sum = wave_sum(sum);
+    sum = group_sum<G>(sum);
     if (a.grad_loss) {
-        cnt = wave_sum(cnt);
+        cnt = group_sum<G>(cnt);
         const float live = (float)*a.routed;
         const float f = cnt > 0.0f && live > 0.0f ? *a.grad_loss * (float)E / (cnt * live) : 0.0f;
 #pragma unroll
-        for (int u = 0; u < V; ++u) g[u] *= f;
+        for (int i = 0; i < V; ++i) g[i] *= f;
     }
-    if (a.grad_weights) {
-        const float dw = lane < a.k ? a.grad_weights[t * a.k + lane] : 0.0f;
-        const float w = lane < a.k ? a.weights[t * a.k + lane] : 0.0f;
-        const int id = lane < a.k ? a.experts[t * a.k + lane] : -1;
-        const float mean = a.renormalize ? wave_sum(id >= 0 ? dw * w : 0.0f) : 0.0f;
-        const float add = a.renormalize ? w * (dw - mean) : dw;
+    if (a.grad_weights && here) {
+        float mean = 0.0f;
+        if (a.renormalize)
+            for (int j = 0; j < a.k; ++j)
+                if (a.experts[t * a.k + j] >= 0) mean += a.grad_weights[t * a.k + j] * a.weights[t * a.k + j];
         for (int j = 0; j < a.k; ++j) {
-            const float x = __shfl(add, j, 64);
-            const int e = __shfl(id, j, 64);
+            const int e = a.experts[t * a.k + j];
+            const float dw = a.grad_weights[t * a.k + j], add = a.renormalize ? a.weights[t * a.k + j] * (dw - mean) : dw;
 #pragma unroll
-            for (int u = 0; u < V; ++u)
-                if (e == lane + 64 * u) {
-                    if (a.renormalize) d[u] += x;
-                    else g[u] += x;
+            for (int i = 0; i < V; ++i)
+                if (e == e0 + i) {
+                    if (a.renormalize) d[i] += add;
+                    else g[i] += add;
                 }
         }
     }
     float dot = 0.0f;
     const float inv = none ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-        p[u] *= inv;
-        dot += p[u] * g[u];
+    for (int i = 0; i < V; ++i) {
+        p[i] *= inv;
+        dot += p[i] * g[i];
     }
-    dot = wave_sum(dot);
+    dot = group_sum<G>(dot);
+    if (!here) return;
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-        const int e = lane + 64 * u;
-        if (e < E) store_cast(a.grad_logits, t * a.ld_grad + e, none ? 0.0f : p[u] * (g[u] - dot) + d[u], a.type);
+    for (int i = 0; i < V; ++i) d[i] = none ? 0.0f : p[i] * (g[i] - dot) + d[i];
+    uint8_t* out = (uint8_t*)a.grad_logits + t * a.ld_grad * es;
+    const bool vec_out = ((uintptr_t)a.grad_logits | (uintptr_t)(a.ld_grad * es)) % 16 == 0;
+    if (vec_out && e0 + V <= E && a.type == DT_F32) {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            ((u32x4*)((float*)out + e0))[i] = (u32x4){__float_as_uint(d[4 * i]), __float_as_uint(d[4 * i + 1]),
+                                                      __float_as_uint(d[4 * i + 2]), __float_as_uint(d[4 * i + 3])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (e0 + i < E) store_cast(out, e0 + i, d[i], a.type);
     }
 }
 
@@ -429,7 +450,7 @@ struct Eight {
     {
         if (!ANY || count >= 8) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) w[i] = ((const row_word<ANY>*)row)[u * W + i];
+            for (int i = 0; i < W; ++i) w[i] = __builtin_nontemporal_load((const row_word<ANY>*)row + u * W + i);
             return;
         }
         w[0] = w[W - 1] = (u32x4){0, 0, 0, 0};
@@ -666,14 +687,25 @@ hipError_t launch_moe_route(MoeRouteArgs a, void* ws, hipStream_t st)
     return hipGetLastError();
 }
 
+namespace {
+template <int G, int V>
+hipError_t launch_grad(const MoeRouteGradArgs& a, hipStream_t st)
+{
+    launch_k((moe_route_grad_kernel<G, V>), dim3((unsigned)((a.T + 256 / G - 1) / (256 / G))), dim3(256), 0u, st, a);
+    return hipGetLastError();
+}
+}  // namespace
+
 hipError_t launch_moe_route_grad(const MoeRouteGradArgs& a, hipStream_t st)
 {
-    const dim3 grid((unsigned)((a.T + 3) / 4)), block(256);
-    if (a.E <= 64) launch_k(moe_route_grad_kernel<1>, grid, block, 0u, st, a);
-    else if (a.E <= 128) launch_k(moe_route_grad_kernel<2>, grid, block, 0u, st, a);
-    else if (a.E <= 256) launch_k(moe_route_grad_kernel<4>, grid, block, 0u, st, a);
-    else launch_k(moe_route_grad_kernel<16>, grid, block, 0u, st, a);
-    return hipGetLastError();
+    if (a.E <= 8) return launch_grad<1, 8>(a, st);
+    if (a.E <= 16) return launch_grad<2, 8>(a, st);
+    if (a.E <= 32) return launch_grad<4, 8>(a, st);
+    if (a.E <= 64) return launch_grad<8, 8>(a, st);
+    if (a.E <= 128) return launch_grad<16, 8>(a, st);
+    if (a.E <= 256) return launch_grad<32, 8>(a, st);
+    if (a.E <= 512) return launch_grad<64, 8>(a, st);
+    return launch_grad<64, 16>(a, st);
 }
 
 hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st)
@@ -694,32 +726,34 @@ bool rows_aligned(const MoeRowsArgs& a)
 }
 }  // namespace
 
+namespace {
+// f(type, any alignment)
+template <class F>
+hipError_t with_row_kernel(const MoeRowsArgs& a, F f)
+{
+    auto types = [&](auto any) {
+        if (a.type == DT_F16) f(std::integral_constant<int, DT_F16>{}, any);
+        else if (a.type == DT_BF16) f(std::integral_constant<int, DT_BF16>{}, any);
+        else f(std::integral_constant<int, DT_F32>{}, any);
+    };
+    if (rows_aligned(a)) types(std::false_type{});
+    else types(std::true_type{});
+    return hipGetLastError();
+}
+}  // namespace
+
 hipError_t launch_moe_combine(const MoeRowsArgs& a, hipStream_t st)
 {
-    const dim3 grid((unsigned)a.T), block(256);
-    auto go = [&](auto any) {
-        constexpr bool ANY = decltype(any)::value;
-        if (a.type == DT_F16) launch_k((moe_combine_kernel<DT_F16, ANY>), grid, block, 0u, st, a);
-        else if (a.type == DT_BF16) launch_k((moe_combine_kernel<DT_BF16, ANY>), grid, block, 0u, st, a);
-        else launch_k((moe_combine_kernel<DT_F32, ANY>), grid, block, 0u, st, a);
-    };
-    if (rows_aligned(a)) go(std::false_type{});
-    else go(std::true_type{});
-    return hipGetLastError();
+    return with_row_kernel(a, [&](auto type, auto any) {
+        launch_k((moe_combine_kernel<decltype(type)::value, decltype(any)::value>), dim3((unsigned)a.T), dim3(256), 0u, st, a);
+    });
 }
 
 hipError_t launch_moe_combine_grad(const MoeRowsArgs& a, hipStream_t st)
 {
-    const dim3 grid((unsigned)a.T), block(256);
-    auto go = [&](auto any) {
-        constexpr bool ANY = decltype(any)::value;
-        if (a.type == DT_F16) launch_k((moe_combine_grad_kernel<DT_F16, ANY>), grid, block, 0u, st, a);
-        else if (a.type == DT_BF16) launch_k((moe_combine_grad_kernel<DT_BF16, ANY>), grid, block, 0u, st, a);
-        else launch_k((moe_combine_grad_kernel<DT_F32, ANY>), grid, block, 0u, st, a);
-    };
-    if (rows_aligned(a)) go(std::false_type{});
-    else go(std::true_type{});
-    return hipGetLastError();
+    return with_row_kernel(a, [&](auto type, auto any) {
+        launch_k((moe_combine_grad_kernel<decltype(type)::value, decltype(any)::value>), dim3((unsigned)a.T), dim3(256), 0u, st, a);
+    });
 }
 
 }  // namespace ascq
