@@ -1,6 +1,7 @@
 // linear.hip -- the quantised linear: 8-bit activations with one scale per token times an 8-bit weight with one scale per
 // channel, and bias, activation and residual in the epilogue (linear.h).  int8 sums are exact (int32); fp8 e4m3 sums are
-// fp32.
+// fp32.  Here: which kernel a call takes -- the weight-streaming one of linear_decode.hip up to 64 rows, the tiles of
+// linear_pipe.h, their K shared by several workgroups where tiles are few, or the one below -- and what is copied for it.
 #include "linear.h"
 
 #include "gemm_pipe.h"
@@ -21,7 +22,8 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t* src, int64_t n, bool 
 }
 
 // Any shape, stride and alignment, 64-bit addresses: 64 x 64 tiles, one stage of 64 K at a time through LDS, a [K, N]
-// weight turned on the way.
+// weight turned on the way.  It takes what nothing else does: K = 0, operands off their alignment without a workspace (1030 x
+// 4100 x 4095 int8: 995 us against 38 with one), and a w [K, N] past 2^31 bytes.
 template <bool F8>
 __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a)
 {
@@ -123,8 +125,9 @@ bool too_large(const LinearArgs& a)
            (a.w_trans ? a.N * kp : a.K * ((a.N + 15) / 16 * 16)) > SPAN;
 }
 
-hipError_t launch_any(const LinearArgs& a, hipStream_t st)
+hipError_t launch_any(const LinearArgs& a, const char* why, hipStream_t st)
 {
+    log_fallback("linear_any_kernel", why);
     const dim3 grid((unsigned)(((a.M + 63) / 64) * ((a.N + 63) / 64)));
     if (a.f8) launch_k(linear_any_kernel<true>, grid, dim3(256), 0u, st, a);
     else launch_k(linear_any_kernel<false>, grid, dim3(256), 0u, st, a);
@@ -168,11 +171,42 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, bool w_trans)
 int64_t part_pitch(int64_t N) { return (N + 7) / 8 * 8; }
 size_t part_bytes(int64_t M, int64_t N, int splits) { return splits > 1 ? (size_t)splits * (size_t)(M * part_pitch(N)) * 4 : 0; }
 
+// Operands past the tiles' 2^31 bytes go in pieces, of rows of x or (w [N, K]) of channels: the rows of a piece, or 0
+int64_t row_piece(const LinearArgs& a)
+{
+    const int64_t kp = (a.K + 15) / 16 * 16, pitch = a.ldx > kp ? a.ldx : kp, most = SPAN / pitch;
+    return a.M > most && most >= 512 ? most / 256 * 256 : 0;
+}
+int64_t channel_piece(const LinearArgs& a)
+{
+    const int64_t kp = (a.K + 15) / 16 * 16, pitch = a.ldw > kp ? a.ldw : kp, most = SPAN / pitch;
+    return a.w_trans && a.N > most && most >= 512 ? most / 256 * 256 : 0;
+}
+LinearArgs piece_of(const LinearArgs& a, int64_t m0, int64_t m, int64_t n0, int64_t n)
+{
+    const int64_t es = a.out_type == DT_F32 ? 4 : 2;
+    LinearArgs b = a;
+    b.x += m0 * a.ldx;
+    b.x_scale += m0;
+    b.w += n0 * a.ldw;  // (n0 > 0: w [N, K])
+    b.w_scale += n0;
+    if (a.bias) b.bias += n0;
+    if (a.residual) b.residual = (const uint8_t*)a.residual + (m0 * a.ldr + n0) * es;
+    b.y = (uint8_t*)a.y + (m0 * a.ldy + n0) * es;
+    b.M = m;
+    b.N = n;
+    return b;
+}
+
 }  // namespace
 
-size_t linear_ws_bytes(const LinearArgs& a)
+size_t linear_ws_bytes(const LinearArgs& in)
 {
-    if (a.M == 0 || a.N == 0 || a.K == 0 || too_large(a)) return 0;
+    LinearArgs a = in;
+    if (a.M == 0 || a.N == 0 || a.K == 0) return 0;
+    if (const int64_t rows = row_piece(a)) a.M = rows;  // (the last piece takes no more)
+    if (const int64_t channels = channel_piece(a)) a.N = channels;
+    if (too_large(a)) return 0;
     const PackPlan p = pack_plan(a);
     const size_t pack = p.x_bytes + p.w_bytes;
     const size_t part = part_bytes(a.M, a.N, plan_of(a.M, a.N, a.w_trans ? p.kp : a.K, a.w_trans).splits);
@@ -182,11 +216,22 @@ size_t linear_ws_bytes(const LinearArgs& a)
 hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hipStream_t st)
 {
     LinearArgs a = in;
-    if (a.K == 0 || too_large(a)) return launch_any(a, st);
+    if (a.K == 0) return launch_any(a, "k = 0", st);
+    const int64_t rows = row_piece(a), channels = rows ? 0 : channel_piece(a);
+    if (rows || channels) {
+        const int64_t step = rows ? rows : channels, end = rows ? a.M : a.N;
+        for (int64_t at = 0; at < end; at += step) {
+            const int64_t n = end - at < step ? end - at : step;
+            const hipError_t e = launch_linear(rows ? piece_of(a, at, n, 0, a.N) : piece_of(a, 0, a.M, at, n), ws, ws_bytes, st);
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    }
+    if (too_large(a)) return launch_any(a, "w [k, n] past 2^31 bytes, or a pitch past 2^24", st);
     const PackPlan p = pack_plan(a);
     const size_t pack = p.x_bytes + p.w_bytes;
     if (pack) {
-        if (pack > ws_bytes) return launch_any(a, st);
+        if (pack > ws_bytes) return launch_any(a, "operands off their alignment and no workspace to copy them to", st);
         uint8_t* px = p.x ? ws : nullptr;
         uint8_t* pw = p.w ? ws + p.x_bytes : nullptr;
         const hipError_t e = launch_pack_rows(PackRows{px, a.x, a.M, a.K, a.ldx},

@@ -12,6 +12,8 @@
 // rows are parked there, then each thread takes runs of eight columns in a rolled loop, so the element-wise code for a row's
 // end is there once per chunk and not once per piece.  That form for all (8192^3 int8, bf16 out): 447 us against 417, 490 against
 // 440 with residual and GELU -- its barriers.
+//
+// 8192^3 int8 411 us plain, 460 with GELU and residual (w [N, K]); 2048 x 4096 x 11008 fp8 71 and 81 with residual.
 #pragma once
 
 #include "gemm_pipe.h"

@@ -13,7 +13,8 @@
 // A chunk of 64 tokens notes those that chose an expert as one 64-bit mask per expert: the rank of a token among them is a
 // population count, and so is the chunk's count.  Blocks of chunks meet through a workspace: their counts and their sums
 // of p; the second launch turns the counts before a block into its rows' offsets.  Up to 64 tokens are one block, which does it all.
-// What bounds it is latency: a chain of k maxima over a token's experts, and two launches.
+// What bounds it is latency: a chain of k maxima over a token's experts, and two launches (16384 tokens, 64 experts, k = 6:
+// 8.6 and 7.3 us of kernels; 16 tokens, 16 experts, k = 2: 4.8).
 #include <type_traits>
 
 #include "common.h"
@@ -277,6 +278,13 @@ __global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int bloc
     const int P = 1024 / E, e = tid % E, part = tid / E;
     int before = 0, all = 0;
     float p = 0.0f;
+    // what comes after the scan is requested in front of it
+    const int64_t chunks = (a.T + CHUNK - 1) / CHUNK;
+    const int64_t c0 = chunks * b0 / blocks, c1 = chunks * (b0 + 1) / blocks;
+    const int64_t end = c1 * CHUNK < a.T ? c1 * CHUNK * k : a.T * k, at0 = c0 * CHUNK * k + tid;
+    const int expert0 = at0 < end ? a.experts[at0] : -1, rank0 = at0 < end ? a.slots[at0] : -1;
+    int live = b0 == 0 && tid < blocks ? a.block_live[tid] : 0;  // (blocks <= MAX_BLOCKS)
+    static_assert(MAX_BLOCKS <= 1024, "one block per thread");
     if (part < P) {
         for (int b = part; b < blocks; b += 8 * P) {  // eight loads in flight
             int c[8];
@@ -313,20 +321,15 @@ __global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int bloc
     const int64_t start = block_exclusive_scan<1024>(all, wtot, &total);
     if (tid < E) base[tid] = (int)start + before;
     __syncthreads();
-    const int64_t chunks = (a.T + CHUNK - 1) / CHUNK;
-    const int64_t c0 = chunks * b0 / blocks, c1 = chunks * (b0 + 1) / blocks;
-    const int64_t end = c1 * CHUNK < a.T ? c1 * CHUNK * k : a.T * k;
-    for (int64_t at = c0 * CHUNK * k + tid; at < end; at += 1024) {
+    for (int64_t at = at0; at < end; at += 1024) {
         if (at >= total) a.row_tokens[at] = -1;
-        const int x = a.experts[at];
+        const int x = at == at0 ? expert0 : a.experts[at];
         if (x < 0) continue;
-        const int slot = base[x] + a.slots[at];
+        const int slot = base[x] + (at == at0 ? rank0 : a.slots[at]);
         a.slots[at] = slot;
         a.row_tokens[slot] = (int)(at / k);
     }
     if (b0 != 0) return;
-    int live = 0;
-    for (int b = tid; b < blocks; b += 1024) live += a.block_live[b];
     if (tid < E) a.counts[tid] = all;
     const float loss = wave_sum(tid < E ? (float)all * p : 0.0f);
 #pragma unroll
@@ -351,7 +354,7 @@ __global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int bloc
 // d loss / d l and d w / d l: G lanes per token, each with V neighbouring experts
 //   g_e = dL E counts_e / (sum counts x routed)  (+ dw_j at choice j without renormalisation),  dl_e = p_e (g_e - sum p g)
 //   renormalised: + w_j (dw_j - sum_i dw_i w_i) at choice j
-// Bound by latency up to some ten thousand tokens, then by memory.
+// Bound by latency up to some ten thousand tokens, then by memory (64 experts: 16384 tokens 8.4 us, 100000 28 us, 3.6 TB/s).
 template <int G, int V>
 __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
 {
@@ -361,6 +364,18 @@ __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
     const int64_t es = a.type == DT_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)a.logits | (uintptr_t)(a.ld * es)) % 16 == 0;
     float p[V], g[V], d[V];
+    // a token's choices, all of them requested in front of the first use
+    int choice[MAX_K];
+    float dw[MAX_K], add[MAX_K];
+    if (a.grad_weights && here) {
+#pragma unroll
+        for (int j = 0; j < MAX_K; ++j) {
+            if (j >= a.k) continue;
+            choice[j] = a.experts[t * a.k + j];
+            dw[j] = a.grad_weights[t * a.k + j];
+            add[j] = a.weights[t * a.k + j];
+        }
+    }
     if (here) load_logits<V>((const uint8_t*)a.logits + t * a.ld * es, a.type, e0, E, vec, p);
     float top = -__builtin_inff(), cnt = 0.0f;
 #pragma unroll
@@ -389,17 +404,21 @@ __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
     }
     if (a.grad_weights && here) {
         float mean = 0.0f;
-        if (a.renormalize)
-            for (int j = 0; j < a.k; ++j)
-                if (a.experts[t * a.k + j] >= 0) mean += a.grad_weights[t * a.k + j] * a.weights[t * a.k + j];
-        for (int j = 0; j < a.k; ++j) {
-            const int e = a.experts[t * a.k + j];
-            const float dw = a.grad_weights[t * a.k + j], add = a.renormalize ? a.weights[t * a.k + j] * (dw - mean) : dw;
+#pragma unroll
+        for (int j = 0; j < MAX_K; ++j) {
+            if (j >= a.k) continue;
+            if (!a.renormalize) add[j] = 1.0f;
+            mean += choice[j] >= 0 ? dw[j] * add[j] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < MAX_K; ++j) {
+            if (j >= a.k) continue;
+            const float x = a.renormalize ? add[j] * (dw[j] - mean) : dw[j];
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (e == e0 + i) {
-                    if (a.renormalize) d[i] += add;
-                    else g[i] += add;
+                if (choice[j] == e0 + i) {
+                    if (a.renormalize) d[i] += x;
+                    else g[i] += x;
                 }
         }
     }
@@ -504,7 +523,7 @@ __device__ __forceinline__ int64_t row_of(const MoeRowsArgs& a, int64_t t, int j
 
 // Rows to the experts' order: one workgroup per token reads its row once and writes it to its k slots, so nothing is read
 // twice; it also clears the rows t k .. t k + k - 1 where no token has them (they lie behind the routed ones).  Bound by
-// memory.
+// memory: 4096 tokens x 2 of 4096 bytes in 9.4 us, 5.3 TB/s.
 template <bool ANY>
 __global__ __launch_bounds__(256) void moe_dispatch_kernel(MoeRowsArgs a)
 {
@@ -542,7 +561,8 @@ __global__ __launch_bounds__(256) void moe_dispatch_kernel(MoeRowsArgs a)
 }
 
 // out_t = sum_j w_tj y[slot_tj] + residual_t: fp32, in the order of j, one rounding.  One workgroup per token; four rows'
-// loads of a thread are in flight together (a choice of no row reads row 0 and is dropped).  Bound by memory.
+// loads of a thread are in flight together (a choice of no row reads row 0 and is dropped).  Bound by memory: 4096 x 2 rows of
+// 4096 bf16 with residual in 25 us, 5.4 TB/s; x 8 rows of 2048 in 31 us.
 template <int T, bool ANY>
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a)
 {
@@ -580,7 +600,8 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a)
 }
 
 // dw_tj = <dout_t, y[slot_tj]>, dy[slot_tj] = w_tj dout_t; rows of no token get 0.  One workgroup per token, four choices at
-// a time; the token's gradient is read once for them.  Bound by memory.
+// a time; the token's gradient is read once for them.  Bound by memory: 4096 x 2 rows of 4096 bf16 in 37 us, 4.5 TB/s.  (Two
+// units of a thread at a time: the same there, 73 us against 67 at 8 rows of 2048; workgroups of 512: 42 against 37.)
 template <int T, bool ANY>
 __global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a)
 {
