@@ -606,7 +606,7 @@ template <int T, bool ANY>
 __global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a)
 {
     constexpr int ES = T == DT_F32 ? 4 : 2;
-    __shared__ float red[4][4];
+    __shared__ float red[4][MAX_K];
     const int64_t t = blockIdx.x, pitch = a.n * ES;
     for (int j0 = 0; j0 < a.k; j0 += 4) {
         float dot[4] = {};
@@ -646,16 +646,16 @@ __global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a)
         }
         if (!a.grad_weights) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dot[j] = wave_sum(dot[j]);
-        __syncthreads();  // (the sums of the choices before are read)
-        if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) red[threadIdx.x >> 6][j] = dot[j];
+        for (int j = 0; j < 4; ++j) {
+            if (j0 + j >= a.k) continue;
+            dot[j] = wave_sum(dot[j]);
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][j0 + j] = dot[j];
         }
-        __syncthreads();
-        const int j = threadIdx.x;
-        if (j < 4 && j0 + j < a.k) a.grad_weights[t * a.k + j0 + j] = (red[0][j] + red[1][j]) + (red[2][j] + red[3][j]);
     }
+    if (!a.grad_weights) return;
+    __syncthreads();
+    const int j = threadIdx.x;
+    if (j < a.k) a.grad_weights[t * a.k + j] = (red[0][j] + red[1][j]) + (red[2][j] + red[3][j]);
 }
 
 namespace {
