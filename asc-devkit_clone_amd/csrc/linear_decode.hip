@@ -2,15 +2,15 @@
 // K a multiple of 16, operands below 2^31 bytes.
 //
 // The weight is read once, so its stream is the bound, and what keeps a stream up is bytes in flight, requested in whole
-// lines.  One workgroup per CU stays for all of its blocks of 16 channels.  Its KW waves share K: wave v has the units
+// lines.  One workgroup per CU stays for all of its blocks of up to 16 channels.  Its KW waves share K: wave v has the units
 // (128 K) v, v + KW, ..., U of them, and holds x's fragments of those in registers for good.  Weight units (16 rows x 128
 // bytes) come by copies into a ring of D slots in LDS that belongs to the wave alone, so nothing in the loop waits for
 // another wave, and the ring runs on from block to block.  At a block's end the waves' sums meet in LDS (int32: exact in
 // any order; fp32: in the order of the waves) and go through the epilogue while the next units arrive.
 // (Fragments loaded from memory straight into registers, sixteen rows apart: a load serves four lines per cycle's four lanes,
 // 14.9 us at 1 x 11008 x 4096 from memory.)
-// From memory (weights of 600 MB in turn), int8: 16 x 11008 x 4096 12.1 us, 3.7 TB/s; 16 x 8192 x 8192 15.0, 4.5; 1 x 32000 x 4096 26.4,
-// 5.0; 16 x 4096 x 11008 13.6; 64 x 4096 x 11008 20 (x's fragments leave room for 4 units: K in three).
+// From memory (weights of 600 MB in turn), int8: 16 x 11008 x 4096 11.8 us, 3.8 TB/s; 16 x 8192 x 8192 15.3, 4.4; 1 x 32000 x 4096
+// 26.8, 4.9; 16 x 4096 x 11008 14.0; 64 x 4096 x 11008 20.4 (x's fragments leave room for 4 units: K in three; 6 units spill: 26).
 // K longer than the registers hold is split over S workgroups, whose sums meet in the workspace in a second launch.
 #include "gemm_pipe.h"
 #include "linear.h"
@@ -37,16 +37,21 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
     const int slices = p.splits;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
+    // this workgroup's slice of K, and every step-th block of R <= 16 channels: R shares them out evenly over whole rounds, and
+    // the rows of a unit past R are not read (16 x 11008 x 4096: 11.8 us, with whole blocks 12.1).  (Neighbours read neighbouring rows: with an even run of channels each, 8192 x
+    // 8192 took 16.6 us against 15.0.  Few workgroups of a split K keep R = 16: more blocks cost them more than rows not read.)
     const int slice = (int)blockIdx.x % slices, b0 = (int)blockIdx.x / slices, step = (int)gridDim.x / slices;
-    const int nblocks = (int)((p.N + 15) / 16);
+    const int rounds = (int)((p.N + 16 * step - 1) / (16 * step));
+    const int R = slices > 1 ? 16 : (int)((p.N + step * rounds - 1) / (step * rounds));
+    const int nblocks = (int)((p.N + R - 1) / R);
     // the slice's units: U KW of them each
     const uint32_t K = (uint32_t)p.K, kbase = ((uint32_t)slice * (U * KW) + (uint32_t)wave) * 128u;
 
     // the epilogue's vectors of this workgroup's blocks
     if (slices == 1)
         for (int i = tid; i < 16 * BLOCKS; i += 64 * KW) {
-            const int64_t n = (int64_t)(b0 + i / 16 * step) * 16 + i % 16;
-            if (n >= p.N) break;
+            const int64_t n = (int64_t)(b0 + i / 16 * step) * R + i % 16;
+            if (n >= p.N || i / 16 >= rounds) continue;
             s_ws[i] = p.w_scale[n];
             s_b[i] = p.bias ? p.bias[n] : -0.0f;
         }
@@ -73,13 +78,15 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
     // the stream: x's units (row block, then u), then the blocks' units; `ask` runs D units ahead of `take`
     uint32_t slot = 0;
     int ask_b = b0, ask_u = 0;
-    auto ask_w = [&](uint32_t s) {
-        request(rw, (uint32_t)p.ldw, ask_b < nblocks ? (uint32_t)ask_b * 16u : 0u, ask_b < nblocks ? (uint32_t)p.N : 0u, ask_u, s);
+    auto ask_w = [&](uint32_t s) {  // (past the last block nothing is read, but the copies are counted)
+        const uint32_t first = ask_b < nblocks ? (uint32_t)(ask_b * R) : 0u, left = ask_b < nblocks ? (uint32_t)p.N - first : 0u;
+        request(rw, (uint32_t)p.ldw, first, first + (left < (uint32_t)R ? left : (uint32_t)R), ask_u, s);
         if (++ask_u == U) {
             ask_u = 0;
             ask_b += step;
         }
     };
+    // chunks g and 4 + g of the lane's row
     const uint32_t f0 = (uint32_t)(r16 * 128 + ((g ^ ((r16 >> 1) & 7)) * 16)), f1 = (uint32_t)(r16 * 128 + (((4 + g) ^ ((r16 >> 1) & 7)) * 16));
     auto take = [&](v4i& lo, v4i& hi, auto ask) {
         __builtin_amdgcn_sched_barrier(0);
@@ -135,8 +142,8 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
             sum_t s = 0;
 #pragma unroll
             for (int v = 0; v < KW; ++v) s += ((const sum_t*)&red[turn][v][m >> 4][(m & 15) + 16 * (n >> 2)])[n & 3];
-            const int64_t col = (int64_t)b * 16 + n;
-            if (m >= p.M || col >= p.N) continue;
+            const int64_t col = (int64_t)b * R + n;
+            if (m >= p.M || n >= R || col >= p.N) continue;
             if (slices > 1) {
                 ((sum_t*)p.part)[((int64_t)slice * p.M + m) * p.part_pitch + col] = s;
                 continue;
@@ -150,41 +157,51 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
     wait_vmcnt<0>();  // no copy may still target LDS when the wave ends
 }
 
-// the sums of a split K, in order, eight columns per thread
+// the sums of a split K, in order, four columns per thread (eight: 1 us more at 64 x 4096, too few threads)
 template <bool F8, int OUT>
 __global__ __launch_bounds__(256) void linear_slices_kernel(LinearArgs p)
 {
-    typedef typename std::conditional<F8, float, int>::type sum_t;
     typedef typename std::conditional<F8, v4f, v4i>::type sum4_t;
+    typedef u32x2 u32x2_any __attribute__((aligned(2)));
     constexpr int ES = OUT == DT_F32 ? 4 : 2;
-    const int64_t runs = p.part_pitch / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= p.M * runs) return;
-    const int64_t m = id / runs, n = id % runs * 8;
-    const int count = p.N - n < 8 ? (int)(p.N - n) : 8;
-    OutRun<OUT> res;
-    if (p.residual) res.load((const uint8_t*)p.residual + m * p.ldr * ES, n, count);
-    const sum_t* at = (const sum_t*)p.part + m * p.part_pitch + n;
-    sum4_t s[2] = {((const sum4_t*)at)[0], ((const sum4_t*)at)[1]};
-    for (int v = 1; v < p.splits; ++v) {
-        at += p.M * p.part_pitch;
-        s[0] += ((const sum4_t*)at)[0];
-        s[1] += ((const sum4_t*)at)[1];
-    }
-    sum_t sum[8];
-    float ws[8], b[8], y[8];
+    const uint32_t runs = (uint32_t)(p.part_pitch / 4);
+    const uint64_t id = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= (uint64_t)p.M * runs) return;
+    const int64_t m = (int64_t)(id / runs), n = (int64_t)(id % runs) * 4;
+    const int count = p.N - n < 4 ? (int)(p.N - n) : 4;
+    if (count <= 0) return;
+    const uint8_t* at = (const uint8_t*)p.part + (m * p.part_pitch + n) * 4;
+    sum4_t s = *(const sum4_t*)at;
+    for (int v = 1; v < p.splits; ++v) s += *(const sum4_t*)(at + v * p.M * p.part_pitch * 4);
+    const float xs = p.x_scale[m];
+    float y[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4; ++e) {
         const int64_t c = e < count ? n + e : n;
-        sum[e] = s[e / 4][e % 4];
-        ws[e] = p.w_scale[c];
-        b[e] = p.bias ? p.bias[c] : -0.0f;
+        y[e] = (float)s[e] * p.w_scale[c] * xs + (p.bias ? p.bias[c] : -0.0f);
     }
-    activate8(sum, ws, p.x_scale[m], b, p.act, y);
+    activation(p.act, [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = f(y[e]);
+    });
     if (p.residual) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] += res.get(e);
+        for (int e = 0; e < 4; ++e)
+            if (e < count) y[e] += load_f32_of(p.residual, m * p.ldr + n + e, OUT);
     }
-    OutRun<OUT>::store((uint8_t*)p.y + m * p.ldy * ES, n, count, y);
+    uint8_t* to = (uint8_t*)p.y + (m * p.ldy + n) * ES;
+    if (count == 4) {
+        if constexpr (OUT == DT_F32) {
+            *(u32x4_any*)to = (u32x4){__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])};
+        } else {
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = OUT == DT_F16 ? f32_to_f16_sat(y[e]) : f32_to_bf16_sat(y[e]);
+            *(u32x2_any*)to = (u32x2){h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+        }
+    } else {
+        for (int e = 0; e < count; ++e) store_cast(to, e, y[e], OUT);
+    }
 }
 
 template <bool F8, int MB, int KW, int U, int D>
@@ -196,10 +213,10 @@ hipError_t go(const LinearArgs& a, hipStream_t st)
     static_assert(2 * D < 64, "vmcnt");
     const hipError_t e = ensure_dynamic_lds<kern>(LDS);
     if (e != hipSuccess) return e;
-    const int nblocks = (int)((a.N + 15) / 16);
-    int per = 256 / a.splits;  // workgroups of a slice
-    if (per * BLOCKS < nblocks) per = (nblocks + BLOCKS - 1) / BLOCKS;
-    if (per > nblocks) per = nblocks;
+    // workgroups of a slice: one per CU in all, with at least four channels, and at most BLOCKS blocks of 16
+    int64_t per = 256 / a.splits;
+    if (per * (BLOCKS * 16) < a.N) per = (a.N + BLOCKS * 16 - 1) / (BLOCKS * 16);
+    if (per > (a.N + 3) / 4) per = (a.N + 3) / 4;
     launch_k(kern, dim3((unsigned)(per * a.splits)), dim3(64 * KW), (uint32_t)LDS, st, a);
     return hipGetLastError();
 }
@@ -254,7 +271,7 @@ hipError_t launch_linear_decode(const LinearArgs& a, hipStream_t st)
 
 hipError_t launch_linear_slices(const LinearArgs& a, hipStream_t st)
 {
-    const dim3 grid((unsigned)((a.M * (a.part_pitch / 8) + 255) / 256)), block(256);
+    const dim3 grid((unsigned)((a.M * (a.part_pitch / 4) + 255) / 256)), block(256);
     auto go_out = [&](auto f8) {
         constexpr bool F8 = decltype(f8)::value;
         if (a.out_type == DT_F16) launch_k((linear_slices_kernel<F8, DT_F16>), grid, block, 0u, st, a);
