@@ -519,56 +519,72 @@ __device__ __forceinline__ int64_t row_of(const MoeRowsArgs& a, int64_t t, int j
     return slot >= 0 && slot < a.T * a.k ? slot : -1;
 }
 
+// four waves per workgroup: the wave's number among all (a scalar, so that what a wave shares is loaded once)
+__device__ __forceinline__ int64_t wave_of() { return (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 }  // namespace
 
-// Rows to the experts' order: one workgroup per token reads its row once and writes it to its k slots, so nothing is read
-// twice; it also clears the rows t k .. t k + k - 1 where no token has them (they lie behind the routed ones).  Bound by
-// memory: 4096 tokens x 2 of 4096 bytes in 9.4 us, 5.3 TB/s.
+// Rows to the experts' order: `waves` waves per token, interleaved by 1 KB, read its row once and write it to its k slots, so
+// nothing is read twice; they also clear the rows t k .. t k + k - 1 where no token has them (they lie behind the routed
+// ones).  Bound by memory: 4096 tokens x 2 of 4096 bytes in 9.8 us, 5.2 TB/s; 512 x 6 of 2048 in 4.7.
 template <bool ANY>
-__global__ __launch_bounds__(256) void moe_dispatch_kernel(MoeRowsArgs a)
+__global__ __launch_bounds__(256) void moe_dispatch_kernel(MoeRowsArgs a, int waves)
 {
-    const int64_t t = blockIdx.x, words = a.row_bytes / 16;
+    const int64_t w = wave_of(), t = w / waves, words = a.row_bytes / 16;
+    if (t >= a.T) return;
+    const int c0 = (int)(w % waves) * 64, lane = threadIdx.x & 63;
     const int rest = ANY ? (int)(a.row_bytes % 16) : 0;
     const uint8_t* src = (const uint8_t*)a.x + t * a.ldx;
     uint8_t* out = (uint8_t*)a.out;
-    for (int64_t c = threadIdx.x; c < words; c += 256) {
-        const u32x4 w = ((const row_word<ANY>*)src)[c];
-        for (int j = 0; j < a.k; ++j) {
-            const int64_t slot = row_of(a, t, j), r = t * a.k + j;
-            if (slot >= 0) __builtin_nontemporal_store(w, (row_word<ANY>*)(out + slot * a.row_bytes) + c);
-            if (a.row_tokens[r] < 0)
-                __builtin_nontemporal_store((u32x4){0, 0, 0, 0}, (row_word<ANY>*)(out + r * a.row_bytes) + c);
+    // f(the token's row of choice j or -1, row t k + j where no token has it, else -1)
+    auto each = [&](auto f) {
+        for (int j0 = 0; j0 < a.k; j0 += 4) {
+            int64_t slot[4], clear[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = j0 + j < a.k ? j0 + j : 0;
+                slot[j] = row_of(a, t, at);
+                clear[j] = a.row_tokens[t * a.k + at] < 0 ? t * a.k + at : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j0 + j < a.k) f(slot[j], clear[j]);
         }
+    };
+    const float scale = a.scale_out ? a.scale[t] : 0.0f;
+    for (int64_t c = c0 + lane; c < words; c += waves * 64) {
+        const u32x4 v = ((const row_word<ANY>*)src)[c];
+        each([&](int64_t slot, int64_t clear) {
+            if (slot >= 0) __builtin_nontemporal_store(v, (row_word<ANY>*)(out + slot * a.row_bytes) + c);
+            if (clear >= 0) __builtin_nontemporal_store((u32x4){0, 0, 0, 0}, (row_word<ANY>*)(out + clear * a.row_bytes) + c);
+        });
     }
     // the bytes behind the last whole word, and the scales
-    const int i = threadIdx.x;
-    if (i < rest || (i == 16 && a.scale_out)) {
-        const int64_t at = words * 16 + i;
-        const uint8_t b = i < rest ? src[at] : 0;
-        const float s = i == 16 ? a.scale[t] : 0.0f;
-        for (int j = 0; j < a.k; ++j) {
-            const int64_t slot = row_of(a, t, j), r = t * a.k + j;
-            const bool clear = a.row_tokens[r] < 0;
-            if (i == 16) {
-                if (slot >= 0) a.scale_out[slot] = s;
-                if (clear) a.scale_out[r] = 0.0f;
+    if (c0 == 0 && (lane < rest || (lane == 16 && a.scale_out))) {
+        const int64_t at = words * 16 + lane;
+        const uint8_t byte = lane < rest ? src[at] : 0;
+        each([&](int64_t slot, int64_t clear) {
+            if (lane == 16) {
+                if (slot >= 0) a.scale_out[slot] = scale;
+                if (clear >= 0) a.scale_out[clear] = 0.0f;
             } else {
-                if (slot >= 0) out[slot * a.row_bytes + at] = b;
-                if (clear) out[r * a.row_bytes + at] = 0;
+                if (slot >= 0) out[slot * a.row_bytes + at] = byte;
+                if (clear >= 0) out[clear * a.row_bytes + at] = 0;
             }
-        }
+        });
     }
 }
 
-// out_t = sum_j w_tj y[slot_tj] + residual_t: fp32, in the order of j, one rounding.  One workgroup per token; four rows'
-// loads of a thread are in flight together (a choice of no row reads row 0 and is dropped).  Bound by memory: 4096 x 2 rows of
-// 4096 bf16 with residual in 25 us, 5.4 TB/s; x 8 rows of 2048 in 31 us.
+// out_t = sum_j w_tj y[slot_tj] + residual_t: fp32, in the order of j, one rounding.  `waves` waves per token, interleaved by
+// 512 elements; four rows' loads of a thread are in flight together (a choice of no row reads row 0 and is dropped).  Bound by
+// memory: 4096 x 2 rows of 4096 bf16 with residual in 26 us, 5.2 TB/s; x 8 rows of 2048 in 33 us.
 template <int T, bool ANY>
-__global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a)
+__global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a, int waves)
 {
     constexpr int ES = T == DT_F32 ? 4 : 2;
-    const int64_t t = blockIdx.x, pitch = a.n * ES;
-    for (int64_t u = threadIdx.x; u * 8 < a.n; u += 256) {
+    const int64_t w = wave_of(), t = w / waves, pitch = a.n * ES;
+    if (t >= a.T) return;
+    for (int64_t u = w % waves * 64 + (threadIdx.x & 63); u * 8 < a.n; u += waves * 64) {
         const int count = ANY && a.n - u * 8 < 8 ? (int)(a.n - u * 8) : 8;
         float v[8] = {};
         Eight<T, ANY> r;
@@ -586,9 +602,9 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j0 + j >= a.k) continue;
-                const float w = a.weights[t * a.k + j0 + j];
+                const float weight = a.weights[t * a.k + j0 + j];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += ok[j] ? w * y[j].get(e) : 0.0f;
+                for (int e = 0; e < 8; ++e) v[e] += ok[j] ? weight * y[j].get(e) : 0.0f;
             }
         }
         if (a.residual) {
@@ -599,63 +615,81 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a)
     }
 }
 
-// dw_tj = <dout_t, y[slot_tj]>, dy[slot_tj] = w_tj dout_t; rows of no token get 0.  One workgroup per token, four choices at
-// a time; the token's gradient is read once for them.  Bound by memory: 4096 x 2 rows of 4096 bf16 in 37 us, 4.5 TB/s.  (Two
-// units of a thread at a time: the same there, 73 us against 67 at 8 rows of 2048; workgroups of 512: 42 against 37.)
-template <int T, bool ANY>
-__global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a)
+// dw_tj = <dout_t, y[slot_tj]>, dy[slot_tj] = w_tj dout_t; rows of no token get 0.  An item is a token and up to `per` <= 4 of its
+// choices, whose gradient it reads once; W waves do it: four, or one for rows of fewer than 2048 (13370 tokens x 2 of 512:
+// 17 us, with four waves 43; 8192 x 2 of 2048: 34, with one wave 42).  Few items take a choice each (14 tokens x 8 of 3904: 4.5
+// us, four choices 7.0; 512 x 6 of 2048: 14, four 10).  Bound by memory: 4096 x 2 rows of 4096 bf16 in 35 us, 4.8 TB/s.
+template <int T, bool ANY, int W>
+__global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a, int per)
 {
     constexpr int ES = T == DT_F32 ? 4 : 2;
-    __shared__ float red[4][MAX_K];
-    const int64_t t = blockIdx.x, pitch = a.n * ES;
-    for (int j0 = 0; j0 < a.k; j0 += 4) {
-        float dot[4] = {};
-        for (int64_t u = threadIdx.x; u * 8 < a.n; u += 256) {
+    __shared__ float red[4][4];
+    const int groups = (a.k + per - 1) / per, lane = (int)threadIdx.x % (64 * W);
+    const int64_t item = wave_of() / W, pitch = a.n * ES;
+    const bool here = item < a.T * groups;  // (an item past the last does nothing, but meets the others)
+    const int64_t t = here ? item / groups : 0;
+    const int j0 = (int)(here ? item % groups : 0) * per, jn = here ? (a.k - j0 < per ? a.k - j0 : per) : 0;
+    float dot[4] = {};
+    if (here) {
+        int64_t slot[4];
+        float w[4];
+        bool clear[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t r = t * a.k + j0 + j;
+            slot[j] = j < jn ? row_of(a, t, j0 + j) : -1;
+            w[j] = j < jn && a.out ? a.weights[r] : 0.0f;
+            clear[j] = j < jn && a.out && a.row_tokens[r] < 0;
+        }
+        for (int64_t u = lane; u * 8 < a.n; u += 64 * W) {
             const int count = ANY && a.n - u * 8 < 8 ? (int)(a.n - u * 8) : 8;
             Eight<T, ANY> d, y[4];
-            int64_t slot[4];
             d.load((const uint8_t*)a.x + t * pitch, u, count);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                slot[j] = j0 + j < a.k ? row_of(a, t, j0 + j) : -1;
-                if (j0 + j < a.k && a.grad_weights) y[j].load((const uint8_t*)a.y + (slot[j] >= 0 ? slot[j] : 0) * pitch, u, count);
-            }
+            for (int j = 0; j < 4; ++j)
+                if (j < jn && a.grad_weights) y[j].load((const uint8_t*)a.y + (slot[j] >= 0 ? slot[j] : 0) * pitch, u, count);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (j0 + j >= a.k) continue;
-                const int64_t r = t * a.k + j0 + j;
+                if (j >= jn) continue;
                 if (a.grad_weights && slot[j] >= 0) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dot[j] = fmaf(d.get(e), y[j].get(e), dot[j]);
                 }
-                if (a.out) {
-                    float f[8];
-                    if (slot[j] >= 0) {
-                        const float w = a.weights[r];
+                float f[8];
+                if (a.out && slot[j] >= 0) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = w * d.get(e);
-                        Eight<T, ANY>::store((uint8_t*)a.out + slot[j] * pitch, u, count, f);
-                    }
-                    if (a.row_tokens[r] < 0) {
+                    for (int e = 0; e < 8; ++e) f[e] = w[j] * d.get(e);
+                    Eight<T, ANY>::store((uint8_t*)a.out + slot[j] * pitch, u, count, f);
+                }
+                if (clear[j]) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-                        Eight<T, ANY>::store((uint8_t*)a.out + r * pitch, u, count, f);
-                    }
+                    for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+                    Eight<T, ANY>::store((uint8_t*)a.out + (t * a.k + j0 + j) * pitch, u, count, f);
                 }
             }
         }
-        if (!a.grad_weights) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j0 + j >= a.k) continue;
-            dot[j] = wave_sum(dot[j]);
-            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][j0 + j] = dot[j];
-        }
     }
     if (!a.grad_weights) return;
-    __syncthreads();
-    const int j = threadIdx.x;
-    if (j < a.k) a.grad_weights[t * a.k + j] = (red[0][j] + red[1][j]) + (red[2][j] + red[3][j]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j >= jn) continue;
+        dot[j] = wave_sum(dot[j]);
+        if constexpr (W == 1) {
+            if (lane == 0) a.grad_weights[t * a.k + j0 + j] = dot[j];
+        } else {
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][j] = dot[j];
+        }
+    }
+    if constexpr (W > 1) {
+        __syncthreads();
+        const int j = lane, first = (int)threadIdx.x / (64 * W) * W;
+        if (j < jn) {
+            float sum = red[first][j];
+#pragma unroll
+            for (int v = 1; v < W; ++v) sum += red[first + v][j];
+            a.grad_weights[t * a.k + j0 + j] = sum;
+        }
+    }
 }
 
 namespace {
@@ -729,25 +763,21 @@ hipError_t launch_moe_route_grad(const MoeRouteGradArgs& a, hipStream_t st)
     return launch_grad<64, 16>(a, st);
 }
 
-hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st)
+namespace {
+// waves that share a token's row of `units` 16-byte (or 8-element) words: one word per thread, which is what is fastest from a
+// handful of tokens (14 x 8 rows of 3904: combine 6.9 us, with half as many waves 13) to 16384, within a grid's bound
+int row_waves(int64_t T, int64_t units)
 {
-    const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.ldx | (uintptr_t)a.row_bytes;
-    const dim3 grid((unsigned)a.T), block(256);
-    if (bits % 16 == 0) launch_k(moe_dispatch_kernel<false>, grid, block, 0u, st, a);
-    else launch_k(moe_dispatch_kernel<true>, grid, block, 0u, st, a);
-    return hipGetLastError();
+    const int64_t all = (units + 63) / 64, most = (1 << 20) / T;
+    return (int)(all < 1 ? 1 : all < most ? all : most > 1 ? most : 1);
 }
 
-namespace {
 // rows of whole 16-byte words (f32: of 8 elements), all of them aligned
 bool rows_aligned(const MoeRowsArgs& a)
 {
     const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.y | (uintptr_t)a.residual;
     return bits % 16 == 0 && a.n % 8 == 0;
 }
-}  // namespace
-
-namespace {
 // f(type, any alignment)
 template <class F>
 hipError_t with_row_kernel(const MoeRowsArgs& a, F f)
@@ -763,17 +793,37 @@ hipError_t with_row_kernel(const MoeRowsArgs& a, F f)
 }
 }  // namespace
 
+hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st)
+{
+    const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.ldx | (uintptr_t)a.row_bytes;
+    const int waves = row_waves(a.T, a.row_bytes / 16);
+    const dim3 grid((unsigned)((a.T * waves + 3) / 4)), block(256);
+    if (bits % 16 == 0) launch_k(moe_dispatch_kernel<false>, grid, block, 0u, st, a, waves);
+    else launch_k(moe_dispatch_kernel<true>, grid, block, 0u, st, a, waves);
+    return hipGetLastError();
+}
+
 hipError_t launch_moe_combine(const MoeRowsArgs& a, hipStream_t st)
 {
+    const int waves = row_waves(a.T, (a.n + 7) / 8);
     return with_row_kernel(a, [&](auto type, auto any) {
-        launch_k((moe_combine_kernel<decltype(type)::value, decltype(any)::value>), dim3((unsigned)a.T), dim3(256), 0u, st, a);
+        launch_k((moe_combine_kernel<decltype(type)::value, decltype(any)::value>), dim3((unsigned)((a.T * waves + 3) / 4)),
+                 dim3(256), 0u, st, a, waves);
     });
 }
 
 hipError_t launch_moe_combine_grad(const MoeRowsArgs& a, hipStream_t st)
 {
+    const int per = a.T * a.k <= 1024 ? 1 : 4;  // (808 rows: alike)
+    const int64_t items = a.T * ((a.k + per - 1) / per);
     return with_row_kernel(a, [&](auto type, auto any) {
-        launch_k((moe_combine_grad_kernel<decltype(type)::value, decltype(any)::value>), dim3((unsigned)a.T), dim3(256), 0u, st, a);
+        constexpr int T = decltype(type)::value;
+        constexpr bool ANY = decltype(any)::value;
+        // (a grid has fewer than 2^32 threads)
+        if (a.n < 2048 || items >= 1 << 24)
+            launch_k((moe_combine_grad_kernel<T, ANY, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0u, st, a, per);
+        else
+            launch_k((moe_combine_grad_kernel<T, ANY, 4>), dim3((unsigned)items), dim3(256), 0u, st, a, per);
     });
 }
 
