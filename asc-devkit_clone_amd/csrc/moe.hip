@@ -42,40 +42,72 @@ __device__ __forceinline__ float wave_sum(float v)
     return v;
 }
 
-// The value of the lane that step S (1, 2, 4, 8) of a butterfly within 16 lanes meets: quad permutations, then mirrors,
-// which reach the other half because the lanes of a half already agree.
-template <int S>
-__device__ __forceinline__ int meet(int v)
+// v of the lane that `ctrl` names among this lane's 16
+template <int ctrl>
+__device__ __forceinline__ uint32_t moved(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true); }
+template <int ctrl>
+__device__ __forceinline__ float moved(float v) { return __uint_as_float(moved<ctrl>(__float_as_uint(v))); }
+
+// op of v and v of the lane 16 or 32 away
+template <int S, class Op>
+__device__ __forceinline__ uint32_t far(uint32_t v, Op op)
 {
-    constexpr int ctrl = S == 1 ? 0xB1 : S == 2 ? 0x4E : S == 4 ? 0x141 : 0x140;
-    return __builtin_amdgcn_update_dpp(0, v, ctrl, 0xf, 0xf, true);
+    if constexpr (S == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return op((uint32_t)r[0], (uint32_t)r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return op((uint32_t)r[0], (uint32_t)r[1]);
+    }
 }
-// (beyond 16 lanes: through the cross-lane network)
-template <int S>
-__device__ __forceinline__ int meet_any(int v)
+template <int S, class Op>
+__device__ __forceinline__ float far(float v, Op op)
 {
-    if constexpr (S < 16) return meet<S>(v);
-    else return __shfl_xor(v, S, 64);
+    return __uint_as_float(far<S>(__float_as_uint(v), [&](uint32_t x, uint32_t y) {
+        return __float_as_uint(op(__uint_as_float(x), __uint_as_float(y)));
+    }));
 }
-template <int S>
-__device__ __forceinline__ float meet_any(float v) { return __int_as_float(meet_any<S>(__float_as_int(v))); }
-// f(step) for the steps of a butterfly over G lanes
-template <int G, class F>
-__device__ __forceinline__ void butterfly(F f)
+
+// op (commutative) over G neighbouring lanes, each of them gets it: within 16 lanes quad permutations, then mirrors, which
+// reach the other half because the lanes of a half already agree
+template <int G, class T, class Op>
+__device__ __forceinline__ T reduce(T v, Op op)
 {
-    if constexpr (G > 1) f(std::integral_constant<int, 1>{});
-    if constexpr (G > 2) f(std::integral_constant<int, 2>{});
-    if constexpr (G > 4) f(std::integral_constant<int, 4>{});
-    if constexpr (G > 8) f(std::integral_constant<int, 8>{});
-    if constexpr (G > 16) f(std::integral_constant<int, 16>{});
-    if constexpr (G > 32) f(std::integral_constant<int, 32>{});
+    if constexpr (G > 1) v = op(v, moved<0xB1>(v));
+    if constexpr (G > 2) v = op(v, moved<0x4E>(v));
+    if constexpr (G > 4) v = op(v, moved<0x141>(v));
+    if constexpr (G > 8) v = op(v, moved<0x140>(v));
+    if constexpr (G > 16) v = far<16>(v, op);
+    if constexpr (G > 32) v = far<32>(v, op);
+    return v;
+}
+// the sum over the wave's lanes G, 2 G, ... away: rotations within 16 lanes, then the swaps
+template <int G>
+__device__ __forceinline__ float sum_across(float v)
+{
+    auto add = [](float x, float y) { return x + y; };
+    if constexpr (G <= 8) v += moved<0x128>(v);
+    if constexpr (G <= 4) v += moved<0x124>(v);
+    if constexpr (G <= 2) v += moved<0x122>(v);
+    if constexpr (G <= 1) v += moved<0x121>(v);
+    if constexpr (G <= 16) v = far<16>(v, add);
+    if constexpr (G <= 32) v = far<32>(v, add);
+    return v;
 }
 template <int G>
 __device__ __forceinline__ float group_sum(float v)
 {
-    butterfly<G>([&](auto s) { v += meet_any<decltype(s)::value>(v); });
-    return v;
+    return reduce<G>(v, [](float x, float y) { return x + y; });
 }
+
+// a logit as a number whose order is the logit's; NOTHING or less: it counts nothing (-inf, or a choice taken)
+constexpr uint32_t NOTHING = 0x007fffffu;
+__device__ __forceinline__ uint32_t key_of(float v)
+{
+    const uint32_t b = __float_as_uint(v + 0.0f);  // (-0 is 0)
+    return b ^ ((int)b < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float((int)k < 0 ? k ^ 0x80000000u : ~k); }
 
 // logits e0 .. e0 + V - 1 of a row (past E: -inf); vec: the row's V are one aligned run
 template <int V>
@@ -139,36 +171,29 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
         __syncthreads();
         for (int token = tid / G; token < CHUNK; token += TOK) {
             const int64_t t = c * CHUNK + token;
-            const bool here = t < a.T;
-            float v[V], p[V];
-            if (here) load_logits<V>((const uint8_t*)a.logits + t * row_bytes, a.type, e0, E, vec, v);
+            if (c * CHUNK + __builtin_amdgcn_readfirstlane(token) >= a.T) break;  // none of the wave's
+            float p[V];
+            uint32_t key[V];
+            if (t < a.T) load_logits<V>((const uint8_t*)a.logits + t * row_bytes, a.type, e0, E, vec, p);
             else {
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = -__builtin_inff();
+                for (int i = 0; i < V; ++i) p[i] = -__builtin_inff();
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) p[i] = v[i];
-            float top = 0.0f, inv = 0.0f, wsum = 0.0f;
+            for (int i = 0; i < V; ++i) key[i] = key_of(p[i]);
+            float top = 0.0f, inv = 0.0f;
             for (int j = 0; j < k; ++j) {
-                // the largest logit left and its expert, the lowest of equals; -1 when nothing is left that counts
-                float best = -__builtin_inff();
-                int e = -1;
+                // the largest logit left, then the lowest expert that has it; -1 when nothing is left that counts
+                uint32_t best = key[0], at = 0xffffffffu;
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (v[i] > best) {
-                        best = v[i];
-                        e = e0 + i;
-                    }
-                butterfly<G>([&](auto s) {
-                    const float ob = meet_any<decltype(s)::value>(best);
-                        const int oe = meet_any<decltype(s)::value>(e);
-                    if (ob > best || (ob == best && (uint32_t)oe < (uint32_t)e)) {
-                        best = ob;
-                        e = oe;
-                    }
-                });
+                for (int i = 1; i < V; ++i) best = best > key[i] ? best : key[i];
+                best = reduce<G>(best, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+#pragma unroll
+                for (int i = V - 1; i >= 0; --i) at = key[i] == best ? (uint32_t)(e0 + i) : at;
+                at = reduce<G>(at, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+                const int e = best > NOTHING ? (int)at : -1;
                 if (j == 0) {
-                    top = e >= 0 ? best : 0.0f;
+                    top = e >= 0 ? of_key(best) : 0.0f;
                     float sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
@@ -179,17 +204,25 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
                     inv = e >= 0 ? 1.0f / sum : 0.0f;
                     live += e >= 0;
                 }
-                const float q = e >= 0 ? expf(best - top) * inv : 0.0f;
-                wsum += q;
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (e == e0 + i) v[i] = -__builtin_inff();
-                if (e0 == 0 && here) {
-                    s_w[token * k + j] = q;
+                for (int i = 0; i < V; ++i) key[i] = e == e0 + i ? 0 : key[i];
+                if (e0 == 0) {
+                    s_w[token * k + j] = of_key(best);
                     s_e[token * k + j] = e;
-                    if (e >= 0) atomicOr((unsigned long long*)&masks[e], 1ull << token);
                 }
             }
+            // the choices' weights, a choice per lane of the token's
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            float wsum = 0.0f;
+            for (int j = tid % G; j < k; j += G) {
+                const int e = s_e[token * k + j];
+                const float q = e >= 0 ? expf(s_w[token * k + j] - top) * inv : 0.0f;
+                wsum += q;
+                s_w[token * k + j] = q;
+                if (e >= 0) atomicOr((unsigned long long*)&masks[e], 1ull << token);
+            }
+            wsum = group_sum<G>(wsum);
             if (e0 == 0) s_f[token] = !a.renormalize ? 1.0f : (wsum > 0.0f ? 1.0f / wsum : 0.0f);
 #pragma unroll
             for (int i = 0; i < V; ++i) psum[i] += p[i] * inv;
@@ -211,11 +244,8 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
     }
     // sums over the block's tokens: the wave's, then the waves' in order
 #pragma unroll
-    for (int o = G; o < 64; o <<= 1) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) psum[i] += __shfl_xor(psum[i], o, 64);
-        live += __shfl_xor(live, o, 64);
-    }
+    for (int i = 0; i < V; ++i) psum[i] = sum_across<G>(psum[i]);
+    live = (int)sum_across<G>((float)live);  // (exact: fewer than 2^24)
     if (lane < G) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -386,7 +416,7 @@ __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
         top = fmaxf(top, p[i]);
         cnt += g[i];
     }
-    butterfly<G>([&](auto s) { top = fmaxf(top, meet_any<decltype(s)::value>(top)); });
+    top = reduce<G>(top, [](float x, float y) { return fmaxf(x, y); });
     const bool none = !(top > -__builtin_inff());  // nothing counts: no gradient
     float sum = 0.0f;
 #pragma unroll
@@ -717,8 +747,8 @@ hipError_t launch_route_experts(const MoeRouteArgs& a, int blocks, hipStream_t s
     if (a.E <= 32) return launch_route<4, 8, SINGLE>(a, blocks, st);
     if (a.E <= 64) return launch_route<8, 8, SINGLE>(a, blocks, st);
     if (a.E <= 128) return launch_route<16, 8, SINGLE>(a, blocks, st);
-    if (a.E <= 256) return launch_route<16, 16, SINGLE>(a, blocks, st);
-    if (a.E <= 512) return launch_route<32, 16, SINGLE>(a, blocks, st);
+    if (a.E <= 256) return launch_route<32, 8, SINGLE>(a, blocks, st);
+    if (a.E <= 512) return launch_route<64, 8, SINGLE>(a, blocks, st);
     return launch_route<64, 16, SINGLE>(a, blocks, st);
 }
 }  // namespace
