@@ -1824,7 +1824,8 @@ ascq_status ascq_moe_route(float* weights, int32_t* experts, int32_t* slots, int
     if (!counts || !routed || !loss || (p->tokens > 0 && (!weights || !experts || !slots || !row_tokens || !logits)))
         return fail(ASCQ_E_INVALID_ARG, "moe_route: null argument");
     const size_t need = ascq::moe_route_ws_bytes(p->tokens, p->experts);
-    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    const bool room = workspace && workspace_bytes >= need && aligned(workspace, 16);
+    if (need && !room && p->tokens > ascq::MOE_ROUTE_ALONE)
         return fail(ASCQ_E_INVALID_ARG, "moe_route: the workspace must be 16-byte aligned and hold %zu bytes", need);
     if (!aligned(weights, 4) || !aligned(experts, 4) || !aligned(slots, 4) || !aligned(row_tokens, 4) || !aligned(counts, 8) ||
         !aligned(routed, 8) || !aligned(loss, 4) || !aligned(logits, float_bytes(p->logits_type)))
@@ -1845,7 +1846,7 @@ ascq_status ascq_moe_route(float* weights, int32_t* experts, int32_t* slots, int
     a.k = p->top_k;
     a.renormalize = p->renormalize ? 1 : 0;
     trace("moe_route: logits %d, T %lld E %lld k %d", a.type, (long long)a.T, (long long)a.E, a.k);
-    return hip_status(ascq::launch_moe_route(a, workspace, S(stream)), "moe_route");
+    return hip_status(ascq::launch_moe_route(a, room ? workspace : nullptr, S(stream)), "moe_route");
 }
 
 ascq_status ascq_moe_route_grad(void* grad_logits, int64_t ld_grad, const void* logits, const float* weights,

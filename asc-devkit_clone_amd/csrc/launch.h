@@ -302,11 +302,13 @@ struct MoeRouteArgs {
     int type;
     int64_t T, E, ld;
     int k, renormalize;
-    int* block_counts;      // (set by the launcher, in the workspace) [blocks][E]
+    int chunk, chunks;      // (this and the rest set by the launcher) tokens of a mask, <= 64; how many
+    int* block_counts;      // in the workspace: [blocks][E]
     float* block_sums;      // [blocks][E]
     int* block_live;        // [blocks]
 };
 size_t moe_route_ws_bytes(int64_t T, int64_t E);
+constexpr int64_t MOE_ROUTE_ALONE = 64;  // tokens that need no workspace, though they may be faster with one
 hipError_t launch_moe_route(MoeRouteArgs a, void* ws, hipStream_t st);
 struct MoeRouteGradArgs {
     void* grad_logits;      // [T, ld_grad] of the logits' type

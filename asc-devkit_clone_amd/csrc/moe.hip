@@ -10,11 +10,13 @@
 //   loss = E sum_e (counts_e / sum counts) (sum_t p_te / routed).
 // Every order is fixed -- no atomic decides a row or the order of a sum -- so equal inputs give equal bits.
 //
-// A chunk of 64 tokens notes those that chose an expert as one 64-bit mask per expert: the rank of a token among them is a
-// population count, and so is the chunk's count.  Blocks of chunks meet through a workspace: their counts and their sums
-// of p; the second launch turns the counts before a block into its rows' offsets.  Up to 64 tokens are one block, which does it all.
-// What bounds it is latency: a chain of k maxima over a token's experts, and two launches (16384 tokens, 64 experts, k = 6:
-// 8.6 and 7.3 us of kernels; 16 tokens, 16 experts, k = 2: 4.8).
+// A chunk of up to 64 tokens notes those that chose an expert as one 64-bit mask per expert: the rank of a token among them
+// is a population count, and so is the chunk's count.  Blocks of chunks meet through a workspace: their counts and their
+// sums of p; the second launch turns the counts before a block into its rows' offsets.  A few tokens are one block, which
+// does it all.
+// What bounds it is latency -- a chain of k maxima over a token's experts, and two launches -- and for many experts the search's
+// instructions, five per logit and choice (16384 tokens, 64 experts, k = 6: 7.5 and 7.3 us of kernels; 16384, 256, k = 8: 17.8
+// and 15; 16 tokens, 16 experts, k = 2: 4.8).
 #include <type_traits>
 
 #include "common.h"
@@ -25,8 +27,8 @@ namespace ascq {
 
 namespace {
 
-constexpr int CHUNK = 64;        // tokens of a mask
-constexpr int MAX_BLOCKS = 512;  // (each block of the second launch reads the counts of all)
+constexpr int CHUNK = 64;        // tokens of a mask, at most
+constexpr int MAX_BLOCKS = 512;  // (each block of the second launch reads the counts of all; fewer, each for a run: slower)
 constexpr int MAX_K = 16;
 
 __device__ __forceinline__ float load_logit(const void* p, int64_t i, int dtype)
@@ -142,6 +144,12 @@ __device__ __forceinline__ void load_logits(const void* row, int type, int e0, i
 
 }  // namespace
 
+// the first chunk of block b of the routing
+__device__ __forceinline__ int64_t first_chunk(const MoeRouteArgs& a, int b, int blocks)
+{
+    return a.chunks <= blocks ? b : (int64_t)a.chunks * b / blocks;
+}
+
 // G lanes per token, each with V neighbouring experts; a chunk at a time, all of its tokens at once up to 16 lanes.
 // SINGLE: one block has all tokens.
 template <int G>
@@ -159,8 +167,8 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
     __shared__ int s_e[CHUNK * MAX_K];
     __shared__ int s_live[NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e0 = tid % G * V;
-    const int64_t chunks = (a.T + CHUNK - 1) / CHUNK;
-    const int64_t c0 = chunks * blockIdx.x / gridDim.x, c1 = chunks * (blockIdx.x + 1) / gridDim.x;
+    const int C = a.chunk;
+    const int64_t c0 = first_chunk(a, blockIdx.x, gridDim.x), c1 = first_chunk(a, blockIdx.x + 1, gridDim.x);
     const bool vec = ((uintptr_t)a.logits | (uintptr_t)(a.ld * (a.type == DT_F32 ? 4 : 2))) % 16 == 0;
     const int64_t row_bytes = a.ld * (a.type == DT_F32 ? 4 : 2);
     if (tid < E) first[tid] = 0;
@@ -169,9 +177,9 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
     for (int64_t c = c0; c < c1; ++c) {
         if (tid < E) masks[tid] = 0;
         __syncthreads();
-        for (int token = tid / G; token < CHUNK; token += TOK) {
-            const int64_t t = c * CHUNK + token;
-            if (c * CHUNK + __builtin_amdgcn_readfirstlane(token) >= a.T) break;  // none of the wave's
+        for (int token = tid / G; token < C; token += TOK) {
+            const int64_t t = c * C + token;
+            if (c * C + __builtin_amdgcn_readfirstlane(token) >= a.T) break;  // none of the wave's
             float p[V];
             uint32_t key[V];
             if (t < a.T) load_logits<V>((const uint8_t*)a.logits + t * row_bytes, a.type, e0, E, vec, p);
@@ -229,10 +237,10 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
         }
         __syncthreads();
         // the choices leave in order; a choice's rank among those of its expert in this block
-        const int64_t left = (a.T - c * CHUNK) * k, n = left < CHUNK * k ? left : CHUNK * k;
+        const int64_t left = (a.T - c * C) * k, n = left < C * k ? left : C * k;
         for (int i = tid; i < n; i += NT) {
             const int e = s_e[i], tk = i / k;
-            const int64_t at = c * CHUNK * k + i;
+            const int64_t at = c * C * k + i;
             a.weights[at] = s_w[i] * s_f[tk];
             a.experts[at] = e;
             const int rank = e < 0 ? -1 : first[e] + __popcll(masks[e] & ((1ull << tk) - 1ull));
@@ -309,9 +317,8 @@ __global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int bloc
     int before = 0, all = 0;
     float p = 0.0f;
     // what comes after the scan is requested in front of it
-    const int64_t chunks = (a.T + CHUNK - 1) / CHUNK;
-    const int64_t c0 = chunks * b0 / blocks, c1 = chunks * (b0 + 1) / blocks;
-    const int64_t end = c1 * CHUNK < a.T ? c1 * CHUNK * k : a.T * k, at0 = c0 * CHUNK * k + tid;
+    const int64_t c0 = first_chunk(a, b0, blocks), c1 = first_chunk(a, b0 + 1, blocks);
+    const int64_t end = c1 * a.chunk < a.T ? c1 * a.chunk * k : a.T * k, at0 = c0 * a.chunk * k + tid;
     const int expert0 = at0 < end ? a.experts[at0] : -1, rank0 = at0 < end ? a.slots[at0] : -1;
     int live = b0 == 0 && tid < blocks ? a.block_live[tid] : 0;  // (blocks <= MAX_BLOCKS)
     static_assert(MAX_BLOCKS <= 1024, "one block per thread");
@@ -723,11 +730,16 @@ __global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a, in
 }
 
 namespace {
-int64_t route_blocks(int64_t T)
+// tokens of a chunk: 64, or 16 where experts are many and tokens few, so that more CUs share the k searches through the logits
+// (512 tokens, 256 experts, k = 8: both launches 13.7 us, with 64 21.4)
+int route_chunk(int64_t T, int64_t E) { return E > 64 && T <= 2048 ? 16 : CHUNK; }
+int64_t route_blocks(int64_t T, int64_t E)
 {
-    const int64_t chunks = (T + CHUNK - 1) / CHUNK;
+    const int64_t chunk = route_chunk(T, E), chunks = (T + chunk - 1) / chunk;
     return chunks < MAX_BLOCKS ? chunks : MAX_BLOCKS;
 }
+// one block for all tokens (64 tokens, 256 experts, k = 8: alone 17 us, by chunks 13.2; 6 tokens 8.7)
+bool route_alone(int64_t T, int64_t E) { return T <= 1 || (T <= MOE_ROUTE_ALONE && T * E <= 8192); }
 
 template <int G, int V, bool SINGLE>
 hipError_t launch_route(const MoeRouteArgs& a, int blocks, hipStream_t st)
@@ -755,14 +767,20 @@ hipError_t launch_route_experts(const MoeRouteArgs& a, int blocks, hipStream_t s
 
 size_t moe_route_ws_bytes(int64_t T, int64_t E)
 {
-    const int64_t blocks = route_blocks(T);
-    return blocks <= 1 ? 0 : (size_t)blocks * ((size_t)E * 8 + 4);
+    const int64_t blocks = route_blocks(T, E);
+    return route_alone(T, E) ? 0 : (size_t)blocks * ((size_t)E * 8 + 4);
 }
 
 hipError_t launch_moe_route(MoeRouteArgs a, void* ws, hipStream_t st)
 {
-    const int blocks = (int)route_blocks(a.T);
-    if (blocks <= 1) return launch_route_experts<true>(a, 1, st);
+    if (route_alone(a.T, a.E) || !ws) {
+        a.chunk = CHUNK;
+        a.chunks = (int)((a.T + CHUNK - 1) / CHUNK);
+        return a.T <= MOE_ROUTE_ALONE ? launch_route_experts<true>(a, 1, st) : hipErrorInvalidValue;
+    }
+    const int blocks = (int)route_blocks(a.T, a.E);
+    a.chunk = route_chunk(a.T, a.E);
+    a.chunks = (int)((a.T + a.chunk - 1) / a.chunk);
     a.block_counts = (int*)ws;
     a.block_sums = (float*)(a.block_counts + (int64_t)blocks * a.E);
     a.block_live = (int*)(a.block_sums + (int64_t)blocks * a.E);

@@ -634,7 +634,8 @@ typedef struct {
  *   routed   int64 [1]: tokens with a choice
  *   loss     f32 [1]: the balance loss experts sum_e (counts_e / sum counts) (sum_t p_te / routed); 0 without a choice
  * tokens * top_k < 2^31.  Equal inputs give equal bits: no order depends on timing.
- * workspace (no counterpart in the reference): ascq_moe_route_workspace_size bytes, 16-byte aligned (NULL when 0). */
+ * workspace (no counterpart in the reference): ascq_moe_route_workspace_size bytes, 16-byte aligned; up to 64 tokens the
+ * call also runs without one (NULL), of many experts slower. */
 ascq_status ascq_moe_route_workspace_size(const ascq_route_param* p, size_t* bytes);
 ascq_status ascq_moe_route(float* weights, int32_t* experts, int32_t* slots, int32_t* row_tokens, int64_t* counts,
                            int64_t* routed, float* loss, const void* logits, const ascq_route_param* p, void* workspace,

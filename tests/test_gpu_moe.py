@@ -8,6 +8,7 @@ products in fp32 (2^-24 (k + 1) of their magnitudes) and rounds once; its weight
 steps."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -355,3 +356,31 @@ def test_on_another_stream(ascq_gpu):
     r = ascq_gpu.moe_route(gx, 4, stream=st)
     st.synchronize()
     _check_route(r, _reference(x, 4, True))
+
+
+@pytest.mark.parametrize("t,e,k", [(64, 256, 8), (40, 1000, 16), (64, 16, 2), (33, 300, 4)])
+def test_route_without_workspace(ascq_gpu, t, e, k):
+    """Up to 64 tokens the C entry runs without a workspace, also where it would use one."""
+    x = _logits(t, e, "f32", 5, 0.1, 0.1).cuda()
+    want = ascq_gpu.moe_route(x, k)
+    r = ascq_gpu.MoeRouting(*(torch.full_like(v, -7) for v in want))
+    p = ascq_gpu._RouteParam(t, e, e, ascq_gpu._FLOAT_CODE[torch.float32], k, 1)
+    status = ascq_gpu.lib().ascq_moe_route(*(v.data_ptr() for v in r), x.data_ptr(), ctypes.byref(p), None, 0,
+                                           torch.cuda.current_stream().cuda_stream)
+    assert status == ascq_gpu.OK
+    for name in ("experts", "slots", "tokens", "counts", "routed", "weights"):
+        assert torch.equal(getattr(r, name), getattr(want, name)), name
+    assert torch.allclose(r.loss, want.loss, rtol=1e-5, atol=0)  # the tokens' sums come in another order
+
+
+@pytest.mark.parametrize("t,e,k", [(17, 700, 3), (500, 100, 5), (2048, 256, 8), (2049, 65, 2), (33000, 9, 1)])
+def test_route_chunks(ascq_gpu, t, e, k):
+    """Short chunks of tokens for many experts, long ones, and more of them than blocks."""
+    x = _logits(t, e, "bf16", 7, 0.2, 0.1, True)
+    _check_route(ascq_gpu.moe_route(x.cuda(), k), _reference(x, k, True))
+
+
+@pytest.mark.parametrize("t,e,k,n", [(300, 60, 8, 2056), (600, 8, 3, 1000), (1100, 16, 1, 2049), (1025, 4, 2, 5)])
+def test_many_rows(ascq_gpu, t, e, k, n):
+    test_dispatch(ascq_gpu, t, e, k, n, 0.2, torch.int8)
+    test_combine_and_its_gradients(ascq_gpu, t, e, k, n, 0.2, "bf16")
