@@ -256,6 +256,23 @@ def _stream(stream) -> int | None:
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
+def _new(stream, shape, dtype, device, private: bool = False) -> torch.Tensor:
+    """An uninitialised tensor for kernels on `stream` (None: the current one), taken from that stream's memory: a block of
+    the current stream's may still be in use by work queued there, which `stream` does not wait for.  The caller reads a
+    result on the current stream as a rule, so a block given back is not reused before that stream's work is done either;
+    `private`: the call's own, which only `stream` uses."""
+    if stream is None or device.type == "cpu":
+        return torch.empty(shape, dtype=dtype, device=device)
+    current = torch.cuda.current_stream(device)
+    if current.cuda_stream == _stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device) if isinstance(stream, int) else stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if not private:
+        t.record_stream(current)
+    return t
+
+
 def _half_bits(v: float) -> int:
     return int(torch.tensor([v], dtype=torch.float16).view(torch.int16).item()) & 0xFFFF
 
@@ -589,15 +606,15 @@ def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, 
     h = x
     if residual is not None:
         ldr = _pitch(what, "residual", residual, shape, dt)
-        h = residual_out if residual_out is not None else torch.empty((m, n), dtype=dt, device=x.device)
+        h = residual_out if residual_out is not None else _new(stream, (m, n), dt, x.device)
         ldh = _pitch(what, "residual_out", h, shape, dt)
     elif residual_out is not None:
         _refuse(what, "residual_out needs a residual")
     if norm_out is not None:
         _dense(what, "norm_out", norm_out, shape, dt)
-    q = out if out is not None else torch.empty((m, n), dtype=_CODE_DTYPE[dst_type], device=x.device)
+    q = out if out is not None else _new(stream, (m, n), _CODE_DTYPE[dst_type], x.device)
     _dense(what, "out", q, shape, _CODE_DTYPE[dst_type])
-    s = scale_out if scale_out is not None else torch.empty((m,), dtype=torch.float32, device=x.device)
+    s = scale_out if scale_out is not None else _new(stream, (m,), torch.float32, x.device)
     _dense(what, "scale_out", s, (m,), torch.float32)
     _same_device(what, x, gamma, residual, h, norm_out, q, s)
     p = _NormQuantParam(m, n, ldx, ldr, ldh, src_type, dst_type, eps)
@@ -621,7 +638,7 @@ def quant_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
     code = _typed(what, "x", x, _CODE_TYPE)
     ldx, ldr = _pitch(what, "x", x, (m, k), x.dtype), 0
     ldw = _pitch(what, "w", w, (n, k) if w_trans else (k, n), x.dtype)
-    y = out if out is not None else torch.empty((m, n), dtype=out_dtype, device=x.device)
+    y = out if out is not None else _new(stream, (m, n), out_dtype, x.device)
     out_type = _typed(what, "out", y, _FLOAT_CODE)
     ldy = _pitch(what, "out", y, (m, n), y.dtype)
     _dense(what, "x_scale", x_scale, (m,), torch.float32)
@@ -636,9 +653,7 @@ def quant_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
         need = ctypes.c_size_t(0)
         check(lib().ascq_quant_linear_workspace_size(_at(x), _at(w), ctypes.byref(p), ctypes.byref(need)), what)
         if need.value:
-            workspace = torch.empty((need.value,), dtype=torch.uint8, device=x.device)
-            if stream is not None:
-                workspace.record_stream(_torch_stream(stream))
+            workspace = _new(stream, (need.value,), torch.uint8, x.device, private=True)
     check(lib().ascq_quant_linear(_at(y), _at(x), _at(x_scale), _at(w), _at(w_scale), _at(bias), _at(residual),
                                   ctypes.byref(p), _at(workspace), _room(workspace), _stream(stream)), what)
     return y
@@ -646,10 +661,6 @@ def quant_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
 
 def _room(workspace) -> int:
     return 0 if workspace is None else workspace.numel() * workspace.element_size()
-
-
-def _torch_stream(stream):
-    return torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream
 
 
 def quant_linear_workspace_size(x: torch.Tensor, w: torch.Tensor, w_trans: bool = True, out_dtype=torch.bfloat16) -> int:
@@ -700,16 +711,14 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True, out=No
     check(lib().ascq_moe_route_workspace_size(ctypes.byref(p), ctypes.byref(need)), what)
     r = out
     if r is None:
-        new = lambda shape, dt: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
+        new = lambda shape, dt: _new(stream, shape, dt, logits.device)  # noqa: E731
         r = MoeRouting(new((t, top_k), torch.float32), new((t, top_k), torch.int32), new((t, top_k), torch.int32),
                        new((t * top_k,), torch.int32), new((e,), torch.int64), new((1,), torch.int64),
                        new((1,), torch.float32))
     _check_routing(what, r, t, e, top_k)
     _same_device(what, logits, *r, workspace)
     if workspace is None and need.value:
-        workspace = torch.empty((need.value,), dtype=torch.uint8, device=logits.device)
-        if stream is not None:
-            workspace.record_stream(_torch_stream(stream))
+        workspace = _new(stream, (need.value,), torch.uint8, logits.device, private=True)
     check(lib().ascq_moe_route(*map(_at, r), _at(logits), ctypes.byref(p), _at(workspace), _room(workspace),
                                _stream(stream)), what)
     return r
@@ -733,7 +742,7 @@ def moe_route_grad(logits: torch.Tensor, weights: torch.Tensor, experts: torch.T
         _dense(what, "grad_weights", grad_weights, (t, k), torch.float32)
     if grad_loss is not None:
         _dense(what, "grad_loss", grad_loss, (1,), torch.float32)
-    g = out if out is not None else torch.empty((t, e), dtype=logits.dtype, device=logits.device)
+    g = out if out is not None else _new(stream, (t, e), logits.dtype, logits.device)
     ldg = _pitch(what, "out", g, (t, e), logits.dtype)
     _same_device(what, logits, weights, experts, counts, routed, grad_weights, grad_loss, g)
     p = _RouteParam(t, e, ld, _typed(what, "logits", logits, _FLOAT_CODE), k, int(renormalize))
@@ -755,12 +764,12 @@ def moe_dispatch(x: torch.Tensor, x_scale, slots: torch.Tensor, tokens: torch.Te
     ldx = _pitch(what, "x", x, (t, n), x.dtype)
     _dense(what, "slots", slots, (t, k), torch.int32)
     _dense(what, "tokens", tokens, (t * k,), torch.int32)
-    rows = out if out is not None else torch.empty((t * k, n), dtype=x.dtype, device=x.device)
+    rows = out if out is not None else _new(stream, (t * k, n), x.dtype, x.device)
     _dense(what, "out", rows, (t * k, n), x.dtype)
     s = None
     if x_scale is not None:
         _dense(what, "x_scale", x_scale, (t,), torch.float32)
-        s = scale_out if scale_out is not None else torch.empty((t * k,), dtype=torch.float32, device=x.device)
+        s = scale_out if scale_out is not None else _new(stream, (t * k,), torch.float32, x.device)
         _dense(what, "scale_out", s, (t * k,), torch.float32)
     elif scale_out is not None:
         _refuse(what, "scale_out needs x_scale")
@@ -784,7 +793,7 @@ def moe_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, res
     _dense(what, "weights", weights, (t, k), torch.float32)
     if residual is not None:
         _dense(what, "residual", residual, (t, n), y.dtype)
-    r = out if out is not None else torch.empty((t, n), dtype=y.dtype, device=y.device)
+    r = out if out is not None else _new(stream, (t, n), y.dtype, y.device)
     _dense(what, "out", r, (t, n), y.dtype)
     _same_device(what, y, slots, weights, residual, r)
     p = _RowsParam(t, n, 0, code, k)
@@ -807,11 +816,11 @@ def moe_combine_grad(grad_out: torch.Tensor, y: torch.Tensor, slots: torch.Tenso
     _dense(what, "slots", slots, (t, k), torch.int32)
     _dense(what, "tokens", tokens, (t * k,), torch.int32)
     _dense(what, "weights", weights, (t, k), torch.float32)
-    dw = out if out is not None else torch.empty((t, k), dtype=torch.float32, device=y.device)
+    dw = out if out is not None else _new(stream, (t, k), torch.float32, y.device)
     _dense(what, "out", dw, (t, k), torch.float32)
     dy = None
     if need_grad_y:
-        dy = grad_y_out if grad_y_out is not None else torch.empty_like(y)
+        dy = grad_y_out if grad_y_out is not None else _new(stream, (t * k, n), y.dtype, y.device)
         _dense(what, "grad_y_out", dy, (t * k, n), y.dtype)
     _same_device(what, y, grad_out, slots, tokens, weights, dw, dy)
     p = _RowsParam(t, n, 0, code, k)
