@@ -288,8 +288,8 @@ def quant_dynamic_per_token(x: torch.Tensor, round_mode: int = ROUND_RINT, out=N
     """Per-row absmax -> int8 q and fp32 scale (= absmax/127).  x: [m, n] f16 / bf16 / f32."""
     m, n = x.shape
     src_type = _FLOAT_CODE[x.dtype]
-    q = out if out is not None else torch.empty((m, n), dtype=torch.int8, device=x.device)
-    s = scale_out if scale_out is not None else torch.empty((m,), dtype=torch.float32, device=x.device)
+    q = out if out is not None else _new(stream, (m, n), torch.int8, x.device)
+    s = scale_out if scale_out is not None else _new(stream, (m,), torch.float32, x.device)
     check(lib().ascq_ascend_quant_dynamic_per_token(_ptr(q), _ptr(s), _ptr(x), src_type, m, n, round_mode,
                                                     _stream(stream)), "quant_dynamic_per_token")
     return q, s
@@ -300,7 +300,7 @@ def quant_per_token(x: torch.Tensor, scale: torch.Tensor, offset=None, round_mod
     """AscendQuant PER_TOKEN: q = sat_s8(round(f32(x) * scale[row] (+ offset[row])))."""
     m, n = x.shape
     src_type = _FLOAT_CODE[x.dtype]
-    q = out if out is not None else torch.empty((m, n), dtype=torch.int8, device=x.device)
+    q = out if out is not None else _new(stream, (m, n), torch.int8, x.device)
     p = _QuantParam(m, n, m * n, 0, 1 if offset is not None else 0, 1, round_mode)
     check(lib().ascq_ascend_quant_per_token(_ptr(q), _ptr(x), src_type, _ptr(scale), _ptr(offset), ctypes.byref(p),
                                             _stream(stream)), "quant_per_token")
@@ -320,9 +320,9 @@ def ascend_quant_policy(x: torch.Tensor, scale: torch.Tensor, policy: int, dst_t
     if out is not None:
         q = out
     elif dst_type in (FP4_E2M1, FP4_E1M2):
-        q = torch.empty((m, n // 2), dtype=torch.uint8, device=x.device)
+        q = _new(stream, (m, n // 2), torch.uint8, x.device)
     else:
-        q = torch.empty((m, n), dtype=torch.int8 if dst_type == INT8 else torch.uint8, device=x.device)
+        q = _new(stream, (m, n), torch.int8 if dst_type == INT8 else torch.uint8, x.device)
     has_off = offset is not None or offset_scalar is not None
     p = _QuantParam(m, n, m * n, group_size, int(has_off), k_dim, round_mode)
     check(lib().ascq_ascend_quant_policy(_ptr(q), dst_type, _ptr(x), src_type, _ptr(scale), _ptr(offset),
@@ -337,8 +337,7 @@ def ascend_quant(x: torch.Tensor, dst_type: int = INT8, scale=None, offset=None,
     source's type; offset None takes offset_scalar as a source-typed value).  dst INT8 / HIF8 (half arithmetic) or
     FP8_E4M3 / FP8_E5M2 (fp32 arithmetic); returns int8 (INT8) or uint8 codes of x's shape."""
     src_type = _FLOAT_CODE[x.dtype]
-    q = out if out is not None else torch.empty(x.shape, dtype=torch.int8 if dst_type == INT8 else torch.uint8,
-                                                device=x.device)
+    q = out if out is not None else _new(stream, x.shape, torch.int8 if dst_type == INT8 else torch.uint8, x.device)
     if scale is not None:
         scale_count = scale_count or scale.numel()
     check(lib().ascq_ascend_quant(_ptr(q), dst_type, _ptr(x), src_type, _ptr(scale), _ptr(offset), float(scale_scalar),
@@ -373,7 +372,7 @@ def ascend_dequant(src: torch.Tensor, scale, dst_dtype=torch.float16, cal_count=
     if scale_type is None:
         scale_type = F32 if scale is None else {torch.float32: F32, torch.bfloat16: BF16, torch.int64: U64}[scale.dtype]
     rows, ldd = dequant_dst_shape(dst_dtype, m, n, cal, mode)
-    y = out if out is not None else torch.empty((rows, ldd), dtype=dst_dtype, device=src.device)
+    y = out if out is not None else _new(stream, (rows, ldd), dst_dtype, src.device)
     p = _DequantParam(m, n, cal)
     check(lib().ascq_ascend_dequant(_ptr(y), dst_type, _ptr(src), src_type, _ptr(scale), scale_type,
                                     float(scale_scalar), PER_TENSOR if scale is None else PER_CHANNEL, mode,
@@ -389,7 +388,7 @@ def ascend_dequant_policy(src: torch.Tensor, scale: torch.Tensor, policy: int, d
     m, n = src.shape
     src_type = _SRC_CODE[src.dtype]
     scale_type = _FLOAT_CODE[scale.dtype]
-    y = out if out is not None else torch.empty((m, n), dtype=dst_dtype, device=src.device)
+    y = out if out is not None else _new(stream, (m, n), dst_dtype, src.device)
     p = _DequantPolicyParam(m, n, m * n if cal_count is None else cal_count, group_size, int(offset is not None), kdim)
     check(lib().ascq_ascend_dequant_policy(_ptr(y), _dtype_code(dst_dtype), _ptr(src), src_type, _ptr(scale),
                                            _ptr(offset), scale_type, policy, ctypes.byref(p), _stream(stream)),
@@ -403,7 +402,7 @@ def ascend_antiquant(src: torch.Tensor, src_type: int, scale: torch.Tensor, offs
     """AscendAntiQuant: dst = (src + offset) * scale.  Returns [K, N] (or [N, K] when is_transpose)."""
     dst_type = {torch.float16: F16, torch.bfloat16: BF16}[dst_dtype]
     shape = (n, k) if is_transpose else (k, n)
-    y = out if out is not None else torch.empty(shape, dtype=dst_dtype, device=src.device)
+    y = out if out is not None else _new(stream, shape, dst_dtype, src.device)
     check(lib().ascq_ascend_antiquant(_ptr(y), dst_type, _ptr(src), src_type, _ptr(offset), _ptr(scale), k, n,
                                       group_size, int(is_transpose), arith, _stream(stream)), "ascend_antiquant")
     return y
@@ -415,7 +414,7 @@ def ascend_antiquant_scalar(src: torch.Tensor, src_type: int, offset: float | No
     scale only); count elements (int4 two per byte)."""
     dst_type = {torch.float16: F16, torch.bfloat16: BF16}[dst_dtype]
     bits = lambda v: int(torch.tensor([v], dtype=dst_dtype).view(torch.int16).item()) & 0xFFFF
-    y = out if out is not None else torch.empty(count, dtype=dst_dtype, device=src.device)
+    y = out if out is not None else _new(stream, count, dst_dtype, src.device)
     check(lib().ascq_ascend_antiquant_scalar(_ptr(y), dst_type, _ptr(src), src_type, bits(offset or 0.0), bits(scale),
                                              int(offset is not None), count, _stream(stream)), "ascend_antiquant_scalar")
     return y
@@ -427,7 +426,7 @@ def ascend_antiquant_policy(src: torch.Tensor, src_type: int, scale: torch.Tenso
     """AscendAntiQuant policy form (PER_TOKEN / PER_GROUP) over [m, n]: int8 / fp8 sources with f16 / bf16 / f32
     scales, fp4 E2M1 / E1M2 sources with E8M0 group scales.  Returns [m, n] of dst_dtype."""
     dst_type = _FLOAT_CODE[dst_dtype]
-    y = out if out is not None else torch.empty((m, n), dtype=dst_dtype, device=src.device)
+    y = out if out is not None else _new(stream, (m, n), dst_dtype, src.device)
     check(lib().ascq_ascend_antiquant_policy(_ptr(y), dst_type, _ptr(src), src_type, _ptr(scale), _ptr(offset),
                                              scale_type, policy, m, n, group_size, k_dim, int(is_transpose),
                                              _stream(stream)), "ascend_antiquant_policy")
@@ -449,9 +448,9 @@ def quantize(x: torch.Tensor, policy: int, dst_type: int = INT8, scale=None, off
     if out is not None:
         q = out
     elif dst_type in (FP4_E2M1, FP4_E1M2):
-        q = torch.empty((m, n // 2), dtype=torch.uint8, device=x.device)
+        q = _new(stream, (m, n // 2), torch.uint8, x.device)
     else:
-        q = torch.empty((m, n), dtype=torch.int8 if dst_type == INT8 else torch.uint8, device=x.device)
+        q = _new(stream, (m, n), torch.int8 if dst_type == INT8 else torch.uint8, x.device)
     has_off = offset is not None or offset_scalar is not None
     p = _QuantizeParam(policy, int(has_off), round_mode, kdim, m, n, group_size)
     check(lib().ascq_quantize(_ptr(q), dst_type, _ptr(x), _FLOAT_CODE[x.dtype], _ptr(scale), _ptr(offset),
@@ -470,7 +469,7 @@ def dequantize(src: torch.Tensor, policy: int, dst_dtype=torch.float32, scale=No
     if scale_type is None:
         scale_type = F32 if scale is None else {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16,
                                                 torch.int64: U64}[scale.dtype]
-    y = out if out is not None else torch.empty((m, n), dtype=dst_dtype, device=src.device)
+    y = out if out is not None else _new(stream, (m, n), dst_dtype, src.device)
     p = _QuantizeParam(policy, 0, ROUND_RINT, kdim, m, n, group_size)
     check(lib().ascq_dequantize(_ptr(y), _FLOAT_CODE[dst_dtype], _ptr(src), src_type, _ptr(scale), float(scale_scalar),
                                 scale_type, ctypes.byref(p), _stream(stream)), "dequantize")
@@ -486,7 +485,7 @@ def antiquantize(src: torch.Tensor, src_type: int, policy: int, m: int, n: int, 
     if scale_type is None:
         scale_type = _FLOAT_CODE[dst_dtype] if scale is None else {torch.float32: F32, torch.float16: F16,
                                                                    torch.bfloat16: BF16, torch.uint8: E8M0}[scale.dtype]
-    y = out if out is not None else torch.empty((m, n), dtype=dst_dtype, device=src.device)
+    y = out if out is not None else _new(stream, (m, n), dst_dtype, src.device)
     has_off = offset is not None or offset_scalar is not None
     p = _QuantizeParam(policy, int(has_off), ROUND_RINT, kdim, m, n, group_size)
     check(lib().ascq_antiquantize(_ptr(y), _FLOAT_CODE[dst_dtype], _ptr(src), src_type, _ptr(scale), _ptr(offset),
@@ -506,7 +505,7 @@ def weight_pack_size(w_type: int, k: int, n: int) -> int:
 
 def weight_pack(w: torch.Tensor, w_type: int, k: int, n: int, is_transpose: bool = False, out=None, stream=None):
     nbytes = weight_pack_size(w_type, k, n)
-    wp = out if out is not None else torch.empty((nbytes,), dtype=torch.uint8, device=w.device)
+    wp = out if out is not None else _new(stream, (nbytes,), torch.uint8, w.device)
     check(lib().ascq_weight_pack(_ptr(wp), _ptr(w), w_type, k, n, int(is_transpose), _stream(stream)), "weight_pack")
     return wp
 
@@ -514,7 +513,7 @@ def weight_pack(w: torch.Tensor, w_type: int, k: int, n: int, is_transpose: bool
 def antiquant_matmul(x: torch.Tensor, w_packed: torch.Tensor, w_type: int, scale: torch.Tensor, offset, group_size: int,
                      n: int, out=None, stream=None):
     m, k = x.shape
-    y = out if out is not None else torch.empty((m, n), dtype=torch.float16, device=x.device)
+    y = out if out is not None else _new(stream, (m, n), torch.float16, x.device)
     check(lib().ascq_antiquant_matmul(_ptr(y), _ptr(x), _ptr(w_packed), w_type, _ptr(scale), _ptr(offset), group_size,
                                       m, n, k, _stream(stream)), "antiquant_matmul")
     return y
@@ -531,7 +530,7 @@ def quant_group_matmul(x: torch.Tensor, per_token_scale: torch.Tensor, w: torch.
     g = scale.shape[0]
     n = scale.shape[1]
     out_type = {torch.bfloat16: BF16, torch.float16: F16}[out_dtype]
-    y = out if out is not None else torch.empty((m, n), dtype=out_dtype, device=x.device)
+    y = out if out is not None else _new(stream, (m, n), out_dtype, x.device)
     check(lib().ascq_quant_group_matmul(_ptr(y), out_type, _ptr(x), _ptr(per_token_scale), _ptr(w), int(w_trans),
                                         _ptr(scale), _ptr(group_list), list_type, g, m, k, n, int(activation),
                                         _stream(stream)),
@@ -842,14 +841,14 @@ def nz_to_nd(src: torch.Tensor, dtype: int, batch: int, rows: int, cols: int, tr
     times the element size"""
     esize = {INT8: 1, UINT8: 1, FP8_E4M3: 1, FP8_E5M2: 1, F16: 2, BF16: 2, INT32: 4, F32: 4}[dtype]
     shape = (batch, cols, rows * esize) if transpose_out else (batch, rows, cols * esize)
-    y = out if out is not None else torch.empty(shape, dtype=torch.uint8, device=src.device)
+    y = out if out is not None else _new(stream, shape, torch.uint8, src.device)
     check(lib().ascq_nz_to_nd(_ptr(y), _ptr(src), dtype, batch, rows, cols, int(transpose_out), _stream(stream)),
           "nz_to_nd")
     return y
 
 
 def nd_to_nz(src: torch.Tensor, dtype: int, batch: int, rows: int, cols: int, out=None, stream=None):
-    y = out if out is not None else torch.empty(nz_size(dtype, batch, rows, cols), dtype=torch.uint8, device=src.device)
+    y = out if out is not None else _new(stream, nz_size(dtype, batch, rows, cols), torch.uint8, src.device)
     check(lib().ascq_nd_to_nz(_ptr(y), _ptr(src), dtype, batch, rows, cols, _stream(stream)), "nd_to_nz")
     return y
 

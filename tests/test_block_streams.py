@@ -72,6 +72,25 @@ CALLS = {
     "dispatch": lambda a, v, st: a.moe_dispatch(v["q"], v["s4"], v["i42"], v["i8"], stream=st),
     "combine": lambda a, v, st: a.moe_combine(v["y"], v["i42"], v["k2"], stream=st),
     "combine_grad": lambda a, v, st: a.moe_combine_grad(v["h"], v["y"], v["i42"], v["i8"], v["k2"], stream=st),
+    "quant_dynamic": lambda a, v, st: a.quant_dynamic_per_token(v["h"], stream=st),
+    "quant_per_token": lambda a, v, st: a.quant_per_token(v["h"], v["s4"], stream=st),
+    "quant_policy": lambda a, v, st: a.ascend_quant_policy(v["h"], v["s4"], a.PER_TOKEN, stream=st),
+    "quant_policy_fp4": lambda a, v, st: a.ascend_quant_policy(v["h"], v["s4"], a.PER_GROUP, a.FP4_E2M1, stream=st),
+    "quant": lambda a, v, st: a.ascend_quant(v["h"], stream=st),
+    "dequant": lambda a, v, st: a.ascend_dequant(v["q"], None, scale_type=a.F32, stream=st),
+    "dequant_policy": lambda a, v, st: a.ascend_dequant_policy(v["q"], v["s4"], a.PER_TOKEN, stream=st),
+    "antiquant": lambda a, v, st: a.ascend_antiquant(v["q"], a.INT8, v["g"], None, 4, 64, stream=st),
+    "antiquant_scalar": lambda a, v, st: a.ascend_antiquant_scalar(v["q"], a.INT8, None, 0.5, 256, stream=st),
+    "antiquant_policy": lambda a, v, st: a.ascend_antiquant_policy(v["q"], a.INT8, v["s4"], a.F32, a.PER_TOKEN, 4, 64, stream=st),
+    "quantize": lambda a, v, st: a.quantize(v["h"], a.PER_TENSOR, stream=st),
+    "quantize_fp4": lambda a, v, st: a.quantize(v["h"], a.PER_TENSOR, a.FP4_E2M1, stream=st),
+    "dequantize": lambda a, v, st: a.dequantize(v["logits"], a.PER_TENSOR, stream=st),
+    "antiquantize": lambda a, v, st: a.antiquantize(v["q"], a.INT8, a.PER_TENSOR, 4, 64, stream=st),
+    "weight_pack": lambda a, v, st: a.weight_pack(v["w"], a.INT8, 64, 32, stream=st),
+    "antiquant_matmul": lambda a, v, st: a.antiquant_matmul(v["h"], v["w"], a.INT8, v["g"], None, 64, 32, stream=st),
+    "group_matmul": lambda a, v, st: a.quant_group_matmul(v["q"], v["s4"], v["w"], v["k2"], v["c8"], stream=st),
+    "nz_to_nd": lambda a, v, st: a.nz_to_nd(v["q"], a.INT8, 1, 16, 32, stream=st),
+    "nd_to_nz": lambda a, v, st: a.nd_to_nz(v["q"], a.INT8, 1, 16, 32, stream=st),
 }
 
 
