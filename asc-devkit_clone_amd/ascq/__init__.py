@@ -646,20 +646,26 @@ def quant_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scal
         _dense(what, "bias", bias, (n,), torch.float32)
     if residual is not None:
         ldr = _pitch(what, "residual", residual, (m, n), y.dtype)
+    room = _room(what, workspace)
     _same_device(what, x, x_scale, w, w_scale, bias, residual, y, workspace)
     p = _LinearParam(m, n, k, ldx, ldw, ldr, ldy, code, out_type, int(w_trans), activation)
     if workspace is None:
         need = ctypes.c_size_t(0)
         check(lib().ascq_quant_linear_workspace_size(_at(x), _at(w), ctypes.byref(p), ctypes.byref(need)), what)
         if need.value:
-            workspace = _new(stream, (need.value,), torch.uint8, x.device, private=True)
+            workspace, room = _new(stream, (need.value,), torch.uint8, x.device, private=True), need.value
     check(lib().ascq_quant_linear(_at(y), _at(x), _at(x_scale), _at(w), _at(w_scale), _at(bias), _at(residual),
-                                  ctypes.byref(p), _at(workspace), _room(workspace), _stream(stream)), what)
+                                  ctypes.byref(p), _at(workspace), room, _stream(stream)), what)
     return y
 
 
-def _room(workspace) -> int:
-    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+def _room(what: str, workspace) -> int:
+    """The bytes of a workspace, which is one run of memory: what lies in a view's gaps is not the call's to write"""
+    if workspace is None:
+        return 0
+    if not workspace.is_contiguous():
+        _refuse(what, "the workspace must be contiguous")
+    return workspace.numel() * workspace.element_size()
 
 
 def quant_linear_workspace_size(x: torch.Tensor, w: torch.Tensor, w_trans: bool = True, out_dtype=torch.bfloat16) -> int:
@@ -715,10 +721,11 @@ def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True, out=No
                        new((t * top_k,), torch.int32), new((e,), torch.int64), new((1,), torch.int64),
                        new((1,), torch.float32))
     _check_routing(what, r, t, e, top_k)
+    room = _room(what, workspace)
     _same_device(what, logits, *r, workspace)
     if workspace is None and need.value:
-        workspace = _new(stream, (need.value,), torch.uint8, logits.device, private=True)
-    check(lib().ascq_moe_route(*map(_at, r), _at(logits), ctypes.byref(p), _at(workspace), _room(workspace),
+        workspace, room = _new(stream, (need.value,), torch.uint8, logits.device, private=True), need.value
+    check(lib().ascq_moe_route(*map(_at, r), _at(logits), ctypes.byref(p), _at(workspace), room,
                                _stream(stream)), what)
     return r
 
