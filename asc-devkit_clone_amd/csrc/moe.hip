@@ -435,7 +435,7 @@ __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
     if (a.grad_loss) {
         cnt = group_sum<G>(cnt);
         const float live = (float)*a.routed;
-        const float f = cnt > 0.0f && live > 0.0f ? *a.grad_loss * (float)E / (cnt * live) : 0.0f;
+        const float f = cnt > 0.0f && live > 0.0f ? *a.grad_loss * ((float)E / (cnt * live)) : 0.0f;  // (no product larger than f)
 #pragma unroll
         for (int i = 0; i < V; ++i) g[i] *= f;
     }

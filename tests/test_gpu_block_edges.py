@@ -34,3 +34,15 @@ def test_side_stream_beside_work_on_the_current_one(ascq_gpu):
             torch.cuda.synchronize()
             assert torch.equal(got, want)
             assert all(torch.equal(p, q) for p, q in zip(r, route))
+
+
+def test_route_gradient_of_a_large_upstream_gradient(ascq_gpu):
+    """grad_loss E counts / (sum counts routed) in an order that does not pass fp32's range while the result is inside it: the
+    gradient of 2e38 is 2^100 times that of 2e38 / 2^100, bit for bit (a power of two; nothing here is subnormal)"""
+    a = ascq_gpu
+    x = torch.randn(40, 16, generator=torch.Generator().manual_seed(3)).cuda()
+    r = a.moe_route(x, 2)
+    grad = lambda v: a.moe_route_grad(x, r.weights, r.experts, r.counts, r.routed,  # noqa: E731
+                                      grad_loss=torch.tensor([v], device="cuda"))
+    large, small = grad(2e38), grad(2e38 / 2.0 ** 100)
+    assert torch.isfinite(large).all() and torch.equal(large, small * 2.0 ** 100)
