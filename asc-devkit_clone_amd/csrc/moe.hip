@@ -37,6 +37,14 @@ __device__ __forceinline__ float load_logit(const void* p, int64_t i, int dtype)
     return v != v ? -__builtin_inff() : fminf(v, 3.402823466e38f);
 }
 
+// a gradient, rounded once: past a 16-bit type's range it is infinite, which is what a loss scaler looks for
+__device__ __forceinline__ void store_grad(void* p, int64_t i, float v, int dtype)
+{
+    if (dtype == DT_F16) ((uint16_t*)p)[i] = f32_to_f16(v);
+    else if (dtype == DT_BF16) ((__bf16*)p)[i] = (__bf16)v;
+    else ((float*)p)[i] = v;
+}
+
 __device__ __forceinline__ float wave_sum(float v)
 {
 #pragma unroll
@@ -480,7 +488,7 @@ __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (e0 + i < E) store_cast(out, e0 + i, d[i], a.type);
+            if (e0 + i < E) store_grad(out, e0 + i, d[i], a.type);
     }
 }
 
@@ -517,6 +525,8 @@ struct Eight {
             else w[0][e / 2] |= (uint32_t)((const uint16_t*)row)[u * 8 + e] << (16 * (e & 1));
         }
     }
+    // SAT: 16-bit types saturate, else they overflow to infinity
+    template <bool SAT>
     __device__ __forceinline__ static void store(void* row, int64_t u, int count, const float (&f)[8])
     {
         uint32_t d[8];
@@ -527,7 +537,7 @@ struct Eight {
             us2_t top = {0, 0};
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = cvt_pair<T == DT_BF16>(f[2 * e], f[2 * e + 1], top);
-            if (__builtin_expect(cvt_special<T == DT_BF16>(top), 0)) {
+            if (SAT && __builtin_expect(cvt_special<T == DT_BF16>(top), 0)) {
                 auto one = [](float x) { return (uint32_t)(T == DT_BF16 ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d[e] = one(f[2 * e]) | (one(f[2 * e + 1]) << 16);
@@ -648,11 +658,11 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a, int wav
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += r.get(e);
         }
-        Eight<T, ANY>::store((uint8_t*)a.out + t * pitch, u, count, v);
+        Eight<T, ANY>::template store<true>((uint8_t*)a.out + t * pitch, u, count, v);
     }
 }
 
-// dw_tj = <dout_t, y[slot_tj]>, dy[slot_tj] = w_tj dout_t; rows of no token get 0.  An item is a token and up to `per` <= 4 of its
+// dw_tj = <dout_t, y[slot_tj]>, dy[slot_tj] = w_tj dout_t (past its type's range infinite); rows of no token get 0.  An item is a token and up to `per` <= 4 of its
 // choices, whose gradient it reads once; W waves do it: four, or one for rows of fewer than 2048 (13370 tokens x 2 of 512:
 // 17 us, with four waves 43; 8192 x 2 of 2048: 34, with one wave 42).  Few items take a choice each (14 tokens x 8 of 3904: 4.5
 // us, four choices 7.0; 512 x 6 of 2048: 14, four 10).  Bound by memory: 4096 x 2 rows of 4096 bf16 in 35 us, 4.8 TB/s.
@@ -696,12 +706,12 @@ __global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a, in
                 if (a.out && slot[j] >= 0) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] = w[j] * d.get(e);
-                    Eight<T, ANY>::store((uint8_t*)a.out + slot[j] * pitch, u, count, f);
+                    Eight<T, ANY>::template store<false>((uint8_t*)a.out + slot[j] * pitch, u, count, f);
                 }
                 if (clear[j]) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-                    Eight<T, ANY>::store((uint8_t*)a.out + (t * a.k + j0 + j) * pitch, u, count, f);
+                    Eight<T, ANY>::template store<false>((uint8_t*)a.out + (t * a.k + j0 + j) * pitch, u, count, f);
                 }
             }
         }

@@ -640,9 +640,10 @@ ascq_status ascq_moe_route_workspace_size(const ascq_route_param* p, size_t* byt
 ascq_status ascq_moe_route(float* weights, int32_t* experts, int32_t* slots, int32_t* row_tokens, int64_t* counts,
                            int64_t* routed, float* loss, const void* logits, const ascq_route_param* p, void* workspace,
                            size_t workspace_bytes, void* stream);
-/* (no counterpart in the reference) The gradient with respect to the logits of grad_loss loss + sum_tj grad_weights_tj weights_tj (counts and choices taken
- * as constants): grad_logits [tokens, ld_grad] of the logits' type; weights, experts, counts and routed as
- * ascq_moe_route left them; grad_weights f32 [tokens, top_k] and grad_loss f32 [1], on the device, either may be NULL. */
+/* (no counterpart in the reference) The gradient with respect to the logits of grad_loss loss + sum_tj grad_weights_tj
+ * weights_tj (counts and choices taken as constants): grad_logits [tokens, ld_grad] of the logits' type, rounded once, infinite
+ * past a 16-bit type's range; weights, experts, counts and routed as ascq_moe_route left them; grad_weights f32 [tokens, top_k]
+ * and grad_loss f32 [1], on the device, either may be NULL. */
 ascq_status ascq_moe_route_grad(void* grad_logits, int64_t ld_grad, const void* logits, const float* weights,
                                 const int32_t* experts, const int64_t* counts, const int64_t* routed,
                                 const float* grad_weights, const float* grad_loss, const ascq_route_param* p,
@@ -663,8 +664,9 @@ ascq_status ascq_moe_dispatch(void* rows, float* row_scale, const void* x, const
  * NULL, or out itself. */
 ascq_status ascq_moe_combine(void* out, const void* y, const int32_t* slots, const float* weights, const void* residual,
                              const ascq_rows_param* p, void* stream);
-/* (no counterpart in the reference) grad_weights[t, j] = <grad_out[t], y[slots[t, j]]> (f32, 0 where there is no row) and grad_y[slots[t, j]] =
- * weights[t, j] grad_out[t] (rows of no token are 0); either may be NULL.  The residual's gradient is grad_out. */
+/* (no counterpart in the reference) grad_weights[t, j] = <grad_out[t], y[slots[t, j]]> (f32, 0 where there is no row) and
+ * grad_y[slots[t, j]] = weights[t, j] grad_out[t] (rounded once, infinite past a 16-bit type's range; rows of no token are 0);
+ * either may be NULL.  The residual's gradient is grad_out. */
 ascq_status ascq_moe_combine_grad(float* grad_weights, void* grad_y, const void* grad_out, const void* y,
                                   const int32_t* slots, const int32_t* row_tokens, const float* weights,
                                   const ascq_rows_param* p, void* stream);

@@ -46,3 +46,61 @@ def test_route_gradient_of_a_large_upstream_gradient(ascq_gpu):
                                       grad_loss=torch.tensor([v], device="cuda"))
     large, small = grad(2e38), grad(2e38 / 2.0 ** 100)
     assert torch.isfinite(large).all() and torch.equal(large, small * 2.0 ** 100)
+
+
+def _same(got, want):
+    """equal bits, any NaN being as good as another"""
+    assert got.dtype == want.dtype
+    nan = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), nan)
+    assert torch.equal(torch.where(nan, 0, got), torch.where(nan, 0, want))
+
+
+@pytest.mark.parametrize("n", [64, 77, 2048, 4099])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+def test_combine_gradient_keeps_infinities(ascq_gpu, dt, n):
+    """grad_y is one fp32 product rounded once to its type (so equal bits): infinities and NaN of grad_out arrive, and a
+    product past the type's range is infinite -- what a loss scaler looks for"""
+    a = ascq_gpu
+    t, k = 5, 2
+    slots = torch.arange(t * k, dtype=torch.int32, device="cuda").view(t, k)
+    tokens = torch.arange(t * k, dtype=torch.int32, device="cuda") // k
+    w = torch.full((t, k), 0.5, device="cuda")
+    w[3] = 1e20
+    g = torch.randn(t, n, generator=torch.Generator().manual_seed(n)).to(dt)
+    g[1, 3], g[1, n - 1], g[2, 0], g[2, n // 2] = float("inf"), -float("inf"), float("nan"), torch.finfo(dt).max
+    g = g.cuda()
+    y = torch.ones(t * k, n, dtype=dt, device="cuda")
+    dw, dy = a.moe_combine_grad(g, y, slots, tokens, w)
+    _same(dy, (w.view(-1, 1) * g.float()[tokens.long()]).to(dt))
+    assert torch.isinf(dy[2, 3]) and torch.isinf(dy[2, n - 1]) and torch.isnan(dy[4, 0])
+    if dt is torch.float16:
+        assert torch.isinf(dy[6:8]).all()  # 1e20 g
+    assert torch.isnan(dw[1]).all() and torch.isnan(dw[2]).all()  # inf - inf, NaN
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("e", [8, 33, 64])
+def test_route_gradient_overflows_to_infinity(ascq_gpu, e, dt, renormalize):
+    """A gradient past its type's range is infinite (the f32 gradient, which the other tests compare, rounded once: its size
+    is at least twice the type's largest, or at most half of it, wherever it is looked at)"""
+    a = ascq_gpu
+    t, k = 9, 2
+    x = torch.randn(t, e, generator=torch.Generator().manual_seed(e)).to(dt).cuda()
+    r = a.moe_route(x, k, renormalize)
+    for scale in (1.0, 1e6, 1e38):
+        up = torch.full((1,), scale, device="cuda")
+        dw = torch.randn(t, k, generator=torch.Generator().manual_seed(1)).cuda() * scale
+        got = a.moe_route_grad(x, r.weights, r.experts, r.counts, r.routed, grad_weights=dw, grad_loss=up, renormalize=renormalize)
+        wide = a.moe_route_grad(x.float(), r.weights, r.experts, r.counts, r.routed, grad_weights=dw, grad_loss=up,
+                                renormalize=renormalize)
+        top = torch.finfo(dt).max
+        over, under = wide.abs() > 2 * top, wide.abs() < top / 2
+        assert torch.isinf(got[over]).all() and torch.equal(got[over].sign().float(), wide[over].sign())
+        assert torch.isfinite(got[under]).all()
+        if dt is torch.float16 and scale > 1e6:
+            assert over.any()
+    up.fill_(float("inf"))
+    got = a.moe_route_grad(x, r.weights, r.experts, r.counts, r.routed, grad_loss=up, renormalize=renormalize)
+    assert not torch.isfinite(got).any()
