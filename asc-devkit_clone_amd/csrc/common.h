@@ -57,6 +57,14 @@ __device__ __forceinline__ uint16_t f32_to_bf16_sat(float x)
     b = (b & 0x7fffu) == 0x7f80u ? ((b & 0x8000u) | 0x7f7fu) : b;
     return (u & 0x7fffffffu) > 0x7f800000u ? (uint16_t)((u >> 16) | 0x40u) : (uint16_t)b;
 }
+// fp32 -> f16 / bf16, rne: a finite value past the type's range saturates, an infinity (and a NaN) stays what it is
+template <bool BF>
+__device__ __forceinline__ uint16_t f32_to_16_keep_inf(float x)
+{
+    const bool inf = __builtin_fabsf(x) == __builtin_inff();
+    const uint16_t b = BF ? f32_to_bf16_sat(x) : f32_to_f16_sat(x);
+    return inf ? (uint16_t)((b & 0x8000u) | (BF ? 0x7f80u : 0x7c00u)) : b;
+}
 // Two fp32 -> two f16 / bf16 (rne, saturating as f32_to_f16_sat / f32_to_bf16_sat) in one gfx950 conversion, as one
 // dword; `top` keeps the largest magnitude bits of both halves seen, so a caller converts many pairs and looks once for
 // the rare ones the conversion alone does not saturate (an exponent of all ones: overflow, infinity, NaN).

@@ -9,8 +9,8 @@
 // stored stream's type), the codes' and norm's.
 // Bound by memory: 8192 x 8192 bf16 with residual to e4m3 in 77 us, 6.1 TB/s of the bytes it cannot do without; f32 4.9 TB/s
 // (4096 x 8192: 88 us); rows that start at any element 4.4 (8192 x 8191: 108 us).  A decode step's 16 x 4096 takes 3.5 us.
-// A row of zeros has codes and scale 0.  A row with a NaN, an infinity, or squares that pass fp32's range has codes 0 and
-// scale NaN, so that its products are NaN and not some number.
+// A row of zeros has codes and scale 0.  A row with a NaN, an infinity (which h keeps: only a finite sum saturates), or squares
+// that pass fp32's range has codes 0 and scale NaN, so that its products are NaN and not some number.
 #include <type_traits>
 
 #include "common.h"
@@ -22,9 +22,15 @@ namespace {
 
 __device__ __forceinline__ float round_to(float v, int dtype)
 {
-    if (dtype == DT_F16) return f16_to_f32(f32_to_f16_sat(v));
-    if (dtype == DT_BF16) return bf16_to_f32(f32_to_bf16_sat(v));
+    if (dtype == DT_F16) return f16_to_f32(f32_to_16_keep_inf<false>(v));
+    if (dtype == DT_BF16) return bf16_to_f32(f32_to_16_keep_inf<true>(v));
     return v;
+}
+__device__ __forceinline__ void store_rounded(void* p, int64_t i, float v, int dtype)
+{
+    if (dtype == DT_F16) ((uint16_t*)p)[i] = f32_to_16_keep_inf<false>(v);
+    else if (dtype == DT_BF16) ((uint16_t*)p)[i] = f32_to_16_keep_inf<true>(v);
+    else ((float*)p)[i] = v;
 }
 
 struct RowScale {
@@ -90,7 +96,7 @@ struct Unit {
         const uint16_t b = (uint16_t)(e & 1 ? d >> 16 : d);
         return T == DT_F16 ? f16_to_f32(b) : bf16_to_f32(b);
     }
-    // the unit of eight floats, rounded (16-bit types: nearest even, saturating)
+    // the unit of eight floats, rounded (16-bit types: nearest even; what is finite saturates)
     __device__ __forceinline__ void set(const float (&f)[8])
     {
         if constexpr (T == DT_F32) {
@@ -101,7 +107,7 @@ struct Unit {
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[0][e] = cvt_pair<T == DT_BF16>(f[2 * e], f[2 * e + 1], top);
             if (__builtin_expect(cvt_special<T == DT_BF16>(top), 0)) {
-                auto one = [](float x) { return (uint32_t)(T == DT_BF16 ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
+                auto one = [](float x) { return (uint32_t)f32_to_16_keep_inf<T == DT_BF16>(x); };
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[0][e] = one(f[2 * e]) | (one(f[2 * e + 1]) << 16);
             }
@@ -283,7 +289,7 @@ __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
     uint32_t top = 0;
     for (int64_t c = threadIdx.x; c < a.n; c += 256) {
         const float h = first(c);
-        if (a.h_out) store_cast(a.h_out, row * a.ldh + c, h, dt);
+        if (a.h_out) store_rounded(a.h_out, row * a.ldh + c, h, dt);
         ss += h * h;
         const uint32_t t = __float_as_uint(h * load_f32_of(a.gamma, c, dt)) & 0x7fffffffu;
         top = t > top ? t : top;
@@ -298,7 +304,7 @@ __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
         const float v = r.mult == 0.0f ? 0.0f : t * r.mult;
         if (a.dst_type == DT_INT8) ((int8_t*)a.q)[row * a.n + c] = (int8_t)quant_s8<RM_RINT>(v);
         else ((uint8_t*)a.q)[row * a.n + c] = f32_to_fp8(v, 0);
-        if (a.norm_out) store_cast(a.norm_out, row * a.n + c, t * r.rstd, dt);
+        if (a.norm_out) store_rounded(a.norm_out, row * a.n + c, t * r.rstd, dt);
     }
 }
 

@@ -581,7 +581,8 @@ typedef struct {
 } ascq_norm_quant_param;
 
 /* Residual addition, RMS norm and an 8-bit output with one scale per token, in one pass (no counterpart in the reference):
- *   h = rnd(x + residual) (rounded to src_type, saturating; without residual h = x), stored to h_out when given
+ *   h = rnd(x + residual) (rounded to src_type: a finite fp32 sum saturates, an infinite one stays infinite; without
+ *       residual h = x), stored to h_out when given
  *   t_c = h_c gamma_c,  rstd = 1 / sqrt(mean_c h_c^2 + eps),  a = max_c |t_c|,  Q = 127 (int8) or 448 (e4m3)
  *   q_c = rint(t_c (Q (1 / a))),  scale[row] = a rstd / Q, so that q scale is the norm h rstd gamma
  *   norm_out (optional): rnd(t_c rstd), the unquantised norm.

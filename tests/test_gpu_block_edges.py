@@ -104,3 +104,41 @@ def test_route_gradient_overflows_to_infinity(ascq_gpu, e, dt, renormalize):
     up.fill_(float("inf"))
     got = a.moe_route_grad(x, r.weights, r.experts, r.counts, r.routed, grad_loss=up, renormalize=renormalize)
     assert not torch.isfinite(got).any()
+
+
+def _rounded(v, dt):
+    """an fp32 value in dt: what is finite saturates, infinities and NaN stay"""
+    top = torch.finfo(dt).max
+    return torch.where(torch.isfinite(v), v.clamp(-top, top), v).to(dt)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [8, 96, 513, 4096, 66000])
+def test_norm_of_an_infinite_sum(ascq_gpu, n, dt, codes):
+    """an infinity or NaN in x or the residual: h keeps it (equal bits), codes 0, scale and norm NaN; the other rows are those of
+    the same call without it"""
+    a = ascq_gpu
+    g = torch.Generator().manual_seed(n)
+    x, r = torch.randn(9, n, generator=g).to(dt), torch.randn(9, n, generator=g).to(dt)
+    gamma = (torch.rand(n, generator=g) + 0.5).to(dt).cuda()
+    code = a.INT8 if codes == "int8" else a.FP8_E4M3
+    plain = a.add_rms_norm_quant(x.cuda(), gamma, 1e-5, code, residual=r.cuda())
+    inf, top = float("inf"), torch.finfo(dt).max
+    x[1, 2] = inf
+    r[2, n - 1] = -inf
+    x[3, 0], r[3, 0] = inf, inf
+    x[4, n // 2], r[4, n // 2] = inf, -inf
+    x[5, 1], r[5, 1] = -inf, top
+    r[7, n // 2] = float("nan")
+    bad, good = [1, 2, 3, 4, 5, 7], [0, 6, 8]
+    norm = torch.empty(9, n, dtype=dt, device="cuda")
+    q, s, h = a.add_rms_norm_quant(x.cuda(), gamma, 1e-5, code, residual=r.cuda(), norm_out=norm)
+    _same(h.cpu(), _rounded(x.float() + r.float(), dt))
+    assert torch.isinf(h.cpu()[[1, 2, 3, 5], [2, n - 1, 0, 1]]).all()
+    assert torch.all(q[bad].float() == 0) and torch.isnan(s[bad]).all() and torch.isnan(norm[bad]).all()
+    assert torch.equal(q[good].view(torch.uint8), plain[0][good].view(torch.uint8)) and torch.equal(s[good], plain[1][good])
+    into = x.cuda()
+    again = a.add_rms_norm_quant(into, gamma, 1e-5, code, residual=r.cuda(), residual_out=into)
+    _same(into, h)
+    assert torch.equal(again[0].view(torch.uint8), q.view(torch.uint8))
