@@ -312,6 +312,13 @@ __device__ __forceinline__ void store_cast(void* p, int64_t i, float v, int dtyp
     else if (dtype == DT_BF16) ((uint16_t*)p)[i] = f32_to_bf16_sat(v);
     else ((float*)p)[i] = v;
 }
+// the same, an infinity staying one
+__device__ __forceinline__ void store_keep_inf(void* p, int64_t i, float v, int dtype)
+{
+    if (dtype == DT_F16) ((uint16_t*)p)[i] = f32_to_16_keep_inf<false>(v);
+    else if (dtype == DT_BF16) ((uint16_t*)p)[i] = f32_to_16_keep_inf<true>(v);
+    else ((float*)p)[i] = v;
+}
 
 __device__ __forceinline__ float load_f32_of(const void* p, int64_t i, int dtype)
 {

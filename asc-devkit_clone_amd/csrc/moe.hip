@@ -525,7 +525,7 @@ struct Eight {
             else w[0][e / 2] |= (uint32_t)((const uint16_t*)row)[u * 8 + e] << (16 * (e & 1));
         }
     }
-    // SAT: 16-bit types saturate, else they overflow to infinity
+    // SAT: what is finite saturates in 16-bit types, else it overflows to infinity
     template <bool SAT>
     __device__ __forceinline__ static void store(void* row, int64_t u, int count, const float (&f)[8])
     {
@@ -538,7 +538,7 @@ struct Eight {
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = cvt_pair<T == DT_BF16>(f[2 * e], f[2 * e + 1], top);
             if (SAT && __builtin_expect(cvt_special<T == DT_BF16>(top), 0)) {
-                auto one = [](float x) { return (uint32_t)(T == DT_BF16 ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
+                auto one = [](float x) { return (uint32_t)f32_to_16_keep_inf<T == DT_BF16>(x); };
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d[e] = one(f[2 * e]) | (one(f[2 * e + 1]) << 16);
             }
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256) void moe_dispatch_kernel(MoeRowsArgs a, int wa
     }
 }
 
-// out_t = sum_j w_tj y[slot_tj] + residual_t: fp32, in the order of j, one rounding.  `waves` waves per token, interleaved by
+// out_t = sum_j w_tj y[slot_tj] + residual_t: fp32, in the order of j, one rounding (a finite sum saturates).  `waves` waves per token, interleaved by
 // 512 elements; four rows' loads of a thread are in flight together (a choice of no row reads row 0 and is dropped).  Bound by
 // memory: 4096 x 2 rows of 4096 bf16 with residual in 26 us, 5.2 TB/s; x 8 rows of 2048 in 33 us.
 template <int T, bool ANY>

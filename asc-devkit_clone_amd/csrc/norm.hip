@@ -26,12 +26,6 @@ __device__ __forceinline__ float round_to(float v, int dtype)
     if (dtype == DT_BF16) return bf16_to_f32(f32_to_16_keep_inf<true>(v));
     return v;
 }
-__device__ __forceinline__ void store_rounded(void* p, int64_t i, float v, int dtype)
-{
-    if (dtype == DT_F16) ((uint16_t*)p)[i] = f32_to_16_keep_inf<false>(v);
-    else if (dtype == DT_BF16) ((uint16_t*)p)[i] = f32_to_16_keep_inf<true>(v);
-    else ((float*)p)[i] = v;
-}
 
 struct RowScale {
     float mult, scale, rstd;  // codes = rnd(t * mult); a row without a finite answer: mult 0, scale NaN
@@ -289,7 +283,7 @@ __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
     uint32_t top = 0;
     for (int64_t c = threadIdx.x; c < a.n; c += 256) {
         const float h = first(c);
-        if (a.h_out) store_rounded(a.h_out, row * a.ldh + c, h, dt);
+        if (a.h_out) store_keep_inf(a.h_out, row * a.ldh + c, h, dt);
         ss += h * h;
         const uint32_t t = __float_as_uint(h * load_f32_of(a.gamma, c, dt)) & 0x7fffffffu;
         top = t > top ? t : top;
@@ -304,7 +298,7 @@ __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
         const float v = r.mult == 0.0f ? 0.0f : t * r.mult;
         if (a.dst_type == DT_INT8) ((int8_t*)a.q)[row * a.n + c] = (int8_t)quant_s8<RM_RINT>(v);
         else ((uint8_t*)a.q)[row * a.n + c] = f32_to_fp8(v, 0);
-        if (a.norm_out) store_rounded(a.norm_out, row * a.n + c, t * r.rstd, dt);
+        if (a.norm_out) store_keep_inf(a.norm_out, row * a.n + c, t * r.rstd, dt);
     }
 }
 

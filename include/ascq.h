@@ -661,8 +661,8 @@ typedef struct {
 /* (no counterpart in the reference) rows[slots[t, j]] = x[t], row_scale[slots[t, j]] = x_scale[t] (both NULL without scales); rows of no token are 0 */
 ascq_status ascq_moe_dispatch(void* rows, float* row_scale, const void* x, const float* x_scale, const int32_t* slots,
                               const int32_t* row_tokens, const ascq_rows_param* p, void* stream);
-/* (no counterpart in the reference) out[t] = sum_j weights[t, j] y[slots[t, j]] + residual[t]: fp32, in the order of j, one rounding.  residual may be
- * NULL, or out itself. */
+/* (no counterpart in the reference) out[t] = sum_j weights[t, j] y[slots[t, j]] + residual[t]: fp32, in the order of j, one
+ * rounding (in f16 and bf16 a finite sum saturates, an infinite one stays infinite).  residual may be NULL, or out itself. */
 ascq_status ascq_moe_combine(void* out, const void* y, const int32_t* slots, const float* weights, const void* residual,
                              const ascq_rows_param* p, void* stream);
 /* (no counterpart in the reference) grad_weights[t, j] = <grad_out[t], y[slots[t, j]]> (f32, 0 where there is no row) and

@@ -142,3 +142,23 @@ def test_norm_of_an_infinite_sum(ascq_gpu, n, dt, codes):
     again = a.add_rms_norm_quant(into, gamma, 1e-5, code, residual=r.cuda(), residual_out=into)
     _same(into, h)
     assert torch.equal(again[0].view(torch.uint8), q.view(torch.uint8))
+
+
+@pytest.mark.parametrize("n", [64, 77, 2048])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+def test_combine_keeps_infinities(ascq_gpu, dt, n):
+    """infinities and NaN of the rows and the residual stay; a finite sum past a 16-bit type's range saturates.  (weights 1 and
+    one choice: the fp32 sum y + residual is rounded once, and the result is equal to that)"""
+    a = ascq_gpu
+    t = 8
+    slots = torch.arange(t, dtype=torch.int32, device="cuda").view(t, 1)
+    g = torch.Generator().manual_seed(n)
+    y, r = torch.randn(t, n, generator=g).to(dt), torch.randn(t, n, generator=g).to(dt)
+    inf, top = float("inf"), torch.finfo(dt).max
+    y[1, 3], r[2, n - 1], y[3, 0], r[3, 0] = inf, -inf, inf, -inf
+    y[4, 5], r[5, 1] = float("nan"), float("nan")
+    y[6], r[6] = top * 0.75, top * 0.5
+    y[7], r[7] = -top, -inf
+    got = a.moe_combine(y.cuda(), slots, torch.ones(t, 1, device="cuda"), residual=r.cuda()).cpu()
+    _same(got, _rounded(y.float() + r.float(), dt))
+    assert got[1, 3] == inf and got[2, n - 1] == -inf and torch.isnan(got[3, 0]) and torch.all(got[7] == -inf)
