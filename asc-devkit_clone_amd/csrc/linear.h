@@ -1,6 +1,6 @@
 // linear.h -- the epilogue of the quantised linear (linear.hip):
 //   y = cast(act(acc w_scale[n] x_scale[m] + bias[n]) + residual[m, n])
-// in fp32, in this order, one rounding at the end (f16 / bf16: nearest even, saturating).
+// in fp32, in this order, one rounding at the end (f16 / bf16: nearest even; a finite value saturates, an infinity stays).
 #pragma once
 
 #include "common.h"
@@ -80,7 +80,7 @@ struct OutRun {
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = cvt_pair<OUT == DT_BF16>(f[2 * e], f[2 * e + 1], top);
             if (__builtin_expect(cvt_special<OUT == DT_BF16>(top), 0)) {
-                auto one = [](float x) { return (uint32_t)(OUT == DT_BF16 ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
+                auto one = [](float x) { return (uint32_t)f32_to_16_keep_inf<OUT == DT_BF16>(x); };
 #pragma unroll
                 for (int e = 0; e < 4; ++e) d[e] = one(f[2 * e]) | (one(f[2 * e + 1]) << 16);
             }

@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a)
                 if (a.bias) v += a.bias[n];
                 v = activate(v, a.act);
                 if (a.residual) v += load_f32_of(a.residual, m * a.ldr + n, a.out_type);
-                store_cast(a.y, m * a.ldy + n, v, a.out_type);
+                store_keep_inf(a.y, m * a.ldy + n, v, a.out_type);
             }
 }
 

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
             float y = scaled(s) * s_ws[i * 16 + n] * s_xs[m] + s_b[i * 16 + n];
             y = activate(y, p.act);
             if (p.residual) y += load_f32_of(p.residual, m * p.ldr + col, p.out_type);
-            store_cast(p.y, m * p.ldy + col, y, p.out_type);
+            store_keep_inf(p.y, m * p.ldy + col, y, p.out_type);
         }
     }
     wait_vmcnt<0>();  // no copy may still target LDS when the wave ends
@@ -196,11 +196,11 @@ __global__ __launch_bounds__(256) void linear_slices_kernel(LinearArgs p)
         } else {
             uint32_t h[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = OUT == DT_F16 ? f32_to_f16_sat(y[e]) : f32_to_bf16_sat(y[e]);
+            for (int e = 0; e < 4; ++e) h[e] = f32_to_16_keep_inf<OUT == DT_BF16>(y[e]);
             *(u32x2_any*)to = (u32x2){h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
         }
     } else {
-        for (int e = 0; e < count; ++e) store_cast(to, e, y[e], OUT);
+        for (int e = 0; e < count; ++e) store_keep_inf(to, e, y[e], OUT);
     }
 }
 

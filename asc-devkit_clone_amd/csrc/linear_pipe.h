@@ -102,7 +102,7 @@ struct LinearEpilogue {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = cvt_pair<BF>(v[q][2 * e], v[q][2 * e + 1], top);
                 if (__builtin_expect(cvt_special<BF>(top), 0)) {
-                    auto one = [](float x) { return (uint32_t)(BF ? f32_to_bf16_sat(x) : f32_to_f16_sat(x)); };
+                    auto one = [](float x) { return (uint32_t)f32_to_16_keep_inf<BF>(x); };
 #pragma unroll
                     for (int e = 0; e < 4; ++e) w[e] = one(v[q][2 * e]) | (one(v[q][2 * e + 1]) << 16);
                 }

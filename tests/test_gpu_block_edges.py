@@ -162,3 +162,26 @@ def test_combine_keeps_infinities(ascq_gpu, dt, n):
     got = a.moe_combine(y.cuda(), slots, torch.ones(t, 1, device="cuda"), residual=r.cuda()).cpu()
     _same(got, _rounded(y.float() + r.float(), dt))
     assert got[1, 3] == inf and got[2, n - 1] == -inf and torch.isnan(got[3, 0]) and torch.all(got[7] == -inf)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k,w_trans", [(3, 80, 128, True), (40, 77, 8192, True), (300, 260, 128, True), (300, 264, 128, False),
+                                           (300, 77, 130, True), (4, 64, 0, True)])
+def test_linear_keeps_infinities(ascq_gpu, m, n, k, w_trans, dt):
+    """infinities and NaN of the bias and the residual stay; a finite value past a 16-bit type's range saturates.  (x is zero, so
+    the result is the fp32 sum bias + residual rounded once, and equal to that.)"""
+    a = ascq_gpu
+    x = torch.zeros(m, k, dtype=torch.int8, device="cuda")
+    w = torch.ones((n, k) if w_trans else (k, n), dtype=torch.int8, device="cuda")
+    g = torch.Generator().manual_seed(n)
+    bias, r = torch.randn(n, generator=g), torch.randn(m, n, generator=g).to(dt)
+    inf, top = float("inf"), torch.finfo(dt).max
+    bias[1], bias[n - 1], bias[5], bias[6] = inf, -inf, float("nan"), top / 2
+    r[0, 3], r[1, n - 2], r[2, 1], r[2, 4] = inf, -inf, -inf, float("nan")
+    r[:, 6] = top
+    if dt is torch.float32:
+        r[:, 6] = top / 4
+    got = a.quant_linear(x, torch.ones(m, device="cuda"), w, torch.ones(n, device="cuda"), bias=bias.cuda(), residual=r.cuda(),
+                         w_trans=w_trans, out_dtype=dt).cpu()
+    _same(got, _rounded(bias + r.float(), dt))
+    assert got[0, 3] == inf and got[1, n - 2] == -inf and torch.isnan(got[2, 1]) and got[0, n - 1] == -inf
