@@ -416,7 +416,8 @@ __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
 #pragma unroll
         for (int j = 0; j < MAX_K; ++j) {
             if (j >= a.k) continue;
-            choice[j] = a.experts[t * a.k + j];
+            const int x = a.experts[t * a.k + j];
+            choice[j] = x < E ? x : -1;  // (no expert: no choice)
             dw[j] = a.grad_weights[t * a.k + j];
             add[j] = a.weights[t * a.k + j];
         }

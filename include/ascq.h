@@ -643,8 +643,8 @@ ascq_status ascq_moe_route(float* weights, int32_t* experts, int32_t* slots, int
                            size_t workspace_bytes, void* stream);
 /* (no counterpart in the reference) The gradient with respect to the logits of grad_loss loss + sum_tj grad_weights_tj
  * weights_tj (counts and choices taken as constants): grad_logits [tokens, ld_grad] of the logits' type, rounded once, infinite
- * past a 16-bit type's range; weights, experts, counts and routed as ascq_moe_route left them; grad_weights f32 [tokens, top_k]
- * and grad_loss f32 [1], on the device, either may be NULL. */
+ * past a 16-bit type's range; weights, experts, counts and routed as ascq_moe_route left them (a choice outside
+ * [0, experts) counts as none); grad_weights f32 [tokens, top_k] and grad_loss f32 [1], on the device, either may be NULL. */
 ascq_status ascq_moe_route_grad(void* grad_logits, int64_t ld_grad, const void* logits, const float* weights,
                                 const int32_t* experts, const int64_t* counts, const int64_t* routed,
                                 const float* grad_weights, const float* grad_loss, const ascq_route_param* p,

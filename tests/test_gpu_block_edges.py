@@ -185,3 +185,21 @@ def test_linear_keeps_infinities(ascq_gpu, m, n, k, w_trans, dt):
                          w_trans=w_trans, out_dtype=dt).cpu()
     _same(got, _rounded(bias + r.float(), dt))
     assert got[0, 3] == inf and got[1, n - 2] == -inf and torch.isnan(got[2, 1]) and got[0, n - 1] == -inf
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("e", [8, 60, 300])
+def test_route_gradient_without_choices_out_of_range(ascq_gpu, e, renormalize):
+    """a choice that is no expert counts as none, for the token's other choices too (equal bits)"""
+    a = ascq_gpu
+    t, k = 12, 3
+    g = torch.Generator().manual_seed(e)
+    x, dw = torch.randn(t, e, generator=g).cuda(), (torch.randn(t, k, generator=g) * 3).cuda()
+    r = a.moe_route(x, k, renormalize)
+    odd, none = r.experts.clone(), r.experts.clone()
+    for i, (j, bad) in enumerate(((1, e), (0, 2 ** 31 - 1), (2, -7), (1, -(2 ** 31)), (0, e + 5))):
+        odd[i, j], none[i, j] = bad, -1
+    grad = lambda experts: a.moe_route_grad(x, r.weights, experts, r.counts, r.routed, grad_weights=dw,  # noqa: E731
+                                            renormalize=renormalize)
+    assert torch.equal(grad(odd), grad(none))
+    assert not torch.equal(grad(odd)[:5], grad(r.experts)[:5]) and torch.equal(grad(odd)[5:], grad(r.experts)[5:])
