@@ -204,8 +204,16 @@ size_t linear_ws_bytes(const LinearArgs& in)
 {
     LinearArgs a = in;
     if (a.M == 0 || a.N == 0 || a.K == 0) return 0;
-    if (const int64_t rows = row_piece(a)) a.M = rows;  // (the last piece takes no more)
-    if (const int64_t channels = channel_piece(a)) a.N = channels;
+    const int64_t rows = row_piece(a), channels = rows ? 0 : channel_piece(a);
+    if (rows || channels) {  // what the whole pieces take or the last one, which may split K where they do not
+        int64_t& size = rows ? a.M : a.N;
+        const int64_t whole = rows ? rows : channels, last = size % whole;
+        size = whole;
+        const size_t most = linear_ws_bytes(a);
+        size = last;
+        const size_t rest = linear_ws_bytes(a);
+        return most > rest ? most : rest;
+    }
     if (too_large(a)) return 0;
     const PackPlan p = pack_plan(a);
     const size_t pack = p.x_bytes + p.w_bytes;
