@@ -23,7 +23,7 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t* src, int64_t n, bool 
 
 // Any shape, stride and alignment, 64-bit addresses: 64 x 64 tiles, one stage of 64 K at a time through LDS, a [K, N]
 // weight turned on the way.  It takes what nothing else does: K = 0, operands off their alignment without a workspace (1030 x
-// 4100 x 4095 int8: 995 us against 38 with one), and a w [K, N] past 2^31 bytes.
+// 4100 x 4095 int8: 995 us against 38 with one), and a w [K, N] past 2^31 bytes or of few rows that are very far apart.
 template <bool F8>
 __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a)
 {
@@ -121,6 +121,9 @@ bool too_large(const LinearArgs& a)
     const int64_t kp = (a.K + 15) / 16 * 16;
     // (the epilogue addresses 16 rows with 32-bit offsets)
     if (a.ldy > (1ll << 24) || (a.residual && a.ldr > (1ll << 24))) return true;
+    // (rows of a w [K, N] past K are asked for, up to the end of x's last 16-byte word or, fp8, of the stage: their 32-bit offsets
+    // must not come round to w again)
+    if (!a.w_trans && a.ldw > ((1ll << 32) - a.N - 4096) / (a.f8 ? (a.K + 127) / 128 * 128 : kp)) return true;
     return a.ldx * (a.M - 1) + kp > SPAN || a.M * kp > SPAN || (a.w_trans ? a.ldw * (a.N - 1) + kp : a.ldw * (a.K - 1) + a.N + 3) > SPAN ||
            (a.w_trans ? a.N * kp : a.K * ((a.N + 15) / 16 * 16)) > SPAN;
 }
@@ -235,7 +238,7 @@ hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hip
         }
         return hipSuccess;
     }
-    if (too_large(a)) return launch_any(a, "w [k, n] past 2^31 bytes, or a pitch past 2^24", st);
+    if (too_large(a)) return launch_any(a, "w [k, n] past 2^31 bytes or of few, very long rows, or a pitch past 2^24", st);
     const PackPlan p = pack_plan(a);
     const size_t pack = p.x_bytes + p.w_bytes;
     if (pack) {

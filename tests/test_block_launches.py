@@ -1,0 +1,27 @@
+"""The block operators' launches (CPU only): the built library driven by the programs of tests/cpp, which record the kernels it
+would launch, their grids and arguments."""
+from __future__ import annotations
+
+import os
+import subprocess
+from pathlib import Path
+
+import ascq
+
+ROOT = Path(__file__).resolve().parent.parent
+HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+
+
+def _run(tmp_path, name):
+    exe = tmp_path / name
+    libdir = Path(ascq.LIB_PATH).parent
+    subprocess.run([HIPCC, "--offload-arch=gfx950", "--offload-host-only", "-x", "hip", "-std=c++17", "-O1", "-I", str(ROOT / "include"),
+                    "-I", str(libdir / "csrc"), str(ROOT / "tests" / "cpp" / f"{name}.cpp"), "-rdynamic", "-L", str(libdir), "-lascq",
+                    f"-Wl,-rpath,{libdir}", "-Wl,-rpath,/opt/rocm/lib", "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
+
+
+def test_rows_past_k_are_past_the_range(tmp_path):
+    """w [K, N] of large row pitches: what the tiles read past K is nothing of w"""
+    _run(tmp_path, "linear_pitches")

@@ -203,3 +203,24 @@ def test_route_gradient_without_choices_out_of_range(ascq_gpu, e, renormalize):
                                             renormalize=renormalize)
     assert torch.equal(grad(odd), grad(none))
     assert not torch.equal(grad(odd)[:5], grad(r.experts)[:5]) and torch.equal(grad(odd)[5:], grad(r.experts)[5:])
+
+
+@pytest.mark.parametrize("k,pitch", [(1, 1 << 32), (2, (1 << 31) - 8192), (3, 1 << 24)])
+def test_linear_over_rows_far_apart(ascq_gpu, k, pitch):
+    """w [k, n] of few rows, gigabytes apart: neither what lies between them nor what follows k in x's rows is multiplied (small
+    whole numbers: exact)"""
+    a = ascq_gpu
+    m, n = 200, 320
+    g = torch.Generator(device="cuda").manual_seed(k)
+    raw = torch.full(((k - 1) * pitch + n,), 3, dtype=torch.int8, device="cuda")
+    w = raw.as_strided((k, n), (pitch, 1))
+    w.copy_(torch.randint(-9, 9, (k, n), generator=g, device="cuda", dtype=torch.int8))
+    x = torch.full((m, 32), 5, dtype=torch.int8, device="cuda")[:, :k]
+    x.copy_(torch.randint(-9, 9, (m, k), generator=g, device="cuda", dtype=torch.int8))
+    ones = torch.ones(max(m, n), device="cuda")
+    want = x.float() @ w.float()
+    assert torch.equal(a.quant_linear(x, ones[:m], w, ones[:n], w_trans=False, out_dtype=torch.float32), want)
+    f8 = torch.float8_e4m3fn
+    xf, wf = torch.full((m, 32), float("nan"), device="cuda").to(f8)[:, :k], raw.float().to(f8).as_strided((k, n), (pitch, 1))
+    xf.copy_(x.float().to(f8))
+    assert torch.equal(a.quant_linear(xf, ones[:m], wf, ones[:n], w_trans=False, out_dtype=torch.float32), want)
