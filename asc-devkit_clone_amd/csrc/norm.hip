@@ -339,7 +339,7 @@ static bool launch_row_of(const NormQuantArgs& a, bool any, hipStream_t st)
     return a.residual ? launch_row<T, true, false>(a, st) : launch_row<T, false, false>(a, st);
 }
 
-hipError_t launch_norm_quant(const NormQuantArgs& a, hipStream_t st)
+static hipError_t launch_rows(const NormQuantArgs& a, hipStream_t st)
 {
     const int64_t es = a.src_type == DT_F32 ? 4 : 2;
     const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.residual | (uintptr_t)a.h_out | (uintptr_t)a.norm_out |
@@ -354,6 +354,25 @@ hipError_t launch_norm_quant(const NormQuantArgs& a, hipStream_t st)
         launch_k(norm_quant_any_kernel, dim3((unsigned)a.m), dim3(256), 0u, st, a);
     }
     return hipGetLastError();
+}
+
+hipError_t launch_norm_quant(const NormQuantArgs& a, hipStream_t st)
+{
+    constexpr int64_t ROWS = 1 << 21;  // of a launch: a grid has fewer than 2^32 threads, a row up to 1024
+    const int64_t es = a.src_type == DT_F32 ? 4 : 2;
+    for (int64_t r = 0; r < a.m; r += ROWS) {
+        NormQuantArgs b = a;
+        b.m = a.m - r < ROWS ? a.m - r : ROWS;
+        b.q = (uint8_t*)a.q + r * a.n;
+        b.scale_out += r;
+        b.x = (const uint8_t*)a.x + r * a.ldx * es;
+        if (a.residual) b.residual = (const uint8_t*)a.residual + r * a.ldr * es;
+        if (a.h_out) b.h_out = (uint8_t*)a.h_out + r * a.ldh * es;
+        if (a.norm_out) b.norm_out = (uint8_t*)a.norm_out + r * a.n * es;
+        const hipError_t e = launch_rows(b, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace ascq

@@ -17,6 +17,7 @@ struct Launch {
     std::string kernel;  // mangled
     dim3 grid, block;
     uint8_t bytes[256];
+    int64_t second;  // the second argument's first bytes, when there is one
     template <class T>
     T args() const
     {
@@ -48,6 +49,11 @@ inline size_t& first_argument()
     return n;
 }
 
+inline size_t& second_argument()
+{
+    static size_t n = 0;
+    return n;
+}
 inline Launch& configured()
 {
     static Launch l{};
@@ -80,6 +86,7 @@ hipError_t hipLaunchKernel(const void* host, dim3 grid, dim3 block, void** args,
     l.grid = grid;
     l.block = block;
     std::memcpy(l.bytes, args[0], first_argument() < sizeof(l.bytes) ? first_argument() : sizeof(l.bytes));
+    if (second_argument()) std::memcpy(&l.second, args[1], second_argument());
     launches().push_back(l);
     return hipSuccess;
 }

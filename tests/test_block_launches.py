@@ -25,3 +25,8 @@ def _run(tmp_path, name):
 def test_rows_past_k_are_past_the_range(tmp_path):
     """w [K, N] of large row pitches: what the tiles read past K is nothing of w"""
     _run(tmp_path, "linear_pitches")
+
+
+def test_norm_of_very_many_rows(tmp_path):
+    """up to 2^31 rows: every row once, no grid of 2^32 threads"""
+    _run(tmp_path, "norm_rows")

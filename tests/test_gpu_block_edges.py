@@ -224,3 +224,15 @@ def test_linear_over_rows_far_apart(ascq_gpu, k, pitch):
     xf, wf = torch.full((m, 32), float("nan"), device="cuda").to(f8)[:, :k], raw.float().to(f8).as_strided((k, n), (pitch, 1))
     xf.copy_(x.float().to(f8))
     assert torch.equal(a.quant_linear(xf, ones[:m], wf, ones[:n], w_trans=False, out_dtype=torch.float32), want)
+
+
+def test_norm_of_very_many_rows(ascq_gpu):
+    """more rows than a grid has room for: each as its like among the first (equal bits)"""
+    a = ascq_gpu
+    m, n, every = (1 << 26) + 5, 8, 1 << 16
+    x = torch.randn(every, n, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").half()
+    gamma = torch.linspace(0.5, 1.5, n, device="cuda").half()
+    q, s, _ = a.add_rms_norm_quant(x, gamma)
+    wide, ws, _ = a.add_rms_norm_quant(x.repeat((m + every - 1) // every, 1)[:m], gamma)
+    assert torch.equal(wide[:-5].view(-1, every, n), q.expand(m // every, -1, -1)) and torch.equal(wide[-5:], q[:5])
+    assert torch.equal(ws[:-5].view(-1, every), s.expand(m // every, -1)) and torch.equal(ws[-5:], s[:5])
