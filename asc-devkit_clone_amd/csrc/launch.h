@@ -334,6 +334,7 @@ struct MoeRowsArgs {
     const float* weights;
     int type, k;
     int64_t T, n, row_bytes, ldx;
+    int64_t first;          // (set by the launcher) the launch's first token (combine_grad: item)
 };
 hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st);
 hipError_t launch_moe_combine(const MoeRowsArgs& a, hipStream_t st);

@@ -578,7 +578,7 @@ __device__ __forceinline__ int64_t wave_of() { return (int64_t)blockIdx.x * 4 + 
 template <bool ANY>
 __global__ __launch_bounds__(256) void moe_dispatch_kernel(MoeRowsArgs a, int waves)
 {
-    const int64_t w = wave_of(), t = w / waves, words = a.row_bytes / 16;
+    const int64_t w = wave_of(), t = a.first + w / waves, words = a.row_bytes / 16;
     if (t >= a.T) return;
     const int c0 = (int)(w % waves) * 64, lane = threadIdx.x & 63;
     const int rest = ANY ? (int)(a.row_bytes % 16) : 0;
@@ -630,7 +630,7 @@ template <int T, bool ANY>
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeRowsArgs a, int waves)
 {
     constexpr int ES = T == DT_F32 ? 4 : 2;
-    const int64_t w = wave_of(), t = w / waves, pitch = a.n * ES;
+    const int64_t w = wave_of(), t = a.first + w / waves, pitch = a.n * ES;
     if (t >= a.T) return;
     for (int64_t u = w % waves * 64 + (threadIdx.x & 63); u * 8 < a.n; u += waves * 64) {
         const int count = ANY && a.n - u * 8 < 8 ? (int)(a.n - u * 8) : 8;
@@ -673,7 +673,7 @@ __global__ __launch_bounds__(256) void moe_combine_grad_kernel(MoeRowsArgs a, in
     constexpr int ES = T == DT_F32 ? 4 : 2;
     __shared__ float red[4][4];
     const int groups = (a.k + per - 1) / per, lane = (int)threadIdx.x % (64 * W);
-    const int64_t item = wave_of() / W, pitch = a.n * ES;
+    const int64_t item = a.first + wave_of() / W, pitch = a.n * ES;
     const bool here = item < a.T * groups;  // (an item past the last does nothing, but meets the others)
     const int64_t t = here ? item / groups : 0;
     const int j0 = (int)(here ? item % groups : 0) * per, jn = here ? (a.k - j0 < per ? a.k - j0 : per) : 0;
@@ -805,8 +805,21 @@ namespace {
 template <int G, int V>
 hipError_t launch_grad(const MoeRouteGradArgs& a, hipStream_t st)
 {
-    launch_k((moe_route_grad_kernel<G, V>), dim3((unsigned)((a.T + 256 / G - 1) / (256 / G))), dim3(256), 0u, st, a);
-    return hipGetLastError();
+    constexpr int64_t TOKENS = (1ll << 31) / G;  // of a launch: a grid has fewer than 2^32 threads
+    const int64_t es = a.type == DT_F32 ? 4 : 2;
+    for (int64_t t = 0; t < a.T; t += TOKENS) {
+        MoeRouteGradArgs b = a;
+        b.T = a.T - t < TOKENS ? a.T - t : TOKENS;
+        b.grad_logits = (uint8_t*)a.grad_logits + t * a.ld_grad * es;
+        b.logits = (const uint8_t*)a.logits + t * a.ld * es;
+        if (a.weights) b.weights += t * a.k;
+        if (a.experts) b.experts += t * a.k;
+        if (a.grad_weights) b.grad_weights += t * a.k;
+        launch_k((moe_route_grad_kernel<G, V>), dim3((unsigned)((b.T + 256 / G - 1) / (256 / G))), dim3(256), 0u, st, b);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 }  // namespace
 
@@ -831,6 +844,19 @@ int row_waves(int64_t T, int64_t units)
     return (int)(all < 1 ? 1 : all < most ? all : most > 1 ? most : 1);
 }
 
+// A grid has fewer than 2^32 threads: launches of up to 2^25 items (tokens; as many have a wave each).  f(args, how many)
+template <class F>
+hipError_t in_pieces(const MoeRowsArgs& a, int64_t items, F f)
+{
+    constexpr int64_t MOST = 1 << 25;
+    MoeRowsArgs b = a;
+    for (b.first = 0; b.first < items; b.first += MOST) {
+        const hipError_t e = f(b, items - b.first < MOST ? items - b.first : MOST);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 // rows of whole 16-byte words (f32: of 8 elements), all of them aligned
 bool rows_aligned(const MoeRowsArgs& a)
 {
@@ -852,37 +878,42 @@ hipError_t with_row_kernel(const MoeRowsArgs& a, F f)
 }
 }  // namespace
 
-hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st)
+hipError_t launch_moe_dispatch(const MoeRowsArgs& in, hipStream_t st)
 {
-    const uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.ldx | (uintptr_t)a.row_bytes;
-    const int waves = row_waves(a.T, a.row_bytes / 16);
-    const dim3 grid((unsigned)((a.T * waves + 3) / 4)), block(256);
-    if (bits % 16 == 0) launch_k(moe_dispatch_kernel<false>, grid, block, 0u, st, a, waves);
-    else launch_k(moe_dispatch_kernel<true>, grid, block, 0u, st, a, waves);
-    return hipGetLastError();
-}
-
-hipError_t launch_moe_combine(const MoeRowsArgs& a, hipStream_t st)
-{
-    const int waves = row_waves(a.T, (a.n + 7) / 8);
-    return with_row_kernel(a, [&](auto type, auto any) {
-        launch_k((moe_combine_kernel<decltype(type)::value, decltype(any)::value>), dim3((unsigned)((a.T * waves + 3) / 4)),
-                 dim3(256), 0u, st, a, waves);
+    const uintptr_t bits = (uintptr_t)in.x | (uintptr_t)in.out | (uintptr_t)in.ldx | (uintptr_t)in.row_bytes;
+    const int waves = row_waves(in.T, in.row_bytes / 16);  // (T > 2^20: 1)
+    return in_pieces(in, in.T, [&](const MoeRowsArgs& a, int64_t tokens) {
+        const dim3 grid((unsigned)((tokens * waves + 3) / 4)), block(256);
+        if (bits % 16 == 0) launch_k(moe_dispatch_kernel<false>, grid, block, 0u, st, a, waves);
+        else launch_k(moe_dispatch_kernel<true>, grid, block, 0u, st, a, waves);
+        return hipGetLastError();
     });
 }
 
-hipError_t launch_moe_combine_grad(const MoeRowsArgs& a, hipStream_t st)
+hipError_t launch_moe_combine(const MoeRowsArgs& in, hipStream_t st)
 {
-    const int per = a.T * a.k <= 1024 ? 1 : 4;  // (808 rows: alike)
-    const int64_t items = a.T * ((a.k + per - 1) / per);
-    return with_row_kernel(a, [&](auto type, auto any) {
-        constexpr int T = decltype(type)::value;
-        constexpr bool ANY = decltype(any)::value;
-        // (a grid has fewer than 2^32 threads)
-        if (a.n < 2048 || items >= 1 << 24)
-            launch_k((moe_combine_grad_kernel<T, ANY, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0u, st, a, per);
-        else
-            launch_k((moe_combine_grad_kernel<T, ANY, 4>), dim3((unsigned)items), dim3(256), 0u, st, a, per);
+    const int waves = row_waves(in.T, (in.n + 7) / 8);
+    return in_pieces(in, in.T, [&](const MoeRowsArgs& a, int64_t tokens) {
+        return with_row_kernel(a, [&](auto type, auto any) {
+            launch_k((moe_combine_kernel<decltype(type)::value, decltype(any)::value>), dim3((unsigned)((tokens * waves + 3) / 4)),
+                     dim3(256), 0u, st, a, waves);
+        });
+    });
+}
+
+hipError_t launch_moe_combine_grad(const MoeRowsArgs& in, hipStream_t st)
+{
+    const int per = in.T * in.k <= 1024 ? 1 : 4;  // (808 rows: alike)
+    const int64_t all = in.T * ((in.k + per - 1) / per);
+    return in_pieces(in, all, [&](const MoeRowsArgs& a, int64_t items) {
+        return with_row_kernel(a, [&](auto type, auto any) {
+            constexpr int T = decltype(type)::value;
+            constexpr bool ANY = decltype(any)::value;
+            if (a.n < 2048 || all >= 1 << 24)  // (four waves each: within a grid)
+                launch_k((moe_combine_grad_kernel<T, ANY, 1>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0u, st, a, per);
+            else
+                launch_k((moe_combine_grad_kernel<T, ANY, 4>), dim3((unsigned)items), dim3(256), 0u, st, a, per);
+        });
     });
 }
 

@@ -30,3 +30,8 @@ def test_rows_past_k_are_past_the_range(tmp_path):
 def test_norm_of_very_many_rows(tmp_path):
     """up to 2^31 rows: every row once, no grid of 2^32 threads"""
     _run(tmp_path, "norm_rows")
+
+
+def test_routing_and_rows_of_very_many_tokens(tmp_path):
+    """up to 2^31 rows: every token once, no grid of 2^32 threads"""
+    _run(tmp_path, "moe_tokens")

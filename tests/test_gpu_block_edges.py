@@ -236,3 +236,43 @@ def test_norm_of_very_many_rows(ascq_gpu):
     wide, ws, _ = a.add_rms_norm_quant(x.repeat((m + every - 1) // every, 1)[:m], gamma)
     assert torch.equal(wide[:-5].view(-1, every, n), q.expand(m // every, -1, -1)) and torch.equal(wide[-5:], q[:5])
     assert torch.equal(ws[:-5].view(-1, every), s.expand(m // every, -1)) and torch.equal(ws[-5:], s[:5])
+
+
+def test_rows_of_very_many_tokens(ascq_gpu):
+    """more tokens than a grid has room for: rows moved to the reverse order and back, and their gradients (equal bits: weights 1
+    and 2, one choice)"""
+    a = ascq_gpu
+    t, n = (1 << 26) + 5, 8
+    slots = torch.arange(t - 1, -1, -1, dtype=torch.int32, device="cuda").view(t, 1)
+    x = torch.randint(-100, 100, (t, n), dtype=torch.int8, device="cuda")
+    rows, _ = a.moe_dispatch(x, None, slots, slots.view(t))
+    assert torch.equal(rows, x.flip(0))
+    y = rows.half()
+    del rows
+    out = a.moe_combine(y, slots, torch.ones(t, 1, device="cuda"))
+    assert torch.equal(out, x.half())
+    two = torch.full((t, 1), 2.0, device="cuda")
+    dw, dy = a.moe_combine_grad(out, y, slots, slots.view(t), two)
+    assert torch.equal(dy, y * 2)
+    assert torch.equal(dw.view(t), (x.float() ** 2).sum(dim=1))
+
+
+def test_route_gradient_of_very_many_tokens(ascq_gpu):
+    """more tokens than a grid of 64 lanes each has room for: each token as its like among the first (equal bits)"""
+    a = ascq_gpu
+    every, e = 1 << 16, 300
+    x = torch.randn(every, e, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").half()
+    r = a.moe_route(x, 1)
+    ones = torch.ones(every, 1, device="cuda")
+    args = dict(grad_loss=torch.full((1,), 64.0, device="cuda"), renormalize=False)
+    want = a.moe_route_grad(x, r.weights, r.experts, r.counts, r.routed, grad_weights=ones, **args)
+    t = (1 << 26) + 5  # (64 lanes a token)
+    more = (t + every - 1) // every
+    wide = x.repeat(more, 1)[:t]
+    got = a.moe_route_grad(wide, r.weights.repeat(more, 1)[:t], r.experts.repeat(more, 1)[:t], r.counts, r.routed,
+                           grad_weights=ones.repeat(more, 1)[:t], out=wide, **args)
+    assert got is wide
+    for at in range(0, t - every, every * 64):
+        part = got[at:at + every * 64]
+        assert torch.equal(part, want.repeat(64, 1)[:part.shape[0]])
+    assert torch.equal(got[-5:], want[:5])
