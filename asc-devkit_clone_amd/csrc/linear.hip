@@ -25,13 +25,13 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t* src, int64_t n, bool 
 // weight turned on the way.  It takes what nothing else does: K = 0, operands off their alignment without a workspace (1030 x
 // 4100 x 4095 int8: 995 us against 38 with one), and a w [K, N] past 2^31 bytes or of few rows that are very far apart.
 template <bool F8>
-__global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a)
+__global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t first)
 {
     constexpr int P = 80;  // bytes of a row in LDS: 64, and 16 that spread the rows over the banks
     __shared__ __attribute__((aligned(16))) uint8_t sx[64 * P], sw[64 * P];
     typedef typename std::conditional<F8, v4f, v4i>::type acc_t;
     const int64_t tiles_n = (a.N + 63) / 64;
-    const int64_t m0 = (int64_t)blockIdx.x / tiles_n * 64, n0 = (int64_t)blockIdx.x % tiles_n * 64;
+    const int64_t tile = first + blockIdx.x, m0 = tile / tiles_n * 64, n0 = tile % tiles_n * 64;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
     const int r = t >> 2, c = (t & 3) * 16;
     const bool ax = ((uintptr_t)a.x | (uintptr_t)a.ldx) % 16 == 0, aw = ((uintptr_t)a.w | (uintptr_t)a.ldw) % 16 == 0;
@@ -131,10 +131,16 @@ bool too_large(const LinearArgs& a)
 hipError_t launch_any(const LinearArgs& a, const char* why, hipStream_t st)
 {
     log_fallback("linear_any_kernel", why);
-    const dim3 grid((unsigned)(((a.M + 63) / 64) * ((a.N + 63) / 64)));
-    if (a.f8) launch_k(linear_any_kernel<true>, grid, dim3(256), 0u, st, a);
-    else launch_k(linear_any_kernel<false>, grid, dim3(256), 0u, st, a);
-    return hipGetLastError();
+    constexpr int64_t MOST = 1 << 23;  // tiles of a launch: a grid has fewer than 2^32 threads
+    const int64_t tiles = ((a.M + 63) / 64) * ((a.N + 63) / 64);
+    for (int64_t at = 0; at < tiles; at += MOST) {
+        const dim3 grid((unsigned)(tiles - at < MOST ? tiles - at : MOST));
+        if (a.f8) launch_k(linear_any_kernel<true>, grid, dim3(256), 0u, st, a, at);
+        else launch_k(linear_any_kernel<false>, grid, dim3(256), 0u, st, a, at);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace

@@ -35,3 +35,8 @@ def test_norm_of_very_many_rows(tmp_path):
 def test_routing_and_rows_of_very_many_tokens(tmp_path):
     """up to 2^31 rows: every token once, no grid of 2^32 threads"""
     _run(tmp_path, "moe_tokens")
+
+
+def test_linear_of_very_many_tiles(tmp_path):
+    """outputs of more tiles than a grid has room for"""
+    _run(tmp_path, "linear_grids")

@@ -276,3 +276,14 @@ def test_route_gradient_of_very_many_tokens(ascq_gpu):
         part = got[at:at + every * 64]
         assert torch.equal(part, want.repeat(64, 1)[:part.shape[0]])
     assert torch.equal(got[-5:], want[:5])
+
+
+def test_linear_of_very_many_tiles(ascq_gpu):
+    """more output tiles than a grid has room for (k = 0: the bias and the residual, exact)"""
+    a = ascq_gpu
+    m = (1 << 30) + 70
+    r = torch.arange(1024, device="cuda").half().repeat(m // 1024 + 1)[:m].view(m, 1)
+    got = a.quant_linear(torch.empty(m, 0, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda"),
+                         torch.empty(1, 0, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"),
+                         bias=torch.full((1,), 0.5, device="cuda"), residual=r, out_dtype=torch.float16)
+    assert torch.equal(got, r + 0.5)
