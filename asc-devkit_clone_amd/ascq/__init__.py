@@ -616,6 +616,10 @@ def add_rms_norm_quant(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-6, 
     s = scale_out if scale_out is not None else _new(stream, (m,), torch.float32, x.device)
     _dense(what, "scale_out", s, (m,), torch.float32)
     _same_device(what, x, gamma, residual, h, norm_out, q, s)
+    if n == 0 and m > 0:  # (the library writes nothing; a row without elements is a row of zeros)
+        with torch.cuda.stream(torch.cuda.ExternalStream(_stream(stream), x.device)):
+            s.zero_()
+        return q, s, h
     p = _NormQuantParam(m, n, ldx, ldr, ldh, src_type, dst_type, eps)
     check(lib().ascq_add_rms_norm_quant(_at(q), _at(s), _at(h) if residual is not None else None, _at(norm_out), _at(x),
                                         _at(residual), _at(gamma), ctypes.byref(p), _stream(stream)), what)

@@ -1900,8 +1900,8 @@ ascq_status ascq_moe_dispatch(void* rows, float* row_scale, const void* x, const
     if (!addressable(p->tokens, ldx)) return fail(ASCQ_E_UNSUPPORTED, "moe_dispatch: tensor too large");
     if ((row_scale == nullptr) != (x_scale == nullptr))
         return fail(ASCQ_E_INVALID_ARG, "moe_dispatch: row_scale and x_scale go together");
-    if (p->tokens == 0 || p->n == 0) return ASCQ_OK;
-    if (!rows || !x || !slots || !row_tokens) return fail(ASCQ_E_INVALID_ARG, "moe_dispatch: null argument");
+    if (p->tokens == 0 || (p->n == 0 && !row_scale)) return ASCQ_OK;  // (empty rows have scales)
+    if ((p->n > 0 && (!rows || !x)) || !slots || !row_tokens) return fail(ASCQ_E_INVALID_ARG, "moe_dispatch: null argument");
     const size_t es = float_type(p->type) ? float_bytes(p->type) : 1;
     if (!aligned(rows, es) || !aligned(x, es) || !aligned(row_scale, 4) || !aligned(x_scale, 4) || !aligned(slots, 4) ||
         !aligned(row_tokens, 4))

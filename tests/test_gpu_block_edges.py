@@ -287,3 +287,27 @@ def test_linear_of_very_many_tiles(ascq_gpu):
                          torch.empty(1, 0, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"),
                          bias=torch.full((1,), 0.5, device="cuda"), residual=r, out_dtype=torch.float16)
     assert torch.equal(got, r + 0.5)
+
+
+def test_rows_without_elements(ascq_gpu):
+    """rows of no elements: the norm's scales are those of a row of zeros, the dispatch moves scales alone, the combine's weight
+    gradients are sums of nothing"""
+    a = ascq_gpu
+    side = torch.cuda.Stream()
+    for st in (None, side, side.cuda_stream):
+        x = torch.empty(5, 0, dtype=torch.float16, device="cuda")
+        full = torch.full((5,), 9.0, device="cuda")
+        torch.cuda.synchronize()
+        q, s, h = a.add_rms_norm_quant(x, torch.empty(0, dtype=torch.float16, device="cuda"), residual=x, scale_out=full, stream=st)
+        torch.cuda.synchronize()
+        assert s is full and torch.all(s == 0) and q.shape == (5, 0) and h.shape == (5, 0)
+    tokens = torch.tensor([1, 0, 2, 2, -1, -1], dtype=torch.int32, device="cuda")
+    slots = torch.tensor([[1, -1], [0, -1], [2, 3]], dtype=torch.int32, device="cuda")
+    scale, got = torch.tensor([1.0, 2.0, 3.0], device="cuda"), torch.full((6,), 9.0, device="cuda")
+    for dt in (torch.int8, torch.float16):
+        rows, got = a.moe_dispatch(torch.empty(3, 0, dtype=dt, device="cuda"), scale, slots, tokens, scale_out=got.fill_(9.0))
+        assert got.tolist() == [2.0, 1.0, 3.0, 3.0, 0.0, 0.0] and rows.shape == (6, 0)
+    y, w = torch.empty(6, 0, device="cuda"), torch.ones(3, 2, device="cuda")
+    dw, dy = a.moe_combine_grad(torch.empty(3, 0, device="cuda"), y, slots, tokens, w, out=torch.full((3, 2), 9.0, device="cuda"))
+    assert torch.all(dw == 0) and dy.shape == (6, 0)
+    assert a.moe_combine(y, slots, w).shape == (3, 0)
