@@ -41,8 +41,7 @@ __device__ __forceinline__ RowScale row_scale(float ss, uint32_t top, float inv_
     }
     const float a = __uint_as_float(top);
     r.rstd = top ? 1.0f / sqrtf(ss * inv_n + eps) : 0.0f;
-    // (it passes fp32's range below a = 1.3e-36, where t times the largest number still is at most Q)
-    r.mult = top ? fminf(q_max * (1.0f / a), 3.402823466e38f) : 0.0f;
+    r.mult = top ? q_max * (1.0f / a) : 0.0f;
     r.scale = a * r.rstd / q_max;
     return r;
 }
@@ -60,6 +59,7 @@ __device__ __forceinline__ void block_reduce(float& ss, uint32_t& top)
         top = other > top ? other : top;
     }
     const int wave = threadIdx.x >> 6;
+    __syncthreads();  // (the row before, or this one's first sums, have been read)
     if ((threadIdx.x & 63) == 0) {
         s_sum[wave] = ss;
         s_top[wave] = top;
@@ -72,6 +72,63 @@ __device__ __forceinline__ void block_reduce(float& ss, uint32_t& top)
         ss += s_sum[w];
         top = s_top[w] > top ? s_top[w] : top;
     }
+}
+
+// Rows whose products t lie below 2^-100 (1 / a and the scale would leave fp32's range), or whose mean square does (squares
+// would: only with an eps as small), are done here from memory, with products times 2^100, h times 2^90, or both; the powers go
+// back into the scale and the norm.  (A row whose products all are 0 in fp32 is an ordinary row of zeros.)  Each thread has the RUN-element pieces threadIdx.x, threadIdx.x + NT, ..., as when it
+// stored h.
+enum : int { SMALL_T = 1, SMALL_H = 2 };
+__device__ __forceinline__ int small_powers(float ss, uint32_t top, float inv_n, float eps)
+{
+    const int p = top == 0 ? 0 : (top < 0x0d800000u ? SMALL_T : 0) | (ss * inv_n + eps < 0x1p-100f ? SMALL_H : 0);  // (2^-100)
+    return __builtin_amdgcn_readfirstlane(p);
+}
+template <int NT, int RUN>
+__device__ __forceinline__ void finish_small_row(const NormQuantArgs& a, int dt, int64_t row, int small, float inv_n)
+{
+    const bool small_t = small & SMALL_T, small_h = small & SMALL_H;
+    auto each = [&](auto f) {
+#pragma unroll 1
+        for (int64_t c = threadIdx.x; c * RUN < a.n; c += NT)
+#pragma unroll 1
+            for (int64_t i = c * RUN; i < c * RUN + RUN && i < a.n; ++i) {
+                float h;
+                if (a.h_out) h = load_f32_of(a.h_out, row * a.ldh + i, dt);  // (x or the residual may be gone)
+                else {
+                    h = load_f32_of(a.x, row * a.ldx + i, dt);
+                    if (a.residual) h = round_to(h + load_f32_of(a.residual, row * a.ldr + i, dt), dt);
+                }
+                const float g = load_f32_of(a.gamma, i, dt);
+                const float k = small_h ? h * 0x1p90f : h;
+                // (no factor overflows: |h g| < 2^-100)
+                f(i, k, !small_t ? h * g : __builtin_fabsf(g) < 1.0f ? k * (g * 0x1p100f) : k * 0x1p100f * g);
+            }
+    };
+    float ss = 0.0f;
+    uint32_t top = 0;
+    each([&](int64_t, float h, float t) {
+        ss = fmaf(h, h, ss);
+        const uint32_t b = __float_as_uint(t) & 0x7fffffffu;
+        top = b > top ? b : top;
+    });
+    block_reduce<NT / 64>(ss, top);
+    const bool int8 = a.dst_type == DT_INT8;
+    const float q_max = int8 ? 127.0f : 448.0f;
+    const RowScale s = row_scale(ss, top, inv_n, small_h ? a.eps * 0x1p90f * 0x1p90f : a.eps, q_max);
+    // t rstd in an order that leaves fp32's range only if the result does
+    const float power = small_t ? 0x1p-100f : 0x1p90f;
+    auto normed = [&](float t) {
+        return (__builtin_fabsf(t) < 1.0f) == (power > 1.0f) ? t * power * s.rstd : t * s.rstd * power;
+    };
+    const float scale = normed(__uint_as_float(top)) / q_max;
+    if (threadIdx.x == 0) a.scale_out[row] = scale;
+    each([&](int64_t i, float, float t) {
+        const float v = scale > 0.0f ? t * s.mult : 0.0f;
+        if (int8) ((int8_t*)a.q)[row * a.n + i] = (int8_t)quant_s8<RM_RINT>(v);
+        else ((uint8_t*)a.q)[row * a.n + i] = f32_to_fp8(v, 0);
+        if (a.norm_out) store_keep_inf(a.norm_out, row * a.n + i, normed(t), dt);
+    });
 }
 
 // 16 (8) bytes at any element's (byte's) address: the memory pipeline takes wide accesses of any alignment
@@ -172,8 +229,10 @@ __device__ __forceinline__ u32x2 codes8(const float (&v)[8], bool int8)
 // and the codes, so every byte moves once.  All loads of a thread are issued in front of its first wait: units past the
 // row read its last whole one and are dropped (in place, another thread may have stored it by then).
 // ANY: rows that start at any element, whose last unit may be a part of one.
+// (bf16, 1024 threads of four 16-byte words: in 64 registers, which are two workgroups per CU.  2048 x 32768 with residual 81 us,
+// in the 68 that it takes by itself 88)
 template <int T, int NT, int U, bool RES, bool ANY>
-__global__ __launch_bounds__(NT) void norm_quant_row_kernel(NormQuantArgs a)
+__global__ __launch_bounds__(NT, T != DT_F16 && NT == 1024 && U * Unit<T>::W <= 4 ? 8 : 1) void norm_quant_row_kernel(NormQuantArgs a)
 {
     const int64_t row = blockIdx.x;
     const uint32_t whole = (uint32_t)(a.n / 8), units = ANY ? (uint32_t)((a.n + 7) / 8) : whole;
@@ -233,8 +292,10 @@ __global__ __launch_bounds__(NT) void norm_quant_row_kernel(NormQuantArgs a)
         }
     }
     block_reduce<NT / 64>(ss, top);
+    const float inv_n = 1.0f / (float)a.n;
+    const int small = T == DT_F16 ? 0 : small_powers(ss, top, inv_n, a.eps);
     const bool int8 = a.dst_type == DT_INT8;
-    const RowScale s = row_scale(ss, top, 1.0f / (float)a.n, a.eps, int8 ? 127.0f : 448.0f);
+    const RowScale s = row_scale(ss, top, inv_n, a.eps, int8 ? 127.0f : 448.0f);
     if (threadIdx.x == 0) a.scale_out[row] = s.scale;
     uint8_t* q = (uint8_t*)a.q + row * a.n;
 #pragma unroll
@@ -267,6 +328,10 @@ __global__ __launch_bounds__(NT) void norm_quant_row_kernel(NormQuantArgs a)
             else o.store_part(to, c, part);
         }
     }
+    // (over what was stored above, and behind it, where the row's registers are free: in front, they cost 9 % to 24 % of long rows)
+    // (f16 has no such rows: its smallest number's square is 2^-48)
+    if constexpr (T != DT_F16)
+        if (__builtin_expect(small, 0)) finish_small_row<NT, 8>(a, T, row, small, inv_n);
 }
 
 // Rows too long for registers: one workgroup per row, element by element, the row read twice (the second time from the
@@ -289,7 +354,9 @@ __global__ __launch_bounds__(256) void norm_quant_any_kernel(NormQuantArgs a)
         top = t > top ? t : top;
     }
     block_reduce<4>(ss, top);
-    const RowScale r = row_scale(ss, top, 1.0f / (float)a.n, a.eps, a.dst_type == DT_INT8 ? 127.0f : 448.0f);
+    const float inv_n = 1.0f / (float)a.n;
+    if (const int small = small_powers(ss, top, inv_n, a.eps)) return finish_small_row<256, 1>(a, dt, row, small, inv_n);
+    const RowScale r = row_scale(ss, top, inv_n, a.eps, a.dst_type == DT_INT8 ? 127.0f : 448.0f);
     if (threadIdx.x == 0) a.scale_out[row] = r.scale;
     for (int64_t c = threadIdx.x; c < a.n; c += 256) {
         const float h = a.h_out ? load_f32_of(a.h_out, row * a.ldh + c, dt) : first(c);

@@ -587,8 +587,9 @@ typedef struct {
  *   q_c = rint(t_c (Q (1 / a))),  scale[row] = a rstd / Q, so that q scale is the norm h rstd gamma
  *   norm_out (optional): rnd(t_c rstd), the unquantised norm.
  * q and norm_out are dense [m, n].  h_out may be x or residual itself (with its stride); it needs a residual.  A row of
- * zeros gives codes and scale 0.  A row with a NaN or an infinity in h or t, or whose sum of squares passes fp32's range,
- * gives codes 0 and scale (and norm_out) NaN.  eps >= 0.  n = 0: nothing is written. */
+ * zeros (products t that all are 0 in fp32) gives codes and scale 0; smaller ones than fp32 has reciprocals or squares of are
+ * as exact as others.  A row with a NaN or an infinity in h or t, or whose sum of squares passes fp32's range, gives codes 0
+ * and scale (and norm_out) NaN.  eps >= 0.  n = 0: nothing is written. */
 ascq_status ascq_add_rms_norm_quant(void* q, float* scale, void* h_out, void* norm_out, const void* x,
                                     const void* residual, const void* gamma, const ascq_norm_quant_param* p,
                                     void* stream);

@@ -311,3 +311,52 @@ def test_rows_without_elements(ascq_gpu):
     dw, dy = a.moe_combine_grad(torch.empty(3, 0, device="cuda"), y, slots, tokens, w, out=torch.full((3, 2), 9.0, device="cuda"))
     assert torch.all(dw == 0) and dy.shape == (6, 0)
     assert a.moe_combine(y, slots, w).shape == (3, 0)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-5])
+@pytest.mark.parametrize("dt,n", [("f32", 64), ("f32", 513), ("f32", 4096), ("f32", 70000), ("bf16", 96), ("bf16", 4100),
+                                  ("bf16", 70000), ("f16", 640)])
+def test_norm_of_tiny_rows(ascq_gpu, dt, n, eps, codes):
+    """Rows, gammas and products far below 1, down to subnormal numbers: codes times scale is the norm of the definition in 64
+    bits, as for ordinary rows, also where the squares or the products' reciprocal leave fp32's range.  Bounds of
+    test_gpu_norm.py (the products' powers of two are exact, so the same roundings are taken), and a scale or norm that is
+    subnormal itself is off by a unit of it."""
+    from test_gpu_norm import DT, ULP, _check
+
+    a = ascq_gpu
+    g = torch.Generator().manual_seed(n)
+    low = {"f32": 2.0 ** -149, "bf16": 2.0 ** -133, "f16": 2.0 ** -24}[dt]
+    size = [1.0, 1e-12, 1e-16, 1e-19, 1e-22, 1e-30, 1e-36, 1e-38, 3e-39, 20 * low]
+    if dt == "f16":
+        size = [1.0, 1e-3, 1e-5, 1e-6, 20 * low]
+    rows = torch.tensor(size, dtype=torch.float64)[:, None]
+    x = (torch.randn(len(size), n, generator=g, dtype=torch.float64) * rows).to(DT[dt])
+    r = (torch.randn(len(size), n, generator=g, dtype=torch.float64) * rows).to(DT[dt])
+    x[0, 1:] = r[0] = 0  # one number, and zeros
+    code = a.INT8 if codes == "int8" else a.FP8_E4M3
+    for power in (0, -10, -60, -90, -120, 40):
+        if dt == "f16" and power not in (0, -10):
+            continue
+        gamma = ((torch.rand(n, generator=g) + 0.5) * 2.0 ** power).to(DT[dt])
+        gamma[3] = 0
+        for residual in (None, r):
+            norm = torch.empty(x.shape, dtype=DT[dt], device="cuda")
+            into = x.cuda()
+            q, s, h = a.add_rms_norm_quant(into, gamma.cuda(), eps, code, residual=None if residual is None else r.cuda(),
+                                           residual_out=None if residual is None else into, norm_out=norm)
+            h, s, norm = h.cpu(), s.cpu(), norm.cpu()
+            t = h.double() * gamma.double()
+            rstd = 1 / torch.sqrt((h.double() ** 2).mean(dim=1) + eps)
+            # (products below half of fp32's smallest number are 0; a scale that rounds to 0 leaves codes of 0)
+            none = t.abs().amax(dim=1) < 2.0 ** -150
+            keep = (t.abs().amax(dim=1) * rstd / (127 if codes == "int8" else 448) > 2.0 ** -148) & ~none
+            assert torch.all(s[none] == 0) and torch.all(q.cpu()[none].float() == 0) and torch.all(norm[none] == 0)
+            assert keep.any()
+            _check(x[keep], gamma, None if residual is None else r[keep], codes, q.cpu()[keep], s[keep], h[keep], eps=eps)
+            assert torch.isfinite(s).all() and torch.all(q.float().abs() <= (127 if codes == "int8" else 448))
+            assert torch.all(s[~keep] <= 2.0 ** -147)
+            want = torch.where((t == 0) | none[:, None], 0.0, t * rstd[:, None])
+            near = want.abs() < torch.finfo(DT[dt]).max / 2
+            bound = (ULP[dt] + (n / 256 + 40) * 2.0 ** -24) * want.abs() + low
+            assert torch.all(((norm.double() - want).abs() <= bound) | ~near)
