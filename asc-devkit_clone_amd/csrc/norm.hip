@@ -76,8 +76,8 @@ __device__ __forceinline__ void block_reduce(float& ss, uint32_t& top)
 
 // Rows whose products t lie below 2^-100 (1 / a and the scale would leave fp32's range), or whose mean square does (squares
 // would: only with an eps as small), are done here from memory, with products times 2^100, h times 2^90, or both; the powers go
-// back into the scale and the norm.  (A row whose products all are 0 in fp32 is an ordinary row of zeros.)  Each thread has the RUN-element pieces threadIdx.x, threadIdx.x + NT, ..., as when it
-// stored h.
+// back into the scale and the norm.  (A row whose products all are 0 in fp32 is an ordinary row of zeros.)  Each thread has the
+// RUN-element pieces threadIdx.x, threadIdx.x + NT, ..., as when it stored h.
 enum : int { SMALL_T = 1, SMALL_H = 2 };
 __device__ __forceinline__ int small_powers(float ss, uint32_t top, float inv_n, float eps)
 {
@@ -328,8 +328,8 @@ __global__ __launch_bounds__(NT, T != DT_F16 && NT == 1024 && U * Unit<T>::W <= 
             else o.store_part(to, c, part);
         }
     }
-    // (over what was stored above, and behind it, where the row's registers are free: in front, they cost 9 % to 24 % of long rows)
-    // (f16 has no such rows: its smallest number's square is 2^-48)
+    // over what was stored above, and behind it, where the row's registers are free (in front: long rows 9 % to 24 % slower).  f16
+    // has no such rows: its smallest number's square is 2^-48.
     if constexpr (T != DT_F16)
         if (__builtin_expect(small, 0)) finish_small_row<NT, 8>(a, T, row, small, inv_n);
 }

@@ -580,7 +580,7 @@ typedef struct {
     float eps;
 } ascq_norm_quant_param;
 
-/* Residual addition, RMS norm and an 8-bit output with one scale per token, in one pass (no counterpart in the reference):
+/* Residual addition, RMS norm and an 8-bit output with one scale per token, in one pass:
  *   h = rnd(x + residual) (rounded to src_type: a finite fp32 sum saturates, an infinite one stays infinite; without
  *       residual h = x), stored to h_out when given
  *   t_c = h_c gamma_c,  rstd = 1 / sqrt(mean_c h_c^2 + eps),  a = max_c |t_c|,  Q = 127 (int8) or 448 (e4m3)
@@ -589,7 +589,7 @@ typedef struct {
  * q and norm_out are dense [m, n].  h_out may be x or residual itself (with its stride); it needs a residual.  A row of
  * zeros (products t that all are 0 in fp32) gives codes and scale 0; smaller ones than fp32 has reciprocals or squares of are
  * as exact as others.  A row with a NaN or an infinity in h or t, or whose sum of squares passes fp32's range, gives codes 0
- * and scale (and norm_out) NaN.  eps >= 0.  n = 0: nothing is written. */
+ * and scale (and norm_out) NaN.  eps >= 0.  n = 0: nothing is written.  (There is no counterpart in the reference.) */
 ascq_status ascq_add_rms_norm_quant(void* q, float* scale, void* h_out, void* norm_out, const void* x,
                                     const void* residual, const void* gamma, const ascq_norm_quant_param* p,
                                     void* stream);
@@ -603,11 +603,12 @@ typedef struct {
     int32_t activation;   /* ascq_activation */
 } ascq_linear_param;
 
-/* The quantised linear (no counterpart in the reference):
+/* The quantised linear:
  * y = cast(act((sum_k x[m, k] w[k, n]) w_scale[n] x_scale[m] + bias[n]) + residual[m, n]), fp32 in this order, one
  * rounding at the end (nearest even; in f16 and bf16 a finite value saturates, an infinite one stays infinite).  int8
  * sums are exact int32 (k below 2^17); fp8 sums are those of the fp8 Matmul.  x_scale f32 [m], w_scale f32 [n]; bias f32 [n]
- * or NULL; residual [m, n] or NULL (it may be y itself, with its stride).  k = 0 gives act(bias) + residual.
+ * or NULL; residual [m, n] or NULL (it may be y itself, with its stride).  k = 0 gives act(bias) + residual.  (There is
+ * no counterpart in the reference.)
  * workspace: optional, 16-byte aligned, ascq_quant_linear_workspace_size bytes (0 for many calls): room for the partial
  * sums of few rows and for operands whose rows are off 16 bytes; a call with less of it, or none, takes kernels that
  * need none and returns the same int8 results. */
