@@ -197,7 +197,7 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) key[i] = key_of(p[i]);
-            float top = 0.0f, inv = 0.0f;
+            float top = 0.0f, all = 1.0f, inv = 0.0f;
             for (int j = 0; j < k; ++j) {
                 // the largest logit left, then the lowest expert that has it; -1 when nothing is left that counts
                 uint32_t best = key[0], at = 0xffffffffu;
@@ -217,7 +217,8 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
                         sum += p[i];
                     }
                     sum = group_sum<G>(sum);
-                    inv = e >= 0 ? 1.0f / sum : 0.0f;
+                    all = e >= 0 ? sum : 1.0f;
+                    inv = e >= 0 ? 1.0f / sum : 0.0f;  // (of the loss's sums; a weight is divided)
                     live += e >= 0;
                 }
 #pragma unroll
@@ -233,13 +234,13 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
             float wsum = 0.0f;
             for (int j = tid % G; j < k; j += G) {
                 const int e = s_e[token * k + j];
-                const float q = e >= 0 ? expf(s_w[token * k + j] - top) * inv : 0.0f;
+                const float q = e >= 0 ? expf(s_w[token * k + j] - top) / all : 0.0f;
                 wsum += q;
                 s_w[token * k + j] = q;
                 if (e >= 0) atomicOr((unsigned long long*)&masks[e], 1ull << token);
             }
             wsum = group_sum<G>(wsum);
-            if (e0 == 0) s_f[token] = !a.renormalize ? 1.0f : (wsum > 0.0f ? 1.0f / wsum : 0.0f);
+            if (e0 == 0) s_f[token] = a.renormalize && wsum > 0.0f ? wsum : 1.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) psum[i] += p[i] * inv;
         }
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(route_threads<G>) void moe_route_kernel(MoeRouteArg
         for (int i = tid; i < n; i += NT) {
             const int e = s_e[i], tk = i / k;
             const int64_t at = c * C * k + i;
-            a.weights[at] = s_w[i] * s_f[tk];
+            a.weights[at] = s_w[i] / s_f[tk];
             a.experts[at] = e;
             const int rank = e < 0 ? -1 : first[e] + __popcll(masks[e] & ((1ull << tk) - 1ull));
             if constexpr (!SINGLE) a.slots[at] = rank;

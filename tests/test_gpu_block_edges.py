@@ -360,3 +360,21 @@ def test_norm_of_tiny_rows(ascq_gpu, dt, n, eps, codes):
             near = want.abs() < torch.finfo(DT[dt]).max / 2
             bound = (ULP[dt] + (n / 256 + 40) * 2.0 ** -24) * want.abs() + low
             assert torch.all(((norm.double() - want).abs() <= bound) | ~near)
+
+
+@pytest.mark.parametrize("t,e", [(9, 8), (64, 64), (3000, 64), (600, 256), (70, 1000)])
+def test_routing_weights_are_quotients(ascq_gpu, t, e):
+    """A weight is a quotient rounded once, not a product with a rounded reciprocal: one choice renormalised has the weight 1,
+    k equal ones 1 / k each, and of E equal logits any choice has 1 / E (powers of two: equal bits), whatever the logits are"""
+    a = ascq_gpu
+    x = (torch.randn(t, e, generator=torch.Generator().manual_seed(e)) * 3).cuda()
+    assert torch.all(a.moe_route(x, 1).weights == 1.0)
+    for k in (2, 4, 8):
+        # (the k largest alike, the others anything below: their share of the softmax leaves the renormalised weights)
+        y = x.clone()
+        y.scatter_(1, x.topk(k).indices, x.amax(dim=1, keepdim=True).expand(-1, k))
+        assert torch.all(a.moe_route(y, k).weights == 1.0 / k)
+    for n in (2, 3, 7, 8):
+        same = torch.randn(t, 1, generator=torch.Generator().manual_seed(n)).expand(t, n).contiguous().cuda()
+        one = torch.ones(1, device="cuda")
+        assert torch.all(a.moe_route(same, 1, renormalize=False).weights == one / n)
