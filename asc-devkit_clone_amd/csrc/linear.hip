@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t f
                 if (m >= a.M || n >= a.N) continue;
                 float v = (float)acc[i][j][e] * a.w_scale[n] * a.x_scale[m];
                 if (a.bias) v += a.bias[n];
-                v = activate(v, a.act);
+                v = a.out_type == DT_F32 ? activate<true>(v, a.act) : activate<false>(v, a.act);
                 if (a.residual) v += load_f32_of(a.residual, m * a.ldr + n, a.out_type);
                 store_keep_inf(a.y, m * a.ldy + n, v, a.out_type);
             }

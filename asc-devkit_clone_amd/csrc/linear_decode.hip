@@ -149,7 +149,7 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
                 continue;
             }
             float y = scaled(s) * s_ws[i * 16 + n] * s_xs[m] + s_b[i * 16 + n];
-            y = activate(y, p.act);
+            y = p.out_type == DT_F32 ? activate<true>(y, p.act) : activate<false>(y, p.act);
             if (p.residual) y += load_f32_of(p.residual, m * p.ldr + col, p.out_type);
             store_keep_inf(p.y, m * p.ldy + col, y, p.out_type);
         }
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void linear_slices_kernel(LinearArgs p)
         const int64_t c = e < count ? n + e : n;
         y[e] = (float)s[e] * p.w_scale[c] * xs + (p.bias ? p.bias[c] : -0.0f);
     }
-    activation(p.act, [&](auto f) {
+    activation<OUT == DT_F32>(p.act, [&](auto f) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = f(y[e]);
     });

@@ -79,7 +79,7 @@ struct LinearEpilogue {
                     }
                 }
             }
-            activation(p.act, [&](auto f) {
+            activation<false>(p.act, [&](auto f) {
 #pragma unroll
                 for (int q = 0; q < R; ++q)
 #pragma unroll
@@ -156,7 +156,7 @@ struct LinearEpilogue {
                         b[4 * h + e] = p.bias ? bias[e] : -0.0f;
                     }
                 }
-                activate8(s, ws, s_xs[row], b, p.act, v);
+                activate8<OUT == DT_F32>(s, ws, s_xs[row], b, p.act, v);
                 if (p.residual) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] += res.get(e);

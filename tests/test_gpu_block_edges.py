@@ -378,3 +378,35 @@ def test_routing_weights_are_quotients(ascq_gpu, t, e):
         same = torch.randn(t, 1, generator=torch.Generator().manual_seed(n)).expand(t, n).contiguous().cuda()
         one = torch.ones(1, device="cuda")
         assert torch.all(a.moe_route(same, 1, renormalize=False).weights == one / n)
+
+
+@pytest.mark.parametrize("m,k", [(1, 64), (3, 8192), (300, 64), (2, 0)])
+@pytest.mark.parametrize("act", ["gelu", "silu", "faster_gelu"])
+def test_activations_of_f32_outputs(ascq_gpu, act, m, k):
+    """An f32 output has the activation to a few units of fp32, also where it is small.  x is zero, so the activation's argument is
+    the bias, exactly.  GELU: the complementary error function is allowed 16 units, and its argument's two roundings move it by
+    at most x^2 units and a few; the others: the exponential 3 units, its argument's rounding |b x|, an addition, a product and a
+    division; a result below 2^-126 is off by units of the smallest number."""
+    a = ascq_gpu
+    v = torch.cat([torch.linspace(-14, 14, 4001), torch.linspace(-100, 100, 401), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e30, -1e30])])
+    n = v.numel()
+    code = dict(gelu=a.ACT_GELU, silu=a.ACT_SILU, faster_gelu=a.ACT_FASTER_GELU)[act]
+    got = a.quant_linear(torch.zeros(m, k, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda"),
+                         torch.zeros(n, k, dtype=torch.int8, device="cuda"), torch.ones(n, device="cuda"), bias=v.cuda(),
+                         activation=code, out_dtype=torch.float32).cpu().double()
+    z = v.double()
+    if act == "gelu":
+        want, units = 0.5 * z * torch.special.erfc(-z * 0.5 ** 0.5), 20 + z * z
+    else:
+        b = 1.0 if act == "silu" else 1.702
+        e = torch.exp(-b * z.abs())
+        want, units = z * torch.where(z < 0, e, 1.0) / (1 + e), 8 + b * z.abs()
+    # (past 2^100 only the side that is the argument itself is left, or nothing)
+    units = units.clamp_max(1e5)
+    off = (got - want).abs() - (units * 2.0 ** -23 * want.abs() + 200 * 2.0 ** -149)
+    assert torch.all(off <= 0), (act, v[off.max(dim=1).indices[0]], off.max())
+    special = torch.tensor([float("inf"), -float("inf"), float("nan")])
+    got = a.quant_linear(torch.zeros(m, k, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda"),
+                         torch.zeros(3, k, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"), bias=special.cuda(),
+                         activation=code, out_dtype=torch.float32).cpu()
+    assert torch.all(torch.isinf(got[:, 0])) and torch.all(got[:, 1] == 0) and torch.all(torch.isnan(got[:, 2]))
