@@ -8,26 +8,30 @@
 
 namespace ascq {
 
-// Activations of 16-bit outputs: the hardware's exponential and reciprocal, and a polynomial; their errors lie below the
-// output's rounding.
-// GELU, x Phi(x) = max(x, 0) - |x| Q(|x|) with the normal tail Q by Abramowitz and Stegun 26.2.17: the density times a
-// polynomial of degree 5 in t = 1 / (1 + p |x|), 7.5e-8 off at most.  The side with the small result is the product alone, so
-// it keeps its sign and falls to 0.  (The density's 1 / sqrt(2 pi) is in the coefficients.)
+// Activations of 16-bit outputs: the hardware's exponential and reciprocal, and a polynomial; their errors lie below a
+// hundredth of the output's rounding.
+// GELU, x Phi(x) = max(x, 0) - |x| Q(|x|), Q the normal tail: exp(-x^2 / 2) times the polynomial of degree 7 in t = 1 / (1 + 0.2 |x|)
+// that is least off relatively over 0 <= |x| <= 14 (1.2e-6; found by linear programming).  The side with the small result is
+// the product alone, so it keeps its sign and its digits, and falls to 0.
 __device__ __forceinline__ float gelu_erf(float x)
 {
     const float ax = fminf(__builtin_fabsf(x), 20.0f);  // (beyond, the tail is 0)
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.2316419f, ax, 1.0f));
-    float q = fmaf(0.53070271f, t, -0.72657601f);
-    q = fmaf(q, t, 0.71070687f);
-    q = fmaf(q, t, -0.14224837f);
-    q = fmaf(q, t, 0.12741479f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.2f, ax, 1.0f));
+    float q = fmaf(0.27908108f, t, -0.38677869f);
+    q = fmaf(q, t, 0.44687112f);
+    q = fmaf(q, t, -0.12313594f);
+    q = fmaf(q, t, 0.132517f);
+    q = fmaf(q, t, 0.07109624f);
+    q = fmaf(q, t, 0.08034985f);
     const float tail = ax * (q * t) * __builtin_amdgcn_exp2f(ax * ax * -0.72134752f);
     return (x < 0.0f ? 0.0f : x) - tail;
 }
-// x / (1 + exp(-b x)): -0 as x -> -inf (SiLU: b = 1, FasterGelu: 1.702)
+// x / (1 + exp(-b x)): -0 as x -> -inf (SiLU: b = 1, FasterGelu: 1.702).  Both sides times 2^-32, so that the reciprocal of a
+// large denominator is a normal number for as long as the result is one.
 __device__ __forceinline__ float swish(float x, float b)
 {
-    return fmaxf(x, -200.0f) * __builtin_amdgcn_rcpf(1.0f + __expf(-b * x));
+    const float e = __builtin_amdgcn_exp2f(fmaf(x, -1.44269504f * b, -32.0f));
+    return fmaxf(x, -200.0f) * 0x1p-32f * __builtin_amdgcn_rcpf(e + 0x1p-32f);
 }
 // The same for f32 outputs, to a few units of fp32 where the result is small too.  GELU: the tail as above, the polynomial of
 // degree 8 that is least off relatively over 0 <= |x| <= 14 (1.3e-7; found by linear programming), and the square's rounding

@@ -410,3 +410,28 @@ def test_activations_of_f32_outputs(ascq_gpu, act, m, k):
                          torch.zeros(3, k, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"), bias=special.cuda(),
                          activation=code, out_dtype=torch.float32).cpu()
     assert torch.all(torch.isinf(got[:, 0])) and torch.all(got[:, 1] == 0) and torch.all(torch.isnan(got[:, 2]))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4000, 64), (3, 4004, 8192), (300, 4000, 64), (300, 4004, 64)])
+@pytest.mark.parametrize("act", ["gelu", "silu", "faster_gelu"])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_activations_of_16_bit_outputs(ascq_gpu, dt, act, m, n, k):
+    """A 16-bit output is the activation rounded once, where it is small too: half a unit of the type, and a hundredth of one for
+    the activation's own error -- GELU's polynomial 1.3e-6, exponentials of rounded arguments x^2 2^-23 and 4 units, some more
+    roundings: below 2e-5 in all where the result is normal.  x is zero, so the activation's argument is the bias, exactly."""
+    a = ascq_gpu
+    v = torch.cat([torch.linspace(-9, 9, 3000), torch.linspace(-60, 60, n - 3000)])
+    code = dict(gelu=a.ACT_GELU, silu=a.ACT_SILU, faster_gelu=a.ACT_FASTER_GELU)[act]
+    got = a.quant_linear(torch.zeros(m, k, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda"),
+                         torch.zeros(n, k, dtype=torch.int8, device="cuda"), torch.ones(n, device="cuda"), bias=v.cuda(),
+                         activation=code, out_dtype=dt).cpu().double()
+    z = v.double()
+    if act == "gelu":
+        want = 0.5 * z * torch.special.erfc(-z * 0.5 ** 0.5)
+    else:
+        e = torch.exp(-(1.0 if act == "silu" else 1.702) * z.abs())
+        want = z * torch.where(z < 0, e, 1.0) / (1 + e)
+    half, low = (2.0 ** -11, 2.0 ** -25) if dt is torch.float16 else (2.0 ** -8, 2.0 ** -126)
+    binade = torch.exp2(torch.floor(torch.log2(want.abs().clamp_min(1e-300))))
+    off = (got - want).abs() - (half * 1.0001 * binade + 2e-5 * want.abs() + low)
+    assert torch.all(off <= 0), (act, v[off.max(dim=1).indices[0]], off.max())
