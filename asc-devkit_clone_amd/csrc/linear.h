@@ -10,9 +10,9 @@ namespace ascq {
 
 // Activations of 16-bit outputs: the hardware's exponential and reciprocal, and a polynomial; their errors lie below a
 // hundredth of the output's rounding.
-// GELU, x Phi(x) = max(x, 0) - |x| Q(|x|), Q the normal tail: exp(-x^2 / 2) times the polynomial of degree 7 in t = 1 / (1 + 0.2 |x|)
-// that is least off relatively over 0 <= |x| <= 14 (1.2e-6; found by linear programming).  The side with the small result is
-// the product alone, so it keeps its sign and its digits, and falls to 0.
+// GELU, x Phi(x) = max(x, 0) - |x| Q(|x|), Q the normal tail: exp(-x^2 / 2) times the polynomial of degree 7 in t = 1 / (1 + 0.2
+// |x|) that is least off relatively over 0 <= |x| <= 14 (1.2e-6; found by linear programming).  The side with the small result
+// is the product alone, so it keeps its sign and its digits, and falls to 0.
 __device__ __forceinline__ float gelu_erf(float x)
 {
     const float ax = fminf(__builtin_fabsf(x), 20.0f);  // (beyond, the tail is 0)

@@ -1,7 +1,11 @@
 // linear.hip -- the quantised linear: 8-bit activations with one scale per token times an 8-bit weight with one scale per
-// channel, and bias, activation and residual in the epilogue (linear.h).  int8 sums are exact (int32); fp8 e4m3 sums are
-// fp32.  Here: which kernel a call takes -- the weight-streaming one of linear_decode.hip up to 64 rows, the tiles of
-// linear_pipe.h, their K shared by several workgroups where tiles are few, or the one below -- and what is copied for it.
+// channel, and bias, activation and residual in the epilogue (linear.h).  int8 sums are exact (int32).  fp8 e4m3 sums are
+// held in fp32, but the matrix unit aligns the products of 16 neighbouring k to the largest and drops what lies 2^-13 below
+// it: normal data come out 1.5e-5 off (normwise, 16 x 4096 x 4096 to 2048 x 4096 x 11008) where fp32 sums are 7e-8 to 1.5e-7.
+// That is below a 16-bit output's rounding (1.7e-3 in bf16 either way) and is taken for f32 outputs too, as by the fp8
+// Matmul: instructions that keep all bits run at half the rate, on operands that would have to be widened first.
+// Here: which kernel a call takes -- the weight-streaming one of linear_decode.hip up to 64 rows, the tiles of linear_pipe.h,
+// their K shared by several workgroups where tiles are few, or the one below -- and what is copied for it.
 #include "linear.h"
 
 #include "gemm_pipe.h"
@@ -158,9 +162,11 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, bool w_trans)
 {
     if (w_trans && M <= 64) return {true, 0, linear_decode_splits(M, K)};
     Plan best{false, (int)pick_pipe_tile(M, N, K), 1};
-    // (up to 256 rows the weight comes from memory, not from a cache that other tiles filled, and few workgroups wait for it:
-    // 128 x 4096 x 4096, 64 tiles, takes 17.7 us against the table's 8.6, w [K, N] 24.7; 256 x 11008 x 4096, 172 tiles, 23.8
-    // against 15.3 but split in two 40)
+    // (Up to 256 rows the weight comes from memory, not from a cache that other tiles filled, and few workgroups wait for it, so
+    // the table, whose operands were cached, is short of what they take.  Weights of 600 MB in turn, us split and unsplit, with
+    // tiles of 64 x 128: 128 x 4096 x 11008, 64 tiles, 22.6 and 42.6, w [K, N] 25.5 and 58.2; 192 x 2048 x 8192, 48, 16.4 and
+    // 21.1; 256 x 4096 x 11008, 128, 30.7 and 41.8; at 96 tiles or K = 4096 alike, up to a fifth either way: 192 x 4096 x 4096 15.9
+    // and 13.1, w [K, N] 100 x 6144 x 4096 21.2 and 25.1.)
     float least = pipe_tile_us(best.tile, M, N, K);
     if (M <= 256 && ((M + 63) / 64) * ((N + 127) / 128) <= (w_trans ? 96 : 128)) least *= w_trans ? 1.6f : 2.2f;
     for (int tile : {PIPE_128x128, PIPE_64x128})

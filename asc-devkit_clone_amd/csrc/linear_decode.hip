@@ -9,8 +9,8 @@
 // any order; fp32: in the order of the waves) and go through the epilogue while the next units arrive.
 // (Fragments loaded from memory straight into registers, sixteen rows apart: a load serves four lines per cycle's four lanes,
 // 14.9 us at 1 x 11008 x 4096 from memory.)
-// From memory (weights of 600 MB in turn), int8: 16 x 11008 x 4096 11.8 us, 3.8 TB/s; 16 x 8192 x 8192 15.3, 4.4; 1 x 32000 x 4096
-// 26.8, 4.9; 16 x 4096 x 11008 14.0; 64 x 4096 x 11008 20.4 (x's fragments leave room for 4 units: K in three; 6 units spill: 26).
+// From memory (weights of 600 MB in turn), int8: 16 x 11008 x 4096 11.8 us, 3.8 TB/s; 16 x 8192 x 8192 15.5, 4.3; 1 x 32000 x 4096
+// 26.5, 4.9; 16 x 4096 x 11008 14 to 15; 64 x 4096 x 11008 20.7 (x's fragments leave room for 4 units: K in three; 6 units spill: 26).
 // K longer than the registers hold is split over S workgroups, whose sums meet in the workspace in a second launch.
 #include "gemm_pipe.h"
 #include "linear.h"
@@ -38,8 +38,9 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     // this workgroup's slice of K, and every step-th block of R <= 16 channels: R shares them out evenly over whole rounds, and
-    // the rows of a unit past R are not read (16 x 11008 x 4096: 11.8 us, with whole blocks 12.1).  (Neighbours read neighbouring rows: with an even run of channels each, 8192 x
-    // 8192 took 16.6 us against 15.0.  Few workgroups of a split K keep R = 16: more blocks cost them more than rows not read.)
+    // the rows of a unit past R are not read (16 x 11008 x 4096: 11.8 us, with whole blocks 12.1).  (Neighbours read neighbouring
+    // rows: with an even run of channels each, 8192 x 8192 took 16.6 us against 15.0.  Few workgroups of a split K keep R = 16:
+    // more blocks cost them more than rows not read.)
     const int slice = (int)blockIdx.x % slices, b0 = (int)blockIdx.x / slices, step = (int)gridDim.x / slices;
     const int rounds = (int)((p.N + 16 * step - 1) / (16 * step));
     const int R = slices > 1 ? 16 : (int)((p.N + step * rounds - 1) / (step * rounds));

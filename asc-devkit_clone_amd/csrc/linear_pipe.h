@@ -6,14 +6,15 @@
 // neighbouring fragment columns.  v_permlane16_swap trades halves of the two, after which a lane owns eight columns of a
 // row; they are scaled, biased, activated (one branch for the step), joined by the residual, rounded and stored in one
 // 16-byte piece.  The residual is requested whole in front of the first step, into the registers that the main loop's operands
-// have left (one step ahead instead: 443 us against 439, bf16 out; a word of each of its lines read in front of the main loop as
-// well: 448).  What it costs is its bytes: all CUs come to their epilogues together and read at memory's rate.
+// have left (one step ahead instead: 1 % more at 8192^3; a word of each of its lines read in front of the main loop as well: 2 %).
+// What it costs is its bytes: all CUs come to their epilogues together and read at memory's rate.
 // f32 outputs, and tiles whose columns end inside a piece, go through LDS, which the main loop has left: chunks of fragment
 // rows are parked there, then each thread takes runs of eight columns in a rolled loop, so the element-wise code for a row's
-// end is there once per chunk and not once per piece.  That form for all (8192^3 int8, bf16 out): 447 us against 417, 490 against
-// 440 with residual and GELU -- its barriers.
+// end is there once per chunk and not once per piece.  That form for all (8192^3 int8, bf16 out): 425 us against 418, with
+// residual and GELU alike.
 //
-// 8192^3 int8 411 us plain, 460 with GELU and residual (w [N, K]); 2048 x 4096 x 11008 fp8 71 and 81 with residual.
+// 8192^3 int8, w [N, K], from card to card: 409 to 418 us plain, 432 with residual, 436 with GELU, 460 to 472 with both; w [K, N] 421
+// and 471 to 487.  2048 x 4096 x 11008 fp8 with residual 73 us (operands cached), 81 from memory.
 #pragma once
 
 #include "gemm_pipe.h"

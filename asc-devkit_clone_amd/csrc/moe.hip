@@ -14,9 +14,9 @@
 // is a population count, and so is the chunk's count.  Blocks of chunks meet through a workspace: their counts and their
 // sums of p; the second launch turns the counts before a block into its rows' offsets.  A few tokens are one block, which
 // does it all.
-// What bounds it is latency -- a chain of k maxima over a token's experts, and two launches -- and for many experts the search's
-// instructions, five per logit and choice (16384 tokens, 64 experts, k = 6: 7.5 and 7.3 us of kernels; 16384, 256, k = 8: 17.8
-// and 15; 16 tokens, 16 experts, k = 2: 4.8).
+// What bounds it is latency: a chain of k maxima over a token's experts, and two launches, the second of which reads the counts
+// of all blocks in each (16384 tokens, 64 experts, k = 6: 7.5 and 7.3 us of kernels; 16384, 256, k = 8: 17.8, of which the
+// search's instructions, five per logit and choice, are some 4 at the chip's rate, and 15; 16 tokens, 16 experts, k = 2: 4.8).
 #include <type_traits>
 
 #include "common.h"
@@ -30,12 +30,6 @@ namespace {
 constexpr int CHUNK = 64;        // tokens of a mask, at most
 constexpr int MAX_BLOCKS = 512;  // (each block of the second launch reads the counts of all; fewer, each for a run: slower)
 constexpr int MAX_K = 16;
-
-__device__ __forceinline__ float load_logit(const void* p, int64_t i, int dtype)
-{
-    const float v = load_f32_of(p, i, dtype);
-    return v != v ? -__builtin_inff() : fminf(v, 3.402823466e38f);
-}
 
 // a gradient, rounded once: past a 16-bit type's range it is infinite, which is what a loss scaler looks for
 __device__ __forceinline__ void store_grad(void* p, int64_t i, float v, int dtype)
@@ -400,7 +394,7 @@ __global__ __launch_bounds__(1024) void moe_rows_kernel(MoeRouteArgs a, int bloc
 // d loss / d l and d w / d l: G lanes per token, each with V neighbouring experts
 //   g_e = dL E counts_e / (sum counts x routed)  (+ dw_j at choice j without renormalisation),  dl_e = p_e (g_e - sum p g)
 //   renormalised: + w_j (dw_j - sum_i dw_i w_i) at choice j
-// Bound by latency up to some ten thousand tokens, then by memory (64 experts: 16384 tokens 8.4 us, 100000 28 us, 3.6 TB/s).
+// Bound by latency (64 experts, k = 6: 16384 tokens 8 to 9 us, 100000 32 us, 1.8 TB/s of what it has to move).
 template <int G, int V>
 __global__ __launch_bounds__(256) void moe_route_grad_kernel(MoeRouteGradArgs a)
 {

@@ -8,7 +8,7 @@
 // the same pass, and the codes need no second reduction.  h, t, the sum and the scale are fp32; the roundings are h's (the
 // stored stream's type), the codes' and norm's.
 // Bound by memory: 8192 x 8192 bf16 with residual to e4m3 in 77 us, 6.1 TB/s of the bytes it cannot do without; f32 4.9 TB/s
-// (4096 x 8192: 88 us); rows that start at any element 4.4 (8192 x 8191: 108 us).  A decode step's 16 x 4096 takes 3.5 us.
+// (4096 x 8192: 88 us); rows that start at any element 4.3 (8192 x 8191: 110 us).  A decode step's 16 x 4096 takes 3.5 us.
 // A row of zeros has codes and scale 0.  A row with a NaN, an infinity (which h keeps: only a finite sum saturates), or squares
 // that pass fp32's range has codes 0 and scale NaN, so that its products are NaN and not some number.
 #include <type_traits>
@@ -229,10 +229,12 @@ __device__ __forceinline__ u32x2 codes8(const float (&v)[8], bool int8)
 // and the codes, so every byte moves once.  All loads of a thread are issued in front of its first wait: units past the
 // row read its last whole one and are dropped (in place, another thread may have stored it by then).
 // ANY: rows that start at any element, whose last unit may be a part of one.
-// (bf16, 1024 threads of four 16-byte words: in 64 registers, which are two workgroups per CU.  2048 x 32768 with residual 81 us,
-// in the 68 that it takes by itself 88)
+// waves_per_simd: bf16 and f32, 1024 threads of four 16-byte words, in 64 registers, which are two workgroups per CU (bf16 2048 x
+// 32768 with residual 81 us, in the 70 that it takes by itself 88).
+template <int T, int NT, int U>
+constexpr int waves_per_simd = T != DT_F16 && NT == 1024 && U * Unit<T>::W <= 4 ? 8 : 1;
 template <int T, int NT, int U, bool RES, bool ANY>
-__global__ __launch_bounds__(NT, T != DT_F16 && NT == 1024 && U * Unit<T>::W <= 4 ? 8 : 1) void norm_quant_row_kernel(NormQuantArgs a)
+__global__ __launch_bounds__(NT, waves_per_simd<T, NT, U>) void norm_quant_row_kernel(NormQuantArgs a)
 {
     const int64_t row = blockIdx.x;
     const uint32_t whole = (uint32_t)(a.n / 8), units = ANY ? (uint32_t)((a.n + 7) / 8) : whole;

@@ -606,7 +606,9 @@ typedef struct {
 /* The quantised linear:
  * y = cast(act((sum_k x[m, k] w[k, n]) w_scale[n] x_scale[m] + bias[n]) + residual[m, n]), fp32 in this order, one
  * rounding at the end (nearest even; in f16 and bf16 a finite value saturates, an infinite one stays infinite).  int8
- * sums are exact int32 (k below 2^17); fp8 sums are those of the fp8 Matmul.  x_scale f32 [m], w_scale f32 [n]; bias f32 [n]
+ * sums are exact int32 (k below 2^17); fp8 sums are the matrix unit's, as the fp8 Matmul's are: fp32, less what lies
+ * 2^-13 below the largest of 16 neighbouring products (1.5e-5 normwise, f32 outputs too); which ones are neighbours, and so
+ * the last bits, may differ with alignment and workspace.  x_scale f32 [m], w_scale f32 [n]; bias f32 [n]
  * or NULL; residual [m, n] or NULL (it may be y itself, with its stride).  k = 0 gives act(bias) + residual.  (There is
  * no counterpart in the reference.)
  * workspace: optional, 16-byte aligned, ascq_quant_linear_workspace_size bytes (0 for many calls): room for the partial
@@ -625,8 +627,8 @@ typedef struct {
     int32_t renormalize;     /* 1: a token's weights are divided by their sum */
 } ascq_route_param;
 
-/* Expert routing (no counterpart in the reference).  logits [tokens, experts]; a logit of -inf or NaN counts nothing (its expert is masked for the token),
- * +inf counts as the largest finite number.  p = softmax over what counts; a token's choices are its top_k largest logits
+/* Expert routing (no counterpart in the reference).  logits [tokens, experts]; a logit of -inf or NaN counts nothing (its
+ * expert is masked for the token), +inf counts as the largest finite number.  p = softmax over what counts; a token's choices are its top_k largest logits
  * in falling order, of equal ones the lowest expert; a token with fewer that count has fewer choices, a token of none
  * (padding) has none.
  *   weights  f32 [tokens, top_k]: p of the choice (renormalize: divided by their sum); 0 where there is none
@@ -660,7 +662,8 @@ typedef struct {
     int32_t type;   /* dispatch: INT8, FP8_E4M3, F16, BF16 or F32; combine, combine_grad: F16, BF16, F32 */
     int32_t top_k;  /* 1 .. 16 */
 } ascq_rows_param;
-/* (no counterpart in the reference) rows[slots[t, j]] = x[t], row_scale[slots[t, j]] = x_scale[t] (both NULL without scales); rows of no token are 0 */
+/* (no counterpart in the reference) rows[slots[t, j]] = x[t], row_scale[slots[t, j]] = x_scale[t] (both NULL without scales);
+ * rows of no token are 0 */
 ascq_status ascq_moe_dispatch(void* rows, float* row_scale, const void* x, const float* x_scale, const int32_t* slots,
                               const int32_t* row_tokens, const ascq_rows_param* p, void* stream);
 /* (no counterpart in the reference) out[t] = sum_j weights[t, j] y[slots[t, j]] + residual[t]: fp32, in the order of j, one

@@ -15,9 +15,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 def _run(tmp_path, name):
     exe = tmp_path / name
     libdir = Path(ascq.LIB_PATH).parent
-    subprocess.run([HIPCC, "--offload-arch=gfx950", "--offload-host-only", "-x", "hip", "-std=c++17", "-O1", "-I", str(ROOT / "include"),
-                    "-I", str(libdir / "csrc"), str(ROOT / "tests" / "cpp" / f"{name}.cpp"), "-rdynamic", "-L", str(libdir), "-lascq",
-                    f"-Wl,-rpath,{libdir}", "-Wl,-rpath,/opt/rocm/lib", "-o", str(exe)], check=True)
+    subprocess.run([HIPCC, "--offload-arch=gfx950", "--offload-host-only", "-x", "hip", "-std=c++17", "-O1",
+                    "-I", str(ROOT / "include"), "-I", str(libdir / "csrc"), str(ROOT / "tests" / "cpp" / f"{name}.cpp"),
+                    "-rdynamic", "-L", str(libdir), "-lascq", f"-Wl,-rpath,{libdir}", "-Wl,-rpath,/opt/rocm/lib", "-o", str(exe)],
+                   check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
 
