@@ -286,7 +286,7 @@ hipError_t launch_linear_pipe_i8(const LinearArgs& a, hipStream_t st);
 hipError_t launch_linear_pipe_f8(const LinearArgs& a, hipStream_t st);
 // linear_decode.hip: x [M <= 64, K] and w [N, K] with 16-byte-aligned rows, K a multiple of 16; K is split a.splits =
 // linear_decode_splits ways
-int linear_decode_splits(int64_t M, int64_t K);
+int linear_decode_splits(int64_t M, int64_t K, bool wide);  // wide: fp8 with f32 outputs
 hipError_t launch_linear_decode(const LinearArgs& a, hipStream_t st);
 // adds the sums that the workgroups of a split K left, in order, and runs the epilogue
 hipError_t launch_linear_slices(const LinearArgs& a, hipStream_t st);

@@ -1,9 +1,10 @@
 // linear.hip -- the quantised linear: 8-bit activations with one scale per token times an 8-bit weight with one scale per
 // channel, and bias, activation and residual in the epilogue (linear.h).  int8 sums are exact (int32).  fp8 e4m3 sums are
-// held in fp32, but the matrix unit aligns the products of 16 neighbouring k to the largest and drops what lies 2^-13 below
-// it: normal data come out 1.5e-5 off (normwise, 16 x 4096 x 4096 to 2048 x 4096 x 11008) where fp32 sums are 7e-8 to 1.5e-7.
-// That is below a 16-bit output's rounding (1.7e-3 in bf16 either way) and is taken for f32 outputs too, as by the fp8
-// Matmul: instructions that keep all bits run at half the rate, on operands that would have to be widened first.
+// held in fp32, but the fp8 MFMA aligns the products of 16 neighbouring k to the largest and drops what lies 2^-13 below it:
+// normal data come out 1.5e-5 off (normwise, 16 x 4096 x 4096 to 2048 x 4096 x 11008) where fp32 sums are 7e-8 to 1.5e-7.  That
+// is below a 16-bit output's rounding (1.7e-3 in bf16 either way), so those take it; for f32 outputs the codes are widened to
+// f16 in registers, for the f16 MFMA, which keeps all bits at half the rate (8192^3 396 -> 811 us; 16 x 32000 x 4096, whose
+// weight comes from memory, 27 either way).
 // Here: which kernel a call takes -- the weight-streaming one of linear_decode.hip up to 64 rows, the tiles of linear_pipe.h,
 // their K shared by several workgroups where tiles are few, or the one below -- and what is copied for it.
 #include "linear.h"
@@ -65,10 +66,11 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearArgs a, int64_t f
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if constexpr (F8) {
-                    typedef long v2l __attribute__((ext_vector_type(2)));
-                    const v2l p = __builtin_bit_cast(v2l, fx[i]), q = __builtin_bit_cast(v2l, fw[j]);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(p[0], q[0], acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(p[1], q[1], acc[i][j], 0, 0, 0);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const h8 p = widen_e4m3(fx[i][2 * h], fx[i][2 * h + 1]), q = widen_e4m3(fw[j][2 * h], fw[j][2 * h + 1]);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, acc[i][j], 0, 0, 0);
+                    }
                 } else {
                     acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fx[i], fw[j], acc[i][j], 0, 0, 0);
                 }
@@ -151,6 +153,7 @@ hipError_t launch_any(const LinearArgs& a, const char* why, hipStream_t st)
 
 namespace {
 
+bool wide(const LinearArgs& a) { return a.f8 && a.out_type == DT_F32; }
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // How an aligned call runs: the weight-streaming kernel for few rows, or tiles, whose K may be shared by several workgroups
@@ -158,10 +161,16 @@ struct Plan {
     bool decode;
     int tile, splits;
 };
-Plan plan_of(int64_t M, int64_t N, int64_t K, bool w_trans)
+// wide: fp8 with f32 outputs, on tiles of 128 x 128 or 64 x 128 (their operands as f16 numbers take more registers)
+int tile_of(int64_t M, int64_t N, int64_t K, bool wide)
 {
-    if (w_trans && M <= 64) return {true, 0, linear_decode_splits(M, K)};
-    Plan best{false, (int)pick_pipe_tile(M, N, K), 1};
+    if (!wide) return (int)pick_pipe_tile(M, N, K);
+    return pipe_tile_us(PIPE_64x128, M, N, K) < pipe_tile_us(PIPE_128x128, M, N, K) ? PIPE_64x128 : PIPE_128x128;
+}
+Plan plan_of(int64_t M, int64_t N, int64_t K, bool w_trans, bool wide)
+{
+    if (w_trans && M <= 64) return {true, 0, linear_decode_splits(M, K, wide)};
+    Plan best{false, tile_of(M, N, K, wide), 1};
     // (Up to 256 rows the weight comes from memory, not from a cache that other tiles filled, and few workgroups wait for it, so
     // the table, whose operands were cached, is short of what they take.  Weights of 600 MB in turn, us split and unsplit, with
     // tiles of 64 x 128: 128 x 4096 x 11008, 64 tiles, 22.6 and 42.6, w [K, N] 25.5 and 58.2; 192 x 2048 x 8192, 48, 16.4 and
@@ -232,7 +241,7 @@ size_t linear_ws_bytes(const LinearArgs& in)
     if (too_large(a)) return 0;
     const PackPlan p = pack_plan(a);
     const size_t pack = p.x_bytes + p.w_bytes;
-    const size_t part = part_bytes(a.M, a.N, plan_of(a.M, a.N, a.w_trans ? p.kp : a.K, a.w_trans).splits);
+    const size_t part = part_bytes(a.M, a.N, plan_of(a.M, a.N, a.w_trans ? p.kp : a.K, a.w_trans, wide(a)).splits);
     return part ? align256(pack) + part : pack;
 }
 
@@ -270,9 +279,9 @@ hipError_t launch_linear(const LinearArgs& in, uint8_t* ws, size_t ws_bytes, hip
         }
         if (a.w_trans) a.K = p.kp;  // (zeros behind K in one operand at least)
     }
-    Plan plan = plan_of(a.M, a.N, a.K, a.w_trans);
+    Plan plan = plan_of(a.M, a.N, a.K, a.w_trans, wide(a));
     if (plan.splits > 1) {
-        if (align256(pack) + part_bytes(a.M, a.N, plan.splits) > ws_bytes) plan = {false, (int)pick_pipe_tile(a.M, a.N, a.K), 1};
+        if (align256(pack) + part_bytes(a.M, a.N, plan.splits) > ws_bytes) plan = {false, tile_of(a.M, a.N, a.K, wide(a)), 1};
         a.part = ws + align256(pack);
         a.part_pitch = part_pitch(a.N);
     }

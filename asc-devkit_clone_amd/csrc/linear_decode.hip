@@ -24,7 +24,8 @@ __device__ __forceinline__ float scaled(int v) { return (float)v; }
 
 constexpr int BLOCKS = 64;  // blocks of 16 channels that a workgroup keeps the scales of
 
-template <bool F8, int MB, int KW, int U, int D>
+// WIDE: fp8 with the sums of the f16 MFMA, for f32 outputs
+template <bool F8, bool WIDE, int MB, int KW, int U, int D>
 __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
 {
     typedef typename std::conditional<F8, v4f, v4i>::type acc_t;
@@ -119,15 +120,20 @@ __global__ __launch_bounds__(64 * KW) void linear_decode_kernel(LinearArgs p)
         acc_t acc[MB] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            if constexpr (WIDE) {  // (x's codes stay codes: widened once for all blocks they do not fit the registers)
+#pragma unroll
+                for (int m = 0; m < MB; ++m) asm volatile("" : "+v"(x[m][u][0]), "+v"(x[m][u][1]));
+            }
             v4i lo, hi;
             take(lo, hi, ask_w);
 #pragma unroll
             for (int m = 0; m < MB; ++m) {
                 if constexpr (F8) {
                     const v4i e = x[m][u][0], f = x[m][u][1];
-                    acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                        (v8i){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]},
-                        (v8i){e[0], e[1], e[2], e[3], f[0], f[1], f[2], f[3]}, acc[m], 0, 0, 0, 0, 0, 0);
+                    const v8i w8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    const v8i x8 = {e[0], e[1], e[2], e[3], f[0], f[1], f[2], f[3]};
+                    if constexpr (WIDE) acc[m] = mfma_wide_e4m3(w8, x8, acc[m]);
+                    else acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[m], 0, 0, 0, 0, 0, 0);
                 } else {
                     acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo, x[m][u][0], acc[m], 0, 0, 0);
                     acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi, x[m][u][1], acc[m], 0, 0, 0);
@@ -205,10 +211,10 @@ __global__ __launch_bounds__(256) void linear_slices_kernel(LinearArgs p)
     }
 }
 
-template <bool F8, int MB, int KW, int U, int D>
+template <bool F8, bool WIDE, int MB, int KW, int U, int D>
 hipError_t go(const LinearArgs& a, hipStream_t st)
 {
-    constexpr auto kern = linear_decode_kernel<F8, MB, KW, U, D>;
+    constexpr auto kern = linear_decode_kernel<F8, WIDE, MB, KW, U, D>;
     constexpr int LDS = KW * D * 2048 + 2 * 16 * KW * MB * 64 + (2 * BLOCKS * 16 + 16 * MB) * 4;
     static_assert(LDS <= 160 * 1024, "LDS");
     static_assert(2 * D < 64, "vmcnt");
@@ -226,12 +232,12 @@ hipError_t go(const LinearArgs& a, hipStream_t st)
 struct DecodePlan {
     int mb, kw, u, slices;
 };
-DecodePlan decode_plan(int64_t M, int64_t K)
+DecodePlan decode_plan(int64_t M, int64_t K, bool wide)
 {
     DecodePlan d{};
     d.mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     d.kw = d.mb == 1 ? 16 : 8;
-    const int most = d.mb == 1 ? 8 : d.mb == 2 ? 10 : 4;
+    const int most = d.mb == 1 ? (wide ? 6 : 8) : d.mb == 2 ? 10 : 4;  // (wide, 8 units: they spill, 16 x 4096 x 14336 23 us)
     const int units = (int)((K + 127) / 128);
     d.slices = (units + d.kw * most - 1) / (d.kw * most);
     const int per = (units + d.slices - 1) / d.slices;
@@ -240,34 +246,36 @@ DecodePlan decode_plan(int64_t M, int64_t K)
     return d;
 }
 
-template <bool F8>
+template <bool F8, bool WIDE>
 hipError_t launch_plan(const LinearArgs& a, const DecodePlan& d, hipStream_t st)
 {
     if (d.mb == 1) {
-        if (d.u == 2) return go<F8, 1, 16, 2, 3>(a, st);
-        if (d.u == 4) return go<F8, 1, 16, 4, 3>(a, st);
-        if (d.u == 6) return go<F8, 1, 16, 6, 3>(a, st);
-        return go<F8, 1, 16, 8, 3>(a, st);
+        if (d.u == 2) return go<F8, WIDE, 1, 16, 2, 3>(a, st);
+        if (d.u == 4) return go<F8, WIDE, 1, 16, 4, 3>(a, st);
+        if (WIDE || d.u == 6) return go<F8, WIDE, 1, 16, 6, 3>(a, st);
+        if constexpr (!WIDE) return go<F8, WIDE, 1, 16, 8, 3>(a, st);
     }
     if (d.mb == 2) {
-        if (d.u == 2) return go<F8, 2, 8, 2, 6>(a, st);
-        if (d.u == 4) return go<F8, 2, 8, 4, 6>(a, st);
-        if (d.u == 6) return go<F8, 2, 8, 6, 6>(a, st);
-        if (d.u == 8) return go<F8, 2, 8, 8, 6>(a, st);
-        return go<F8, 2, 8, 10, 6>(a, st);
+        if (d.u == 2) return go<F8, WIDE, 2, 8, 2, 6>(a, st);
+        if (d.u == 4) return go<F8, WIDE, 2, 8, 4, 6>(a, st);
+        if (d.u == 6) return go<F8, WIDE, 2, 8, 6, 6>(a, st);
+        if (d.u == 8) return go<F8, WIDE, 2, 8, 8, 6>(a, st);
+        return go<F8, WIDE, 2, 8, 10, 6>(a, st);
     }
-    if (d.u == 2) return go<F8, 4, 8, 2, 5>(a, st);
-    return go<F8, 4, 8, 4, 5>(a, st);
+    if (d.u == 2) return go<F8, WIDE, 4, 8, 2, 5>(a, st);
+    return go<F8, WIDE, 4, 8, 4, 5>(a, st);
 }
 
 }  // namespace
 
-int linear_decode_splits(int64_t M, int64_t K) { return decode_plan(M, K).slices; }
+int linear_decode_splits(int64_t M, int64_t K, bool wide) { return decode_plan(M, K, wide).slices; }
 
 hipError_t launch_linear_decode(const LinearArgs& a, hipStream_t st)
 {
-    const DecodePlan d = decode_plan(a.M, a.K);
-    return a.f8 ? launch_plan<true>(a, d, st) : launch_plan<false>(a, d, st);
+    const bool wide = a.f8 && a.out_type == DT_F32;
+    const DecodePlan d = decode_plan(a.M, a.K, wide);
+    if (!a.f8) return launch_plan<false, false>(a, d, st);
+    return wide ? launch_plan<true, true>(a, d, st) : launch_plan<true, false>(a, d, st);
 }
 
 hipError_t launch_linear_slices(const LinearArgs& a, hipStream_t st)

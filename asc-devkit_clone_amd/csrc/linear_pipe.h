@@ -177,10 +177,11 @@ private:
 
 // SPLIT: few tiles of a long K, each shared by p.splits workgroups, which leave their sums (fp32 / int32) in p.part,
 // [split][M][part_pitch]; linear_slices_kernel adds them and runs the epilogue.
-template <int BM, int BN, int WM, int WN, int OP, bool BTR, bool SPLIT>
+// FMT: 0 (e4m3 x e4m3), or 64, whose sums keep all bits.
+template <int BM, int BN, int WM, int WN, int OP, bool BTR, bool SPLIT, int FMT>
 __global__ __launch_bounds__(WM * WN * 64, 2) void linear_pipe_kernel(LinearArgs p)
 {
-    using T = GemmPipe<BM, BN, WM, WN, OP, 0, BTR>;  // (e4m3 x e4m3)
+    using T = GemmPipe<BM, BN, WM, WN, OP, FMT, BTR>;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     int tm, tn;
     const int tiles_m = (int)((p.M + BM - 1) / BM), tiles_n = (int)((p.N + BN - 1) / BN);
@@ -240,21 +241,30 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_pipe_kernel(LinearArgs
     }
 }
 
-template <int BM, int BN, int WM, int WN, int OP, bool BTR, bool SPLIT = false>
+template <int BM, int BN, int WM, int WN, int OP, bool BTR, bool SPLIT = false, int FMT = 0>
 static hipError_t launch_linear_tile(const LinearArgs& a, hipStream_t st)
 {
-    using T = GemmPipe<BM, BN, WM, WN, OP, 0, BTR>;
+    using T = GemmPipe<BM, BN, WM, WN, OP, FMT, BTR>;
     constexpr int LDS = (int)T::LDS_BYTES + (SPLIT ? 0 : 3072);  // the ring, the vectors
     const int tiles = (int)(((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN)) * (SPLIT ? a.splits : 1);
-    const hipError_t e = ensure_dynamic_lds<linear_pipe_kernel<BM, BN, WM, WN, OP, BTR, SPLIT>>(LDS);
+    const hipError_t e = ensure_dynamic_lds<linear_pipe_kernel<BM, BN, WM, WN, OP, BTR, SPLIT, FMT>>(LDS);
     if (e != hipSuccess) return e;
-    launch_k((linear_pipe_kernel<BM, BN, WM, WN, OP, BTR, SPLIT>), dim3(tiles), dim3(T::NT), (uint32_t)LDS, st, a);
+    launch_k((linear_pipe_kernel<BM, BN, WM, WN, OP, BTR, SPLIT, FMT>), dim3(tiles), dim3(T::NT), (uint32_t)LDS, st, a);
     return hipGetLastError();
 }
 
 template <int OP, bool BTR>
 static hipError_t launch_linear_layout(const LinearArgs& a, hipStream_t st)
 {
+    if constexpr (OP == OP_F8)
+        if (a.out_type == DT_F32) {
+            const bool large = a.tile == PIPE_128x128;  // (linear.hip plans these calls on two shapes)
+            if (a.splits > 1)
+                return large ? launch_linear_tile<128, 128, 2, 2, OP, BTR, true, 64>(a, st)
+                             : launch_linear_tile<64, 128, 2, 2, OP, BTR, true, 64>(a, st);
+            return large ? launch_linear_tile<128, 128, 2, 2, OP, BTR, false, 64>(a, st)
+                         : launch_linear_tile<64, 128, 2, 2, OP, BTR, false, 64>(a, st);
+        }
     if (a.splits > 1)
         return a.tile == PIPE_128x128 ? launch_linear_tile<128, 128, 2, 2, OP, BTR, true>(a, st)
                                       : launch_linear_tile<64, 128, 2, 2, OP, BTR, true>(a, st);

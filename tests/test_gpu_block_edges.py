@@ -435,3 +435,29 @@ def test_activations_of_16_bit_outputs(ascq_gpu, dt, act, m, n, k):
     binade = torch.exp2(torch.floor(torch.log2(want.abs().clamp_min(1e-300))))
     off = (got - want).abs() - (half * 1.0001 * binade + 2e-5 * want.abs() + low)
     assert torch.all(off <= 0), (act, v[off.max(dim=1).indices[0]], off.max())
+
+
+@pytest.mark.parametrize("w_trans", [True, False])
+@pytest.mark.parametrize("m,n,k,shift", [(1, 512, 4096, 0), (16, 1024, 1024, 0), (17, 512, 8192, 0), (40, 256, 11008, 0),
+                                         (64, 512, 2048, 0), (100, 384, 11008, 0), (300, 516, 4096, 0), (1030, 1100, 1003, 0),
+                                         (2048, 2048, 1024, 0), (70, 100, 515, 3), (5, 64, 144, 1)])
+def test_fp8_sums_of_f32_outputs(ascq_gpu, m, n, k, shift, w_trans):
+    """An f32 output of e4m3 operands has fp32 sums.  Of normal data, against 64 bits, normwise: K / 32 accumulations that each
+    round the sum so far (2^-24 of it, in both directions alike: their square root), and eight roundings more for the products
+    inside one, the scales and the store."""
+    a = ascq_gpu
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+
+    def codes(rows, cols):
+        pad = torch.zeros(rows * cols + 64, device="cuda").to(torch.float8_e4m3fn)
+        v = pad[shift:shift + rows * cols].view(rows, cols)
+        v.copy_((torch.randn(rows, cols, generator=g, device="cuda") * 64).clamp(-448, 448).to(torch.float8_e4m3fn))
+        return v
+
+    x, w = codes(m, k), codes(n, k) if w_trans else codes(k, n)
+    xs, ws = (torch.rand(s, generator=g, device="cuda") + 0.5 for s in (m, n))
+    wf = w.float().double()
+    want = x.float().double() @ (wf.t().contiguous() if w_trans else wf) * ws.double() * xs.double()[:, None]
+    for room in (None, torch.empty(1, dtype=torch.uint8, device="cuda")):
+        got = a.quant_linear(x, xs, w, ws, w_trans=w_trans, out_dtype=torch.float32, workspace=room)
+        assert (got.double() - want).norm() <= ((k / 32) ** 0.5 + 8) * 2.0 ** -24 * want.norm()
