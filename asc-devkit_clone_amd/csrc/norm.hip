@@ -234,7 +234,7 @@ __device__ __forceinline__ u32x2 codes8(const float (&v)[8], bool int8)
 template <int T, int NT, int U>
 constexpr int waves_per_simd = T != DT_F16 && NT == 1024 && U * Unit<T>::W <= 4 ? 8 : 1;
 template <int T, int NT, int U, bool RES, bool ANY>
-__global__ __launch_bounds__(NT, waves_per_simd<T, NT, U>) void norm_quant_row_kernel(NormQuantArgs a)
+__global__ __launch_bounds__(NT, (waves_per_simd<T, NT, U>)) void norm_quant_row_kernel(NormQuantArgs a)
 {
     const int64_t row = blockIdx.x;
     const uint32_t whole = (uint32_t)(a.n / 8), units = ANY ? (uint32_t)((a.n + 7) / 8) : whole;

@@ -609,8 +609,8 @@ typedef struct {
  * sums are exact int32 (k below 2^17).  fp8 sums are fp32 where out_type is F32; for 16-bit outputs they may be the fp8
  * Matmul's, which leave out what lies 2^-13 below the largest of 16 neighbouring products (1.5e-5 normwise, below those
  * outputs' rounding); their last bits may differ with alignment and workspace.  x_scale f32 [m], w_scale f32 [n]; bias f32
- * [n] or NULL; residual [m, n] or NULL (it may be y itself, with its stride).  k = 0 gives act(bias) + residual.  (There is no
- * counterpart in the reference.)
+ * [n] or NULL; residual [m, n] or NULL (it may be y itself, with its stride).  k = 0 gives act(bias) + residual.  (There is
+ * no counterpart in the reference.)
  * workspace: optional, 16-byte aligned, ascq_quant_linear_workspace_size bytes (0 for many calls): room for the partial
  * sums of few rows and for operands whose rows are off 16 bytes; a call with less of it, or none, takes kernels that
  * need none and returns the same int8 results. */
