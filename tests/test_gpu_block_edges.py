@@ -315,8 +315,9 @@ def test_rows_without_elements(ascq_gpu):
 
 @pytest.mark.parametrize("codes", ["int8", "fp8"])
 @pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-5])
-@pytest.mark.parametrize("dt,n", [("f32", 64), ("f32", 513), ("f32", 4096), ("f32", 70000), ("bf16", 96), ("bf16", 4100),
-                                  ("bf16", 70000), ("f16", 640)])
+@pytest.mark.parametrize("dt,n", [("f32", 64), ("f32", 513), ("f32", 4096), ("f32", 16000), ("f32", 20001), ("f32", 70000),
+                                  ("bf16", 96), ("bf16", 1000), ("bf16", 4100), ("bf16", 20000), ("bf16", 20001),
+                                  ("bf16", 60000), ("bf16", 70000), ("f16", 640)])
 def test_norm_of_tiny_rows(ascq_gpu, dt, n, eps, codes):
     """Rows, gammas and products far below 1, down to subnormal numbers: codes times scale is the norm of the definition in 64
     bits, as for ordinary rows, also where the squares or the products' reciprocal leave fp32's range.  Bounds of
