@@ -104,6 +104,33 @@ class _RowsParam(ctypes.Structure):
                 ("top_k", ctypes.c_int32)]
 
 
+class _KvCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("ld_codes", ctypes.c_int64), ("ld_scales", ctypes.c_int64),
+                ("kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("d", ctypes.c_int32), ("group", ctypes.c_int32)]
+
+
+class _KvSequences(ctypes.Structure):
+    _fields_ = [("page_table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("starts", ctypes.c_void_p),
+                ("ld_table", ctypes.c_int64), ("batch", ctypes.c_int32), ("table_pages", ctypes.c_int32)]
+
+
+class _KvAppendParam(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("ld_k", ctypes.c_int64), ("hd_k", ctypes.c_int64), ("ld_v", ctypes.c_int64),
+                ("hd_v", ctypes.c_int64), ("type", ctypes.c_int32)]
+
+
+class _KvAttentionParam(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("max_queries", ctypes.c_int64), ("ld_q", ctypes.c_int64), ("hd_q", ctypes.c_int64),
+                ("ld_out", ctypes.c_int64), ("hd_out", ctypes.c_int64), ("window", ctypes.c_int64), ("type", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("causal", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+class _KvEvictParam(ctypes.Structure):
+    _fields_ = [("cap", ctypes.c_int64), ("cap_out", ctypes.c_int64), ("ld_into", ctypes.c_int64), ("keep", ctypes.c_int32),
+                ("recent", ctypes.c_int32), ("into_pages", ctypes.c_int32)]
+
+
 class _MatmulTypes(ctypes.Structure):
     _fields_ = [
         ("a_type", ctypes.c_int32),
@@ -190,6 +217,15 @@ SIGNATURES = {
     "ascq_moe_dispatch": (_I32, [_P] * 6 + [ctypes.POINTER(_RowsParam), _P]),
     "ascq_moe_combine": (_I32, [_P] * 5 + [ctypes.POINTER(_RowsParam), _P]),
     "ascq_moe_combine_grad": (_I32, [_P] * 7 + [ctypes.POINTER(_RowsParam), _P]),
+    "ascq_kv_append": (_I32, [ctypes.POINTER(_KvCache), _P, _P, _P, ctypes.POINTER(_KvAppendParam), _P]),
+    "ascq_kv_attention_workspace_size": (_I32, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvSequences),
+                                                ctypes.POINTER(_KvAttentionParam), ctypes.POINTER(ctypes.c_size_t)]),
+    "ascq_kv_attention": (_I32, [_P] * 3 + [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvSequences),
+                                            ctypes.POINTER(_KvAttentionParam), _P, ctypes.c_size_t, _P]),
+    "ascq_kv_weights": (_I32, [_P, _P, _I64, _F32, _P, _P, ctypes.POINTER(_KvCache), ctypes.POINTER(_KvSequences),
+                               ctypes.POINTER(_KvAttentionParam), _P]),
+    "ascq_kv_evict": (_I32, [_P] * 5 + [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvSequences), ctypes.POINTER(_KvEvictParam),
+                                        _P]),
     "ascq_nz_size": (ctypes.c_size_t, [_I32, _I64, _I64, _I64]),
     "ascq_nz_to_nd": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _I32, _P]),
     "ascq_nd_to_nz": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _P]),
@@ -837,6 +873,226 @@ def moe_combine_grad(grad_out: torch.Tensor, y: torch.Tensor, slots: torch.Tenso
     check(lib().ascq_moe_combine_grad(_at(dw), _at(dy), _at(grad_out), _at(y), _at(slots), _at(tokens), _at(weights),
                                       ctypes.byref(p), _stream(stream)), what)
     return dw, dy
+
+
+# ------------------------------------------------------------------------------------------
+# attention over the paged int4 key / value cache
+# ------------------------------------------------------------------------------------------
+class KvCache(NamedTuple):
+    """A paged key / value cache: int4 codes (uint8 [pages, kv_heads, page_size, d / 2]) and f16 (scale, offset) pairs
+    ([pages, kv_heads, page_size, d / group, 2]); a page's elements are contiguous, pages at any pitch of 16 bytes.  A code stands
+    for f16(code * scale + offset)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def kv_cache(pages: int, kv_heads: int, page_size: int, d: int, group: int = 32, device="cuda") -> KvCache:
+    """An empty cache (its memory is not set: nothing is read that was not appended)"""
+    new = lambda shape, dt: torch.empty(shape, dtype=dt, device=device)  # noqa: E731
+    code, scale = (pages, kv_heads, page_size, d // 2), (pages, kv_heads, page_size, d // group, 2)
+    return KvCache(new(code, torch.uint8), new(code, torch.uint8), new(scale, torch.float16), new(scale, torch.float16))
+
+
+def _page_pitch(what: str, name: str, t: torch.Tensor, shape, dtype) -> int:
+    """elements from page to page of a pool whose pages are contiguous"""
+    if t.shape != shape or t.dtype is not dtype:
+        _refuse(what, f"{name} must be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+    if not t.is_contiguous() and not (t.shape[0] > 0 and t[0].is_contiguous()):
+        _refuse(what, f"{name}: the elements of a page must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _cache_arg(what: str, c: KvCache) -> _KvCache:
+    if c.k.dim() != 4 or c.k_scale.dim() != 5:
+        _refuse(what, "codes must be [pages, kv_heads, page_size, d / 2], scales [pages, kv_heads, page_size, d / group, 2]")
+    shape, pairs = c.k.shape, c.k_scale.shape
+    groups = pairs[3]
+    if pairs[:3] != shape[:3] or pairs[4] != 2 or groups < 1 or 2 * shape[3] % groups:
+        _refuse(what, f"k_scale {tuple(pairs)} does not fit codes {tuple(shape)}")
+    ld = _page_pitch(what, "k", c.k, shape, torch.uint8)
+    ld_scale = _page_pitch(what, "k_scale", c.k_scale, pairs, torch.float16)
+    if ld != _page_pitch(what, "v", c.v, shape, torch.uint8) or \
+            ld_scale != _page_pitch(what, "v_scale", c.v_scale, pairs, torch.float16):
+        _refuse(what, "keys and values must have one page pitch")
+    return _KvCache(c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), shape[0], ld, ld_scale, shape[1],
+                    shape[2], 2 * shape[3], 2 * shape[3] // groups)
+
+
+def _heads_pitch(what: str, name: str, t: torch.Tensor, shape, dtype):
+    """pitches of tokens and heads of t [tokens, heads, d], whose rows of d are contiguous"""
+    if t.shape != shape or t.dtype is not dtype:
+        _refuse(what, f"{name} must be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
+    tokens, heads, d = shape
+    ld, hd, unit = t.stride()
+    if heads <= 1:
+        hd = d  # (torch gives a single one any stride)
+    if tokens <= 1:
+        ld = max(heads, 1) * hd
+    if unit != 1 or hd < d or ld < d:
+        _refuse(what, f"{name}: the channels of a head must be contiguous, and rows apart")
+    return ld, hd
+
+
+def _sequences_arg(what: str, page_table: torch.Tensor, lengths: torch.Tensor, starts) -> _KvSequences:
+    if page_table.dim() != 2:
+        _refuse(what, "page_table must be [batch, pages]")
+    batch, columns = page_table.shape
+    ld = _pitch(what, "page_table", page_table, page_table.shape, torch.int32)
+    _dense(what, "lengths", lengths, (batch,), torch.int32)
+    if starts is not None:
+        _dense(what, "starts", starts, (batch + 1,), torch.int32)
+    return _KvSequences(page_table.data_ptr(), lengths.data_ptr(), _at(starts), ld, batch, columns)
+
+
+_QUERY_CODE = {torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _queries_arg(what: str, q: torch.Tensor, c: _KvCache, starts, max_queries, scale, causal, window) -> _KvAttentionParam:
+    if q.dim() != 3 or q.shape[2] != c.d:
+        _refuse(what, f"q must be [tokens, heads, {c.d}]")
+    code = _typed(what, "q", q, _QUERY_CODE)
+    ld, hd = _heads_pitch(what, "q", q, q.shape, q.dtype)
+    tokens, heads, d = q.shape
+    if starts is None:
+        max_queries = 1
+    elif max_queries is None:
+        max_queries = tokens
+    return _KvAttentionParam(tokens, max_queries, ld, hd, 0, 0, window, code, heads, int(causal),
+                             d ** -0.5 if scale is None else scale)
+
+
+def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
+    """Quantises rows k, v [tokens, kv_heads, d] (f16 / bf16 / f32; tokens and heads at any pitch, so slices of a fused projection
+    too) into the cache: token t to row slots[t] % page_size of page slots[t] // page_size (int64; a slot outside the cache, -1 for
+    padding, is not written; slots are distinct)."""
+    what = "kv_append"
+    c = _cache_arg(what, cache)
+    if k.dim() != 3:
+        _refuse(what, "k must be [tokens, kv_heads, d]")
+    t = k.shape[0]
+    shape = (t, c.kv_heads, c.d)
+    code = _typed(what, "k", k, _FLOAT_CODE)
+    ldk, hdk = _heads_pitch(what, "k", k, shape, k.dtype)
+    ldv, hdv = _heads_pitch(what, "v", v, shape, k.dtype)
+    _dense(what, "slots", slots, (t,), torch.int64)
+    _same_device(what, k, v, slots, *cache)
+    p = _KvAppendParam(t, ldk, hdk, ldv, hdv, code)
+    check(lib().ascq_kv_append(ctypes.byref(c), _at(k), _at(v), _at(slots), ctypes.byref(p), _stream(stream)), what)
+
+
+def kv_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, starts=None, max_queries=None,
+                 scale=None, causal: bool = True, window: int = 0, need_lse: bool = False, out=None, lse=None, workspace=None,
+                 stream=None):
+    """softmax(scale q k^T) v over the cached tokens of each sequence: q [tokens, heads, d] (f16 / bf16, tokens and heads at any
+    pitch), page_table int32 [batch, pages], lengths int32 [batch] (tokens cached, the queries' own among them).  starts int32
+    [batch + 1]: sequence b has the queries starts[b] .. starts[b + 1] - 1 (max_queries at most; give it, the launch is sized by it);
+    None: one each.  A query sees the tokens up to its own (causal) and, with window, no more than that many.  scale: 1 / sqrt(d)
+    if None.  Returns (out, lse): lse f32 [tokens, heads] when need_lse or a tensor for it is given, else None; rows of no sequence
+    are left as they were.  A table narrowed to the longest sequence's pages (page_table[:, :n]) makes the launch smaller.
+    workspace: a uint8 tensor of kv_attention_workspace_size bytes; without one the call takes it from torch's allocator."""
+    what = "kv_attention"
+    c = _cache_arg(what, cache)
+    s = _sequences_arg(what, page_table, lengths, starts)
+    p = _queries_arg(what, q, c, starts, max_queries, scale, causal, window)
+    o = out if out is not None else _new(stream, q.shape, q.dtype, q.device)
+    p.ld_out, p.hd_out = _heads_pitch(what, "out", o, q.shape, q.dtype)
+    if lse is None and need_lse:
+        lse = _new(stream, q.shape[:2], torch.float32, q.device)
+    if lse is not None:
+        _dense(what, "lse", lse, q.shape[:2], torch.float32)
+    room = _room(what, workspace)
+    _same_device(what, q, page_table, lengths, starts, o, lse, workspace, *cache)
+    if workspace is None:
+        need = ctypes.c_size_t(0)
+        check(lib().ascq_kv_attention_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(p), ctypes.byref(need)), what)
+        if need.value:
+            workspace, room = _new(stream, (need.value,), torch.uint8, q.device, private=True), need.value
+    check(lib().ascq_kv_attention(_at(o), _at(lse), _at(q), ctypes.byref(c), ctypes.byref(s), ctypes.byref(p), _at(workspace), room,
+                                  _stream(stream)), what)
+    return o, lse
+
+
+def kv_attention_workspace_size(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, starts=None, max_queries=None,
+                                causal: bool = True, window: int = 0) -> int:
+    """Bytes of the workspace that kv_attention uses for such a call (0: none)"""
+    what = "kv_attention_workspace_size"
+    c = _cache_arg(what, cache)
+    if page_table.dim() != 2:
+        _refuse(what, "page_table must be [batch, pages]")
+    s = _KvSequences(page_table.data_ptr(), page_table.data_ptr(), _at(starts), 0, *page_table.shape)
+    p = _queries_arg(what, q, c, starts, max_queries, None, causal, window)
+    need = ctypes.c_size_t(0)
+    check(lib().ascq_kv_attention_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(p), ctypes.byref(need)), what)
+    return need.value
+
+
+def kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weights=None,
+               decay: float = 1.0, starts=None, max_queries=None, scale=None, causal: bool = True, window: int = 0, out=None,
+               stream=None) -> torch.Tensor:
+    """The attention each cached token received from these queries, summed over them and over the heads of its key head, on top of
+    decay * weights: f32 [batch, kv_heads, cap], cap at least the page table's tokens.  lse as kv_attention returns it for the same
+    arguments.  out may be weights; positions from a sequence's length on stay as they were, or, without weights, are zeros."""
+    what = "kv_weights"
+    c = _cache_arg(what, cache)
+    s = _sequences_arg(what, page_table, lengths, starts)
+    p = _queries_arg(what, q, c, starts, max_queries, scale, causal, window)
+    _dense(what, "lse", lse, q.shape[:2], torch.float32)
+    cap = s.table_pages * c.page_size
+    for t in (weights, out):
+        if t is not None and t.dim() == 3:
+            cap = t.shape[2]
+    shape = (s.batch, c.kv_heads, cap)
+    if weights is not None:
+        _dense(what, "weights", weights, shape, torch.float32)
+    w = out
+    if w is None:
+        # (positions that the call leaves as they were hold what they held)
+        w = _new(stream, shape, torch.float32, q.device)
+        if weights is not None:
+            with torch.cuda.stream(torch.cuda.ExternalStream(_stream(stream), q.device)):
+                w.copy_(weights)
+    _dense(what, "out", w, shape, torch.float32)
+    _same_device(what, q, lse, page_table, lengths, starts, weights, w, *cache)
+    check(lib().ascq_kv_weights(_at(w), _at(weights), cap, decay, _at(q), _at(lse), ctypes.byref(c), ctypes.byref(s), ctypes.byref(p),
+                                _stream(stream)), what)
+    return w
+
+
+def kv_evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weights: torch.Tensor, keep: int, recent: int = 0,
+             into=None, kept=None, lengths_out=None, weights_out=None, stream=None):
+    """Cuts every sequence to its `keep` tokens of most weight (f32 [batch, kv_heads, cap], see kv_weights), the last `recent` always
+    among them, per key head.  They move in order to the sequence's first places: in its own pages, which no other sequence shares
+    then, or in the pages into (int32 [batch, n], none of page_table's), the old ones staying as they are.  Returns (kept, lengths,
+    weights): kept int32 [batch, kv_heads, keep], the tokens' former positions, -1 behind the last; the new lengths, a tensor of their
+    own; the kept tokens' weights, zeros behind them, in weights itself unless weights_out [batch, kv_heads, n] is given."""
+    what = "kv_evict"
+    c = _cache_arg(what, cache)
+    s = _sequences_arg(what, page_table, lengths, None)
+    if weights.dim() != 3 or keep < 1:
+        _refuse(what, "weights must be [batch, kv_heads, cap], keep at least 1")
+    heads = (s.batch, c.kv_heads)
+    _dense(what, "weights", weights, (*heads, weights.shape[2]), torch.float32)
+    w = weights if weights_out is None else weights_out
+    if w.dim() != 3:
+        _refuse(what, "weights_out must be [batch, kv_heads, n]")
+    _dense(what, "weights_out", w, (*heads, w.shape[2]), torch.float32)
+    ld_into = columns = 0
+    if into is not None:
+        if into.dim() != 2:
+            _refuse(what, "into must be [batch, pages]")
+        columns = into.shape[1]
+        ld_into = _pitch(what, "into", into, (s.batch, columns), torch.int32)
+    at = kept if kept is not None else _new(stream, (*heads, keep), torch.int32, weights.device)
+    _dense(what, "kept", at, (*heads, keep), torch.int32)
+    n = lengths_out if lengths_out is not None else _new(stream, (s.batch,), torch.int32, weights.device)
+    _dense(what, "lengths_out", n, (s.batch,), torch.int32)
+    _same_device(what, weights, page_table, lengths, into, at, n, w, *cache)
+    p = _KvEvictParam(weights.shape[2], w.shape[2], ld_into, keep, recent, columns)
+    check(lib().ascq_kv_evict(_at(at), _at(n), _at(w), _at(weights), _at(into), ctypes.byref(c), ctypes.byref(s), ctypes.byref(p),
+                              _stream(stream)), what)
+    return at, n, w
 
 
 # ------------------------------------------------------------------------------------------

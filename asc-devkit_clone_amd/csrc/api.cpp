@@ -1980,6 +1980,247 @@ ascq_status ascq_moe_combine_grad(float* grad_weights, void* grad_y, const void*
 }
 
 // ------------------------------------------------------------------------------------------------
+// attention over the paged int4 key / value cache
+// ------------------------------------------------------------------------------------------------
+namespace {
+ascq_status kv_cache_check(const char* what, const ascq_kv_cache* c, ascq::KvCacheArgs& a)
+{
+    if (!c) return fail(ASCQ_E_INVALID_ARG, "%s: null cache", what);
+    if (c->d != 64 && c->d != 128 && c->d != 256) return fail(ASCQ_E_UNSUPPORTED, "%s: d must be 64, 128 or 256", what);
+    if ((c->group != 32 && c->group != 64 && c->group != 128) || c->group > c->d)
+        return fail(ASCQ_E_UNSUPPORTED, "%s: group must be 32, 64 or 128, and at most d", what);
+    if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+        return fail(ASCQ_E_UNSUPPORTED, "%s: page_size must be a power of two, 16 .. 1024", what);
+    if (c->pages < 1 || c->kv_heads < 1) return fail(ASCQ_E_INVALID_ARG, "%s: bad cache shape", what);
+    if (c->pages > INT32_MAX || c->kv_heads > 1024) return fail(ASCQ_E_UNSUPPORTED, "%s: too many pages or heads", what);
+    const int64_t rows = (int64_t)c->kv_heads * c->page_size;
+    a.ld_code = c->ld_codes;
+    int64_t words = c->ld_scales;
+    if (!pitch(a.ld_code, rows * (c->d / 2)) || !pitch(words, rows * (c->d / c->group) * 2))
+        return fail(ASCQ_E_INVALID_ARG, "%s: a page pitch is smaller than the page", what);
+    if (a.ld_code % 16 || words % 8) return fail(ASCQ_E_INVALID_ARG, "%s: page pitches must be multiples of 16 bytes", what);
+    if (!addressable(c->pages, a.ld_code) || !addressable(c->pages, words)) return fail(ASCQ_E_UNSUPPORTED, "%s: cache too large", what);
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(ASCQ_E_INVALID_ARG, "%s: null argument", what);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))
+        return fail(ASCQ_E_INVALID_ARG, "%s: the cache must be 16-byte aligned", what);
+    a.k = (uint8_t*)c->k;
+    a.v = (uint8_t*)c->v;
+    a.k_scale = (uint32_t*)c->k_scale;
+    a.v_scale = (uint32_t*)c->v_scale;
+    a.pages = c->pages;
+    a.ld_scale = words / 2;
+    a.kv_heads = c->kv_heads;
+    a.page_shift = __builtin_ctz((unsigned)c->page_size);
+    a.d = c->d;
+    a.group = c->group;
+    return ASCQ_OK;
+}
+
+ascq_status kv_sequences_check(const char* what, const ascq_kv_sequences* s, const ascq::KvCacheArgs& c, ascq::KvSequences& a)
+{
+    if (!s) return fail(ASCQ_E_INVALID_ARG, "%s: null sequences", what);
+    if (s->batch < 0 || s->table_pages < 0) return fail(ASCQ_E_INVALID_ARG, "%s: bad shape", what);
+    if (((int64_t)s->table_pages << c.page_shift) > (1 << 30))
+        return fail(ASCQ_E_UNSUPPORTED, "%s: a sequence has room for more than 2^30 tokens", what);
+    a.ld_table = s->ld_table;
+    if (!pitch(a.ld_table, s->table_pages)) return fail(ASCQ_E_INVALID_ARG, "%s: a row pitch is smaller than the row", what);
+    if (!addressable(s->batch, a.ld_table)) return fail(ASCQ_E_UNSUPPORTED, "%s: tensor too large", what);
+    if (s->batch > 0 && ((s->table_pages > 0 && !s->page_table) || !s->lengths))
+        return fail(ASCQ_E_INVALID_ARG, "%s: null argument", what);
+    if (!aligned(s->page_table, 4) || !aligned(s->lengths, 4) || !aligned(s->starts, 4))
+        return fail(ASCQ_E_INVALID_ARG, "%s: a pointer is not aligned to its element type", what);
+    a.table = s->page_table;
+    a.lengths = s->lengths;
+    a.starts = s->starts;
+    a.batch = s->batch;
+    a.table_pages = s->table_pages;
+    return ASCQ_OK;
+}
+
+// (workgroups of one sequence go in one launch)
+constexpr int64_t kKvGroups = 1 << 23;
+
+ascq_status kv_attention_args(const char* what, const ascq_kv_cache* cache, const ascq_kv_sequences* sequences,
+                              const ascq_kv_attention_param* p, ascq::KvAttentionArgs& a)
+{
+    if (!p) return fail(ASCQ_E_INVALID_ARG, "%s: null params", what);
+    ascq_status s = kv_cache_check(what, cache, a.c);
+    if (s != ASCQ_OK) return s;
+    s = kv_sequences_check(what, sequences, a.c, a.s);
+    if (s != ASCQ_OK) return s;
+    if (p->type != ASCQ_DT_F16 && p->type != ASCQ_DT_BF16) return fail(ASCQ_E_UNSUPPORTED, "%s: queries must be f16 or bf16", what);
+    if (p->tokens < 0 || p->max_queries < 0 || p->window < 0) return fail(ASCQ_E_INVALID_ARG, "%s: bad shape", what);
+    if (p->heads < 1 || p->heads % a.c.kv_heads) return fail(ASCQ_E_INVALID_ARG, "%s: heads must be a multiple of the key heads", what);
+    if (p->heads > 65536) return fail(ASCQ_E_UNSUPPORTED, "%s: at most 65536 heads", what);
+    if (p->causal != 0 && p->causal != 1) return fail(ASCQ_E_INVALID_ARG, "%s: causal must be 0 or 1", what);
+    if (!(__builtin_fabsf(p->scale) <= 3.402823466e38f)) return fail(ASCQ_E_INVALID_ARG, "%s: scale must be finite", what);
+    if (!a.s.starts && p->tokens != a.s.batch) return fail(ASCQ_E_INVALID_ARG, "%s: without starts q has one row per sequence", what);
+    if (p->tokens > INT32_MAX) return fail(ASCQ_E_UNSUPPORTED, "%s: at most 2^31 - 1 tokens", what);
+    a.hd_q = p->hd_q;
+    a.hd_out = p->hd_out;
+    if (!pitch(a.hd_q, a.c.d) || !pitch(a.hd_out, a.c.d)) return fail(ASCQ_E_INVALID_ARG, "%s: a head pitch is smaller than d", what);
+    a.ld_q = p->ld_q ? p->ld_q : a.hd_q * p->heads;
+    a.ld_out = p->ld_out ? p->ld_out : a.hd_out * p->heads;
+    if (a.ld_q < a.c.d || a.ld_out < a.c.d) return fail(ASCQ_E_INVALID_ARG, "%s: a row pitch is smaller than the row", what);
+    if (!addressable(p->tokens, a.ld_q) || !addressable(p->heads, a.hd_q) || !addressable(p->tokens, a.ld_out) ||
+        !addressable(p->heads, a.hd_out))
+        return fail(ASCQ_E_UNSUPPORTED, "%s: tensor too large", what);
+    a.T = (int)p->tokens;
+    const int64_t queries = a.s.starts ? p->max_queries : 1;
+    a.max_q = (int)(queries < p->tokens ? queries : p->tokens);
+    a.type = p->type;
+    a.heads = p->heads;
+    a.causal = p->causal;
+    a.window = p->window >= 1 << 30 ? 0 : (int)p->window;  // (a sequence has fewer tokens)
+    a.scale = p->scale;
+    const int64_t tiles = ((int64_t)a.max_q * (p->heads / a.c.kv_heads) + 15) / 16;
+    if (tiles * a.c.kv_heads > kKvGroups) return fail(ASCQ_E_UNSUPPORTED, "%s: too many queries of one sequence", what);
+    return ASCQ_OK;
+}
+}  // namespace
+
+ascq_status ascq_kv_append(const ascq_kv_cache* cache, const void* k, const void* v, const int64_t* slots,
+                           const ascq_kv_append_param* p, void* stream)
+{
+    CallScope scope;
+    const char* what = "kv_append";
+    if (!p) return fail(ASCQ_E_INVALID_ARG, "%s: null params", what);
+    ascq::KvAppendArgs a{};
+    const ascq_status s = kv_cache_check(what, cache, a.c);
+    if (s != ASCQ_OK) return s;
+    if (!float_type(p->type)) return fail(ASCQ_E_UNSUPPORTED, "%s: rows must be f16, bf16 or f32", what);
+    if (p->tokens < 0) return fail(ASCQ_E_INVALID_ARG, "%s: bad shape", what);
+    a.hd_k = p->hd_k;
+    a.hd_v = p->hd_v;
+    if (!pitch(a.hd_k, a.c.d) || !pitch(a.hd_v, a.c.d)) return fail(ASCQ_E_INVALID_ARG, "%s: a head pitch is smaller than d", what);
+    a.ld_k = p->ld_k ? p->ld_k : a.hd_k * a.c.kv_heads;
+    a.ld_v = p->ld_v ? p->ld_v : a.hd_v * a.c.kv_heads;
+    if (a.ld_k < a.c.d || a.ld_v < a.c.d) return fail(ASCQ_E_INVALID_ARG, "%s: a row pitch is smaller than the row", what);
+    if (p->tokens > INT32_MAX || !addressable(p->tokens, a.ld_k) || !addressable(p->tokens, a.ld_v) ||
+        !addressable(a.c.kv_heads, a.hd_k) || !addressable(a.c.kv_heads, a.hd_v))
+        return fail(ASCQ_E_UNSUPPORTED, "%s: tensor too large", what);
+    if (p->tokens == 0) return ASCQ_OK;
+    if (!k || !v || !slots) return fail(ASCQ_E_INVALID_ARG, "%s: null argument", what);
+    if (!aligned(k, float_bytes(p->type)) || !aligned(v, float_bytes(p->type)) || !aligned(slots, 8))
+        return fail(ASCQ_E_INVALID_ARG, "%s: a pointer is not aligned to its element type", what);
+    a.k = k;
+    a.v = v;
+    a.slots = slots;
+    a.type = p->type;
+    a.T = p->tokens;
+    trace("kv_append: type %d, T %lld, heads %d d %d group %d", a.type, (long long)a.T, a.c.kv_heads, a.c.d, a.c.group);
+    return hip_status(ascq::launch_kv_append(a, S(stream)), what);
+}
+
+ascq_status ascq_kv_attention_workspace_size(const ascq_kv_cache* cache, const ascq_kv_sequences* sequences,
+                                             const ascq_kv_attention_param* p, size_t* bytes)
+{
+    if (!bytes) return fail(ASCQ_E_INVALID_ARG, "kv_attention_workspace_size: null argument");
+    ascq::KvAttentionArgs a{};
+    const ascq_status s = kv_attention_args("kv_attention_workspace_size", cache, sequences, p, a);
+    if (s != ASCQ_OK) return s;
+    *bytes = a.s.batch == 0 || a.max_q == 0 ? 0 : ascq::kv_attention_ws_bytes(a);
+    return ASCQ_OK;
+}
+
+ascq_status ascq_kv_attention(void* out, float* lse, const void* q, const ascq_kv_cache* cache,
+                              const ascq_kv_sequences* sequences, const ascq_kv_attention_param* p, void* workspace,
+                              size_t workspace_bytes, void* stream)
+{
+    CallScope scope;
+    ascq::KvAttentionArgs a{};
+    const ascq_status s = kv_attention_args("kv_attention", cache, sequences, p, a);
+    if (s != ASCQ_OK) return s;
+    if (a.s.batch == 0 || a.max_q == 0) return ASCQ_OK;
+    if (!out || !q) return fail(ASCQ_E_INVALID_ARG, "kv_attention: null argument");
+    if (!aligned(out, 2) || !aligned(q, 2) || !aligned(lse, 4))
+        return fail(ASCQ_E_INVALID_ARG, "kv_attention: a pointer is not aligned to its element type");
+    a.q = q;
+    a.out = out;
+    a.lse = lse;
+    trace("kv_attention: type %d, B %d, queries %d, heads %d / %d d %d group %d, pages of %d", a.type, a.s.batch, a.max_q, a.heads,
+          a.c.kv_heads, a.c.d, a.c.group, 1 << a.c.page_shift);
+    // (a workspace off its alignment is none)
+    void* ws = workspace && aligned(workspace, 16) ? workspace : nullptr;
+    return hip_status(ascq::launch_kv_attention(a, ws, ws ? workspace_bytes : 0, S(stream)), "kv_attention");
+}
+
+ascq_status ascq_kv_weights(float* weights_out, const float* weights, int64_t cap, float decay, const void* q, const float* lse,
+                            const ascq_kv_cache* cache, const ascq_kv_sequences* sequences, const ascq_kv_attention_param* p,
+                            void* stream)
+{
+    CallScope scope;
+    ascq::KvAttentionArgs a{};
+    const ascq_status s = kv_attention_args("kv_weights", cache, sequences, p, a);
+    if (s != ASCQ_OK) return s;
+    if (cap < (int64_t)a.s.table_pages << a.c.page_shift)
+        return fail(ASCQ_E_INVALID_ARG, "kv_weights: rows of weights are shorter than the page table's tokens");
+    if (cap > (1 << 30) || (cap / 128 + 1) * a.c.kv_heads > kKvGroups) return fail(ASCQ_E_UNSUPPORTED, "kv_weights: rows too long");
+    if (!(__builtin_fabsf(decay) <= 3.402823466e38f)) return fail(ASCQ_E_INVALID_ARG, "kv_weights: decay must be finite");
+    if (a.s.batch == 0 || cap == 0) return ASCQ_OK;
+    if (!weights_out || (a.max_q > 0 && (!q || !lse))) return fail(ASCQ_E_INVALID_ARG, "kv_weights: null argument");
+    if (!aligned(weights_out, 4) || !aligned(weights, 4) || !aligned(q, 2) || !aligned(lse, 4))
+        return fail(ASCQ_E_INVALID_ARG, "kv_weights: a pointer is not aligned to its element type");
+    a.q = q;
+    a.lse = const_cast<float*>(lse);
+    a.w_in = weights;
+    a.w_out = weights_out;
+    a.cap = (int)cap;
+    a.decay = decay;
+    trace("kv_weights: type %d, B %d, queries %d, heads %d / %d d %d group %d", a.type, a.s.batch, a.max_q, a.heads, a.c.kv_heads,
+          a.c.d, a.c.group);
+    return hip_status(ascq::launch_kv_weights(a, S(stream)), "kv_weights");
+}
+
+ascq_status ascq_kv_evict(int32_t* kept, int32_t* new_lengths, float* weights_out, const float* weights, const int32_t* into,
+                          const ascq_kv_cache* cache, const ascq_kv_sequences* sequences, const ascq_kv_evict_param* p,
+                          void* stream)
+{
+    CallScope scope;
+    const char* what = "kv_evict";
+    if (!p) return fail(ASCQ_E_INVALID_ARG, "%s: null params", what);
+    ascq::KvEvictArgs a{};
+    ascq_status s = kv_cache_check(what, cache, a.c);
+    if (s != ASCQ_OK) return s;
+    s = kv_sequences_check(what, sequences, a.c, a.s);
+    if (s != ASCQ_OK) return s;
+    if (p->keep < 1 || p->recent < 0 || p->recent > p->keep)
+        return fail(ASCQ_E_INVALID_ARG, "%s: 0 <= recent <= keep and keep >= 1", what);
+    if (p->cap < (int64_t)a.s.table_pages << a.c.page_shift)
+        return fail(ASCQ_E_INVALID_ARG, "%s: rows of weights are shorter than the page table's tokens", what);
+    if (p->cap_out < (p->keep < p->cap ? p->keep : p->cap))
+        return fail(ASCQ_E_INVALID_ARG, "%s: rows of weights_out are shorter than what is kept", what);
+    if (p->cap > 1 << 30 || p->cap_out > 1 << 30 || p->keep > 1 << 30) return fail(ASCQ_E_UNSUPPORTED, "%s: rows too long", what);
+    a.ld_into = p->ld_into;
+    if (into && (p->into_pages < 0 || !pitch(a.ld_into, p->into_pages)))
+        return fail(ASCQ_E_INVALID_ARG, "%s: a row pitch is smaller than the row", what);
+    if (into && (int64_t)p->into_pages << a.c.page_shift < p->keep)
+        return fail(ASCQ_E_INVALID_ARG, "%s: the pages of into hold less than what is kept", what);
+    if (into && !addressable(a.s.batch, a.ld_into)) return fail(ASCQ_E_UNSUPPORTED, "%s: tensor too large", what);
+    if (a.s.batch == 0) return ASCQ_OK;
+    if (!kept || !new_lengths || (p->cap > 0 && !weights) || (p->cap_out > 0 && !weights_out))
+        return fail(ASCQ_E_INVALID_ARG, "%s: null argument", what);
+    if (new_lengths == a.s.lengths) return fail(ASCQ_E_INVALID_ARG, "%s: new_lengths must not be lengths", what);
+    if (weights == weights_out && p->cap != p->cap_out) return fail(ASCQ_E_INVALID_ARG, "%s: weights in place need their row length", what);
+    if (into && into == a.s.table) return fail(ASCQ_E_INVALID_ARG, "%s: into must not be the page table (NULL: in place)", what);
+    if (!aligned(kept, 4) || !aligned(new_lengths, 4) || !aligned(weights, 4) || !aligned(weights_out, 4) || !aligned(into, 4))
+        return fail(ASCQ_E_INVALID_ARG, "%s: a pointer is not aligned to its element type", what);
+    a.weights = weights;
+    a.weights_out = weights_out;
+    a.kept = kept;
+    a.lengths_out = new_lengths;
+    a.into = into;
+    a.cap = p->cap;
+    a.cap_out = p->cap_out;
+    a.into_pages = p->into_pages;
+    a.keep = p->keep;
+    a.recent = p->recent;
+    trace("kv_evict: B %d, heads %d d %d group %d, keep %d recent %d%s", a.s.batch, a.c.kv_heads, a.c.d, a.c.group, a.keep, a.recent,
+          into ? "" : ", in place");
+    return hip_status(ascq::launch_kv_evict(a, S(stream)), what);
+}
+
+// ------------------------------------------------------------------------------------------------
 // NZ fractal <-> ND
 // ------------------------------------------------------------------------------------------------
 namespace {

@@ -340,4 +340,63 @@ hipError_t launch_moe_dispatch(const MoeRowsArgs& a, hipStream_t st);
 hipError_t launch_moe_combine(const MoeRowsArgs& a, hipStream_t st);
 hipError_t launch_moe_combine_grad(const MoeRowsArgs& a, hipStream_t st);
 
+// The paged int4 key / value cache (kv_cache.hip, kv_attention.hip): codes [pages][kv_heads][1 << page_shift][d / 2] and
+// scales [pages][kv_heads][1 << page_shift][d / group] words (f16 scale, f16 offset); pages ld_code bytes and ld_scale
+// words apart
+struct KvCacheArgs {
+    uint8_t *k, *v;
+    uint32_t *k_scale, *v_scale;
+    int64_t pages, ld_code, ld_scale;
+    int kv_heads, page_shift, d, group;
+};
+// the sequences: sequence b holds lengths[b] tokens, token t on page table[b * ld_table + (t >> page_shift)]; its queries are
+// rows starts[b] .. starts[b + 1] of q, the last at the sequence's last token (starts null: row b alone)
+struct KvSequences {
+    const int *table, *lengths, *starts;
+    int64_t ld_table;
+    int table_pages, batch;
+};
+struct KvAppendArgs {
+    KvCacheArgs c;
+    const void *k, *v;      // [T] rows of kv_heads x d, ld_* elements from token to token, hd_* from head to head
+    int type;
+    int64_t T, ld_k, hd_k, ld_v, hd_v;
+    const int64_t* slots;   // [T]: page * page_size + token of the page; others are not written
+    int64_t first;          // (set by the launcher) the launch's first token
+};
+hipError_t launch_kv_append(KvAppendArgs a, hipStream_t st);
+struct KvAttentionArgs {
+    KvCacheArgs c;
+    KvSequences s;
+    const void* q;          // [T, heads, d] f16 / bf16 (type), ld_q from token to token, hd_q from head to head
+    void* out;              // attention: [T, heads, d] of q's type
+    float* lse;             // [T, heads]; attention: may be null; weights: read
+    const float* w_in;      // weights: [batch, kv_heads, cap] or null
+    float* w_out;
+    float* part;            // (set by the launcher) where the splits leave their sums
+    int64_t ld_q, hd_q, ld_out, hd_out;
+    int T, cap, type, heads, max_q, window, causal;
+    float scale, decay;
+    // (set by the launcher) heads per key head, tiles of 16 rows per sequence and key head, rows in use of a tile, token
+    // range of a split and how many, the launch's first sequence
+    int ratio, tiles, rows, chunk, splits, first;
+};
+// workspace (16-byte aligned, or null): room for the sums of ranges of tokens; with less a sequence is one range
+size_t kv_attention_ws_bytes(KvAttentionArgs a);
+hipError_t launch_kv_attention(KvAttentionArgs a, void* ws, size_t ws_bytes, hipStream_t st);
+hipError_t launch_kv_weights(KvAttentionArgs a, hipStream_t st);
+struct KvEvictArgs {
+    KvCacheArgs c;
+    KvSequences s;
+    const float* weights;   // [batch, kv_heads, cap]
+    float* weights_out;     // [batch, kv_heads, cap_out]; may be weights (cap_out = cap)
+    int* kept;              // [batch, kv_heads, keep]
+    int* lengths_out;       // [batch]
+    const int* into;        // pages that the kept tokens go to [batch, ld_into], or null: the sequence's own
+    int64_t cap, cap_out, ld_into;
+    int into_pages, keep, recent;
+    int64_t first;          // (set by the launcher) the launch's first sequence
+};
+hipError_t launch_kv_evict(KvEvictArgs a, hipStream_t st);
+
 }  // namespace ascq

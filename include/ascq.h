@@ -678,6 +678,111 @@ ascq_status ascq_moe_combine_grad(float* grad_weights, void* grad_y, const void*
                                   const ascq_rows_param* p, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention over a paged key / value cache held in int4: no counterpart in the reference's hot path.
+ *
+ * A cached row -- a token's keys or values in one key head, d channels -- is d / 2 bytes of int4 codes (two's complement,
+ * even channel in the low nibble) and one f16 pair (scale, offset) per `group` channels, and stands for
+ *     value(c) = f16(c scale + offset), one rounding.
+ * Pools, 16-byte aligned: codes k, v [pages, kv_heads, page_size, d / 2] bytes; k_scale, v_scale [pages, kv_heads, page_size,
+ * d / group, 2] f16; ld_codes bytes (a multiple of 16) and ld_scales f16 elements (a multiple of 8) from page to page, 0 for
+ * dense pools.  d 64, 128 or 256; group 32, 64 or 128, at most d; page_size a power of two, 16 .. 1024.
+ *
+ * Sequence b holds lengths[b] tokens, token t in row t % page_size of page page_table[b, t / page_size].  A length counts as at
+ * least 0 and at most table_pages * page_size; a token whose page is not in [0, pages) is masked.  Sequence b's queries are
+ * the rows starts[b] .. starts[b + 1] - 1 of q, of which max_queries at most are computed (starts NULL: row b alone, and q has
+ * `batch` rows).  Rows past those, and rows of no sequence, are left as they were.  The last query stands at the sequence's
+ * last token: query i of n sees token t when t <= length - n + i (causal) and, with a window, t > length - n + i - window.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+    void *k, *v;
+    void *k_scale, *v_scale;
+    int64_t pages, ld_codes, ld_scales;
+    int32_t kv_heads, page_size, d, group;
+} ascq_kv_cache;
+
+typedef struct {
+    const int32_t* page_table; /* [batch, table_pages], rows ld_table apart (0: dense) */
+    const int32_t* lengths;    /* [batch] */
+    const int32_t* starts;     /* [batch + 1] or NULL */
+    int64_t ld_table;
+    int32_t batch, table_pages;
+} ascq_kv_sequences;
+
+typedef struct {
+    int64_t tokens;
+    int64_t ld_k, hd_k, ld_v, hd_v; /* elements from token to token (0: dense) and from head to head (0: d) */
+    int32_t type;                   /* F16, BF16, F32: k, v */
+} ascq_kv_append_param;
+
+/* Rows k, v [tokens, kv_heads, d] into the cache: token t goes to row slots[t] % page_size of page slots[t] / page_size; a slot
+ * outside [0, pages * page_size) is not written.  The slots of a call are distinct (which of two equal ones stays, or parts of
+ * which, is not defined).  Per group, in fp32 and in this order, with NaN taken as 0 and magnitudes as 61440 at most (so that
+ * every value is a finite f16):
+ *   scale = f16((max - min) / 15),  offset = f16(min + 8 scale),
+ *   c = clamp(rint((x - offset) (1 / scale)), -8, 7), or 0 where scale is 0.
+ * (There is no counterpart in the reference.) */
+ascq_status ascq_kv_append(const ascq_kv_cache* cache, const void* k, const void* v, const int64_t* slots,
+                           const ascq_kv_append_param* p, void* stream);
+
+typedef struct {
+    int64_t tokens;                     /* rows of q */
+    int64_t max_queries;                /* of a sequence, at most; not read without starts */
+    int64_t ld_q, hd_q, ld_out, hd_out; /* elements from token to token (0: dense) and from head to head (0: d) */
+    int64_t window;                     /* tokens up to its own that a query sees; 0: all */
+    int32_t type;                       /* F16, BF16: q, out */
+    int32_t heads;                      /* query heads, a multiple of kv_heads */
+    int32_t causal;                     /* 0, 1 */
+    float scale;
+} ascq_kv_attention_param;
+
+/* out [tokens, heads, d] = softmax(scale q k^T over what a query sees) v, query head h on key head h / (heads / kv_heads); lse (f32
+ * [tokens, heads], or NULL) the log of the sum of exp of the scaled scores.  A query that sees nothing gives zeros and -inf.
+ * Scores and sums are fp32 over the cache's exact values, softmax weights are rounded to f16.  What a query sees has to be finite
+ * (as ascq_kv_append leaves it); what lies behind a sequence's length may be anything.
+ * workspace: optional, 16-byte aligned, ascq_kv_attention_workspace_size bytes (0 for many calls; it depends on the sizes alone):
+ * room for partial sums where several workgroups share a sequence's tokens; with less, or none, they do not.
+ * (There is no counterpart in the reference.) */
+ascq_status ascq_kv_attention(void* out, float* lse, const void* q, const ascq_kv_cache* cache,
+                              const ascq_kv_sequences* sequences, const ascq_kv_attention_param* p, void* workspace,
+                              size_t workspace_bytes, void* stream);
+/* (There is no counterpart in the reference.) */
+ascq_status ascq_kv_attention_workspace_size(const ascq_kv_cache* cache, const ascq_kv_sequences* sequences,
+                                             const ascq_kv_attention_param* p, size_t* bytes);
+
+/* The attention that cached tokens received:
+ *   weights_out[b, g, t] = decay weights[b, g, t] + sum over sequence b's queries that see t, and over the heads of key head g, of
+ *                          exp(scale q k_t - lse)
+ * with lse as ascq_kv_attention leaves it (-inf: the query gives nothing).  weights, weights_out f32 [batch, kv_heads, cap], cap >=
+ * table_pages * page_size; weights_out may be weights.  Positions from a sequence's length on are left as they were; with weights
+ * NULL the rows of weights_out are written whole, zeros from the length on.  Sums are fp32 in a fixed order: equal inputs give equal
+ * bits.  ld_out and hd_out are not read.  (There is no counterpart in the reference.) */
+ascq_status ascq_kv_weights(float* weights_out, const float* weights, int64_t cap, float decay, const void* q, const float* lse,
+                            const ascq_kv_cache* cache, const ascq_kv_sequences* sequences, const ascq_kv_attention_param* p,
+                            void* stream);
+
+typedef struct {
+    int64_t cap, cap_out; /* row lengths of weights and weights_out */
+    int64_t ld_into;      /* rows of into (0: dense) */
+    int32_t keep;         /* >= 1 */
+    int32_t recent;       /* 0 .. keep */
+    int32_t into_pages;   /* columns of into */
+} ascq_kv_evict_param;
+
+/* Cuts every sequence to `keep` tokens, per key head: of a longer one the last `recent` stay, and of the others the keep - recent
+ * with the largest weights (NaN below every number; of equal ones the first).  They move, in order, to the first places -- of the
+ * sequence's own pages (into NULL), which no other sequence shares then, or of the pages into [batch, into_pages] (into_pages *
+ * page_size >= keep), which are none of page_table's and distinct.  A shorter sequence moves to into whole.
+ *   kept        int32 [batch, kv_heads, keep]: the former positions of what stays, -1 behind the last
+ *   new_lengths int32 [batch]: min(length, keep); not lengths itself
+ *   weights_out f32 [batch, kv_heads, cap_out]: the weights of what stays, then zeros; may be weights (cap_out = cap)
+ * weights f32 [batch, kv_heads, cap], cap >= table_pages * page_size; cap_out >= min(keep, cap).  sequences->starts is not read.  A
+ * token on a page that does not exist moves as zeros; nothing is written to a page that does not exist.
+ * (There is no counterpart in the reference.) */
+ascq_status ascq_kv_evict(int32_t* kept, int32_t* new_lengths, float* weights_out, const float* weights, const int32_t* into,
+                          const ascq_kv_cache* cache, const ascq_kv_sequences* sequences, const ascq_kv_evict_param* p,
+                          void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * NZ fractal <-> ND layout converters
  * CubeFormat::NZ (include/adv_api/matmul/matmul_config.h:23-35): each [rows, cols] matrix of a batch is stored
  * [ceil(cols / C0)][ceil(rows / 16)][16][C0], C0 = 32 bytes of elements (int8 / fp8: 32, f16 / bf16: 16,
