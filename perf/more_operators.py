@@ -226,7 +226,8 @@ def prepare(case, seed):
     if own:
         s["kv"] = _lib().KvCache(**s["cache"])
         if op == "attention":
-            bytes_ = _lib().kv_attention_workspace_size(s["q"], s["kv"], s["table"], starts=s["starts"], max_queries=c["queries"])
+            bytes_ = _lib().kv_attention_workspace_size(s["q"], s["kv"], s["table"], starts=s["starts"], max_queries=c["queries"],
+                                                        window=c["window"])
             s["buf"]["workspace"] = empty(max(bytes_, 1), torch.uint8)
     return s
 
