@@ -17,6 +17,8 @@
 // fp32.
 #include "common.h"
 
+#include <type_traits>
+
 namespace ascq {
 
 namespace {
@@ -52,8 +54,8 @@ struct Range {
 };
 __device__ __forceinline__ Range range_of(const KvAttentionArgs& a, const View& v, int tile)
 {
-    const int first = tile * 16 / a.ratio;
-    int last = (tile * 16 + 15) / a.ratio;
+    const int first = tile * a.tile_rows / a.ratio;
+    int last = (tile * a.tile_rows + a.tile_rows - 1) / a.ratio;
     last = last < v.rows ? last : v.rows - 1;
     Range r{0, v.len};
     const int64_t at = (int64_t)v.len - v.n;  // the first query's token
@@ -73,10 +75,13 @@ struct Half {
     int64_t code, scale;  // bytes, words
     bool ok;
 };
-__device__ __forceinline__ Half half_at(const KvAttentionArgs& a, const int* table, int h, int token)
+__device__ __forceinline__ int page_at(const KvAttentionArgs& a, const int* table, int token)
 {
     const int col = token >> a.c.page_shift;
-    const int page = col < a.s.table_pages ? table[col] : -1;
+    return col < a.s.table_pages ? table[col] : -1;
+}
+__device__ __forceinline__ Half half_at(const KvAttentionArgs& a, int page, int h, int token)
+{
     Half r;
     r.ok = page >= 0 && page < a.c.pages;
     const int64_t p = r.ok ? page : 0;
@@ -137,62 +142,79 @@ struct Step {
     uint32_t k[2][Shape<D>::KW], ks[2][KS], v[8][Shape<D>::VW], vs[8];
 };
 
+// Where a lane's parts begin, in bytes behind the row of 16 tokens that a scalar address gives
+struct Lane {
+    uint32_t k, ks, v, vs;
+};
+template <class T>
+__device__ __forceinline__ T read(const void* row, uint32_t lane, int words = 0)
+{
+    return *(const T*)((const uint8_t*)row + lane + 4 * words);
+}
+
 template <int D, int G>
-__device__ __forceinline__ void load_step(Step<D, G>& x, const KvAttentionArgs& a, const Half (&half)[2], int r, int j)
+__device__ __forceinline__ void load_step(Step<D, G>& x, const KvAttentionArgs& a, const Half (&half)[2], const Lane& at)
 {
     constexpr int W = D / 8, GR = D / G;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const uint32_t* k = (const uint32_t*)(a.c.k + half[h].code) + r * W + j * (W / 4);
+        const uint8_t *k = a.c.k + half[h].code, *v = a.c.v + half[h].code;
+        const uint32_t *ks = a.c.k_scale + half[h].scale, *vs = a.c.v_scale + half[h].scale;
         if constexpr (Shape<D>::KW == 2) {
-            const u32x2 t = *(const u32x2*)k;
+            const u32x2 t = read<u32x2>(k, at.k);
             x.k[h][0] = t[0], x.k[h][1] = t[1];
         } else {
 #pragma unroll
             for (int i = 0; i < Shape<D>::KW; i += 4) {
-                const u32x4 t = *(const u32x4*)(k + i);
+                const u32x4 t = read<u32x4>(k, at.k, i);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x.k[h][i + e] = t[e];
             }
         }
-        const uint32_t* ks = a.c.k_scale + half[h].scale + r * GR + j * (D / 4) / G;
 #pragma unroll
-        for (int i = 0; i < Step<D, G>::KS; ++i) x.ks[h][i] = ks[i];
-        const uint32_t* v = (const uint32_t*)(a.c.v + half[h].code) + 4 * j * W + (D == 64 ? r >> 1 : r * Shape<D>::VW);
-        const uint32_t* vs = a.c.v_scale + half[h].scale + 4 * j * GR + r * (D / 16) / G;
+        for (int i = 0; i < Step<D, G>::KS; ++i) x.ks[h][i] = read<uint32_t>(ks, at.ks, i);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (Shape<D>::VW == 2) {
-                const u32x2 t = *(const u32x2*)(v + i * W);
+                const u32x2 t = read<u32x2>(v, at.v, i * W);
                 x.v[4 * h + i][0] = t[0], x.v[4 * h + i][1] = t[1];
             } else {
-                x.v[4 * h + i][0] = v[i * W];
+                x.v[4 * h + i][0] = read<uint32_t>(v, at.v, i * W);
             }
-            x.vs[4 * h + i] = vs[i * GR];
+            x.vs[4 * h + i] = read<uint32_t>(vs, at.vs, i * GR);
         }
     }
 }
-
-// the scores of 16 rows against 32 tokens: s[h][i] is row r, token 16 h + 4 j + i
 template <int D, int G>
-__device__ __forceinline__ void scores(v4f (&s)[2], const uint32_t (&k)[2][Shape<D>::KW],
-                                       const uint32_t (&ks)[2][Step<D, G>::KS], const h8 (&q)[Shape<D>::STEPS])
+__device__ __forceinline__ Lane lane_of_step(int r, int j)
+{
+    constexpr int W = D / 8, GR = D / G;
+    return Lane{4u * (r * W + j * (W / 4)), 4u * (r * GR + j * (D / 4) / G),
+                4u * (4 * j * W + (D == 64 ? r >> 1 : r * Shape<D>::VW)), 4u * (4 * j * GR + r * (D / 16) / G)};
+}
+
+// the scores of NQ times 16 rows against 32 tokens: s[c][h][i] is row 16 c + r, token 16 h + 4 j + i
+template <int D, int G, int NQ>
+__device__ __forceinline__ void scores(v4f (&s)[NQ][2], const uint32_t (&k)[2][Shape<D>::KW],
+                                       const uint32_t (&ks)[2][Step<D, G>::KS], const h8 (&q)[NQ][Shape<D>::STEPS])
 {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        s[h] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) s[c][h] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < Shape<D>::STEPS; ++i) {
             const uint32_t w = ks[h][i * Step<D, G>::KS / Shape<D>::STEPS];
             const h8 f = key_fragment(k[h][i], low_pair(w, w), high_pair(w, w));
-            s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[i], s[h], 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) s[c][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, q[c][i], s[c][h], 0, 0, 0);
         }
     }
 }
 
 // O^T += V^T P^T of 32 tokens: tile n's rows are the channels r (D / 16) + n
-template <int D, int G>
-__device__ __forceinline__ void add_values(v4f (&acc)[Shape<D>::TILES], const Step<D, G>& x, h8 p, int r)
+template <int D, int G, int NQ>
+__device__ __forceinline__ void add_values(v4f (&acc)[NQ][Shape<D>::TILES], const Step<D, G>& x, const h8 (&p)[NQ], int r)
 {
     h2 s[4], o[4];
 #pragma unroll
@@ -205,18 +227,14 @@ __device__ __forceinline__ void add_values(v4f (&acc)[Shape<D>::TILES], const St
         constexpr int HALVES = D == 64 ? 1 : 2;
 #pragma unroll
         for (int half = 0; half < HALVES; ++half) {
-            uint32_t y[4];  // a pair of tokens: 4 channels each
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint32_t sel = D == 64 ? (r & 1 ? 0x07060302u : 0x05040100u) : half ? 0x07060302u : 0x05040100u;
-                y[u] = __builtin_amdgcn_perm(x.v[2 * u + 1][w], x.v[2 * u][w], sel);
-            }
             h8 f[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const uint32_t y8 = y[u] >> 8;
-                const h2 c0 = __builtin_elementwise_fma(codes_of<0>(y[u]), s[u], o[u]);
-                const h2 c1 = __builtin_elementwise_fma(codes_of<1>(y[u]), s[u], o[u]);
+                const uint32_t sel = D == 64 ? (r & 1 ? 0x07060302u : 0x05040100u) : half ? 0x07060302u : 0x05040100u;
+                const uint32_t y = __builtin_amdgcn_perm(x.v[2 * u + 1][w], x.v[2 * u][w], sel);  // a pair of tokens: 4 channels each
+                const uint32_t y8 = y >> 8;
+                const h2 c0 = __builtin_elementwise_fma(codes_of<0>(y), s[u], o[u]);
+                const h2 c1 = __builtin_elementwise_fma(codes_of<1>(y), s[u], o[u]);
                 const h2 c2 = __builtin_elementwise_fma(codes_of<0>(y8), s[u], o[u]);
                 const h2 c3 = __builtin_elementwise_fma(codes_of<1>(y8), s[u], o[u]);
                 f[0][2 * u] = c0[0], f[0][2 * u + 1] = c0[1];
@@ -225,19 +243,24 @@ __device__ __forceinline__ void add_values(v4f (&acc)[Shape<D>::TILES], const St
                 f[3][2 * u] = c3[0], f[3][2 * u + 1] = c3[1];
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                v4f& t = acc[w * 8 + half * 4 + n];
-                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[n], p, t, 0, 0, 0);
-            }
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int c = 0; c < NQ; ++c) {
+                    v4f& t = acc[c][w * 8 + half * 4 + n];
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[n], p[c], t, 0, 0, 0);
+                }
         }
     }
 }
 
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
 // Row r of a tile as fragments (8 channels of lane j's quarter a step, in K's order), scaled by a power of two that brings its
-// largest magnitude to [2^14, 2^15): f16 then keeps every bit that matters (39 powers of two below the largest).  Returns what
-// a score is multiplied by to undo that; rows that are not there are zeros.
+// largest magnitude to [2^14, 2^15): f16 then keeps every bit that matters (39 powers of two below the largest).  The scale's
+// sign goes into the row too, so that what is returned -- a score to base 2 is that times the product -- is positive, never 0
+// or infinite, and masked products of -inf stay that.  Rows that are not there are zeros.
 template <int D>
-__device__ __forceinline__ float load_row(h8 (&q)[Shape<D>::STEPS], const uint16_t* row, bool there, bool bf16, int j)
+__device__ __forceinline__ float load_row(h8 (&q)[Shape<D>::STEPS], const uint16_t* row, bool there, bool bf16, int j, float scale)
 {
     u32x4 raw[Shape<D>::STEPS];
     float top = 0.0f;
@@ -255,7 +278,8 @@ __device__ __forceinline__ float load_row(h8 (&q)[Shape<D>::STEPS], const uint16
     top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
     int e = (int)(__float_as_uint(top) >> 23) - 127;
     e = e < -100 ? -100 : e > 127 ? 14 : e;  // (0 and tiny rows; infinite ones pass as they are)
-    const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+    float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+    up = scale > 0.0f ? up : scale < 0.0f ? -up : 0.0f;
 #pragma unroll
     for (int i = 0; i < Shape<D>::STEPS; ++i) {
         float x[8];
@@ -269,29 +293,118 @@ __device__ __forceinline__ float load_row(h8 (&q)[Shape<D>::STEPS], const uint16
                       (_Float16)x[2], (_Float16)x[6], (_Float16)x[3], (_Float16)x[7]};
         q[i] = f;
     }
-    return __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+    const float undo = __uint_as_float((uint32_t)(127 - 14 + e) << 23) * (__builtin_fabsf(scale) * LOG2E);
+    return __builtin_fminf(__builtin_fmaxf(undo, 0x1p-126f), 0x1p127f);
 }
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float MARGIN = 15.0f, BELOW = 8.0f;  // a weight is exp2(score - reference), 2^8 at the maximum, 2^15 at most
 
+// where the splits of a row leave their sums: d of O, the reference, the sum of weights, for each
+template <int D>
+__device__ __forceinline__ float* part_of(const KvAttentionArgs& a, int64_t b, int tile, int h, int row)
+{
+    const int64_t all = (int64_t)a.max_q * a.ratio;
+    const int rows = (int)(all < a.tile_rows ? all : a.tile_rows);
+    return a.part + ((((b - a.first) * a.tiles + tile) * a.c.kv_heads + h) * (int64_t)rows + row) * a.splits * (D + 2);
+}
+
+__device__ __forceinline__ void store8(uint16_t* to, const float (&o)[8], float by, bool bf16)
+{
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float lo = o[2 * e] * by, hi = o[2 * e + 1] * by;
+        if (bf16) w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){lo, hi}, bf2_t));
+        else w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){lo, hi}, h2_t));
+    }
+    *(u32x4_any*)to = w;
+}
+
+// What a lane knows of the row it scores: its tokens [low, limit), what undoes the scaling of its query, the softmax's reference
+// (none yet: -inf), what is subtracted for it, and the sum of its weights.
+struct Row {
+    int low, limit;
+    float undo, ref, base, sum;
+};
+
+// the tokens that query `query` of a sequence sees
+__device__ __forceinline__ void sees(const KvAttentionArgs& a, const View& v, int query, int& low, int& limit)
+{
+    const int64_t at = (int64_t)v.len - v.n + query;
+    limit = a.causal ? (at + 1 < 0 ? 0 : at + 1 < v.len ? (int)(at + 1) : v.len) : v.len;
+    low = a.window ? (at - a.window + 1 < 0 ? 0 : at - a.window + 1 < v.len ? (int)(at - a.window + 1) : v.len) : 0;
+}
+
+// scores -> weights (f16) of the tokens t .. t + 31 below `end`; `edge`: some row does not see some of them;
+// `meanwhile` is work that the weights do not depend on
+template <int NQ, int TILES, class F>
+__device__ __forceinline__ void weigh(h8 (&p)[NQ], v4f (&s)[NQ][2], Row (&row)[NQ], v4f (&acc)[NQ][TILES], bool edge, int t, int end,
+                                      bool ok0, bool ok1, int j, F meanwhile)
+{
+    if (edge) {
+#pragma unroll
+        for (int c = 0; c < NQ; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int token = t + (e >> 2) * 16 + 4 * j + (e & 3);
+                const bool seen = token >= row[c].low && token < row[c].limit && token < end && (e < 4 ? ok0 : ok1);
+                s[c][e >> 2][e & 3] = seen ? s[c][e >> 2][e & 3] : -__builtin_inff();
+            }
+    }
+    float top[NQ];
+    bool moves = false;
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        top[c] = s[c][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top[c] = __builtin_fmaxf(top[c], s[c][e >> 2][e & 3]);
+        top[c] *= row[c].undo;
+        moves |= top[c] > row[c].ref + MARGIN;
+    }
+    if (__ballot(moves)) {
+#pragma unroll
+        for (int c = 0; c < NQ; ++c) {
+            top[c] = __builtin_fmaxf(top[c], __shfl_xor(top[c], 16, 64));
+            top[c] = __builtin_fmaxf(top[c], __shfl_xor(top[c], 32, 64));
+            const float to = __builtin_fmaxf(row[c].ref, top[c] - BELOW);
+            const float f = to == row[c].ref ? 1.0f : __builtin_amdgcn_exp2f(row[c].ref - to);
+            row[c].sum *= f;
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) acc[c][n] *= f;
+            row[c].ref = to;
+            row[c].base = to == -__builtin_inff() ? 0.0f : to;
+        }
+    }
+    meanwhile();
+#pragma unroll
+    for (int c = 0; c < NQ; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c][e >> 2][e & 3], row[c].undo, -row[c].base));
+            row[c].sum += w;
+            p[c][e] = (_Float16)w;
+        }
+}
+
 // Four waves share a range of a sequence's tokens, a wave every fourth step of 32; their sums meet in LDS.  One range: the
-// result.  Several: each leaves its sums, and kv_join_kernel adds them.
-template <int D, int G>
-__global__ __launch_bounds__(256) void kv_attention_kernel(KvAttentionArgs a)
+// result.  Several: each leaves its sums, and kv_join_kernel adds them.  Workgroups go through the first ranges of all tiles and
+// heads, then the second ones (those behind short sequences come last and end at once), a place further each time: workgroups
+// are dealt to the eight XCDs in turn, and neither a sequence nor the first ranges, which all sequences have, fall to one of them.
+template <int D, int G, int NQ>
+__global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 3) void kv_attention_kernel(KvAttentionArgs a, uint32_t groups)
 {
     constexpr int TILES = Shape<D>::TILES, MD = Shape<D>::MD;
     __shared__ float merge[4][16][MD + 4];
-    __shared__ float stat[2][4][16];
-    uint32_t id = blockIdx.x;
-    const int split = (int)(id % a.splits);
-    id /= a.splits;
+    __shared__ float stat[2][4][NQ * 16];
+    const int split = (int)(blockIdx.x / groups);
+    uint32_t id = blockIdx.x % groups + split;
+    while (id >= groups) id -= groups;
     const int h = (int)(id % a.c.kv_heads);
     id /= a.c.kv_heads;
     const int tile = (int)(id % a.tiles);
     const int64_t b = a.first + id / a.tiles;
     const View v = view_of(a, b);
-    if (tile * 16 >= v.rows * a.ratio) return;
+    if (tile * a.tile_rows >= v.rows * a.ratio) return;
     const Range range = range_of(a, v, tile);
     const int64_t begin64 = range.lo + (int64_t)split * a.chunk;
     if (split > 0 && begin64 >= range.hi) return;
@@ -301,18 +414,43 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(KvAttentionArgs a)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int* table = a.s.table + b * a.s.ld_table;
 
-    const int row = tile * 16 + r, query = row / a.ratio;
-    const bool there = query < v.rows;
-    h8 q[Shape<D>::STEPS];
-    const uint16_t* from = (const uint16_t*)a.q + (int64_t)(v.start + (there ? query : 0)) * a.ld_q +
-                           (int64_t)(h * a.ratio + row % a.ratio) * a.hd_q;
-    const float undo = load_row<D>(q, from, there, a.type == DT_BF16, j) * (a.scale * LOG2E);
-    // the row's tokens [low, limit); rows that are not there take those of the last query
-    const int mine = there ? query : v.rows - 1;
-    const int64_t at = (int64_t)v.len - v.n + mine;
-    const int limit = a.causal ? (at + 1 < 0 ? 0 : at + 1 < v.len ? (int)(at + 1) : v.len) : v.len;
-    const int low = a.window ? (at - a.window + 1 < 0 ? 0 : at - a.window + 1 < v.len ? (int)(at - a.window + 1) : v.len) : 0;
-    int all_limit = limit, all_low = low;  // what every row sees
+    // the first step is on its way before the queries
+    const Lane at = lane_of_step<D, G>(r, j);
+    Step<D, G> x0, x1;
+    Half at0[2], at1[2];
+    int pages[2];
+    int t = begin + 32 * wave;
+    auto fetch = [&](Step<D, G>& x, Half(&half)[2], int token) {
+        half[0] = half_at(a, pages[0], h, token);
+        half[1] = half_at(a, pages[1], h, token + 16);
+        load_step<D, G>(x, a, half, at);
+    };
+    auto look = [&](int token) {
+        pages[0] = page_at(a, table, token);
+        pages[1] = page_at(a, table, token + 16);
+    };
+    if (t < end) {
+        look(t);
+        fetch(x0, at0, t);
+        look(t + 128);
+    }
+
+    h8 q[NQ][Shape<D>::STEPS];
+    Row row[NQ];
+    int all_limit = v.len, all_low = 0;  // what every row sees
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        const int at = tile * a.tile_rows + c * 16 + r, query = at / a.ratio;
+        const bool there = query < v.rows;
+        const uint16_t* from = (const uint16_t*)a.q + (int64_t)(v.start + (there ? query : 0)) * a.ld_q +
+                               (int64_t)(h * a.ratio + at % a.ratio) * a.hd_q;
+        row[c].undo = load_row<D>(q[c], from, there, a.type == DT_BF16, j, a.scale);
+        sees(a, v, there ? query : v.rows - 1, row[c].low, row[c].limit);  // (rows that are not there: as the last query)
+        row[c].ref = -__builtin_inff();
+        row[c].base = row[c].sum = 0.0f;
+        all_limit = all_limit < row[c].limit ? all_limit : row[c].limit;
+        all_low = all_low > row[c].low ? all_low : row[c].low;
+    }
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) {
         const int x = __shfl_xor(all_limit, off, 64), y = __shfl_xor(all_low, off, 64);
@@ -321,297 +459,707 @@ __global__ __launch_bounds__(256) void kv_attention_kernel(KvAttentionArgs a)
     }
     all_limit = __builtin_amdgcn_readfirstlane(all_limit);
     all_low = __builtin_amdgcn_readfirstlane(all_low);
+    all_limit = all_limit < end ? all_limit : end;
 
-    v4f acc[TILES];
+    v4f acc[NQ][TILES];
 #pragma unroll
-    for (int n = 0; n < TILES; ++n) acc[n] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    float ref = -__builtin_inff(), base = 0.0f, sum = 0.0f;  // reference (none yet) and what is subtracted; sum of weights
+    for (int c = 0; c < NQ; ++c)
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) acc[c][n] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 
-    Step<D, G> now, next;
-    Half here[2], there_half[2];
-    int t = begin + 32 * wave;
-    if (t < end) {
-        here[0] = half_at(a, table, h, t);
-        here[1] = half_at(a, table, h, t + 16);
-        load_step<D, G>(now, a, here, r, j);
-    }
-    for (; t < end; t += 128) {
+    auto work = [&](Step<D, G>& x, const Half(&half)[2], int token) {
+        v4f s[NQ][2];
+        scores<D, G, NQ>(s, x.k, x.ks, q);
+        const bool edge = token < all_low || token + 32 > all_limit || !half[0].ok || !half[1].ok;
+        if (edge) {
+            // what lies behind the sequence may be anything: its values become 0
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x.vs[e] = token + (e >> 2) * 16 + 4 * j + (e & 3) < end && half[e >> 2].ok ? x.vs[e] : 0u;
+        }
+        h8 p[NQ];
+        weigh<NQ, TILES>(p, s, row, acc, edge, token, end, half[0].ok, half[1].ok, j, [] {});
+        add_values<D, G, NQ>(acc, x, p, r);
+    };
+    for (; t < end; t += 256) {
         if (t + 128 < end) {
-            there_half[0] = half_at(a, table, h, t + 128);
-            there_half[1] = half_at(a, table, h, t + 144);
-            load_step<D, G>(next, a, there_half, r, j);
+            fetch(x1, at1, t + 128);
+            look(t + 256);
         }
-        v4f s[2];
-        scores<D, G>(s, now.k, now.ks, q);
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * undo;
-        if (t < all_low || t + 32 > all_limit || t + 32 > end || !here[0].ok || !here[1].ok) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int token = t + (e >> 2) * 16 + 4 * j + (e & 3);
-                const bool seen = token >= low && token < limit && token < end && here[e >> 2].ok;
-                x[e] = seen ? x[e] : -__builtin_inff();
-                // (what lies behind the sequence may be anything: its values become 0)
-                now.vs[e] = token < end && here[e >> 2].ok ? now.vs[e] : 0u;
-            }
+        work(x0, at0, t);
+        if (t + 128 >= end) break;
+        if (t + 256 < end) {
+            fetch(x0, at0, t + 256);
+            look(t + 384);
         }
-        float top = x[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) top = __builtin_fmaxf(top, x[e]);
-        if (__ballot(top > ref + MARGIN)) {
-            top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
-            top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
-            const float to = __builtin_fmaxf(ref, top - BELOW);
-            const float f = to == ref ? 1.0f : __builtin_amdgcn_exp2f(ref - to);
-            sum *= f;
-#pragma unroll
-            for (int n = 0; n < TILES; ++n) acc[n] *= f;
-            ref = to;
-            base = to == -__builtin_inff() ? 0.0f : to;
-        }
-        h8 p;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float w = __builtin_amdgcn_exp2f(x[e] - base);
-            sum += w;
-            p[e] = (_Float16)w;
-        }
-        add_values<D, G>(acc, now, p, r);
-        now = next;
-        here[0] = there_half[0];
-        here[1] = there_half[1];
+        work(x1, at1, t + 128);
     }
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
 
     // the waves' sums
-    if (j == 0) stat[0][wave][r] = ref, stat[1][wave][r] = sum;
-    __syncthreads();
-    float top = -__builtin_inff();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, stat[0][w][r]);
-    const float f = ref == -__builtin_inff() && sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(base - top);
+    for (int c = 0; c < NQ; ++c) {
+        row[c].sum += __shfl_xor(row[c].sum, 16, 64);
+        row[c].sum += __shfl_xor(row[c].sum, 32, 64);
+        if (j == 0) stat[0][wave][c * 16 + r] = row[c].ref, stat[1][wave][c * 16 + r] = row[c].sum;
+    }
+    __syncthreads();
     constexpr int EACH = 8, PER = MD / EACH;  // channels of a thread, threads of a row
     const int orow = threadIdx.x / PER, och = threadIdx.x % PER * EACH;
-    float total = 0.0f, most = -__builtin_inff();
-    if (orow < 16) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) most = __builtin_fmaxf(most, stat[0][w][orow]);
+    for (int c = 0; c < NQ; ++c) {
+        float top = -__builtin_inff();
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float c = stat[0][w][orow], l = stat[1][w][orow];
-            total += l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f((c == -__builtin_inff() ? 0.0f : c) - most);
-        }
-    }
-    const int out_row = tile * 16 + orow, out_query = out_row / a.ratio;
-    const bool writes = orow < 16 && out_query < v.rows;
-    const int head = h * a.ratio + out_row % a.ratio;
-    const int64_t token = v.start + out_query;
-    float* part = a.part;
-    if (a.splits > 1 && writes)
-        part += ((((b - a.first) * a.tiles + tile) * a.c.kv_heads + h) * (int64_t)a.rows + orow) * a.splits * (D + 2) +
-                (int64_t)split * (D + 2);
+        for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, stat[0][w][c * 16 + r]);
+        const float f = row[c].ref == -__builtin_inff() && row[c].sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(row[c].base - top);
+        float total = 0.0f, most = -__builtin_inff();
+        if (orow < 16) {
 #pragma unroll
-    for (int piece = 0; piece < D / MD; ++piece) {
-        // lane (r, j) has channels j (D / 4) .. of row r: 4 runs of TILES
+            for (int w = 0; w < 4; ++w) most = __builtin_fmaxf(most, stat[0][w][c * 16 + orow]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c0 = j * (D / 4) + i * TILES - piece * MD;
-            if (c0 >= 0 && c0 < MD) {
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) merge[wave][r][c0 + n] = acc[n][i] * f;
+            for (int w = 0; w < 4; ++w) {
+                const float ref = stat[0][w][c * 16 + orow], l = stat[1][w][c * 16 + orow];
+                total += l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f((ref == -__builtin_inff() ? 0.0f : ref) - most);
             }
         }
-        __syncthreads();
-        if (writes) {
-            float o[EACH];
+        const int out_row = tile * a.tile_rows + c * 16 + orow, out_query = out_row / a.ratio;
+        const bool writes = orow < 16 && out_query < v.rows;
+        const int head = h * a.ratio + out_row % a.ratio;
+        const int64_t token = v.start + out_query;
+        float* part = nullptr;
+        if (a.splits > 1 && writes) part = part_of<D>(a, b, tile, h, c * 16 + orow) + (int64_t)split * (D + 2);
 #pragma unroll
-            for (int e = 0; e < EACH; ++e)
-                o[e] = merge[0][orow][och + e] + merge[1][orow][och + e] + merge[2][orow][och + e] + merge[3][orow][och + e];
-            if (a.splits > 1) {
+        for (int piece = 0; piece < D / MD; ++piece) {
+            if (c + piece > 0) __syncthreads();
+            // lane (r, j) has channels j (D / 4) .. of row r: 4 runs of TILES
 #pragma unroll
-                for (int e = 0; e < EACH; ++e) part[piece * MD + och + e] = o[e];
-            } else {
-                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                u32x4 w;
+            for (int i = 0; i < 4; ++i) {
+                const int c0 = j * (D / 4) + i * TILES - piece * MD;
+                if (c0 >= 0 && c0 < MD) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float lo = o[2 * e] * inv, hi = o[2 * e + 1] * inv;
-                    if (a.type == DT_BF16) w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){lo, hi}, bf2_t));
-                    else w[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){lo, hi}, h2_t));
+                    for (int n = 0; n < TILES; ++n) merge[wave][r][c0 + n] = acc[c][n][i] * f;
                 }
-                *(u32x4_any*)((uint16_t*)a.out + token * a.ld_out + head * a.hd_out + piece * MD + och) = w;
+            }
+            __syncthreads();
+            if (writes) {
+                float o[EACH];
+#pragma unroll
+                for (int e = 0; e < EACH; ++e)
+                    o[e] = merge[0][orow][och + e] + merge[1][orow][och + e] + merge[2][orow][och + e] + merge[3][orow][och + e];
+                if (a.splits > 1) {
+#pragma unroll
+                    for (int e = 0; e < EACH; ++e) part[piece * MD + och + e] = o[e];
+                } else {
+                    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                    store8((uint16_t*)a.out + token * a.ld_out + head * a.hd_out + piece * MD + och, o, inv, a.type == DT_BF16);
+                }
             }
         }
-        if (piece + 1 < D / MD) __syncthreads();
-    }
-    if (writes && och == 0) {
-        if (a.splits > 1) part[D] = most, part[D + 1] = total;
-        else if (a.lse) a.lse[token * a.heads + head] = total == 0.0f ? -__builtin_inff() : LN2 * (most + log2f(total));
+        if (writes && och == 0) {
+            if (a.splits > 1) part[D] = most, part[D + 1] = total;
+            else if (a.lse) a.lse[token * a.heads + head] = total == 0.0f ? -__builtin_inff() : LN2 * (most + log2f(total));
+        }
     }
 }
 
-// adds what the ranges of a row left, in their order: a wave per row
-template <int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a)
+// Many rows: WAVES waves of 16 NQ rows each go through the tokens together, and codes become fragments once for all of them.  A step
+// is 32 tokens for every four waves: each converts a quarter of 32 tokens into a ring of three steps in LDS, laid out lane by
+// lane as the matrix instruction reads them.  While a wave weighs the scores of 32 tokens, its products of the next 32's keys
+// run, and the values' products follow.  A quarter: in K half the words of one of the two halves, in V 2 (d = 256: 4) of the D /
+// 16 tiles.
+template <int D, int G>
+struct Quarter {
+    static constexpr int KN = Shape<D>::KW / 2, VN = D == 256 ? 4 : 2;
+    uint32_t k[KN], ks, v[8], vs[8];
+    bool ok0, ok1;
+};
+
+template <int D, int G>
+__device__ __forceinline__ void load_quarter(Quarter<D, G>& x, const KvAttentionArgs& a, const int (&pages)[2], int h, int t, int wave,
+                                             const Lane& at)
 {
-    const int lane = threadIdx.x & 63;
-    int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int orow = (int)(id % a.rows);
-    id /= a.rows;
+    constexpr int W = D / 8, GR = D / G, KN = Quarter<D, G>::KN;
+    const Half half[2] = {half_at(a, pages[0], h, t), half_at(a, pages[1], h, t + 16)};
+    x.ok0 = half[0].ok, x.ok1 = half[1].ok;
+    const Half& mine = wave >> 1 ? half[1] : half[0];
+    const uint8_t* k = a.c.k + mine.code;
+    if constexpr (KN == 4) {
+        const u32x4 w = read<u32x4>(k, at.k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.k[i] = w[i];
+    } else if constexpr (KN == 2) {
+        const u32x2 w = read<u32x2>(k, at.k);
+        x.k[0] = w[0], x.k[1] = w[1];
+    } else {
+        x.k[0] = read<uint32_t>(k, at.k);
+    }
+    x.ks = read<uint32_t>(a.c.k_scale + mine.scale, at.ks);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x.v[e] = read<uint32_t>(a.c.v + half[e >> 2].code, at.v, (e & 3) * W);
+        x.vs[e] = read<uint32_t>(a.c.v_scale + half[e >> 2].scale, at.vs, (e & 3) * GR);
+    }
+}
+template <int D, int G>
+__device__ __forceinline__ Lane lane_of_quarter(int wave, int r, int j)
+{
+    constexpr int W = D / 8, GR = D / G, KN = Quarter<D, G>::KN;
+    const int part = wave & 1;
+    return Lane{4u * (r * W + j * (W / 4) + part * KN), 4u * (r * GR + (j * (D / 4) + part * (D / 8)) / G),
+                4u * (4 * j * W + (D == 64 ? r >> 1 : D == 128 ? r : 2 * r + (wave >> 1))),
+                4u * (4 * j * GR + r * (D / 16) / G)};
+}
+
+template <int D, int G>
+__device__ __forceinline__ void convert_quarter(h8* slot, Quarter<D, G>& x, int t, int end, int wave, int r, int j, int lane)
+{
+    constexpr int STEPS = Shape<D>::STEPS, KN = Quarter<D, G>::KN;
+    const int part = wave & 1, half = wave >> 1;
+    const h2 ks = low_pair(x.ks, x.ks), ko = high_pair(x.ks, x.ks);
+#pragma unroll
+    for (int i = 0; i < KN; ++i) slot[(half * STEPS + part * KN + i) * 64 + lane] = key_fragment(x.k[i], ks, ko);
+    if (D == 64 && half) return;  // (four tiles: two waves have them)
+    if (t + 32 > end || !x.ok0 || !x.ok1) {
+        // what lies behind the sequence may be anything: its values become 0
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.vs[e] = t + (e >> 2) * 16 + 4 * j + (e & 3) < end && (e < 4 ? x.ok0 : x.ok1) ? x.vs[e] : 0u;
+    }
+    // this wave's channels of a word: of the half `high`, those of `odd` (or all four)
+    const uint32_t high = D == 64 ? r & 1 : D == 128 ? half : part;
+    const uint32_t sel = high ? 0x07060302u : 0x05040100u;
+    h8 f[Quarter<D, G>::VN];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const h2 s = low_pair(x.vs[2 * u], x.vs[2 * u + 1]), o = high_pair(x.vs[2 * u], x.vs[2 * u + 1]);
+        uint32_t y = __builtin_amdgcn_perm(x.v[2 * u + 1], x.v[2 * u], sel);
+        if constexpr (D == 256) {
+            const h2 c0 = __builtin_elementwise_fma(codes_of<0>(y), s, o), c1 = __builtin_elementwise_fma(codes_of<1>(y), s, o);
+            f[0][2 * u] = c0[0], f[0][2 * u + 1] = c0[1];
+            f[1][2 * u] = c1[0], f[1][2 * u + 1] = c1[1];
+            y >>= 8;
+            const h2 c2 = __builtin_elementwise_fma(codes_of<0>(y), s, o), c3 = __builtin_elementwise_fma(codes_of<1>(y), s, o);
+            f[2][2 * u] = c2[0], f[2][2 * u + 1] = c2[1];
+            f[3][2 * u] = c3[0], f[3][2 * u + 1] = c3[1];
+        } else {
+            y >>= 8 * part;
+            const h2 c0 = __builtin_elementwise_fma(codes_of<0>(y), s, o), c1 = __builtin_elementwise_fma(codes_of<1>(y), s, o);
+            f[0][2 * u] = c0[0], f[0][2 * u + 1] = c0[1];
+            f[1][2 * u] = c1[0], f[1][2 * u + 1] = c1[1];
+        }
+    }
+    const int first = D == 256 ? half * 8 + part * 4 : D == 128 ? half * 4 + part * 2 : part * 2;
+#pragma unroll
+    for (int n = 0; n < Quarter<D, G>::VN; ++n) slot[(2 * STEPS + first + n) * 64 + lane] = f[n];
+}
+
+template <int D, int G, int NQ, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, NQ * D > 256 ? 1 : 2) void kv_chunk_kernel(KvAttentionArgs a, uint32_t groups)
+{
+    constexpr int STEPS = Shape<D>::STEPS, TILES = Shape<D>::TILES, SET = (2 * STEPS + TILES) * 64;
+    constexpr int SETS = WAVES / 4, TOKENS = 32 * SETS, SLOT = SETS * SET;
+    extern __shared__ h8 ring[];  // three steps
+    const int split = (int)(blockIdx.x / groups);
+    uint32_t id = blockIdx.x % groups;
     const int h = (int)(id % a.c.kv_heads);
     id /= a.c.kv_heads;
     const int tile = (int)(id % a.tiles);
     const int64_t b = a.first + id / a.tiles;
-    if (b >= a.s.batch) return;
     const View v = view_of(a, b);
-    const int row = tile * 16 + orow, query = row / a.ratio;
+    if (tile * a.tile_rows >= v.rows * a.ratio) return;
+    const Range range = range_of(a, v, tile);
+    const int64_t begin64 = range.lo + (int64_t)split * a.chunk;
+    if (split > 0 && begin64 >= range.hi) return;
+    const int begin = (int)(begin64 < range.hi ? begin64 : range.hi);
+    const int end = range.hi - begin > a.chunk ? begin + a.chunk : range.hi;
+    const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = wave & 3, mine = 32 * (wave >> 2);
+    const int* table = a.s.table + b * a.s.ld_table;
+
+    // codes of step t: looked up two steps ahead, loaded one ahead (of the conversion, which is one ahead of their use)
+    const Lane place = lane_of_quarter<D, G>(quarter, r, j);
+    Quarter<D, G> x{};
+    int pages[2];
+    auto look = [&](int t) {
+        pages[0] = page_at(a, table, t + mine);
+        pages[1] = page_at(a, table, t + mine + 16);
+    };
+    auto load = [&](int t) {
+        load_quarter<D, G>(x, a, pages, h, t + mine, quarter, place);
+        look(t + TOKENS);
+    };
+    // which pages of a set exist, for every wave
+    __shared__ uint32_t good[3][2];
+    auto convert = [&](int at, h8* slot, int t) {
+        if (quarter == 0 && lane == 0) good[at][wave >> 2] = (x.ok0 ? 1u : 0u) | (x.ok1 ? 2u : 0u);
+        convert_quarter<D, G>(slot + (wave >> 2) * SET, x, t + mine, end, quarter, r, j, lane);
+    };
+    look(begin);
+    load(begin);
+
+    h8 q[NQ][STEPS];
+    Row row[NQ];
+    int all_limit = v.len, all_low = 0, any_limit = 0, any_low = v.len;
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        const int at = tile * a.tile_rows + (wave * NQ + c) * 16 + r, query = at / a.ratio;
+        const bool there = query < v.rows;
+        const uint16_t* from = (const uint16_t*)a.q + (int64_t)(v.start + (there ? query : 0)) * a.ld_q +
+                               (int64_t)(h * a.ratio + at % a.ratio) * a.hd_q;
+        row[c].undo = load_row<D>(q[c], from, there, a.type == DT_BF16, j, a.scale);
+        sees(a, v, there ? query : v.rows - 1, row[c].low, row[c].limit);
+        row[c].ref = -__builtin_inff();
+        row[c].base = row[c].sum = 0.0f;
+        all_limit = all_limit < row[c].limit ? all_limit : row[c].limit;
+        all_low = all_low > row[c].low ? all_low : row[c].low;
+        any_limit = any_limit > row[c].limit ? any_limit : row[c].limit;
+        any_low = any_low < row[c].low ? any_low : row[c].low;
+    }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+        const int y0 = __shfl_xor(all_limit, off, 64), y1 = __shfl_xor(all_low, off, 64);
+        const int y2 = __shfl_xor(any_limit, off, 64), y3 = __shfl_xor(any_low, off, 64);
+        all_limit = all_limit < y0 ? all_limit : y0;
+        all_low = all_low > y1 ? all_low : y1;
+        any_limit = any_limit > y2 ? any_limit : y2;
+        any_low = any_low < y3 ? any_low : y3;
+    }
+    all_limit = __builtin_amdgcn_readfirstlane(all_limit);
+    all_low = __builtin_amdgcn_readfirstlane(all_low);
+    any_limit = __builtin_amdgcn_readfirstlane(any_limit);
+    any_low = __builtin_amdgcn_readfirstlane(any_low);
+    all_limit = all_limit < end ? all_limit : end;
+    any_limit = any_limit < end ? any_limit : end;
+    if ((tile * a.tile_rows + wave * NQ * 16) / a.ratio >= v.rows) any_limit = 0;  // (no rows of its own)
+
+    v4f acc[NQ][TILES];
+#pragma unroll
+    for (int c = 0; c < NQ; ++c)
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) acc[c][n] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+
+    auto products = [&](v4f(&s)[NQ][2], const h8(&k)[2 * STEPS]) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) s[c][hh] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int c = 0; c < NQ; ++c)
+                    s[c][hh] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[hh * STEPS + i], q[c][i], s[c][hh], 0, 0, 0);
+        }
+    };
+    auto keys = [&](h8(&k)[2 * STEPS], const h8* set) {
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i) k[i] = set[i * 64 + lane];
+    };
+    // 32 tokens from t on, whose scores are in `s` and values in `set`; the scores of the next 32, in `other`, go to `n`
+    auto attend = [&](int t, v4f(&s)[NQ][2], const h8* set, uint32_t ok, v4f(&n)[NQ][2], const h8* other) {
+        h8 k[2 * STEPS];
+        keys(k, other);
+        if (t < any_limit && t + 32 > any_low) {
+            const bool edge = t < all_low || t + 32 > all_limit || ok != 3u;
+            h8 p[NQ], vals[TILES];
+            weigh<NQ, TILES>(p, s, row, acc, edge, t, end, ok & 1u, ok & 2u, j, [&] {
+#pragma unroll
+                for (int m = 0; m < TILES; ++m) vals[m] = set[(2 * STEPS + m) * 64 + lane];
+                products(n, k);
+            });
+#pragma unroll
+            for (int m = 0; m < TILES; ++m)
+#pragma unroll
+                for (int c = 0; c < NQ; ++c) acc[c][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vals[m], p[c], acc[c][m], 0, 0, 0);
+        } else {
+            products(n, k);
+        }
+    };
+
+    v4f s0[NQ][2], s1[NQ][2];
+    int now = 0, next = 1, spare = 2;
+    if (begin < end) convert(0, ring, begin);
+    if (begin + TOKENS < end) {
+        load(begin + TOKENS);
+        convert(1, ring + SLOT, begin + TOKENS);
+    }
+    if (begin + 2 * TOKENS < end) load(begin + 2 * TOKENS);
+    __syncthreads();
+    {
+        h8 k[2 * STEPS];
+        keys(k, ring);
+        products(s0, k);
+    }
+    for (int t = begin; t < end; t += TOKENS) {
+        const h8 *set = ring + now * SLOT, *following = ring + next * SLOT;
+        const uint32_t ok0 = __builtin_amdgcn_readfirstlane(good[now][0]), ok1 = __builtin_amdgcn_readfirstlane(good[now][SETS - 1]);
+        auto feed = [&] {
+            if (t + 2 * TOKENS < end) {
+                convert(spare, ring + spare * SLOT, t + 2 * TOKENS);
+                if (t + 3 * TOKENS < end) load(t + 3 * TOKENS);
+            }
+        };
+        if constexpr (SETS == 2) {
+            // (waves w and w + 4 share a SIMD: one converts while the other multiplies)
+            if (wave < 4) feed();
+            attend(t, s0, set, ok0, s1, set + SET);
+            if (wave >= 4) feed();
+            attend(t + 32, s1, set + SET, ok1, s0, following);
+        } else {
+            feed();
+            attend(t, s0, set, ok0, s1, following);
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) s0[c][0] = s1[c][0], s0[c][1] = s1[c][1];
+        }
+        __syncthreads();  // the step after next is written, this one is read
+        const int old = now;
+        now = next;
+        next = spare;
+        spare = old;
+    }
+
+    // each wave has its rows' sums: lane (r, j) the channels j (D / 4) .. of row r
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) {
+        float sum = row[c].sum;
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        const int in_tile = (wave * NQ + c) * 16 + r, at = tile * a.tile_rows + in_tile, query = at / a.ratio;
+        if (query >= v.rows) continue;
+        const int head = h * a.ratio + at % a.ratio;
+        const int64_t token = v.start + query;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        float* part = a.splits > 1 ? part_of<D>(a, b, tile, h, in_tile) + (int64_t)split * (D + 2) : nullptr;
+        uint16_t* out = (uint16_t*)a.out + token * a.ld_out + head * a.hd_out;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c0 = j * (D / 4) + i * TILES;
+            if (a.splits > 1) {
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) part[c0 + n] = acc[c][n][i];
+            } else if constexpr (TILES >= 8) {
+#pragma unroll
+                for (int n = 0; n < TILES; n += 8) {
+                    float o[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = acc[c][n + e][i];
+                    store8(out + c0 + n, o, inv, a.type == DT_BF16);
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+                    const float o = acc[c][n][i] * inv;
+                    out[c0 + n] = a.type == DT_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)o) : f32_to_f16(o);
+                }
+            }
+        }
+        if (j == 0) {
+            if (a.splits > 1) part[D] = row[c].ref, part[D + 1] = sum;
+            else if (a.lse) a.lse[token * a.heads + head] = sum == 0.0f ? -__builtin_inff() : LN2 * (row[c].base + log2f(sum));
+        }
+    }
+}
+
+// Adds what the ranges of a row left, a workgroup per row: a wave takes every fourth range, eight at a time so that their loads
+// are in flight together, and the waves' sums are added in order.
+template <int D>
+__global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a)
+{
+    constexpr int E = D / 64;
+    __shared__ float o_of[4][D], l_of[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t all = (int64_t)a.max_q * a.ratio;
+    const int rows = (int)(all < a.tile_rows ? all : a.tile_rows);
+    uint32_t id = blockIdx.x;
+    const int orow = (int)(id % rows);
+    id /= rows;
+    const int h = (int)(id % a.c.kv_heads);
+    id /= a.c.kv_heads;
+    const int tile = (int)(id % a.tiles);
+    const int64_t b = a.first + id / a.tiles;
+    const View v = view_of(a, b);
+    const int row = tile * a.tile_rows + orow, query = row / a.ratio;
     if (query >= v.rows) return;
     const Range range = range_of(a, v, tile);
     const int64_t span = (int64_t)range.hi - range.lo;
     const int n = span <= a.chunk ? 1 : (int)((span + a.chunk - 1) / a.chunk);
-    const float* part = a.part + ((((b - a.first) * a.tiles + tile) * a.c.kv_heads + h) * (int64_t)a.rows + orow) * a.splits * (D + 2);
+    const float* part = part_of<D>(a, b, tile, h, orow);
     float most = -__builtin_inff();
     for (int s = lane; s < n; s += 64) most = __builtin_fmaxf(most, part[(int64_t)s * (D + 2) + D]);
     most = wave_max(most);
-    float total = 0.0f, o[D / 64];
+    float total = 0.0f, o[E] = {};
+    for (int s0 = wave; s0 < n; s0 += 32) {
+        float x[8][E], c[8], l[8];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
-    for (int s = 0; s < n; ++s) {
-        const float* from = part + (int64_t)s * (D + 2);
-        const float c = from[D], l = from[D + 1];
-        const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(c - most);
-        total += l * f;
+        for (int u = 0; u < 8; ++u) {
+            const int s = s0 + 4 * u < n ? s0 + 4 * u : n - 1;
+            const float* from = part + (int64_t)s * (D + 2);
+            c[u] = from[D], l[u] = from[D + 1];
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) o[e] += from[e * 64 + lane] * f;
+            for (int e = 0; e < E; ++e) x[u][e] = from[lane * E + e];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float f = s0 + 4 * u >= n || l[u] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(c[u] - most);
+            total += f == 0.0f ? 0.0f : l[u] * f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += f == 0.0f ? 0.0f : x[u][e] * f;
+        }
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) o_of[wave][lane * E + e] = o[e];
+    if (lane == 0) l_of[wave] = total;
+    __syncthreads();
+    if (threadIdx.x >= D / 2) return;
+    total = l_of[0] + l_of[1] + l_of[2] + l_of[3];
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    const int head = h * a.ratio + row % a.ratio;
+    const int head = h * a.ratio + row % a.ratio, at = 2 * threadIdx.x;
     const int64_t token = v.start + query;
-    uint16_t* out = (uint16_t*)a.out + token * a.ld_out + head * a.hd_out;
+    float y[2];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-        const float x = o[e] * inv;
-        out[e * 64 + lane] = a.type == DT_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)x) : f32_to_f16(x);
-    }
-    if (a.lse && lane == 0) a.lse[token * a.heads + head] = total == 0.0f ? -__builtin_inff() : LN2 * (most + log2f(total));
+    for (int e = 0; e < 2; ++e) y[e] = (o_of[0][at + e] + o_of[1][at + e] + o_of[2][at + e] + o_of[3][at + e]) * inv;
+    uint16_t* out = (uint16_t*)a.out + token * a.ld_out + head * a.hd_out + at;
+    const uint32_t w = a.type == DT_BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){y[0], y[1]}, bf2_t))
+                                         : __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){y[0], y[1]}, h2_t));
+    out[0] = (uint16_t)w, out[1] = (uint16_t)(w >> 16);
+    if (a.lse && threadIdx.x == 0) a.lse[token * a.heads + head] = total == 0.0f ? -__builtin_inff() : LN2 * (most + log2f(total));
 }
 
-// The weight that 32 tokens per wave received: the scores again, exp(score - lse) summed over the rows of every tile, in order.
+// The weight that cached tokens received: the scores again, exp(score - lse) summed over a tile's rows, tile after tile.  Here S = Q
+// K^T, the operands the other way round, so that a lane's scores belong to one token (its column) and to the rows 4 j .. 4 j + 3: the
+// sum over rows stays in the lane until the end.  A wave takes 64 tokens at a time (d = 256: 32), whose keys stay in registers while
+// the rows, converted once per workgroup, come from LDS, eight tiles at a time; more tiles take another turn over the tokens,
+// adding to what the turn before left in the output.
+constexpr int TURN = 8;  // tiles of rows in LDS
+struct TileRows {
+    float undo[16], lse[16];
+    int low[16], limit[16];
+    int any_low, any_limit, all_low, all_limit;
+};
+
 template <int D, int G>
-__global__ __launch_bounds__(256) void kv_weights_kernel(KvAttentionArgs a, int blocks)
+__global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_weights_kernel(KvAttentionArgs a, uint32_t groups)
 {
-    uint32_t id = blockIdx.x;
-    const int block = (int)(id % blocks);
-    id /= blocks;
+    constexpr int STEPS = Shape<D>::STEPS, KW = Shape<D>::KW, NT = D == 256 ? 2 : 4, TOKENS = 16 * NT;
+    constexpr int W = D / 8, GR = D / G, KS = Step<D, G>::KS;
+    extern __shared__ h8 rows_of[];
+    __shared__ TileRows info[TURN];
+    const int part = (int)(blockIdx.x / groups);
+    uint32_t id = blockIdx.x % groups + part;
+    while (id >= groups) id -= groups;
     const int h = (int)(id % a.c.kv_heads);
     const int64_t b = a.first + id / a.c.kv_heads;
     const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
-    const int64_t first = ((int64_t)block * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const View v = view_of(a, b);
     float* out = a.w_out + (b * a.c.kv_heads + h) * (int64_t)a.cap;
     const float* in = a.w_in ? a.w_in + (b * a.c.kv_heads + h) * (int64_t)a.cap : nullptr;
-    if (first >= v.len) {
-        // no tokens here: a row without earlier weights is written to its end
-        if (!in && lane < 32 && first + lane < a.cap) out[first + lane] = 0.0f;
-        return;
-    }
-    const int t = (int)first;
+    const int64_t begin64 = (int64_t)part * a.chunk;
+    const int begin = (int)begin64, stop = a.cap - begin > a.chunk ? begin + a.chunk : a.cap;  // (begin < cap)
+    const int end = stop < v.len ? stop : v.len;
     const int* table = a.s.table + b * a.s.ld_table;
-    const Half half[2] = {half_at(a, table, h, t), half_at(a, table, h, t + 16)};
-    Step<D, G> x;
-    load_step<D, G>(x, a, half, r, j);
-    float got[8] = {};
-    const int tiles = (v.rows * a.ratio + 15) / 16;
-    for (int tile = 0; tile < tiles; ++tile) {
-        const Range range = range_of(a, v, tile);
-        if (t >= range.hi || t + 32 <= range.lo) continue;
-        const int row = tile * 16 + r, query = row / a.ratio;
-        const bool there = query < v.rows;
-        const int64_t token = v.start + (there ? query : 0);
-        const int head = h * a.ratio + row % a.ratio;
-        h8 q[Shape<D>::STEPS];
-        const float undo = load_row<D>(q, (const uint16_t*)a.q + token * a.ld_q + (int64_t)head * a.hd_q, there,
-                                       a.type == DT_BF16, j) * (a.scale * LOG2E);
-        float lse = there ? a.lse[token * a.heads + head] : __builtin_inff();
-        lse = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;  // (a row that saw nothing gives nothing)
-        const int64_t at = (int64_t)v.len - v.n + query;
-        v4f s[2];
-        scores<D, G>(s, x.k, x.ks, q);
+    if (!in)
+        for (int i = (begin > v.len ? begin : v.len) + (int)threadIdx.x; i < stop; i += 256) out[i] = 0.0f;
+    if (begin >= end) return;
+
+    const uint32_t at_k = 4u * (r * W + j * (W / 4)), at_s = 4u * (r * GR + j * (D / 4) / G);
+    uint32_t k[NT][KW], ks[NT][KS], ok = 0;
+    auto load = [&](int t) {
+        ok = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int64_t pos = t + (e >> 2) * 16 + 4 * j + (e & 3);
-            const bool seen = there && pos < v.len && (!a.causal || pos <= at) && (!a.window || pos > at - a.window) && half[e >> 2].ok;
-            const float w = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] * undo - lse);
-            got[e] += seen ? w : 0.0f;
+        for (int n = 0; n < NT; ++n) {
+            const Half half = half_at(a, page_at(a, table, t + 16 * n), h, t + 16 * n);
+            ok |= half.ok ? 1u << n : 0u;
+            const uint8_t* from = a.c.k + half.code;
+            if constexpr (KW == 2) {
+                const u32x2 w = read<u32x2>(from, at_k);
+                k[n][0] = w[0], k[n][1] = w[1];
+            } else {
+#pragma unroll
+                for (int i = 0; i < KW; i += 4) {
+                    const u32x4 w = read<u32x4>(from, at_k, i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) k[n][i + e] = w[e];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) ks[n][i] = read<uint32_t>(a.c.k_scale + half.scale, at_s, i);
         }
-    }
+    };
+
+    const int tiles = (v.rows * a.ratio + 15) / 16;
+    for (int turn = 0; turn == 0 || turn < tiles; turn += TURN) {
+        int t = begin + TOKENS * wave;
+        if (t < end) load(t);
+        if (turn > 0) __syncthreads();
+        for (int tile = turn + wave; tile < tiles && tile < turn + TURN; tile += 4) {
+            const int row = tile * 16 + r, query = row / a.ratio;
+            const bool there = query < v.rows;
+            const int64_t token = v.start + (there ? query : 0);
+            const int head = h * a.ratio + row % a.ratio;
+            h8 q[STEPS];
+            const float undo = load_row<D>(q, (const uint16_t*)a.q + token * a.ld_q + (int64_t)head * a.hd_q, there,
+                                           a.type == DT_BF16, j, a.scale);
+            float lse = there ? a.lse[token * a.heads + head] : __builtin_inff();
+            lse = lse == -__builtin_inff() ? __builtin_inff() : lse * LOG2E;  // (a row that saw nothing gives nothing)
+            int low = 0, limit = v.len;
+            if (there) sees(a, v, query, low, limit);
+            TileRows& x = info[tile - turn];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+            for (int i = 0; i < STEPS; ++i) rows_of[((tile - turn) * STEPS + i) * 64 + lane] = q[i];
+            if (j == 0) x.undo[r] = undo, x.lse[r] = lse, x.low[r] = low, x.limit[r] = limit;
+            int any_low = there ? low : v.len, any_limit = there ? limit : 0, all_low = low, all_limit = limit;
 #pragma unroll
-        for (int off = 1; off < 16; off <<= 1) got[e] += __shfl_xor(got[e], off, 64);
-        const int64_t pos = first + (e >> 2) * 16 + 4 * j + (e & 3);
-        if (r == e && pos < a.cap) {
-            if (pos < v.len) out[pos] = in ? __builtin_fmaf(a.decay, in[pos], got[e]) : got[e];
-            else if (!in) out[pos] = 0.0f;
+            for (int off = 1; off < 16; off <<= 1) {
+                const int y0 = __shfl_xor(any_low, off, 64), y1 = __shfl_xor(any_limit, off, 64);
+                const int y2 = __shfl_xor(all_low, off, 64), y3 = __shfl_xor(all_limit, off, 64);
+                any_low = any_low < y0 ? any_low : y0;
+                any_limit = any_limit > y1 ? any_limit : y1;
+                all_low = all_low > y2 ? all_low : y2;
+                all_limit = all_limit < y3 ? all_limit : y3;
+            }
+            if (lane == 0) x.any_low = any_low, x.any_limit = any_limit, x.all_low = all_low, x.all_limit = all_limit;
+        }
+        __syncthreads();
+        const int here = tiles - turn < TURN ? tiles - turn : TURN;
+        for (; t < end; t += 4 * TOKENS) {
+            h8 f[NT][STEPS];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const uint32_t w = ks[n][i * KS / STEPS];
+                    f[n][i] = key_fragment(k[n][i], low_pair(w, w), high_pair(w, w));
+                }
+            const uint32_t good = ok;
+            if (t + 4 * TOKENS < end) load(t + 4 * TOKENS);
+            float got[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) got[n] = 0.0f;
+            for (int tile = 0; tile < here; ++tile) {
+                const TileRows& x = info[tile];
+                if (t >= __builtin_amdgcn_readfirstlane(x.any_limit) || t + TOKENS <= __builtin_amdgcn_readfirstlane(x.any_low)) continue;
+                const bool edge = t < __builtin_amdgcn_readfirstlane(x.all_low) ||
+                                  t + TOKENS > __builtin_amdgcn_readfirstlane(x.all_limit) || good != (1u << NT) - 1;
+                v4f s[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[n] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const h8 q = rows_of[(tile * STEPS + i) * 64 + lane];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) s[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q, f[n][i], s[n], 0, 0, 0);
+                }
+                const v4f undo = *(const v4f*)(x.undo + 4 * j), lse = *(const v4f*)(x.lse + 4 * j);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], undo[i], -lse[i]));
+                if (edge) {
+                    const v4i low = *(const v4i*)(x.low + 4 * j), limit = *(const v4i*)(x.limit + 4 * j);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const int token = t + 16 * n + r;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[n][i] = token >= low[i] && token < limit[i] && (good >> n & 1u) ? s[n][i] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) got[n] += (s[n][0] + s[n][1]) + (s[n][2] + s[n][3]);
+            }
+            float mine = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                got[n] += __shfl_xor(got[n], 16, 64);
+                got[n] += __shfl_xor(got[n], 32, 64);
+                mine = j == n ? got[n] : mine;
+            }
+            const int pos = t + lane;  // (lane 16 n + r: token r of tile n)
+            if (lane < TOKENS && pos < end) {
+                if (turn > 0) out[pos] += mine;
+                else out[pos] = in ? __builtin_fmaf(a.decay, in[pos], mine) : mine;
+            }
         }
     }
 }
 
-// tokens that a tile of 16 rows can see at most
+constexpr int UNIT = 128;  // tokens of a range: a step of each of four waves, or two steps of eight
+
+// tokens that a tile can see at most
 int64_t widest(const KvAttentionArgs& a)
 {
     const int64_t all = (int64_t)a.s.table_pages << a.c.page_shift;
-    const int64_t seen = a.window && a.causal ? (int64_t)a.window + 16 / a.ratio + 1 + 31 : all;
+    const int64_t seen = a.window && a.causal ? (int64_t)a.window + a.tile_rows / a.ratio + 1 + 31 : all;
     return seen < all ? seen : all;
 }
 
-void plan(KvAttentionArgs& a, bool room)
+int rows_in_use(const KvAttentionArgs& a)
+{
+    const int64_t rows = (int64_t)a.max_q * a.ratio;
+    return (int)(rows < a.tile_rows ? rows : a.tile_rows);
+}
+
+// bytes that one split of every row takes in the workspace
+size_t split_bytes(const KvAttentionArgs& a)
+{
+    return (size_t)a.s.batch * a.tiles * a.c.kv_heads * rows_in_use(a) * (a.c.d + 2) * sizeof(float);
+}
+
+// tiles of rows, and ranges of tokens as far as `room` bytes go
+void plan(KvAttentionArgs& a, size_t room)
 {
     a.ratio = a.heads / a.c.kv_heads;
     const int64_t rows = (int64_t)a.max_q * a.ratio;
-    a.tiles = (int)((rows + 15) / 16);
-    a.rows = (int)(rows < 16 ? rows : 16);
+    a.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 && a.c.d == 256 ? 64 : rows <= 128 || a.c.d == 256 ? 128 : 256;
+    a.tiles = (int)((rows + a.tile_rows - 1) / a.tile_rows);
     const int64_t span = widest(a);
     const int64_t groups = (int64_t)a.s.batch * a.tiles * a.c.kv_heads;
-    int64_t splits = 1;
-    if (room && groups < 1024) {
-        splits = 1024 / groups;
-        const int64_t most = (span + 255) / 256;
-        splits = splits < most ? splits : most;
-    }
-    if (splits < 1) splits = 1;
-    const int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;
-    a.chunk = (int)(chunk < 128 ? 128 : chunk);
+    // Up to 32 rows about six workgroups per CU in all, three of which fit at a time: fewer leave the end of ragged lengths to few,
+    // more pay for their starts (us, 32 sequences of up to 8192 tokens, 8 key heads / 8 of 131072: 1024 42 / 215, 2048 43 / 211,
+    // 4096 48 / 223).  More rows: one per CU, as the rows' sums of further ranges are many.
+    const int64_t wanted = a.tile_rows > 32 ? 256 : 1536;
+    int64_t splits = wanted / groups;
+    const int64_t most = (span + UNIT - 1) / UNIT, fit = (int64_t)(room / split_bytes(a));
+    splits = splits < most ? splits : most;
+    splits = splits < fit ? splits : fit;
+    splits = splits < 1 ? 1 : splits;
+    const int64_t chunk = ((span + splits - 1) / splits + UNIT - 1) / UNIT * UNIT;
+    a.chunk = (int)(chunk < UNIT ? UNIT : chunk);
     a.splits = (int)((span + a.chunk - 1) / a.chunk);
     if (a.splits < 1) a.splits = 1;
-}
-
-size_t part_bytes(const KvAttentionArgs& a)
-{
-    if (a.splits < 2) return 0;
-    return (size_t)a.s.batch * a.tiles * a.c.kv_heads * a.rows * a.splits * (a.c.d + 2) * sizeof(float);
 }
 
 template <int D, int G>
 hipError_t run_attention(KvAttentionArgs a, hipStream_t st)
 {
-    const int64_t per = (int64_t)a.tiles * a.c.kv_heads * a.splits;  // workgroups of a sequence
-    const int64_t most = ((int64_t)1 << 23) / per;                   // sequences of a launch: below 2^31 threads
+    const int64_t per = (int64_t)a.tiles * a.c.kv_heads;         // tiles and heads of a sequence
+    const int64_t most = ((int64_t)1 << 22) / (per * a.splits);  // sequences of a launch: at most 2^31 threads
     float* part = a.part;
     for (int64_t at = 0; at < a.s.batch; at += most) {
         const int64_t n = a.s.batch - at < most ? a.s.batch - at : most;
         a.first = (int)at;
         KvAttentionArgs now = a;
         now.s.batch = (int)(at + n);
-        now.part = part + at * a.tiles * a.c.kv_heads * a.rows * a.splits * (a.c.d + 2);
-        launch_k(kv_attention_kernel<D, G>, dim3((uint32_t)(n * per)), dim3(256), 0, st, now);
-        hipError_t e = hipGetLastError();
+        const int64_t rows = per * rows_in_use(a);
+        now.part = part + at * rows * a.splits * (a.c.d + 2);
+        const uint32_t groups = (uint32_t)(n * per);
+        const dim3 grid(groups * a.splits);
+        hipError_t e = hipSuccess;
+        auto chunk = [&](auto nq, auto waves) {
+            constexpr int NQ = decltype(nq)::value, WAVES = decltype(waves)::value;
+            constexpr int LDS = 3 * (WAVES / 4) * (2 * Shape<D>::STEPS + Shape<D>::TILES) * 1024;
+            e = ensure_dynamic_lds<kv_chunk_kernel<D, G, NQ, WAVES>>(LDS);
+            if (e == hipSuccess) launch_k(kv_chunk_kernel<D, G, NQ, WAVES>, grid, dim3(64 * WAVES), LDS, st, now, groups);
+        };
+        using one = std::integral_constant<int, 1>;
+        using two = std::integral_constant<int, 2>;
+        using waves = std::integral_constant<int, D == 256 ? 4 : 8>;
+        if (a.tile_rows == 16) launch_k(kv_attention_kernel<D, G, 1>, grid, dim3(256), 0, st, now, groups);
+        else if (a.tile_rows == 32) launch_k(kv_attention_kernel<D, G, 2>, grid, dim3(256), 0, st, now, groups);
+        else if (a.tile_rows == 16 * waves::value) chunk(one{}, waves{});
+        else chunk(two{}, waves{});
+        if (e == hipSuccess) e = hipGetLastError();
         if (e != hipSuccess) return e;
         if (a.splits > 1) {
-            const int64_t rows = n * a.tiles * a.c.kv_heads * a.rows;
-            hipLaunchKernelGGL(kv_join_kernel<D>, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, st, now);
+            hipLaunchKernelGGL(kv_join_kernel<D>, dim3((uint32_t)(n * rows)), dim3(256), 0, st, now);
             e = hipGetLastError();
             if (e != hipSuccess) return e;
         }
@@ -622,13 +1170,25 @@ hipError_t run_attention(KvAttentionArgs a, hipStream_t st)
 template <int D, int G>
 hipError_t run_weights(KvAttentionArgs a, hipStream_t st)
 {
-    const int64_t blocks = ((int64_t)a.cap + 127) / 128, per = blocks * a.c.kv_heads;
-    const int64_t most = ((int64_t)1 << 23) / per;
+    a.ratio = a.heads / a.c.kv_heads;
+    const int64_t tiles = ((int64_t)a.max_q * a.ratio + 15) / 16;
+    const int lds = (int)(tiles < TURN ? tiles : TURN) * Shape<D>::STEPS * 1024;
+    hipError_t e = ensure_dynamic_lds<kv_weights_kernel<D, G>>(TURN * Shape<D>::STEPS * 1024);
+    if (e != hipSuccess) return e;
+    // ranges of tokens: about six workgroups per CU in all, as for the attention
+    const int64_t groups = (int64_t)a.s.batch * a.c.kv_heads;
+    const int unit = D == 256 ? 128 : 256;
+    int64_t parts = 1536 / groups;
+    parts = parts < 1 ? 1 : parts;
+    int64_t chunk = ((a.cap + parts - 1) / parts + unit - 1) / unit * unit;
+    a.chunk = (int)chunk;
+    parts = (a.cap + chunk - 1) / chunk;
+    const int64_t per = parts * a.c.kv_heads, most = ((int64_t)1 << 23) / per;  // sequences of a launch: below 2^31 threads
     for (int64_t at = 0; at < a.s.batch; at += most) {
         const int64_t n = a.s.batch - at < most ? a.s.batch - at : most;
         a.first = (int)at;
-        launch_k(kv_weights_kernel<D, G>, dim3((uint32_t)(n * per)), dim3(256), 0, st, a, (int)blocks);
-        const hipError_t e = hipGetLastError();
+        launch_k(kv_weights_kernel<D, G>, dim3((uint32_t)(n * per)), dim3(256), (uint32_t)lds, st, a, (uint32_t)(n * a.c.kv_heads));
+        e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -651,21 +1211,19 @@ hipError_t run_weights(KvAttentionArgs a, hipStream_t st)
 
 size_t kv_attention_ws_bytes(KvAttentionArgs a)
 {
-    plan(a, true);
-    return part_bytes(a);
+    plan(a, SIZE_MAX);
+    return a.splits < 2 ? 0 : split_bytes(a) * a.splits;
 }
 
 hipError_t launch_kv_attention(KvAttentionArgs a, void* ws, size_t ws_bytes, hipStream_t st)
 {
-    plan(a, ws != nullptr);
-    if (part_bytes(a) > ws_bytes) plan(a, false);
+    plan(a, ws ? ws_bytes : 0);
     a.part = (float*)ws;
     KV_SHAPES(run_attention)
 }
 
 hipError_t launch_kv_weights(KvAttentionArgs a, hipStream_t st)
 {
-    plan(a, false);
     KV_SHAPES(run_weights)
 }
 

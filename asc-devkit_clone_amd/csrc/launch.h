@@ -377,9 +377,9 @@ struct KvAttentionArgs {
     int64_t ld_q, hd_q, ld_out, hd_out;
     int T, cap, type, heads, max_q, window, causal;
     float scale, decay;
-    // (set by the launcher) heads per key head, tiles of 16 rows per sequence and key head, rows in use of a tile, token
-    // range of a split and how many, the launch's first sequence
-    int ratio, tiles, rows, chunk, splits, first;
+    // (set by the launcher) heads per key head, tiles of tile_rows rows per sequence and key head, token range of a split and
+    // how many, the launch's first sequence
+    int ratio, tiles, tile_rows, chunk, splits, first;
 };
 // workspace (16-byte aligned, or null): room for the sums of ranges of tokens; with less a sequence is one range
 size_t kv_attention_ws_bytes(KvAttentionArgs a);

@@ -45,8 +45,8 @@ int main()
                         const ascq_kv_cache c{p, p, p, p, 1 << 20, 0, 0, kv, 64, 128, 32};
                         const ascq_kv_sequences s{(int32_t*)p, (int32_t*)p, (int32_t*)p, 0, batch, pages};
                         const ascq_kv_attention_param ap{INT32_MAX, queries, 0, 0, 0, 0, 0, ASCQ_DT_F16, kv * ratio, 1, 1.0f};
-                        const int64_t tiles = (queries * ratio + 15) / 16;
-                        if (tiles * kv > 1 << 23 || (double)batch * tiles * kv > 1e10) continue;  // (refused; thousands of launches)
+                        const int64_t most_tiles = (queries * ratio + 15) / 16;
+                        if (most_tiles * kv > 1 << 23 || (double)batch * most_tiles * kv > 1e10) continue;  // (refused; thousands of launches)
                         size_t bytes = 0;
                         expect(ascq_kv_attention_workspace_size(&c, &s, &ap, &bytes) == ASCQ_OK, "size", batch, queries, kv);
                         for (int room = 0; room < 2; ++room) {
@@ -55,10 +55,11 @@ int main()
                             int64_t at = 0, joined = 0;
                             for (const Launch& l : launches()) {
                                 const auto a = l.args<ascq::KvAttentionArgs>();
-                                good &= fits(l) && a.ratio == ratio && a.tiles == tiles;
+                                const int64_t all = queries * ratio, tiles = a.tiles, rows = all < a.tile_rows ? all : a.tile_rows;
+                                good &= fits(l) && a.ratio == ratio && tiles * a.tile_rows >= all && (tiles - 1) * a.tile_rows < all;
                                 const int64_t groups = (int64_t)(a.s.batch - a.first) * tiles * kv;
                                 if (l.is("kv_join")) {
-                                    good &= a.first == joined && l.grid.x * 4ull >= (uint64_t)groups * a.rows;
+                                    good &= a.first == joined && l.grid.x * 4ull >= (uint64_t)groups * rows;
                                     joined = a.s.batch;
                                 } else {
                                     good &= a.first == at && l.grid.x == (uint64_t)groups * a.splits;
@@ -66,7 +67,7 @@ int main()
                                     at = a.s.batch;
                                 }
                                 if (a.splits > 1) {
-                                    const uint64_t end = ((uint8_t*)a.part - (uint8_t*)p) + (uint64_t)groups * a.rows * a.splits * 130 * 4;
+                                    const uint64_t end = ((uint8_t*)a.part - (uint8_t*)p) + (uint64_t)groups * rows * a.splits * 130 * 4;
                                     good &= room && end <= bytes;
                                 }
                             }
@@ -80,7 +81,7 @@ int main()
                         for (const Launch& l : launches()) {
                             const auto a = l.args<ascq::KvAttentionArgs>();
                             good &= fits(l) && a.first == at;
-                            const int64_t blocks = (cap + 127) / 128;
+                            const int64_t blocks = (cap + a.chunk - 1) / a.chunk;
                             good &= l.grid.x % (blocks * kv) == 0;
                             at += l.grid.x / (blocks * kv);
                         }

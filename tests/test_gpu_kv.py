@@ -128,6 +128,16 @@ def test_attention_queries(ascq_gpu, d, group, causal):
     _check_attention(ascq_gpu, p, causal=causal, window=9)
 
 
+@pytest.mark.parametrize("ratio,kv", [(1, 2), (4, 1), (7, 1)])
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 32), (256, 64), (256, 128)])
+def test_attention_many_queries(ascq_gpu, d, group, ratio, kv):
+    """tiles of 64 to 256 rows, in part filled; sequences of fewer tokens than queries; more rows than one tile"""
+    for queries, lengths, page, dt in (([40], [70], 16, "f16"), ([100, 3], [100, 9], 32, "bf16"), ([70, 1, 200], [300, 33, 150], 64, "f16")):
+        p = K.Problem(d + ratio, lengths, queries=queries, heads=ratio * kv, kv=kv, d=d, group=group, page=page, dt=dt)
+        _check_attention(ascq_gpu, p)
+        _check_attention(ascq_gpu, p, window=37)
+
+
 @pytest.mark.parametrize("window", [1, 2, 31, 32, 33, 100, 1000, 1 << 40])
 def test_attention_window(ascq_gpu, window):
     p = K.Problem(window % 1000, [1, 31, 64, 99, 333], heads=4, kv=4, page=16, d=64, group=64)
