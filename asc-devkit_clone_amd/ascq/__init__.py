@@ -225,7 +225,9 @@ SIGNATURES = {
     "ascq_kv_weights": (_I32, [_P, _P, _I64, _F32, _P, _P, ctypes.POINTER(_KvCache), ctypes.POINTER(_KvSequences),
                                ctypes.POINTER(_KvAttentionParam), _P]),
     "ascq_kv_evict": (_I32, [_P] * 5 + [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvSequences), ctypes.POINTER(_KvEvictParam),
-                                        _P]),
+                                        _P, ctypes.c_size_t, _P]),
+    "ascq_kv_evict_workspace_size": (_I32, [ctypes.POINTER(_KvCache), ctypes.POINTER(_KvSequences),
+                                            ctypes.POINTER(ctypes.c_size_t)]),
     "ascq_nz_size": (ctypes.c_size_t, [_I32, _I64, _I64, _I64]),
     "ascq_nz_to_nd": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _I32, _P]),
     "ascq_nd_to_nz": (_I32, [_P, _P, _I32, _I64, _I64, _I64, _P]),
@@ -1061,12 +1063,13 @@ def kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: KvCache, page_table: t
 
 
 def kv_evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, weights: torch.Tensor, keep: int, recent: int = 0,
-             into=None, kept=None, lengths_out=None, weights_out=None, stream=None):
+             into=None, kept=None, lengths_out=None, weights_out=None, workspace=None, stream=None):
     """Cuts every sequence to its `keep` tokens of most weight (f32 [batch, kv_heads, cap], see kv_weights), the last `recent` always
     among them, per key head.  They move in order to the sequence's first places: in its own pages, which no other sequence shares
     then, or in the pages into (int32 [batch, n], none of page_table's), the old ones staying as they are.  Returns (kept, lengths,
     weights): kept int32 [batch, kv_heads, keep], the tokens' former positions, -1 behind the last; the new lengths, a tensor of their
-    own; the kept tokens' weights, zeros behind them, in weights itself unless weights_out [batch, kv_heads, n] is given."""
+    own; the kept tokens' weights, zeros behind them, in weights itself unless weights_out [batch, kv_heads, n] is given.
+    workspace: a uint8 tensor of kv_evict_workspace_size bytes; without one the call takes it from torch's allocator."""
     what = "kv_evict"
     c = _cache_arg(what, cache)
     s = _sequences_arg(what, page_table, lengths, None)
@@ -1088,11 +1091,29 @@ def kv_evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, we
     _dense(what, "kept", at, (*heads, keep), torch.int32)
     n = lengths_out if lengths_out is not None else _new(stream, (s.batch,), torch.int32, weights.device)
     _dense(what, "lengths_out", n, (s.batch,), torch.int32)
-    _same_device(what, weights, page_table, lengths, into, at, n, w, *cache)
+    room = _room(what, workspace)
+    _same_device(what, weights, page_table, lengths, into, at, n, w, workspace, *cache)
     p = _KvEvictParam(weights.shape[2], w.shape[2], ld_into, keep, recent, columns)
+    if workspace is None:
+        need = ctypes.c_size_t(0)
+        check(lib().ascq_kv_evict_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(need)), what)
+        if need.value:
+            workspace, room = _new(stream, (need.value,), torch.uint8, weights.device, private=True), need.value
     check(lib().ascq_kv_evict(_at(at), _at(n), _at(w), _at(weights), _at(into), ctypes.byref(c), ctypes.byref(s), ctypes.byref(p),
-                              _stream(stream)), what)
+                              _at(workspace), room, _stream(stream)), what)
     return at, n, w
+
+
+def kv_evict_workspace_size(cache: KvCache, page_table: torch.Tensor) -> int:
+    """Bytes of the workspace that kv_evict uses for such a call (0: none)"""
+    what = "kv_evict_workspace_size"
+    c = _cache_arg(what, cache)
+    if page_table.dim() != 2:
+        _refuse(what, "page_table must be [batch, pages]")
+    s = _KvSequences(page_table.data_ptr(), page_table.data_ptr(), None, 0, *page_table.shape)
+    need = ctypes.c_size_t(0)
+    check(lib().ascq_kv_evict_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(need)), what)
+    return need.value
 
 
 # ------------------------------------------------------------------------------------------

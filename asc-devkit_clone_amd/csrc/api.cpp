@@ -2174,7 +2174,7 @@ ascq_status ascq_kv_weights(float* weights_out, const float* weights, int64_t ca
 
 ascq_status ascq_kv_evict(int32_t* kept, int32_t* new_lengths, float* weights_out, const float* weights, const int32_t* into,
                           const ascq_kv_cache* cache, const ascq_kv_sequences* sequences, const ascq_kv_evict_param* p,
-                          void* stream)
+                          void* workspace, size_t workspace_bytes, void* stream)
 {
     CallScope scope;
     const char* what = "kv_evict";
@@ -2217,7 +2217,22 @@ ascq_status ascq_kv_evict(int32_t* kept, int32_t* new_lengths, float* weights_ou
     a.recent = p->recent;
     trace("kv_evict: B %d, heads %d d %d group %d, keep %d recent %d%s", a.s.batch, a.c.kv_heads, a.c.d, a.c.group, a.keep, a.recent,
           into ? "" : ", in place");
-    return hip_status(ascq::launch_kv_evict(a, S(stream)), what);
+    // (a workspace off its alignment is none)
+    void* ws = workspace && aligned(workspace, 16) ? workspace : nullptr;
+    return hip_status(ascq::launch_kv_evict(a, ws, ws ? workspace_bytes : 0, S(stream)), what);
+}
+
+ascq_status ascq_kv_evict_workspace_size(const ascq_kv_cache* cache, const ascq_kv_sequences* sequences, size_t* bytes)
+{
+    const char* what = "kv_evict_workspace_size";
+    if (!bytes) return fail(ASCQ_E_INVALID_ARG, "%s: null argument", what);
+    ascq::KvEvictArgs a{};
+    ascq_status s = kv_cache_check(what, cache, a.c);
+    if (s != ASCQ_OK) return s;
+    s = kv_sequences_check(what, sequences, a.c, a.s);
+    if (s != ASCQ_OK) return s;
+    *bytes = ascq::kv_evict_ws_bytes(a);
+    return ASCQ_OK;
 }
 
 // ------------------------------------------------------------------------------------------------

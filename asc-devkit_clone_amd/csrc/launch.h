@@ -395,8 +395,13 @@ struct KvEvictArgs {
     const int* into;        // pages that the kept tokens go to [batch, ld_into], or null: the sequence's own
     int64_t cap, cap_out, ld_into;
     int into_pages, keep, recent;
-    int64_t first;          // (set by the launcher) the launch's first sequence
+    // (set by the launcher) the launch's first sequence; parts that a selection is shared by, and where they leave their counts
+    int64_t first;
+    int parts;
+    uint32_t* counts;
 };
-hipError_t launch_kv_evict(KvEvictArgs a, hipStream_t st);
+// workspace (16-byte aligned, or null): counts of long selections; with less a workgroup selects alone
+size_t kv_evict_ws_bytes(const KvEvictArgs& a);
+hipError_t launch_kv_evict(KvEvictArgs a, void* ws, size_t ws_bytes, hipStream_t st);
 
 }  // namespace ascq

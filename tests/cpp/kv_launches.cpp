@@ -31,7 +31,7 @@ int main()
             int64_t at = 0;
             for (const Launch& l : launches()) {
                 const auto a = l.args<ascq::KvAppendArgs>();
-                good &= fits(l) && a.first == at && l.threads() >= (uint64_t)(a.T - a.first) * kv * 32;
+                good &= fits(l) && a.first == at && l.threads() >= (uint64_t)(a.T - a.first) * kv * 16;
                 at = a.T;
             }
             expect(good && at == t, "append", t, kv, at);
@@ -94,23 +94,32 @@ int main()
                 const ascq_kv_cache c{p, p, p, p, 1 << 20, 0, 0, kv, 64, 128, 32};
                 const ascq_kv_sequences s{(int32_t*)p, (int32_t*)p, nullptr, 0, batch, 1 << 15};
                 const ascq_kv_evict_param ep{1 << 21, 1 << 21, 0, keep, 0, 1 << 15};
-                for (void* into : {(void*)nullptr, (void*)0x300000000000}) {
-                    launches().clear();
-                    bool good = ascq_kv_evict((int32_t*)p, (int32_t*)p + 1, (float*)p, (float*)p, (int32_t*)into, &c, &s, &ep, nullptr) == ASCQ_OK;
-                    int64_t selected = 0, moved = 0;
-                    for (const Launch& l : launches()) {
-                        const auto a = l.args<ascq::KvEvictArgs>();
-                        good &= fits(l);
-                        if (l.is("select")) {
-                            good &= a.first == selected && l.grid.x % kv == 0;
-                            selected += l.grid.x / kv;
-                        } else {
-                            good &= a.first == moved && l.grid.y % kv == 0 && (into || l.grid.x == 1);
-                            moved += l.grid.y / kv;
+                size_t bytes = 0;
+                expect(ascq_kv_evict_workspace_size(&c, &s, &bytes) == ASCQ_OK && bytes > 0, "evict size", batch, kv, keep);
+                for (int room = 0; room < 2; ++room)
+                    for (void* into : {(void*)nullptr, (void*)0x300000000000}) {
+                        launches().clear();
+                        bool good = ascq_kv_evict((int32_t*)p, (int32_t*)p + 1, (float*)p, (float*)p, (int32_t*)into, &c, &s, &ep,
+                                                  room ? p : nullptr, room ? bytes : 0, nullptr) == ASCQ_OK;
+                        int64_t selected[5] = {}, moved = 0;
+                        for (const Launch& l : launches()) {
+                            const auto a = l.args<ascq::KvEvictArgs>();
+                            good &= fits(l);
+                            if (l.is("select")) {
+                                const int digit = l.is("part_kernelILi0") ? 1 : l.is("part_kernelILi1") ? 2 : l.is("part_kernelILi2") ? 3
+                                                  : l.is("part_kernelILi3") ? 4 : 0;
+                                good &= a.first == selected[digit] && l.grid.x % (kv * a.parts) == 0 && (a.parts > 1) == (digit > 0);
+                                good &= digit == 0 || (room && l.grid.x * (size_t)(5122 * a.parts + 4) / a.parts * 4 <= bytes &&
+                                                       (int64_t)a.parts * 8192 >= (int64_t)s.table_pages * 64);
+                                selected[digit] += l.grid.x / (kv * a.parts);
+                            } else if (!l.is("weights")) {
+                                good &= a.first == moved && l.grid.y % kv == 0 && (into || l.grid.x == 1);
+                                moved += l.grid.y / kv;
+                            }
                         }
+                        for (int i = 0; i < 5; ++i) good &= selected[i] == ((i > 0) == (room > 0) ? batch : 0);
+                        expect(good && moved == batch, "evict", batch, selected[room], moved);
                     }
-                    expect(good && selected == batch && moved == batch, "evict", batch, selected, moved);
-                }
             }
     std::printf("%d failure(s)\n", failures);
     return failures != 0;

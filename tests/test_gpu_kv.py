@@ -310,14 +310,14 @@ def test_weights_add_up(ascq_gpu):
 
 
 # ---------------------------------------------------------------------------------------------- evict
-def _check_evict(ascq, p, w, keep, recent, into=None, cap_out=None):
+def _check_evict(ascq, p, w, keep, recent, into=None, cap_out=None, **more):
     cache = p.gpu(ascq)
     before = [x.cpu().clone() for x in cache]
     wt = w.cuda()
     out = None if cap_out is None else torch.full((*w.shape[:2], cap_out), math.nan).cuda()
     n0 = torch.tensor(p.lengths).int().cuda()
     kept, n, got = ascq.kv_evict(cache, p.table.cuda(), n0, wt, keep, recent, into=None if into is None else into.cuda(),
-                                 weights_out=out)
+                                 weights_out=out, **more)
     assert n.tolist() == [min(x, keep) for x in p.lengths]
     want = [x.clone() for x in before]
     for b, length in enumerate(p.lengths):
@@ -327,11 +327,11 @@ def _check_evict(ascq, p, w, keep, recent, into=None, cap_out=None):
             row = torch.zeros(got.shape[2])
             row[:len(stay)] = w[b, h][stay]
             assert torch.equal(got[b, h].cpu().nan_to_num(nan=-5.0), row.nan_to_num(nan=-5.0))
-            for i, t in enumerate(stay):
-                src = int(p.table[b, t // p.page])
-                dst = int((p.table if into is None else into)[b, i // p.page])
-                for pool, old in zip(want, before):
-                    pool[dst, h, i % p.page] = old[src, h, t % p.page]
+            i, t = torch.arange(len(stay)), torch.tensor(stay, dtype=torch.long)
+            src = p.table[b].long()[t // p.page]
+            dst = (p.table if into is None else into)[b].long()[i // p.page]
+            for pool, old in zip(want, before):
+                pool[dst, h, i % p.page] = old[src, h, t % p.page]
     for a, b in zip(cache, want):
         assert torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
     if out is not None:
@@ -352,15 +352,22 @@ def test_evict(ascq_gpu, d, group, away):
         _check_evict(ascq_gpu, p, w, keep, recent, into, cap_out=keep + 7 if away else None)
 
 
+@pytest.mark.parametrize("alone", [False, True])
 @pytest.mark.parametrize("away", [False, True])
-def test_evict_long(ascq_gpu, away):
-    """tens of thousands of tokens, in place and elsewhere; all weights equal, and all zero but few"""
-    p = K.Problem(2, [20000, 9000, 12000], heads=1, kv=1, d=64, group=64, page=64, spare=450)
-    w = torch.exp(3 * torch.randn(3, 1, p.columns * 64, generator=p.g))
+@pytest.mark.parametrize("keep,recent", [(9500, 1000), (1, 0), (5000, 5000), (8193, 1), (14000, 30)])
+def test_evict_long(ascq_gpu, keep, recent, away, alone):
+    """tens of thousands of tokens, in place and elsewhere, with and without the workspace; all weights equal, all zero but few,
+    weights that differ in their last bits alone, negative ones and NaN"""
+    p = K.Problem(2, [20000, 9000, 12000, 17001, 30, 16385], heads=1, kv=1, d=64, group=64, page=64, spare=6 * 220)
+    w = torch.exp(3 * torch.randn(6, 1, p.columns * 64, generator=p.g))
     w[1] = 0.25
     w[2] = torch.where(torch.rand(w[2].shape, generator=p.g) < 0.9, 0.0, w[2])
-    into = p.spare[:3 * 150].view(3, 150) if away else None
-    _check_evict(ascq_gpu, p, w, 9500, 1000, into)
+    w[3] = 1 + torch.randint(0, 5000, w[3].shape, generator=p.g) * 2.0 ** -23
+    w[5] = torch.where(torch.rand(w[5].shape, generator=p.g) < 0.2, math.nan, w[5] - 1)
+    into = p.spare[:6 * 220].view(6, 220) if away else None
+    more = dict(workspace=torch.zeros(0, dtype=torch.uint8, device="cuda")) if alone else {}
+    assert ascq_gpu.kv_evict_workspace_size(p.gpu(ascq_gpu), p.table.cuda()) > 0
+    _check_evict(ascq_gpu, p, w, keep, recent, into, **more)
 
 
 def test_evict_bad_pages(ascq_gpu):

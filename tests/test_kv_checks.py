@@ -101,9 +101,9 @@ def test_evict_arguments():
     def call(kept=D, n=ctypes.c_void_p(0x2000), wo=D, w=D, into=None, cap=64, cap_out=64, ldi=0, keep=32, recent=4, pages=2,
              cache=None, seq=None):
         p = ascq._KvEvictParam(cap, cap_out, ldi, keep, recent, pages)
-        return ascq.lib().ascq_kv_evict(kept, n, wo, w, into, cache or _cache(), seq or _seq(), ctypes.byref(p), None)
+        return ascq.lib().ascq_kv_evict(kept, n, wo, w, into, cache or _cache(), seq or _seq(), ctypes.byref(p), None, 0, None)
 
-    _err(ascq.lib().ascq_kv_evict(D, D, D, D, None, _cache(), _seq(), None, None), ascq.E_INVALID_ARG, "null params")
+    _err(ascq.lib().ascq_kv_evict(D, D, D, D, None, _cache(), _seq(), None, None, 0, None), ascq.E_INVALID_ARG, "null params")
     for bad, status in BAD_CACHE:
         _err(call(cache=_cache(**bad)), status)
     for bad, status in BAD_SEQ:
@@ -117,6 +117,17 @@ def test_evict_arguments():
     _err(call(cap=1 << 31, cap_out=1 << 31), ascq.E_UNSUPPORTED)
     _err(call(into=other, ldi=1 << 60), ascq.E_UNSUPPORTED)
     _err(call(seq=_seq(table=None, lengths=None, batch=0), kept=None, n=None), ascq.OK)
+    need = ctypes.c_size_t(7)
+    size = ascq.lib().ascq_kv_evict_workspace_size
+    _err(size(_cache(), _seq(), None), ascq.E_INVALID_ARG)
+    for bad, status in BAD_CACHE:
+        _err(size(_cache(**bad), _seq(), ctypes.byref(need)), status)
+    for bad, status in BAD_SEQ:
+        _err(size(_cache(), _seq(**bad), ctypes.byref(need)), status)
+    _err(size(_cache(), _seq(), ctypes.byref(need)), ascq.OK)
+    assert need.value == 0
+    _err(size(_cache(), _seq(columns=1025), ctypes.byref(need)), ascq.OK)
+    assert need.value > 0
 
 
 def test_binding_refusals():
@@ -173,6 +184,7 @@ def test_binding_refusals():
     _refused(ev, cache, table, lengths, w, 8, kept=torch.zeros(3, 2, 7).int())
     _refused(ev, cache, table, lengths, w, 8, lengths_out=lengths.long())
     _refused(ev, cache, table, lengths, w, 8, weights_out=w[:, :, ::2])
+    _refused(ev, cache, table, lengths, w, 8, workspace=w[:, :, ::2])
 
 
 def _calls(v):
