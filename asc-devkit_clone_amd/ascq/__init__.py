@@ -880,14 +880,41 @@ def moe_combine_grad(grad_out: torch.Tensor, y: torch.Tensor, slots: torch.Tenso
 # ------------------------------------------------------------------------------------------
 # attention over the paged int4 key / value cache
 # ------------------------------------------------------------------------------------------
-class KvCache(NamedTuple):
-    """A paged key / value cache: int4 codes (uint8 [pages, kv_heads, page_size, d / 2]) and f16 (scale, offset) pairs
-    ([pages, kv_heads, page_size, d / group, 2]); a page's elements are contiguous, pages at any pitch of 16 bytes.  A code stands
-    for f16(code * scale + offset)."""
-    k: torch.Tensor
-    v: torch.Tensor
-    k_scale: torch.Tensor
-    v_scale: torch.Tensor
+class KvCache:
+    """A paged key / value cache: int4 codes k, v (uint8 [pages, kv_heads, page_size, d / 2]) and f16 (scale, offset) pairs k_scale,
+    v_scale ([pages, kv_heads, page_size, d / group, 2]); a page's elements are contiguous, pages at any pitch of 16 bytes.  A code
+    stands for f16(code * scale + offset).  The tensors are checked here, once, and stay the cache's; iterating gives the four."""
+    __slots__ = ("_tensors", "_c", "_ref", "_device")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        what = "KvCache"
+        if k.dim() != 4 or k_scale.dim() != 5:
+            _refuse(what, "codes must be [pages, kv_heads, page_size, d / 2], scales [pages, kv_heads, page_size, d / group, 2]")
+        shape, pairs = k.shape, k_scale.shape
+        groups = pairs[3]
+        if pairs[:3] != shape[:3] or pairs[4] != 2 or groups < 1 or 2 * shape[3] % groups:
+            _refuse(what, f"k_scale {tuple(pairs)} does not fit codes {tuple(shape)}")
+        ld = _page_pitch(what, "k", k, shape, torch.uint8)
+        ld_scale = _page_pitch(what, "k_scale", k_scale, pairs, torch.float16)
+        if ld != _page_pitch(what, "v", v, shape, torch.uint8) or \
+                ld_scale != _page_pitch(what, "v_scale", v_scale, pairs, torch.float16):
+            _refuse(what, "keys and values must have one page pitch")
+        self._device = k.get_device()
+        for t in (v, k_scale, v_scale):
+            if t.get_device() != self._device:
+                _refuse(what, f"tensors on {k.device} and {t.device}")
+        self._tensors = (k, v, k_scale, v_scale)
+        self._c = _KvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), shape[0], ld, ld_scale, shape[1],
+                           shape[2], 2 * shape[3], 2 * shape[3] // groups)
+        self._ref = ctypes.byref(self._c)
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
+
+    def __iter__(self):
+        return iter(self._tensors)
 
 
 def kv_cache(pages: int, kv_heads: int, page_size: int, d: int, group: int = 32, device="cuda") -> KvCache:
@@ -906,20 +933,10 @@ def _page_pitch(what: str, name: str, t: torch.Tensor, shape, dtype) -> int:
     return t.stride(0) if t.shape[0] > 1 else 0
 
 
-def _cache_arg(what: str, c: KvCache) -> _KvCache:
-    if c.k.dim() != 4 or c.k_scale.dim() != 5:
-        _refuse(what, "codes must be [pages, kv_heads, page_size, d / 2], scales [pages, kv_heads, page_size, d / group, 2]")
-    shape, pairs = c.k.shape, c.k_scale.shape
-    groups = pairs[3]
-    if pairs[:3] != shape[:3] or pairs[4] != 2 or groups < 1 or 2 * shape[3] % groups:
-        _refuse(what, f"k_scale {tuple(pairs)} does not fit codes {tuple(shape)}")
-    ld = _page_pitch(what, "k", c.k, shape, torch.uint8)
-    ld_scale = _page_pitch(what, "k_scale", c.k_scale, pairs, torch.float16)
-    if ld != _page_pitch(what, "v", c.v, shape, torch.uint8) or \
-            ld_scale != _page_pitch(what, "v_scale", c.v_scale, pairs, torch.float16):
-        _refuse(what, "keys and values must have one page pitch")
-    return _KvCache(c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), shape[0], ld, ld_scale, shape[1],
-                    shape[2], 2 * shape[3], 2 * shape[3] // groups)
+def _cache_arg(what: str, cache: KvCache, on: torch.Tensor) -> _KvCache:
+    if cache._device != on.get_device():
+        _refuse(what, f"the cache on {cache.k.device}, other tensors on {on.device}")
+    return cache._c
 
 
 def _heads_pitch(what: str, name: str, t: torch.Tensor, shape, dtype):
@@ -970,7 +987,7 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
     too) into the cache: token t to row slots[t] % page_size of page slots[t] // page_size (int64; a slot outside the cache, -1 for
     padding, is not written; slots are distinct)."""
     what = "kv_append"
-    c = _cache_arg(what, cache)
+    c = _cache_arg(what, cache, k)
     if k.dim() != 3:
         _refuse(what, "k must be [tokens, kv_heads, d]")
     t = k.shape[0]
@@ -979,9 +996,9 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Ten
     ldk, hdk = _heads_pitch(what, "k", k, shape, k.dtype)
     ldv, hdv = _heads_pitch(what, "v", v, shape, k.dtype)
     _dense(what, "slots", slots, (t,), torch.int64)
-    _same_device(what, k, v, slots, *cache)
+    _same_device(what, k, v, slots)
     p = _KvAppendParam(t, ldk, hdk, ldv, hdv, code)
-    check(lib().ascq_kv_append(ctypes.byref(c), _at(k), _at(v), _at(slots), ctypes.byref(p), _stream(stream)), what)
+    check(lib().ascq_kv_append(cache._ref, _at(k), _at(v), _at(slots), ctypes.byref(p), _stream(stream)), what)
 
 
 def kv_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, starts=None, max_queries=None,
@@ -995,7 +1012,7 @@ def kv_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, leng
     are left as they were.  A table narrowed to the longest sequence's pages (page_table[:, :n]) makes the launch smaller.
     workspace: a uint8 tensor of kv_attention_workspace_size bytes; without one the call takes it from torch's allocator."""
     what = "kv_attention"
-    c = _cache_arg(what, cache)
+    c = _cache_arg(what, cache, q)
     s = _sequences_arg(what, page_table, lengths, starts)
     p = _queries_arg(what, q, c, starts, max_queries, scale, causal, window)
     o = out if out is not None else _new(stream, q.shape, q.dtype, q.device)
@@ -1005,13 +1022,13 @@ def kv_attention(q: torch.Tensor, cache: KvCache, page_table: torch.Tensor, leng
     if lse is not None:
         _dense(what, "lse", lse, q.shape[:2], torch.float32)
     room = _room(what, workspace)
-    _same_device(what, q, page_table, lengths, starts, o, lse, workspace, *cache)
+    _same_device(what, q, page_table, lengths, starts, o, lse, workspace)
     if workspace is None:
         need = ctypes.c_size_t(0)
-        check(lib().ascq_kv_attention_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(p), ctypes.byref(need)), what)
+        check(lib().ascq_kv_attention_workspace_size(cache._ref, ctypes.byref(s), ctypes.byref(p), ctypes.byref(need)), what)
         if need.value:
             workspace, room = _new(stream, (need.value,), torch.uint8, q.device, private=True), need.value
-    check(lib().ascq_kv_attention(_at(o), _at(lse), _at(q), ctypes.byref(c), ctypes.byref(s), ctypes.byref(p), _at(workspace), room,
+    check(lib().ascq_kv_attention(_at(o), _at(lse), _at(q), cache._ref, ctypes.byref(s), ctypes.byref(p), _at(workspace), room,
                                   _stream(stream)), what)
     return o, lse
 
@@ -1020,13 +1037,13 @@ def kv_attention_workspace_size(q: torch.Tensor, cache: KvCache, page_table: tor
                                 causal: bool = True, window: int = 0) -> int:
     """Bytes of the workspace that kv_attention uses for such a call (0: none)"""
     what = "kv_attention_workspace_size"
-    c = _cache_arg(what, cache)
+    c = _cache_arg(what, cache, q)
     if page_table.dim() != 2:
         _refuse(what, "page_table must be [batch, pages]")
     s = _KvSequences(page_table.data_ptr(), page_table.data_ptr(), _at(starts), 0, *page_table.shape)
     p = _queries_arg(what, q, c, starts, max_queries, None, causal, window)
     need = ctypes.c_size_t(0)
-    check(lib().ascq_kv_attention_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(p), ctypes.byref(need)), what)
+    check(lib().ascq_kv_attention_workspace_size(cache._ref, ctypes.byref(s), ctypes.byref(p), ctypes.byref(need)), what)
     return need.value
 
 
@@ -1037,7 +1054,7 @@ def kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: KvCache, page_table: t
     decay * weights: f32 [batch, kv_heads, cap], cap at least the page table's tokens.  lse as kv_attention returns it for the same
     arguments.  out may be weights; positions from a sequence's length on stay as they were, or, without weights, are zeros."""
     what = "kv_weights"
-    c = _cache_arg(what, cache)
+    c = _cache_arg(what, cache, q)
     s = _sequences_arg(what, page_table, lengths, starts)
     p = _queries_arg(what, q, c, starts, max_queries, scale, causal, window)
     _dense(what, "lse", lse, q.shape[:2], torch.float32)
@@ -1056,8 +1073,8 @@ def kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: KvCache, page_table: t
             with torch.cuda.stream(torch.cuda.ExternalStream(_stream(stream), q.device)):
                 w.copy_(weights)
     _dense(what, "out", w, shape, torch.float32)
-    _same_device(what, q, lse, page_table, lengths, starts, weights, w, *cache)
-    check(lib().ascq_kv_weights(_at(w), _at(weights), cap, decay, _at(q), _at(lse), ctypes.byref(c), ctypes.byref(s), ctypes.byref(p),
+    _same_device(what, q, lse, page_table, lengths, starts, weights, w)
+    check(lib().ascq_kv_weights(_at(w), _at(weights), cap, decay, _at(q), _at(lse), cache._ref, ctypes.byref(s), ctypes.byref(p),
                                 _stream(stream)), what)
     return w
 
@@ -1071,7 +1088,7 @@ def kv_evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, we
     own; the kept tokens' weights, zeros behind them, in weights itself unless weights_out [batch, kv_heads, n] is given.
     workspace: a uint8 tensor of kv_evict_workspace_size bytes; without one the call takes it from torch's allocator."""
     what = "kv_evict"
-    c = _cache_arg(what, cache)
+    c = _cache_arg(what, cache, weights)
     s = _sequences_arg(what, page_table, lengths, None)
     if weights.dim() != 3 or keep < 1:
         _refuse(what, "weights must be [batch, kv_heads, cap], keep at least 1")
@@ -1092,14 +1109,14 @@ def kv_evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, we
     n = lengths_out if lengths_out is not None else _new(stream, (s.batch,), torch.int32, weights.device)
     _dense(what, "lengths_out", n, (s.batch,), torch.int32)
     room = _room(what, workspace)
-    _same_device(what, weights, page_table, lengths, into, at, n, w, workspace, *cache)
+    _same_device(what, weights, page_table, lengths, into, at, n, w, workspace)
     p = _KvEvictParam(weights.shape[2], w.shape[2], ld_into, keep, recent, columns)
     if workspace is None:
         need = ctypes.c_size_t(0)
-        check(lib().ascq_kv_evict_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(need)), what)
+        check(lib().ascq_kv_evict_workspace_size(cache._ref, ctypes.byref(s), ctypes.byref(need)), what)
         if need.value:
             workspace, room = _new(stream, (need.value,), torch.uint8, weights.device, private=True), need.value
-    check(lib().ascq_kv_evict(_at(at), _at(n), _at(w), _at(weights), _at(into), ctypes.byref(c), ctypes.byref(s), ctypes.byref(p),
+    check(lib().ascq_kv_evict(_at(at), _at(n), _at(w), _at(weights), _at(into), cache._ref, ctypes.byref(s), ctypes.byref(p),
                               _at(workspace), room, _stream(stream)), what)
     return at, n, w
 
@@ -1107,12 +1124,12 @@ def kv_evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, we
 def kv_evict_workspace_size(cache: KvCache, page_table: torch.Tensor) -> int:
     """Bytes of the workspace that kv_evict uses for such a call (0: none)"""
     what = "kv_evict_workspace_size"
-    c = _cache_arg(what, cache)
+    c = _cache_arg(what, cache, page_table)
     if page_table.dim() != 2:
         _refuse(what, "page_table must be [batch, pages]")
     s = _KvSequences(page_table.data_ptr(), page_table.data_ptr(), None, 0, *page_table.shape)
     need = ctypes.c_size_t(0)
-    check(lib().ascq_kv_evict_workspace_size(ctypes.byref(c), ctypes.byref(s), ctypes.byref(need)), what)
+    check(lib().ascq_kv_evict_workspace_size(cache._ref, ctypes.byref(s), ctypes.byref(need)), what)
     return need.value
 
 

@@ -15,7 +15,7 @@
 // Scores are fp32 sums of exact f16 products (bf16 queries are scaled by a power of two per row into f16's range, which
 // keeps all their bits); P is rounded to f16 after exp2 (2^-12 a weight at most, and independent), sums and statistics are
 // fp32.
-#include "common.h"
+#include "gemm_core.h"
 
 #include <type_traits>
 
@@ -25,6 +25,11 @@ namespace {
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
+// Tables that a kernel reads and nobody writes meanwhile, so that their uniform loads go through the scalar cache whatever is
+// stored in between: as vector loads they would wait for all loads before them.
+typedef const int __attribute__((address_space(4))) * Table;
+__device__ __forceinline__ Table table_of(const int* p) { return (Table)(uintptr_t)p; }
+
 struct View {
     int start, rows, n, len;  // first row of q; queries computed; queries there are; tokens
 };
@@ -33,8 +38,8 @@ __device__ __forceinline__ View view_of(const KvAttentionArgs& a, int64_t b)
     View v;
     int64_t start = b, n = 1;
     if (a.s.starts) {
-        start = a.s.starts[b];
-        n = (int64_t)a.s.starts[b + 1] - start;
+        start = table_of(a.s.starts)[b];
+        n = (int64_t)table_of(a.s.starts)[b + 1] - start;
     }
     if (start < 0 || start > a.T || n < 0) start = 0, n = 0;
     int64_t rows = n < a.max_q ? n : a.max_q;
@@ -43,7 +48,7 @@ __device__ __forceinline__ View view_of(const KvAttentionArgs& a, int64_t b)
     v.rows = (int)rows;
     v.n = (int)n;
     const int64_t most = (int64_t)a.s.table_pages << a.c.page_shift;
-    const int64_t len = a.s.lengths[b];
+    const int64_t len = table_of(a.s.lengths)[b];
     v.len = (int)(len < 0 ? 0 : len > most ? most : len);
     return v;
 }
@@ -75,10 +80,12 @@ struct Half {
     int64_t code, scale;  // bytes, words
     bool ok;
 };
-__device__ __forceinline__ int page_at(const KvAttentionArgs& a, const int* table, int token)
+__device__ __forceinline__ int page_at(const KvAttentionArgs& a, Table table, int token)
 {
-    const int col = token >> a.c.page_shift;
-    return col < a.s.table_pages ? table[col] : -1;
+    // (called for sequences of tokens alone, whose table has columns; a load without a branch around it)
+    const int col = token >> a.c.page_shift, last = a.s.table_pages - 1;
+    const int page = table[col < last ? col : last];
+    return col <= last ? page : -1;
 }
 __device__ __forceinline__ Half half_at(const KvAttentionArgs& a, int page, int h, int token)
 {
@@ -412,7 +419,7 @@ __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 3) void kv_at
     const int end = range.hi - begin > a.chunk ? begin + a.chunk : range.hi;
     const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int* table = a.s.table + b * a.s.ld_table;
+    const Table table = table_of(a.s.table + b * a.s.ld_table);
 
     // the first step is on its way before the queries
     const Lane at = lane_of_step<D, G>(r, j);
@@ -672,7 +679,7 @@ __global__ __launch_bounds__(64 * WAVES, NQ * D > 256 ? 1 : 2) void kv_chunk_ker
     const int end = range.hi - begin > a.chunk ? begin + a.chunk : range.hi;
     const int lane = threadIdx.x & 63, r = lane & 15, j = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = wave & 3, mine = 32 * (wave >> 2);
-    const int* table = a.s.table + b * a.s.ld_table;
+    const Table table = table_of(a.s.table + b * a.s.ld_table);
 
     // codes of step t: looked up two steps ahead, loaded one ahead (of the conversion, which is one ahead of their use)
     const Lane place = lane_of_quarter<D, G>(quarter, r, j);
@@ -692,8 +699,10 @@ __global__ __launch_bounds__(64 * WAVES, NQ * D > 256 ? 1 : 2) void kv_chunk_ker
         if (quarter == 0 && lane == 0) good[at][wave >> 2] = (x.ok0 ? 1u : 0u) | (x.ok1 ? 2u : 0u);
         convert_quarter<D, G>(slot + (wave >> 2) * SET, x, t + mine, end, quarter, r, j, lane);
     };
-    look(begin);
-    load(begin);
+    if (begin < end) {
+        look(begin);
+        load(begin);
+    }
 
     h8 q[NQ][STEPS];
     Row row[NQ];
@@ -935,7 +944,7 @@ struct TileRows {
 };
 
 template <int D, int G>
-__global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_weights_kernel(KvAttentionArgs a, uint32_t groups)
+__global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, uint32_t groups)
 {
     constexpr int STEPS = Shape<D>::STEPS, KW = Shape<D>::KW, NT = D == 256 ? 2 : 4, TOKENS = 16 * NT;
     constexpr int W = D / 8, GR = D / G, KS = Step<D, G>::KS;
@@ -954,18 +963,28 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_weights_kernel(KvAtt
     const int64_t begin64 = (int64_t)part * a.chunk;
     const int begin = (int)begin64, stop = a.cap - begin > a.chunk ? begin + a.chunk : a.cap;  // (begin < cap)
     const int end = stop < v.len ? stop : v.len;
-    const int* table = a.s.table + b * a.s.ld_table;
+    const Table table = table_of(a.s.table + b * a.s.ld_table);
     if (!in)
         for (int i = (begin > v.len ? begin : v.len) + (int)threadIdx.x; i < stop; i += 256) out[i] = 0.0f;
     if (begin >= end) return;
 
     const uint32_t at_k = 4u * (r * W + j * (W / 4)), at_s = 4u * (r * GR + j * (D / 4) / G);
     uint32_t k[NT][KW], ks[NT][KS], ok = 0;
-    auto load = [&](int t) {
+    int pages[NT];  // (looked up a step ahead of the loads)
+    auto look = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) pages[n] = page_at(a, table, t + 16 * n);
+    };
+    // What a lane's token has, before the call or from earlier turns: loaded whether it counts or not, as its store is issued
+    // whether it has a token or not (one behind the range is dropped), so that no branch hides how many are on their way.
+    float had = 0.0f;
+    const rsrc_t results = make_rsrc(out + begin, 4u * (uint32_t)(end - begin));
+    auto load = [&](int t, int turn) {
         ok = 0;
+        had = (in && turn == 0 ? in : out)[t + lane < end ? t + lane : end - 1];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const Half half = half_at(a, page_at(a, table, t + 16 * n), h, t + 16 * n);
+            const Half half = half_at(a, pages[n], h, t + 16 * n);
             ok |= half.ok ? 1u << n : 0u;
             const uint8_t* from = a.c.k + half.code;
             if constexpr (KW == 2) {
@@ -982,12 +1001,16 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_weights_kernel(KvAtt
 #pragma unroll
             for (int i = 0; i < KS; ++i) ks[n][i] = read<uint32_t>(a.c.k_scale + half.scale, at_s, i);
         }
+        look(t + 4 * TOKENS);
     };
 
     const int tiles = (v.rows * a.ratio + 15) / 16;
     for (int turn = 0; turn == 0 || turn < tiles; turn += TURN) {
         int t = begin + TOKENS * wave;
-        if (t < end) load(t);
+        if (t < end) {
+            look(t);
+            load(t, turn);
+        }
         if (turn > 0) __syncthreads();
         for (int tile = turn + wave; tile < tiles && tile < turn + TURN; tile += 4) {
             const int row = tile * 16 + r, query = row / a.ratio;
@@ -1029,7 +1052,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_weights_kernel(KvAtt
                     f[n][i] = key_fragment(k[n][i], low_pair(w, w), high_pair(w, w));
                 }
             const uint32_t good = ok;
-            if (t + 4 * TOKENS < end) load(t + 4 * TOKENS);
+            const float before = turn > 0 ? had : in ? a.decay * had : 0.0f;
+            if (t + 4 * TOKENS < end) load(t + 4 * TOKENS, turn);
             float got[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) got[n] = 0.0f;
@@ -1072,11 +1096,9 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void kv_weights_kernel(KvAtt
                 got[n] += __shfl_xor(got[n], 32, 64);
                 mine = j == n ? got[n] : mine;
             }
-            const int pos = t + lane;  // (lane 16 n + r: token r of tile n)
-            if (lane < TOKENS && pos < end) {
-                if (turn > 0) out[pos] += mine;
-                else out[pos] = in ? __builtin_fmaf(a.decay, in[pos], mine) : mine;
-            }
+            // (lane 16 n + r: token r of tile n)
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(before + mine), results,
+                                                  lane < TOKENS ? 4u * (uint32_t)(t - begin + lane) : ~3u, 0, 0);
         }
     }
 }
@@ -1177,12 +1199,11 @@ hipError_t run_weights(KvAttentionArgs a, hipStream_t st)
     if (e != hipSuccess) return e;
     // ranges of tokens: about six workgroups per CU in all, as for the attention
     const int64_t groups = (int64_t)a.s.batch * a.c.kv_heads;
-    const int unit = D == 256 ? 128 : 256;
+    constexpr int unit = D == 256 ? 128 : 256;
     int64_t parts = 1536 / groups;
-    parts = parts < 1 ? 1 : parts;
-    int64_t chunk = ((a.cap + parts - 1) / parts + unit - 1) / unit * unit;
-    a.chunk = (int)chunk;
-    parts = (a.cap + chunk - 1) / chunk;
+    parts = parts < 4 ? 4 : parts;  // (a range is below 2^30 bytes)
+    a.chunk = (int)(((a.cap + parts - 1) / parts + unit - 1) / unit * unit);
+    parts = (a.cap + (int64_t)a.chunk - 1) / a.chunk;
     const int64_t per = parts * a.c.kv_heads, most = ((int64_t)1 << 23) / per;  // sequences of a launch: below 2^31 threads
     for (int64_t at = 0; at < a.s.batch; at += most) {
         const int64_t n = a.s.batch - at < most ? a.s.batch - at : most;

@@ -60,7 +60,7 @@ def test_append(ascq_gpu, d, group, dt):
                 scales[slot // page, :, slot % page] = pairs[i]
     for a, b in zip(cache, want):
         assert torch.equal(a.cpu().view(torch.uint8), b.view(torch.uint8))
-    assert all(torch.isfinite(K.values(a.cpu(), b.cpu())).all() for a, b in zip(cache[:2], cache[2:]))
+    assert all(torch.isfinite(K.values(a.cpu(), b.cpu())).all() for a, b in zip(list(cache)[:2], list(cache)[2:]))
 
 
 @pytest.mark.parametrize("d,group", [(64, 64), (128, 32), (256, 128)])
@@ -72,7 +72,7 @@ def test_append_error(ascq_gpu, d, group):
     cache = ascq_gpu.kv_cache(4, 2, 16, d, group)
     ascq_gpu.kv_append(cache, x.cuda(), (2 * x).cuda(), torch.arange(64).cuda())
     for which, want in ((0, x), (1, 2 * x)):
-        got = K.values(cache[which].cpu(), cache[which + 2].cpu()).transpose(1, 2).flatten(0, 1)
+        got = K.values(list(cache)[which].cpu(), list(cache)[which + 2].cpu()).transpose(1, 2).flatten(0, 1)
         r = want.double().unflatten(-1, (-1, group))
         step = ((r.amax(-1) - r.amin(-1)) / 15).repeat_interleave(group, dim=-1)
         big = r.abs().amax(-1).repeat_interleave(group, dim=-1)
@@ -250,8 +250,8 @@ def test_attention_strides_and_rows_of_nobody(ascq_gpu):
     assert torch.equal(res, want)
     ascq_gpu.kv_attention(q, args[1], args[2][:, :6], args[3], **more, out=res)
     assert torch.equal(res, want)
-    both = torch.stack(list(args[1][:2]), dim=1).contiguous()
-    pairs = torch.stack(list(args[1][2:]), dim=1).contiguous()
+    both = torch.stack(list(args[1])[:2], dim=1).contiguous()
+    pairs = torch.stack(list(args[1])[2:], dim=1).contiguous()
     ascq_gpu.kv_attention(q, ascq_gpu.KvCache(both[:, 0], both[:, 1], pairs[:, 0], pairs[:, 1]), *args[2:], **more, out=res)
     assert torch.equal(res, want)
 
@@ -387,4 +387,4 @@ def test_evict_bad_pages(ascq_gpu):
                 src, dst = int(p.table[b, t // 16]), int(into[b, i // 16])
                 if 0 <= dst < want.shape[0]:
                     want[dst, 0, i % 16] = before[which][src, 0, t % 16].cpu() if src >= 0 else 0
-        assert torch.equal(cache[which].cpu().view(torch.uint8), want.view(torch.uint8))
+        assert torch.equal(list(cache)[which].cpu().view(torch.uint8), want.view(torch.uint8))

@@ -146,12 +146,15 @@ def test_binding_refusals():
     _refused(ascq.kv_append, cache, torch.zeros(3, 2, 256, dtype=torch.float16)[:, :, ::2], k, slots)
     _refused(ascq.kv_append, cache, k[:, :1].expand(3, 2, 128), k, slots)
     _refused(ascq.kv_append, cache, k.int(), k.int(), slots, status=ascq.E_UNSUPPORTED)
-    for bad in (cache._replace(k=cache.k.int()), cache._replace(v=cache.v[:3]), cache._replace(k_scale=cache.k_scale.float()),
-                cache._replace(v_scale=cache.v_scale[:, :, :, :2]), cache._replace(k=cache.k.transpose(1, 2)),
-                cache._replace(k=torch.zeros(8, 2, 16, 64, dtype=torch.uint8)[::2]), cache._replace(k=cache.k[0]),
-                cache._replace(k_scale=cache.k_scale[..., :1], v_scale=cache.v_scale[..., :1]),
-                cache._replace(k_scale=cache.k_scale[:, :, :, :3], v_scale=cache.v_scale[:, :, :, :3])):
-        _refused(ascq.kv_append, bad, k, k, slots)
+    good = dict(zip(("k", "v", "k_scale", "v_scale"), cache))
+    for bad in (dict(k=cache.k.int()), dict(v=cache.v[:3]), dict(k_scale=cache.k_scale.float()),
+                dict(v_scale=cache.v_scale[:, :, :, :2]), dict(k=cache.k.transpose(1, 2)),
+                dict(k=torch.zeros(8, 2, 16, 64, dtype=torch.uint8)[::2]), dict(k=cache.k[0]),
+                dict(k_scale=cache.k_scale[..., :1], v_scale=cache.v_scale[..., :1]),
+                dict(k_scale=cache.k_scale[:, :, :, :3], v_scale=cache.v_scale[:, :, :, :3])):
+        _refused(lambda **kw: ascq.KvCache(**kw), **{**good, **bad})
+    with pytest.raises(AttributeError):
+        cache.k = cache.v
     q, table, lengths = torch.zeros(3, 4, 128, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.int32), torch.ones(3).int()
     att = ascq.kv_attention
     _refused(att, q, cache, table, lengths)  # CPU tensors
@@ -202,7 +205,7 @@ def _calls(v):
 def test_memory_of_a_call_comes_from_its_stream(host, name, side):  # noqa: F811
     real = host.args["h"].new_empty
     v = dict(cache=ascq.KvCache(real(4, 2, 16, 64, dtype=torch.uint8), real(4, 2, 16, 64, dtype=torch.uint8),
-                                real(4, 2, 16, 4, 2), real(4, 2, 16, 4, 2)),
+                                real(4, 2, 16, 4, 2, dtype=torch.float16), real(4, 2, 16, 4, 2, dtype=torch.float16)),
              table=real(3, 2, dtype=torch.int32), n=real(3, dtype=torch.int32), q=real(3, 4, 128), lse=real(3, 4, dtype=torch.float32),
              w=real(3, 2, 32, dtype=torch.float32), stream=host.Stream(SIDE) if side else None)
     host.taken.clear()
