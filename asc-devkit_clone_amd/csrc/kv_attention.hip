@@ -270,19 +270,19 @@ template <int D>
 __device__ __forceinline__ float load_row(h8 (&q)[Shape<D>::STEPS], const uint16_t* row, bool there, bool bf16, int j, float scale)
 {
     u32x4 raw[Shape<D>::STEPS];
-    float top = 0.0f;
+    us2_t most = {0, 0};  // magnitudes order as their bits do, NaN above all
 #pragma unroll
     for (int i = 0; i < Shape<D>::STEPS; ++i) {
         raw[i] = there ? *(const u32x4_any*)(row + j * (D / 4) + 8 * i) : (u32x4){0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint16_t lo = (uint16_t)raw[i][e], hi = (uint16_t)(raw[i][e] >> 16);
-            top = __builtin_fmaxf(top, __builtin_fabsf(bf16 ? bf16_to_f32(lo) : f16_to_f32(lo)));
-            top = __builtin_fmaxf(top, __builtin_fabsf(bf16 ? bf16_to_f32(hi) : f16_to_f32(hi)));
-        }
+        for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(us2_t, raw[i][e] & 0x7fff7fffu));
     }
-    top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
-    top = __builtin_fmaxf(top, __shfl_xor(top, 32, 64));
+    uint32_t bits = most[0] > most[1] ? most[0] : most[1];
+    const uint32_t b16 = __shfl_xor(bits, 16, 64);
+    bits = bits > b16 ? bits : b16;
+    const uint32_t b32 = __shfl_xor(bits, 32, 64);
+    bits = bits > b32 ? bits : b32;
+    const float top = bf16 ? bf16_to_f32((uint16_t)bits) : f16_to_f32((uint16_t)bits);
     int e = (int)(__float_as_uint(top) >> 23) - 127;
     e = e < -100 ? -100 : e > 127 ? 14 : e;  // (0 and tiny rows; infinite ones pass as they are)
     float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
@@ -866,17 +866,18 @@ __global__ __launch_bounds__(64 * WAVES, NQ * D > 256 ? 1 : 2) void kv_chunk_ker
     }
 }
 
-// Adds what the ranges of a row left, a workgroup per row: a wave takes every fourth range, eight at a time so that their loads
-// are in flight together, and the waves' sums are added in order.
-template <int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a)
+// Adds what the ranges of a row left, eight at a time so that their loads are in flight together: WAVES waves a row, each taking
+// every WAVES-th range, their sums added in order.
+template <int D, int WAVES>
+__global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, uint32_t all_rows)
 {
-    constexpr int E = D / 64;
-    __shared__ float o_of[4][D], l_of[4];
+    constexpr int E = D / 64, ROWS = 4 / WAVES;
+    __shared__ float o_of[WAVES][D], l_of[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t all = (int64_t)a.max_q * a.ratio;
     const int rows = (int)(all < a.tile_rows ? all : a.tile_rows);
-    uint32_t id = blockIdx.x;
+    uint32_t id = blockIdx.x * ROWS + (WAVES == 1 ? wave : 0);
+    if (id >= all_rows) return;
     const int orow = (int)(id % rows);
     id /= rows;
     const int h = (int)(id % a.c.kv_heads);
@@ -894,11 +895,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a)
     for (int s = lane; s < n; s += 64) most = __builtin_fmaxf(most, part[(int64_t)s * (D + 2) + D]);
     most = wave_max(most);
     float total = 0.0f, o[E] = {};
-    for (int s0 = wave; s0 < n; s0 += 32) {
+    for (int s0 = WAVES == 1 ? 0 : wave; s0 < n; s0 += 8 * WAVES) {
         float x[8][E], c[8], l[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const int s = s0 + 4 * u < n ? s0 + 4 * u : n - 1;
+            const int s = s0 + WAVES * u < n ? s0 + WAVES * u : n - 1;
             const float* from = part + (int64_t)s * (D + 2);
             c[u] = from[D], l[u] = from[D + 1];
 #pragma unroll
@@ -906,29 +907,35 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a)
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const float f = s0 + 4 * u >= n || l[u] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(c[u] - most);
+            const float f = s0 + WAVES * u >= n || l[u] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(c[u] - most);
             total += f == 0.0f ? 0.0f : l[u] * f;
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] += f == 0.0f ? 0.0f : x[u][e] * f;
         }
     }
+    if constexpr (WAVES > 1) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) o_of[wave][lane * E + e] = o[e];
-    if (lane == 0) l_of[wave] = total;
-    __syncthreads();
-    if (threadIdx.x >= D / 2) return;
-    total = l_of[0] + l_of[1] + l_of[2] + l_of[3];
+        for (int e = 0; e < E; ++e) o_of[wave][lane * E + e] = o[e];
+        if (lane == 0) l_of[wave] = total;
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) {
+            total += l_of[w];
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += o_of[w][lane * E + e];
+        }
+    }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    const int head = h * a.ratio + row % a.ratio, at = 2 * threadIdx.x;
+    const int head = h * a.ratio + row % a.ratio;
     const int64_t token = v.start + query;
-    float y[2];
+    uint16_t* out = (uint16_t*)a.out + token * a.ld_out + head * a.hd_out + lane * E;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) y[e] = (o_of[0][at + e] + o_of[1][at + e] + o_of[2][at + e] + o_of[3][at + e]) * inv;
-    uint16_t* out = (uint16_t*)a.out + token * a.ld_out + head * a.hd_out + at;
-    const uint32_t w = a.type == DT_BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){y[0], y[1]}, bf2_t))
-                                         : __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t){y[0], y[1]}, h2_t));
-    out[0] = (uint16_t)w, out[1] = (uint16_t)(w >> 16);
-    if (a.lse && threadIdx.x == 0) a.lse[token * a.heads + head] = total == 0.0f ? -__builtin_inff() : LN2 * (most + log2f(total));
+    for (int e = 0; e < E; ++e) {
+        const float y = o[e] * inv;
+        out[e] = a.type == DT_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)y) : f32_to_f16(y);
+    }
+    if (a.lse && lane == 0) a.lse[token * a.heads + head] = total == 0.0f ? -__builtin_inff() : LN2 * (most + log2f(total));
 }
 
 // The weight that cached tokens received: the scores again, exp(score - lse) summed over a tile's rows, tile after tile.  Here S = Q
@@ -1098,7 +1105,7 @@ __global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, u
             }
             // (lane 16 n + r: token r of tile n)
             __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(before + mine), results,
-                                                  lane < TOKENS ? 4u * (uint32_t)(t - begin + lane) : ~3u, 0, 0);
+                                                  lane < TOKENS ? 4u * (uint32_t)(t - begin + lane) : OOB, 0, 0);
         }
     }
 }
@@ -1181,7 +1188,9 @@ hipError_t run_attention(KvAttentionArgs a, hipStream_t st)
         if (e == hipSuccess) e = hipGetLastError();
         if (e != hipSuccess) return e;
         if (a.splits > 1) {
-            hipLaunchKernelGGL(kv_join_kernel<D>, dim3((uint32_t)(n * rows)), dim3(256), 0, st, now);
+            const uint32_t all = (uint32_t)(n * rows);
+            if (a.splits > 16) hipLaunchKernelGGL(HIP_KERNEL_NAME(kv_join_kernel<D, 4>), dim3(all), dim3(256), 0, st, now, all);
+            else hipLaunchKernelGGL(HIP_KERNEL_NAME(kv_join_kernel<D, 1>), dim3((all + 3) / 4), dim3(256), 0, st, now, all);
             e = hipGetLastError();
             if (e != hipSuccess) return e;
         }
@@ -1200,7 +1209,7 @@ hipError_t run_weights(KvAttentionArgs a, hipStream_t st)
     // ranges of tokens: about six workgroups per CU in all, as for the attention
     const int64_t groups = (int64_t)a.s.batch * a.c.kv_heads;
     constexpr int unit = D == 256 ? 128 : 256;
-    int64_t parts = 1536 / groups;
+    int64_t parts = (tiles > 4 ? 512 : 1536) / groups;
     parts = parts < 4 ? 4 : parts;  // (a range is below 2^30 bytes)
     a.chunk = (int)(((a.cap + parts - 1) / parts + unit - 1) / unit * unit);
     parts = (a.cap + (int64_t)a.chunk - 1) / a.chunk;

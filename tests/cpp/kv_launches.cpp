@@ -59,7 +59,7 @@ int main()
                                 good &= fits(l) && a.ratio == ratio && tiles * a.tile_rows >= all && (tiles - 1) * a.tile_rows < all;
                                 const int64_t groups = (int64_t)(a.s.batch - a.first) * tiles * kv;
                                 if (l.is("kv_join")) {
-                                    good &= a.first == joined && l.grid.x * 4ull >= (uint64_t)groups * rows;
+                                    good &= a.first == joined && l.grid.x * (l.is("Li1EEE") ? 4ull : 1ull) >= (uint64_t)groups * rows;
                                     joined = a.s.batch;
                                 } else {
                                     good &= a.first == at && l.grid.x == (uint64_t)groups * a.splits;
