@@ -160,13 +160,12 @@ __device__ __forceinline__ T read(const void* row, uint32_t lane, int words = 0)
 }
 
 template <int D, int G>
-__device__ __forceinline__ void load_step(Step<D, G>& x, const KvAttentionArgs& a, const Half (&half)[2], const Lane& at)
+__device__ __forceinline__ void load_keys(Step<D, G>& x, const KvAttentionArgs& a, const Half (&half)[2], const Lane& at)
 {
-    constexpr int W = D / 8, GR = D / G;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const uint8_t *k = a.c.k + half[h].code, *v = a.c.v + half[h].code;
-        const uint32_t *ks = a.c.k_scale + half[h].scale, *vs = a.c.v_scale + half[h].scale;
+        const uint8_t* k = a.c.k + half[h].code;
+        const uint32_t* ks = a.c.k_scale + half[h].scale;
         if constexpr (Shape<D>::KW == 2) {
             const u32x2 t = read<u32x2>(k, at.k);
             x.k[h][0] = t[0], x.k[h][1] = t[1];
@@ -180,6 +179,16 @@ __device__ __forceinline__ void load_step(Step<D, G>& x, const KvAttentionArgs& 
         }
 #pragma unroll
         for (int i = 0; i < Step<D, G>::KS; ++i) x.ks[h][i] = read<uint32_t>(ks, at.ks, i);
+    }
+}
+template <int D, int G>
+__device__ __forceinline__ void load_values(Step<D, G>& x, const KvAttentionArgs& a, const Half (&half)[2], const Lane& at)
+{
+    constexpr int W = D / 8, GR = D / G;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint8_t* v = a.c.v + half[h].code;
+        const uint32_t* vs = a.c.v_scale + half[h].scale;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (Shape<D>::VW == 2) {
@@ -398,7 +407,7 @@ __device__ __forceinline__ void weigh(h8 (&p)[NQ], v4f (&s)[NQ][2], Row (&row)[N
 // heads, then the second ones (those behind short sequences come last and end at once), a place further each time: workgroups
 // are dealt to the eight XCDs in turn, and neither a sequence nor the first ranges, which all sequences have, fall to one of them.
 template <int D, int G, int NQ>
-__global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 3) void kv_attention_kernel(KvAttentionArgs a, uint32_t groups)
+__global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 4) void kv_attention_kernel(KvAttentionArgs a, uint32_t groups)
 {
     constexpr int TILES = Shape<D>::TILES, MD = Shape<D>::MD;
     __shared__ float merge[4][16][MD + 4];
@@ -421,25 +430,24 @@ __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 3) void kv_at
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Table table = table_of(a.s.table + b * a.s.ld_table);
 
-    // the first step is on its way before the queries
+    // The first step is on its way before the queries.  Keys of the next step are loaded when this one's have become scores, values
+    // when they have been added: a set of registers each, a step's arithmetic of the other waves to arrive in.  Behind the last
+    // step it is loaded again, so that no branch hides how many loads are on their way.
     const Lane at = lane_of_step<D, G>(r, j);
-    Step<D, G> x0, x1;
-    Half at0[2], at1[2];
-    int pages[2];
-    int t = begin + 32 * wave;
-    auto fetch = [&](Step<D, G>& x, Half(&half)[2], int token) {
-        half[0] = half_at(a, pages[0], h, token);
-        half[1] = half_at(a, pages[1], h, token + 16);
-        load_step<D, G>(x, a, half, at);
-    };
+    Step<D, G> x;
+    Half here[2];
+    int pages[2], t = begin + 32 * wave;
     auto look = [&](int token) {
         pages[0] = page_at(a, table, token);
         pages[1] = page_at(a, table, token + 16);
     };
     if (t < end) {
         look(t);
-        fetch(x0, at0, t);
-        look(t + 128);
+        here[0] = half_at(a, pages[0], h, t);
+        here[1] = half_at(a, pages[1], h, t + 16);
+        load_keys<D, G>(x, a, here, at);
+        load_values<D, G>(x, a, here, at);
+        look(t + 128 < end ? t + 128 : t);
     }
 
     h8 q[NQ][Shape<D>::STEPS];
@@ -474,32 +482,25 @@ __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 3) void kv_at
 #pragma unroll
         for (int n = 0; n < TILES; ++n) acc[c][n] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto work = [&](Step<D, G>& x, const Half(&half)[2], int token) {
+    for (; t < end; t += 128) {
+        const int then = t + 128 < end ? t + 128 : t;
         v4f s[NQ][2];
         scores<D, G, NQ>(s, x.k, x.ks, q);
-        const bool edge = token < all_low || token + 32 > all_limit || !half[0].ok || !half[1].ok;
+        const Half next[2] = {half_at(a, pages[0], h, then), half_at(a, pages[1], h, then + 16)};
+        load_keys<D, G>(x, a, next, at);
+        look(then + 128 < end ? then + 128 : then);
+        const bool edge = t < all_low || t + 32 > all_limit || !here[0].ok || !here[1].ok;
         if (edge) {
             // what lies behind the sequence may be anything: its values become 0
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x.vs[e] = token + (e >> 2) * 16 + 4 * j + (e & 3) < end && half[e >> 2].ok ? x.vs[e] : 0u;
+            for (int e = 0; e < 8; ++e) x.vs[e] = t + (e >> 2) * 16 + 4 * j + (e & 3) < end && here[e >> 2].ok ? x.vs[e] : 0u;
         }
         h8 p[NQ];
-        weigh<NQ, TILES>(p, s, row, acc, edge, token, end, half[0].ok, half[1].ok, j, [] {});
+        weigh<NQ, TILES>(p, s, row, acc, edge, t, end, here[0].ok, here[1].ok, j, [] {});
         add_values<D, G, NQ>(acc, x, p, r);
-    };
-    for (; t < end; t += 256) {
-        if (t + 128 < end) {
-            fetch(x1, at1, t + 128);
-            look(t + 256);
-        }
-        work(x0, at0, t);
-        if (t + 128 >= end) break;
-        if (t + 256 < end) {
-            fetch(x0, at0, t + 256);
-            look(t + 384);
-        }
-        work(x1, at1, t + 128);
+        load_values<D, G>(x, a, next, at);
+        here[0] = next[0];
+        here[1] = next[1];
     }
 
     // the waves' sums
@@ -943,16 +944,18 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, uint32_
 // sum over rows stays in the lane until the end.  A wave takes 64 tokens at a time (d = 256: 32), whose keys stay in registers while
 // the rows, converted once per workgroup, come from LDS, eight tiles at a time; more tiles take another turn over the tokens,
 // adding to what the turn before left in the output.
-constexpr int TURN = 8;  // tiles of rows in LDS
+template <int D, int WAVES>
+constexpr int TURN = WAVES == 8 && D < 256 ? 16 : 8;  // tiles of rows in LDS
 struct TileRows {
     float undo[16], lse[16];
     int low[16], limit[16];
-    int any_low, any_limit, all_low, all_limit;
+    v4i span;  // what any row sees begins and ends there; what all do
 };
 
-template <int D, int G>
-__global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, uint32_t groups)
+template <int D, int G, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 3) void kv_weights_kernel(KvAttentionArgs a, uint32_t groups)
 {
+    constexpr int TURN = ascq::TURN<D, WAVES>;
     constexpr int STEPS = Shape<D>::STEPS, KW = Shape<D>::KW, NT = D == 256 ? 2 : 4, TOKENS = 16 * NT;
     constexpr int W = D / 8, GR = D / G, KS = Step<D, G>::KS;
     extern __shared__ h8 rows_of[];
@@ -972,7 +975,7 @@ __global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, u
     const int end = stop < v.len ? stop : v.len;
     const Table table = table_of(a.s.table + b * a.s.ld_table);
     if (!in)
-        for (int i = (begin > v.len ? begin : v.len) + (int)threadIdx.x; i < stop; i += 256) out[i] = 0.0f;
+        for (int i = (begin > v.len ? begin : v.len) + (int)threadIdx.x; i < stop; i += 64 * WAVES) out[i] = 0.0f;
     if (begin >= end) return;
 
     const uint32_t at_k = 4u * (r * W + j * (W / 4)), at_s = 4u * (r * GR + j * (D / 4) / G);
@@ -1008,7 +1011,7 @@ __global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, u
 #pragma unroll
             for (int i = 0; i < KS; ++i) ks[n][i] = read<uint32_t>(a.c.k_scale + half.scale, at_s, i);
         }
-        look(t + 4 * TOKENS);
+        look(t + WAVES * TOKENS);
     };
 
     const int tiles = (v.rows * a.ratio + 15) / 16;
@@ -1019,7 +1022,7 @@ __global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, u
             load(t, turn);
         }
         if (turn > 0) __syncthreads();
-        for (int tile = turn + wave; tile < tiles && tile < turn + TURN; tile += 4) {
+        for (int tile = turn + wave; tile < tiles && tile < turn + TURN; tile += WAVES) {
             const int row = tile * 16 + r, query = row / a.ratio;
             const bool there = query < v.rows;
             const int64_t token = v.start + (there ? query : 0);
@@ -1045,11 +1048,11 @@ __global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, u
                 all_low = all_low > y2 ? all_low : y2;
                 all_limit = all_limit < y3 ? all_limit : y3;
             }
-            if (lane == 0) x.any_low = any_low, x.any_limit = any_limit, x.all_low = all_low, x.all_limit = all_limit;
+            if (lane == 0) x.span = (v4i){any_low, any_limit, all_low, all_limit};
         }
         __syncthreads();
         const int here = tiles - turn < TURN ? tiles - turn : TURN;
-        for (; t < end; t += 4 * TOKENS) {
+        for (; t < end; t += WAVES * TOKENS) {
             h8 f[NT][STEPS];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -1060,25 +1063,31 @@ __global__ __launch_bounds__(256, 3) void kv_weights_kernel(KvAttentionArgs a, u
                 }
             const uint32_t good = ok;
             const float before = turn > 0 ? had : in ? a.decay * had : 0.0f;
-            if (t + 4 * TOKENS < end) load(t + 4 * TOKENS, turn);
+            if (t + WAVES * TOKENS < end) load(t + WAVES * TOKENS, turn);
             float got[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) got[n] = 0.0f;
             for (int tile = 0; tile < here; ++tile) {
+                // (a tile's reads together: they take longer than its products)
                 const TileRows& x = info[tile];
-                if (t >= __builtin_amdgcn_readfirstlane(x.any_limit) || t + TOKENS <= __builtin_amdgcn_readfirstlane(x.any_low)) continue;
-                const bool edge = t < __builtin_amdgcn_readfirstlane(x.all_low) ||
-                                  t + TOKENS > __builtin_amdgcn_readfirstlane(x.all_limit) || good != (1u << NT) - 1;
+                const v4i span = x.span;
+                const v4f undo = *(const v4f*)(x.undo + 4 * j), lse = *(const v4f*)(x.lse + 4 * j);
+                h8 q[STEPS];
+                if constexpr (WAVES == 8)
+#pragma unroll
+                    for (int i = 0; i < STEPS; ++i) q[i] = rows_of[(tile * STEPS + i) * 64 + lane];
+                if (t >= __builtin_amdgcn_readfirstlane(span[1]) || t + TOKENS <= __builtin_amdgcn_readfirstlane(span[0])) continue;
+                const bool edge = t < __builtin_amdgcn_readfirstlane(span[2]) ||
+                                  t + TOKENS > __builtin_amdgcn_readfirstlane(span[3]) || good != (1u << NT) - 1;
                 v4f s[NT];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) s[n] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < STEPS; ++i) {
-                    const h8 q = rows_of[(tile * STEPS + i) * 64 + lane];
+                    if constexpr (WAVES < 8) q[i] = rows_of[(tile * STEPS + i) * 64 + lane];  // (registers for more waves)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) s[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q, f[n][i], s[n], 0, 0, 0);
+                    for (int n = 0; n < NT; ++n) s[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[i], f[n][i], s[n], 0, 0, 0);
                 }
-                const v4f undo = *(const v4f*)(x.undo + 4 * j), lse = *(const v4f*)(x.lse + 4 * j);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1141,12 +1150,13 @@ void plan(KvAttentionArgs& a, size_t room)
     a.tiles = (int)((rows + a.tile_rows - 1) / a.tile_rows);
     const int64_t span = widest(a);
     const int64_t groups = (int64_t)a.s.batch * a.tiles * a.c.kv_heads;
-    // Up to 32 rows about six workgroups per CU in all, three of which fit at a time: fewer leave the end of ragged lengths to few,
-    // more pay for their starts (us, 32 sequences of up to 8192 tokens, 8 key heads / 8 of 131072: 1024 42 / 215, 2048 43 / 211,
-    // 4096 48 / 223).  More rows: one per CU, as the rows' sums of further ranges are many.
-    const int64_t wanted = a.tile_rows > 32 ? 256 : 1536;
-    int64_t splits = wanted / groups;
-    const int64_t most = (span + UNIT - 1) / UNIT, fit = (int64_t)(room / split_bytes(a));
+    // Ranges: one workgroup per CU where a step of each of its waves (UNIT tokens) is left to it, and more of them while three steps
+    // are: up to six per CU of few rows (four fit at a time), two of 32 rows, one of more rows, whose sums of further ranges are many.
+    const int64_t wanted = a.tile_rows == 16 ? 1536 : a.tile_rows == 32 ? 512 : 256;
+    const int64_t short_ones = (span + UNIT - 1) / UNIT, long_ones = (span + 3 * UNIT - 1) / (3 * UNIT);
+    int64_t splits = wanted / groups, few = 256 / groups;
+    few = few < short_ones ? few : short_ones;
+    const int64_t most = few > long_ones ? few : long_ones, fit = (int64_t)(room / split_bytes(a));
     splits = splits < most ? splits : most;
     splits = splits < fit ? splits : fit;
     splits = splits < 1 ? 1 : splits;
@@ -1198,30 +1208,38 @@ hipError_t run_attention(KvAttentionArgs a, hipStream_t st)
     return hipSuccess;
 }
 
+template <int D, int G, int WAVES>
+hipError_t run_weights_by(KvAttentionArgs a, int64_t tiles, int64_t wanted, hipStream_t st)
+{
+    constexpr int TILE = Shape<D>::STEPS * 1024, MOST = ascq::TURN<D, WAVES>;
+    hipError_t e = ensure_dynamic_lds<kv_weights_kernel<D, G, WAVES>>(MOST * TILE);
+    if (e != hipSuccess) return e;
+    const int64_t groups = (int64_t)a.s.batch * a.c.kv_heads;
+    constexpr int unit = (D == 256 ? 32 : 64) * WAVES;
+    int64_t parts = wanted / groups;
+    parts = parts < 4 ? 4 : parts;  // (a range is below 2^30 bytes)
+    a.chunk = (int)(((a.cap + parts - 1) / parts + unit - 1) / unit * unit);
+    parts = (a.cap + (int64_t)a.chunk - 1) / a.chunk;
+    const int64_t per = parts * a.c.kv_heads, most = ((int64_t)1 << 22) / per;  // sequences of a launch: at most 2^31 threads
+    for (int64_t at = 0; at < a.s.batch; at += most) {
+        const int64_t n = a.s.batch - at < most ? a.s.batch - at : most;
+        a.first = (int)at;
+        launch_k(kv_weights_kernel<D, G, WAVES>, dim3((uint32_t)(n * per)), dim3(64 * WAVES),
+                 (uint32_t)((tiles < MOST ? tiles : MOST) * TILE), st, a, (uint32_t)(n * a.c.kv_heads));
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 template <int D, int G>
 hipError_t run_weights(KvAttentionArgs a, hipStream_t st)
 {
     a.ratio = a.heads / a.c.kv_heads;
     const int64_t tiles = ((int64_t)a.max_q * a.ratio + 15) / 16;
-    const int lds = (int)(tiles < TURN ? tiles : TURN) * Shape<D>::STEPS * 1024;
-    hipError_t e = ensure_dynamic_lds<kv_weights_kernel<D, G>>(TURN * Shape<D>::STEPS * 1024);
-    if (e != hipSuccess) return e;
-    // ranges of tokens: about six workgroups per CU in all, as for the attention
-    const int64_t groups = (int64_t)a.s.batch * a.c.kv_heads;
-    constexpr int unit = D == 256 ? 128 : 256;
-    int64_t parts = (tiles > 4 ? 512 : 1536) / groups;
-    parts = parts < 4 ? 4 : parts;  // (a range is below 2^30 bytes)
-    a.chunk = (int)(((a.cap + parts - 1) / parts + unit - 1) / unit * unit);
-    parts = (a.cap + (int64_t)a.chunk - 1) / a.chunk;
-    const int64_t per = parts * a.c.kv_heads, most = ((int64_t)1 << 23) / per;  // sequences of a launch: below 2^31 threads
-    for (int64_t at = 0; at < a.s.batch; at += most) {
-        const int64_t n = a.s.batch - at < most ? a.s.batch - at : most;
-        a.first = (int)at;
-        launch_k(kv_weights_kernel<D, G>, dim3((uint32_t)(n * per)), dim3(256), (uint32_t)lds, st, a, (uint32_t)(n * a.c.kv_heads));
-        e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    // Up to 4 tiles of rows ranges as in the attention; more rows: eight waves share the conversion of the rows, a workgroup per CU
+    // (us, 64 queries of 2 x 32 heads over 16384 tokens: 4 waves 50, 8 37)
+    return tiles > 4 ? run_weights_by<D, G, 8>(a, tiles, 256, st) : run_weights_by<D, G, 4>(a, tiles, 1536, st);
 }
 
 #define KV_SHAPES(RUN)                                              \
