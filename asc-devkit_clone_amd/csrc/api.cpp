@@ -2155,7 +2155,7 @@ ascq_status ascq_kv_weights(float* weights_out, const float* weights, int64_t ca
     if (s != ASCQ_OK) return s;
     if (cap < (int64_t)a.s.table_pages << a.c.page_shift)
         return fail(ASCQ_E_INVALID_ARG, "kv_weights: rows of weights are shorter than the page table's tokens");
-    if (cap > (1 << 30) || (cap / 128 + 1) * a.c.kv_heads > kKvGroups) return fail(ASCQ_E_UNSUPPORTED, "kv_weights: rows too long");
+    if (cap > (1 << 30)) return fail(ASCQ_E_UNSUPPORTED, "kv_weights: rows too long");
     if (!(__builtin_fabsf(decay) <= 3.402823466e38f)) return fail(ASCQ_E_INVALID_ARG, "kv_weights: decay must be finite");
     if (a.s.batch == 0 || cap == 0) return ASCQ_OK;
     if (!weights_out || (a.max_q > 0 && (!q || !lse))) return fail(ASCQ_E_INVALID_ARG, "kv_weights: null argument");

@@ -73,7 +73,7 @@ int main()
                             }
                             expect(good && at == batch && (joined == 0 || joined == batch), "attention", batch, queries, at);
                         }
-                        if (pages / 2 * kv > 1 << 23 || (double)batch * pages * kv > 1e10) continue;
+                        if ((double)batch * kv > 1e9) continue;
                         launches().clear();
                         const int64_t cap = pages * 64 + 1;
                         bool good = ascq_kv_weights((float*)p, nullptr, cap, 1.0f, p, (float*)p, &c, &s, &ap, nullptr) == ASCQ_OK;
@@ -82,7 +82,7 @@ int main()
                             const auto a = l.args<ascq::KvAttentionArgs>();
                             good &= fits(l) && a.first == at;
                             const int64_t blocks = (cap + a.chunk - 1) / a.chunk;
-                            good &= l.grid.x % (blocks * kv) == 0;
+                            good &= l.grid.x % (blocks * kv) == 0 && a.chunk > 0 && (int64_t)a.chunk * 4 < 1ll << 31;
                             at += l.grid.x / (blocks * kv);
                         }
                         expect(good && at == batch, "weights", batch, cap, at);

@@ -94,7 +94,6 @@ def test_attention_arguments(name):
         for bad in (dict(lse=None), dict(cap=63), dict(cap=-1), dict(decay=float("inf")), dict(decay=float("nan")), dict(w=ODD)):
             _err(call(**bad), ascq.E_INVALID_ARG)
         _err(call(cap=1 << 31), ascq.E_UNSUPPORTED)
-        _err(call(cap=1 << 30, cache=_cache(kv=1024), heads=1024), ascq.E_UNSUPPORTED)
 
 
 def test_evict_arguments():
