@@ -12,7 +12,7 @@ namespace {
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef v4f v4f_any __attribute__((aligned(4)));
 
-// 8 channels of a row as fp32: NaN counts as 0, magnitudes end at 61440 -- beyond it a code's value could round past f16
+// 8 channels of a row as fp32
 template <int TYPE>
 __device__ __forceinline__ void load8(float (&x)[8], const void* p)
 {
@@ -28,11 +28,6 @@ __device__ __forceinline__ void load8(float (&x)[8], const void* p)
             x[2 * i] = TYPE == DT_BF16 ? bf16_to_f32(lo) : f16_to_f32(lo);
             x[2 * i + 1] = TYPE == DT_BF16 ? bf16_to_f32(hi) : f16_to_f32(hi);
         }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = x[i] != x[i] ? 0.0f : x[i];
-        x[i] = __builtin_fminf(__builtin_fmaxf(x[i], -61440.0f), 61440.0f);
     }
 }
 
@@ -69,7 +64,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int word
     const int64_t page = slot >> a.c.page_shift;
     const bool live = slot >= 0 && page < a.c.pages;
     float x[2][8] = {};
-    if (live) {
+    if (t < a.T) {  // (whether they are written or not: the loads do not wait for the slot)
         load8<TYPE>(x[0], (const uint8_t*)a.k + (t * a.ld_k + h * a.hd_k + 8 * w) * (TYPE == DT_F32 ? 4 : 2));
         load8<TYPE>(x[1], (const uint8_t*)a.v + (t * a.ld_v + h * a.hd_v + 8 * w) * (TYPE == DT_F32 ? 4 : 2));
     }
@@ -78,8 +73,24 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int word
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         float lo = x[i][0], hi = x[i][0];
+        uint32_t big = __float_as_uint(x[i][0]) & 0x7fffffffu;  // (NaN above all)
 #pragma unroll
-        for (int e = 1; e < 8; ++e) lo = __builtin_fminf(lo, x[i][e]), hi = __builtin_fmaxf(hi, x[i][e]);
+        for (int e = 1; e < 8; ++e) {
+            lo = __builtin_fminf(lo, x[i][e]), hi = __builtin_fmaxf(hi, x[i][e]);
+            const uint32_t bits = __float_as_uint(x[i][e]) & 0x7fffffffu;
+            big = big > bits ? big : bits;
+        }
+        if (__ballot(big > __float_as_uint(61440.0f))) {
+            // NaN counts as 0, magnitudes end at 61440: beyond it a code's value could round past f16
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[i][e] = x[i][e] != x[i][e] ? 0.0f : x[i][e];
+                x[i][e] = __builtin_fminf(__builtin_fmaxf(x[i][e], -61440.0f), 61440.0f);
+            }
+            lo = hi = x[i][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) lo = __builtin_fminf(lo, x[i][e]), hi = __builtin_fmaxf(hi, x[i][e]);
+        }
         lo = of_group<0>(lo, lanes);
         hi = of_group<1>(hi, lanes);
         const _Float16 s = (_Float16)((hi - lo) / 15.0f);
@@ -88,8 +99,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int word
         uint32_t code = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float c = __builtin_rintf((x[i][e] - (float)o) * inv);
-            code |= ((uint32_t)(int)__builtin_fminf(__builtin_fmaxf(c, -8.0f), 7.0f) & 15u) << (4 * e);
+            // clamp(rint(t)) = rint(clamp(t)) for these bounds; added to 1.5 2^23 a number rounds to an integer, its low bits
+            const float t = __builtin_amdgcn_fmed3f((x[i][e] - (float)o) * inv, -8.0f, 7.0f) + 12582912.0f;
+            code |= (__float_as_uint(t) & 15u) << (4 * e);
         }
         if (!live) continue;
         ((uint32_t*)((i ? a.c.v : a.c.k) + page * a.c.ld_code + place * (a.c.d / 2)))[w] = code;
@@ -154,7 +166,8 @@ __device__ __forceinline__ void pick_bin(uint32_t c0, uint32_t c1, uint32_t bins
     if (lane == 63) sums[wave] = sum;
     __syncthreads();
     uint32_t before = sum - c0 - c1;
-    for (int i = 0; i < wave; ++i) before += sums[i];
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) before += i < wave ? sums[i] : 0;
     if (before < need && need <= before + c0 + c1) {
         const uint32_t top = bins - 1 - 2 * threadIdx.x;
         const bool first = need <= before + c0;
@@ -259,6 +272,7 @@ __global__ __launch_bounds__(SEL) void kv_select_kernel(KvEvictArgs a)
         if (lane == 0) above[wave] = more, equal[wave] = same;
         __syncthreads();
         uint32_t here = at, tied = ties;
+#pragma unroll
         for (int i = 0; i < WAVES; ++i) {
             if (i < wave) here += above[i], tied += equal[i];
             at += above[i], ties += equal[i];
@@ -359,6 +373,7 @@ __global__ __launch_bounds__(SEL) void kv_select_part_kernel(KvEvictArgs a)
             __syncthreads();
             if (tid == 0) {
                 uint32_t sum = 0;
+#pragma unroll
                 for (int i = 0; i < WAVES; ++i) sum += sides[0][i];
                 own[5120 + LAST] = sum;
                 if (part == 0) found[LAST] = f;
@@ -412,6 +427,7 @@ __global__ __launch_bounds__(SEL) void kv_select_part_kernel(KvEvictArgs a)
         if (lane == 0) before[0][wave] = more, before[1][wave] = same, sides[0][wave] = here, sides[1][wave] = equal;
         __syncthreads();
         uint32_t place = 0, tied = 0;
+#pragma unroll
         for (int i = 0; i < WAVES; ++i) {
             place += before[0][i], tied += before[1][i];
             if (i < wave) place += sides[0][i], tied += sides[1][i];
