@@ -405,7 +405,13 @@ __device__ __forceinline__ void weigh(h8 (&p)[NQ], v4f (&s)[NQ][2], Row (&row)[N
 // Four waves share a range of a sequence's tokens, a wave every fourth step of 32; their sums meet in LDS.  One range: the
 // result.  Several: each leaves its sums, and kv_join_kernel adds them.  Workgroups go through the first ranges of all tiles and
 // heads, then the second ones (those behind short sequences come last and end at once), a place further each time: workgroups
-// are dealt to the eight XCDs in turn, and neither a sequence nor the first ranges, which all sequences have, fall to one of them.
+// are dealt to the eight XCDs in turn, and neither a sequence nor the first ranges, which all sequences have, fall to one of them
+// (32 sequences of 1 to 8192 tokens: 56 us without that, 41 with it).
+// Bound by vector arithmetic on its way to HBM's rate: codes to values, the exponentials, and what the matrix instructions leave.
+// One set of registers a step, at four waves a SIMD, is faster than two sets at three: the other waves cover the loads.  One query
+// each of 32 heads, 8 key heads of 128: 8 sequences of 131072 tokens 205 us, 1090 MB at 5.3 TB/s, the vector units busy 70 %; 32
+// ragged ones up to 8192 40.6 us, 4.0 TB/s, busy 43 %: they end unevenly; 16 x 5 queries (NQ 2) over up to 4099 tokens 26.8 us for
+// 39 MB, and one query over 4096 7.0 us: the way of a step or two, from table over codes to merge, rather than any rate.
 template <int D, int G, int NQ>
 __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 4) void kv_attention_kernel(KvAttentionArgs a, uint32_t groups)
 {
@@ -574,6 +580,10 @@ __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 4) void kv_at
 // lane as the matrix instruction reads them.  While a wave weighs the scores of 32 tokens, its products of the next 32's keys
 // run, and the values' products follow.  A quarter: in K half the words of one of the two halves, in V 2 (d = 256: 4) of the D /
 // 16 tiles.
+// Bound by the waves' arithmetic beside the matrix products, and the meeting at each step: 2 x 1024 queries of 32 heads over 8192
+// tokens, 258 GFLOP below the diagonal: 292 us (880 TFLOP/s; a plain product of large matrices 1355), matrix cores busy 35 %, vector
+// units 47 %, waiting 28 % of the waves' time, no bank conflicts.  Four waves of 32 rows in 32-token
+// steps: 538; 64 rows a wave do not fit the registers (990).
 template <int D, int G>
 struct Quarter {
     static constexpr int KN = Shape<D>::KW / 2, VN = D == 256 ? 4 : 2;
@@ -868,7 +878,7 @@ __global__ __launch_bounds__(64 * WAVES, NQ * D > 256 ? 1 : 2) void kv_chunk_ker
 }
 
 // Adds what the ranges of a row left, eight at a time so that their loads are in flight together: WAVES waves a row, each taking
-// every WAVES-th range, their sums added in order.
+// every WAVES-th range, their sums added in order.  A launch of its own: 4 to 5 us for 2 MB, latency.
 template <int D, int WAVES>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, uint32_t all_rows)
 {
@@ -943,7 +953,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, uint32_
 // K^T, the operands the other way round, so that a lane's scores belong to one token (its column) and to the rows 4 j .. 4 j + 3: the
 // sum over rows stays in the lane until the end.  A wave takes 64 tokens at a time (d = 256: 32), whose keys stay in registers while
 // the rows, converted once per workgroup, come from LDS, eight tiles at a time; more tiles take another turn over the tokens,
-// adding to what the turn before left in the output.
+// adding to what the turn before left in the output.  One query each of 16 ragged sequences up to 8192 (32 heads, 8 key heads of 128):
+// 25 us for 56 MB read and written, waves waiting 44 % of their time: a range is a step or two long.  64 queries of 2 sequences
+// over 16384: 33 us, 17 GFLOP of products, matrix cores busy 17 %, vector units (exp2 of each score) 36 %.
 template <int D, int WAVES>
 constexpr int TURN = WAVES == 8 && D < 256 ? 16 : 8;  // tiles of rows in LDS
 struct TileRows {
@@ -1152,6 +1164,7 @@ void plan(KvAttentionArgs& a, size_t room)
     const int64_t groups = (int64_t)a.s.batch * a.tiles * a.c.kv_heads;
     // Ranges: one workgroup per CU where a step of each of its waves (UNIT tokens) is left to it, and more of them while three steps
     // are: up to six per CU of few rows (four fit at a time), two of 32 rows, one of more rows, whose sums of further ranges are many.
+    // (up to 16 rows, us: 32 ragged sequences up to 8192 / 8 of 131072: 1024 ranges 53 / 205, 1536 41 / 206, 2048 43 / 207)
     const int64_t wanted = a.tile_rows == 16 ? 1536 : a.tile_rows == 32 ? 512 : 256;
     const int64_t short_ones = (span + UNIT - 1) / UNIT, long_ones = (span + 3 * UNIT - 1) / (3 * UNIT);
     int64_t splits = wanted / groups, few = 256 / groups;

@@ -51,7 +51,9 @@ __device__ __forceinline__ float of_group(float x, int lanes)
 
 // A lane takes 8 channels (one word of codes) of a token's keys and values in a head, the group / 8 lanes of a group find its range
 // by exchanges.  fp32 in the order that the header states, every operation IEEE: the same bits as that order anywhere.
-// Bound by memory, once the two rows' loads are in flight together and no index needs a division (8192 tokens x 8 heads of 128, f16: us).
+// The two rows' loads are in flight together, and no index needs a division.  8192 tokens x 8 heads of 128, f16, a group a row, to
+// slots in no order: 14.6 us for 42 MB (2.9 TB/s), the vector units busy 55 % of it, and every row's codes and pair are pieces of
+// 64 and 4 bytes at a place of their own.  16 tokens: 3.6 us, launch and latency.
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int word_bits, FastDiv heads)
 {
@@ -150,8 +152,9 @@ constexpr int SEL = 1024, WAVES = SEL / 64;  // threads of a selection
 // Which tokens of a (sequence, head) stay.  The threshold -- the need-th largest weight among the tokens before the last `recent` --
 // is found digit by digit (11, 11 and 10 bits of the ordered key) by counting; then positions are written in order, those above the
 // threshold and, of those equal to it, the first.  Each wave has a run of neighbouring positions, in registers (HELD a thread) unless
-// the sequence has more than SEL HELD, and then SEL HELD at a time; zeros, which many tokens of a long context have, are counted a wave at a time, as counting them one
-// by one in LDS would be one after the other.
+// the sequence has more than SEL HELD, and then SEL HELD at a time.  Zeros, which many tokens of a long context have, are counted a
+// wave at a time, as counting them one by one in LDS would be one after the other.  Bound by the chain of scans and barriers, not by
+// its bytes (16 x 8 rows of up to 4096 weights: 10.9 us, 0.8 MB).
 // From the top bin down, a thread two of them (c0 the higher): where the need-th is.  pick: the bin, how many are needed of it.
 __device__ __forceinline__ void pick_bin(uint32_t c0, uint32_t c1, uint32_t bins, uint32_t need, uint32_t (&sums)[WAVES],
                                          uint32_t (&pick)[2])
@@ -295,7 +298,8 @@ __global__ __launch_bounds__(SEL) void kv_select_kernel(KvEvictArgs a)
 // The same for long sequences, a part of PART positions to a workgroup and a launch to a digit.  A launch first finds the digit
 // before it from all parts' counts (each workgroup for itself: they lie in L2), then counts its own part; the last one writes the
 // positions, behind those of the parts before.  Of a (sequence, head), in `counts`: per part the counts of the three digits and
-// how many of it lie above the first two, and what was found.
+// how many of it lie above the first two, and what was found.  2 x 8 rows of 131072: 4.1, 8.3, 8.0 and 10.7 us, of which a launch
+// is about 3 and the sums over the parts' counts 4 (24 MB from L2); by one workgroup a row 182.
 constexpr int PART = 8 * SEL;
 constexpr int COUNTS = 2048 + 2048 + 1024 + 2;
 struct Found {
@@ -497,6 +501,8 @@ struct Rows {
 // then all their rows are read before any is written.  To other pages nothing is in the way, and the runs of tokens are shared by
 // gridDim.x workgroups.  In place one workgroup takes the tokens of a plane (keys, values, scales, weights: gridDim.z) in order: the
 // token of place i comes from a position >= i, so that a run's reads lie behind all earlier runs' writes.
+// Bound by rows of 64 and 16 bytes read from anywhere: 2 sequences x 8 heads, 16384 kept of 131072, d 128: 28 us for 42 MB kept
+// (108 MB read in whole lines, 48 written: 5.6 TB/s); 16 sequences of up to 4096 cut to 2048 15 us (40 MB read, 33 written).
 template <int D, int G, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_move_kernel(KvEvictArgs a)
 {
