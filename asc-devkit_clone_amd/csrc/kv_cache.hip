@@ -349,6 +349,8 @@ __global__ __launch_bounds__(SEL) void kv_select_part_kernel(KvEvictArgs a)
     }
     Found f{0, (uint32_t)(a.keep - a.recent)};
     uint32_t mask = 0;
+    // of a thread's two bins, this part's counts (the last launch: those of the parts before), and its share of what lies above
+    uint32_t m0 = 0, m1 = 0, more = 0, same = 0;
     if constexpr (DIGIT > 0) {
         constexpr int LAST = DIGIT - 1;
         constexpr uint32_t bins = bins_of(LAST);
@@ -356,21 +358,24 @@ __global__ __launch_bounds__(SEL) void kv_select_part_kernel(KvEvictArgs a)
         const uint32_t top = bins - 1 - 2 * tid;
         const bool counts = 2 * tid < (int)bins;
         uint32_t c0 = 0, c1 = 0;
-        if (counts)
-#pragma unroll 8
+        if (counts) {
+#pragma unroll 16
             for (int p = 0; p < parts; ++p) {
                 const u32x2 c = *(const u32x2*)(all + (int64_t)p * COUNTS + 2048 * LAST + top - 1);
                 c0 += c[1], c1 += c[0];
+                const bool of_part = DIGIT < 3 ? p == part : p < part;
+                m0 += of_part ? c[1] : 0, m1 += of_part ? c[0] : 0;
             }
+        } else if (DIGIT == 3 && wave == WAVES - 1) {  // (above the first two digits; this wave has no bins of the third)
+            for (int p = lane >> 1; p < part; p += 32) more += all[(int64_t)p * COUNTS + 5120 + (lane & 1)];
+        }
         pick_bin(c0, c1, bins, f.need, sums, pick);
         f.prefix |= pick[0] << shift_of(LAST);
         f.need = pick[1];
         mask = ~((1u << shift_of(LAST)) - 1);
         if constexpr (DIGIT < 3) {
             // how many of this part lie above
-            u32x2 c = {0, 0};
-            if (counts) c = *(const u32x2*)(own + 2048 * LAST + top - 1);
-            uint32_t more = (counts && top > pick[0] ? c[1] : 0) + (counts && top - 1 > pick[0] ? c[0] : 0);
+            more = (top > pick[0] ? m0 : 0) + (top - 1 > pick[0] ? m1 : 0);
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) more += __shfl_xor(more, off, 64);
             if (lane == 0) sides[0][wave] = more;
@@ -404,17 +409,9 @@ __global__ __launch_bounds__(SEL) void kv_select_part_kernel(KvEvictArgs a)
         if (2 * tid < (int)bins) *(u32x2*)(own + 2048 * DIGIT + 2 * tid) = (u32x2){hist[2 * tid], hist[2 * tid + 1]};
     } else {
         // places before this part: above the threshold, and equal to it
-        uint32_t more = 0, same = 0;
-        const uint32_t digit = f.prefix & 1023u;
-        uint32_t sum = 0;
-#pragma unroll 8
-        for (int p = 0; p < part; ++p) {
-            const uint32_t* c = all + (int64_t)p * COUNTS;
-            sum += c[4096 + tid];
-            more += tid < 2 ? c[5120 + tid] : 0;
-        }
-        more += (uint32_t)tid > digit ? sum : 0;
-        same = (uint32_t)tid == digit ? sum : 0;
+        const uint32_t top = bins_of(2) - 1 - 2 * tid;
+        more += (top > pick[0] ? m0 : 0) + (top - 1 > pick[0] ? m1 : 0);
+        same = top == pick[0] ? m0 : top - 1 == pick[0] ? m1 : 0;
         uint32_t here = 0, equal = 0;  // of this wave
 #pragma unroll
         for (int k = 0; k < 8; ++k) {

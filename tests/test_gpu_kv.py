@@ -370,6 +370,16 @@ def test_evict_long(ascq_gpu, keep, recent, away, alone):
     _check_evict(ascq_gpu, p, w, keep, recent, into, **more)
 
 
+@pytest.mark.parametrize("equal", [False, True])
+def test_evict_many_parts(ascq_gpu, equal):
+    """more parts of a selection than a wave has lanes, with ties all over them"""
+    p = K.Problem(2, [600001, 540000], heads=1, kv=1, d=64, group=64, page=1024, spare=0)
+    w = torch.rand(2, 1, p.columns * 1024, generator=p.g)
+    if equal:
+        w = (4 * w).round()
+    _check_evict(ascq_gpu, p, w, 3001, 17, None)
+
+
 def test_evict_bad_pages(ascq_gpu):
     """tokens on no page move as zeros, and nothing is written to a page that does not exist"""
     p = K.Problem(4, [60, 60], heads=1, kv=1, d=64, group=32, page=16, spare=8)
