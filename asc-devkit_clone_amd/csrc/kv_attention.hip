@@ -411,7 +411,8 @@ __device__ __forceinline__ void weigh(h8 (&p)[NQ], v4f (&s)[NQ][2], Row (&row)[N
 // One set of registers a step, at four waves a SIMD, is faster than two sets at three: the other waves cover the loads.  One query
 // each of 32 heads, 8 key heads of 128: 8 sequences of 131072 tokens 205 us, 1090 MB at 5.3 TB/s, the vector units busy 70 %; 32
 // ragged ones up to 8192 40.6 us, 4.0 TB/s, busy 43 %: they end unevenly; 16 x 5 queries (NQ 2) over up to 4099 tokens 26.8 us for
-// 39 MB, and one query over 4096 7.0 us: the way of a step or two, from table over codes to merge, rather than any rate.
+// 39 MB: some 500 vector instructions a step, at most eight steps a wave and uneven (a second set of registers, which 32 rows have room
+// for: 27.5).  One query over 4096 tokens 7.0 us: the way of a step or two, from table over codes to merge, rather than any rate.
 template <int D, int G, int NQ>
 __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 4) void kv_attention_kernel(KvAttentionArgs a, uint32_t groups)
 {
@@ -1164,7 +1165,9 @@ void plan(KvAttentionArgs& a, size_t room)
     const int64_t groups = (int64_t)a.s.batch * a.tiles * a.c.kv_heads;
     // Ranges: one workgroup per CU where a step of each of its waves (UNIT tokens) is left to it, and more of them while three steps
     // are: up to six per CU of few rows (four fit at a time), two of 32 rows, one of more rows, whose sums of further ranges are many.
-    // (up to 16 rows, us: 32 ragged sequences up to 8192 / 8 of 131072: 1024 ranges 53 / 205, 1536 41 / 206, 2048 43 / 207)
+    // (up to 16 rows, us: 32 ragged sequences up to 8192 / 8 of 131072: 1024 ranges 53 / 205, 1536 41 / 206, 2048 43 / 207;
+    // 32 rows, 2 x 8 queries over 65536 / 32 ragged ones: 256 48 / 78, 512 44 / 76 with the join, 1024 51 / 74; more rows, 64
+    // queries over 16384 / 4 x 256 over ragged ones: 256 42 / 299, 512 62 / 265)
     const int64_t wanted = a.tile_rows == 16 ? 1536 : a.tile_rows == 32 ? 512 : 256;
     const int64_t short_ones = (span + UNIT - 1) / UNIT, long_ones = (span + 3 * UNIT - 1) / (3 * UNIT);
     int64_t splits = wanted / groups, few = 256 / groups;

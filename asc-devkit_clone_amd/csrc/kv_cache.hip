@@ -298,8 +298,8 @@ __global__ __launch_bounds__(SEL) void kv_select_kernel(KvEvictArgs a)
 // The same for long sequences, a part of PART positions to a workgroup and a launch to a digit.  A launch first finds the digit
 // before it from all parts' counts (each workgroup for itself: they lie in L2), then counts its own part; the last one writes the
 // positions, behind those of the parts before.  Of a (sequence, head), in `counts`: per part the counts of the three digits and
-// how many of it lie above the first two, and what was found.  2 x 8 rows of 131072: 4.1, 8.3, 8.0 and 10.7 us, of which a launch
-// is about 3 and the sums over the parts' counts 4 (24 MB from L2); by one workgroup a row 182.
+// how many of it lie above the first two, and what was found.  2 x 8 rows of 131072: 4.2, 7.4, 7.5 and 7.8 us, of which a launch
+// is about 3 and the sums over the parts' counts 3 (24 MB from L2); by one workgroup a row 182.
 constexpr int PART = 8 * SEL;
 constexpr int COUNTS = 2048 + 2048 + 1024 + 2;
 struct Found {
