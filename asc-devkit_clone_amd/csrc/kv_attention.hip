@@ -1254,7 +1254,8 @@ hipError_t run_weights(KvAttentionArgs a, hipStream_t st)
     a.ratio = a.heads / a.c.kv_heads;
     const int64_t tiles = ((int64_t)a.max_q * a.ratio + 15) / 16;
     // Up to 4 tiles of rows ranges as in the attention; more rows: eight waves share the conversion of the rows, a workgroup per CU
-    // (us, 64 queries of 2 x 32 heads over 16384 tokens: 4 waves 50, 8 37)
+    // (us, 64 queries of 2 x 32 heads over 16384 tokens: 4 waves 50, 8 37; ranges of up to 4 tiles, one query of 64 ragged sequences
+    // up to 4096 / 8 queries of 8 up to 8192 / one of 2 x 65536: 768 33 / 18 / 25, 1024 34 / 15 / 27, 1536 33 / 15 / 28, 2304 35 / 17 / 29)
     return tiles > 4 ? run_weights_by<D, G, 8>(a, tiles, 256, st) : run_weights_by<D, G, 4>(a, tiles, 1536, st);
 }
 
