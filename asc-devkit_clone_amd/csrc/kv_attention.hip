@@ -53,16 +53,17 @@ __device__ __forceinline__ View view_of(const KvAttentionArgs& a, int64_t b)
     return v;
 }
 
-// the tokens [lo, hi) that the rows of tile `t` see together; a row's own limits follow from its query
+// the tokens [low, hi) that the rows of a tile see together, and where their first step begins (at most 31 tokens before); a row's own
+// limits follow from its query
 struct Range {
-    int lo, hi;
+    int lo, hi, low;
 };
 __device__ __forceinline__ Range range_of(const KvAttentionArgs& a, const View& v, int tile)
 {
     const int first = tile * a.tile_rows / a.ratio;
     int last = (tile * a.tile_rows + a.tile_rows - 1) / a.ratio;
     last = last < v.rows ? last : v.rows - 1;
-    Range r{0, v.len};
+    Range r{0, v.len, 0};
     const int64_t at = (int64_t)v.len - v.n;  // the first query's token
     if (a.causal) {
         const int64_t hi = at + last + 1;
@@ -70,7 +71,8 @@ __device__ __forceinline__ Range range_of(const KvAttentionArgs& a, const View& 
     }
     if (a.window) {
         const int64_t lo = at + first - a.window + 1;
-        r.lo = lo < 0 ? 0 : lo < v.len ? (int)lo & ~31 : v.len;
+        r.low = lo < 0 ? 0 : lo < v.len ? (int)lo : v.len;
+        r.lo = r.low < v.len ? r.low & ~31 : v.len;
     }
     return r;
 }
@@ -498,9 +500,13 @@ __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 4) void kv_at
         look(then + 128 < end ? then + 128 : then);
         const bool edge = t < all_low || t + 32 > all_limit || !here[0].ok || !here[1].ok;
         if (edge) {
-            // what lies behind the sequence may be anything: its values become 0
+            // what no row sees -- behind the sequence, or before all windows -- may be anything: its values become 0 (a weight of 0
+            // would not: 0 times NaN)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x.vs[e] = t + (e >> 2) * 16 + 4 * j + (e & 3) < end && here[e >> 2].ok ? x.vs[e] : 0u;
+            for (int e = 0; e < 8; ++e) {
+                const int token = t + (e >> 2) * 16 + 4 * j + (e & 3);
+                x.vs[e] = token >= range.low && token < end && here[e >> 2].ok ? x.vs[e] : 0u;
+            }
         }
         h8 p[NQ];
         weigh<NQ, TILES>(p, s, row, acc, edge, t, end, here[0].ok, here[1].ok, j, [] {});
@@ -629,7 +635,7 @@ __device__ __forceinline__ Lane lane_of_quarter(int wave, int r, int j)
 }
 
 template <int D, int G>
-__device__ __forceinline__ void convert_quarter(h8* slot, Quarter<D, G>& x, int t, int end, int wave, int r, int j, int lane)
+__device__ __forceinline__ void convert_quarter(h8* slot, Quarter<D, G>& x, int t, int low, int end, int wave, int r, int j, int lane)
 {
     constexpr int STEPS = Shape<D>::STEPS, KN = Quarter<D, G>::KN;
     const int part = wave & 1, half = wave >> 1;
@@ -637,10 +643,13 @@ __device__ __forceinline__ void convert_quarter(h8* slot, Quarter<D, G>& x, int 
 #pragma unroll
     for (int i = 0; i < KN; ++i) slot[(half * STEPS + part * KN + i) * 64 + lane] = key_fragment(x.k[i], ks, ko);
     if (D == 64 && half) return;  // (four tiles: two waves have them)
-    if (t + 32 > end || !x.ok0 || !x.ok1) {
-        // what lies behind the sequence may be anything: its values become 0
+    if (t < low || t + 32 > end || !x.ok0 || !x.ok1) {
+        // what no row of the tile sees may be anything: its values become 0
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x.vs[e] = t + (e >> 2) * 16 + 4 * j + (e & 3) < end && (e < 4 ? x.ok0 : x.ok1) ? x.vs[e] : 0u;
+        for (int e = 0; e < 8; ++e) {
+            const int token = t + (e >> 2) * 16 + 4 * j + (e & 3);
+            x.vs[e] = token >= low && token < end && (e < 4 ? x.ok0 : x.ok1) ? x.vs[e] : 0u;
+        }
     }
     // this wave's channels of a word: of the half `high`, those of `odd` (or all four)
     const uint32_t high = D == 64 ? r & 1 : D == 128 ? half : part;
@@ -709,7 +718,7 @@ __global__ __launch_bounds__(64 * WAVES, NQ * D > 256 ? 1 : 2) void kv_chunk_ker
     __shared__ uint32_t good[3][2];
     auto convert = [&](int at, h8* slot, int t) {
         if (quarter == 0 && lane == 0) good[at][wave >> 2] = (x.ok0 ? 1u : 0u) | (x.ok1 ? 2u : 0u);
-        convert_quarter<D, G>(slot + (wave >> 2) * SET, x, t + mine, end, quarter, r, j, lane);
+        convert_quarter<D, G>(slot + (wave >> 2) * SET, x, t + mine, range.low, end, quarter, r, j, lane);
     };
     if (begin < end) {
         look(begin);

@@ -1,0 +1,66 @@
+"""The paged cache where a call's masks end inside its steps: rows that no query sees hold anything."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kv_lib as K
+from test_gpu_kv import _check_attention
+
+pytestmark = pytest.mark.gpu
+
+SHAPES = [(64, 32), (64, 64), (128, 32), (128, 128), (256, 32), (256, 128)]
+# queries of each sequence (None: one each), lengths, heads (two key heads), window: a step begins up to 31 tokens before the first
+# that any row sees, a whole page and more of them.  One query: (2000, 984) begins at token 1016, its step at 992.  5 x 4 rows are two
+# tiles of 16; 60, 80 and 400 rows share converted steps, in tiles of 64 to 256 rows.
+WINDOWS = [(None, [2000, 70, 333, 1001, 17, 0], 8, 984), (None, [2000, 70, 333, 1001, 17, 0], 8, 21), (None, [5000], 4, 4500),
+           ([5, 1, 4], [99, 200, 1000], 8, 33), ([15, 2], [333, 40], 8, 50), ([40, 3, 0, 17], [333, 64, 20, 19], 4, 37), ([100, 70], [1000, 160], 8, 45)]
+
+
+def _unseen(p, causal, window):
+    """tokens [batch, table's tokens] that no query of their sequence sees"""
+    t = torch.arange(p.columns * p.page)
+    out = torch.ones(len(p.lengths), t.numel(), dtype=torch.bool)
+    for b, length in enumerate(p.lengths):
+        for i in range(p.queries[b]):
+            at = length - p.queries[b] + i
+            out[b] &= ~((t < length) & (t > at - window) & ((t <= at) | (not causal)))
+    return out
+
+
+def _spoil(p, unseen, which, given_back):
+    """every (scale, offset) pair of such tokens becomes NaN, infinite or large, as are those of the spare pages; given_back: whole
+    pages of them are no longer the sequence's, their columns name a spare page"""
+    bad = torch.tensor([math.nan, math.inf, -math.inf, 65504.0]).half()
+    for w in which:
+        pool = p.cache[w]
+        fill = bad[torch.randint(0, 4, pool.shape, generator=p.g)]
+        spoiled = torch.zeros(pool.shape[0], p.page, dtype=torch.bool)
+        spoiled[p.spare.long()] = True
+        for b in range(len(p.lengths)):
+            for t in unseen[b].nonzero().flatten().tolist():
+                page = int(p.table[b, t // p.page])
+                if page >= 0:
+                    spoiled[page, t % p.page] = True
+        p.cache[w] = torch.where(spoiled[:, None, :, None, None], fill, pool)
+    if given_back:
+        whole = unseen.view(len(p.lengths), p.columns, p.page).all(dim=2)
+        p.table = torch.where(whole & (p.table >= 0), p.spare[0], p.table)
+
+
+@pytest.mark.parametrize("given_back", [False, True])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,group", SHAPES)
+def test_attention_garbage_before_the_window(ascq_gpu, d, group, causal, given_back):
+    """nothing of a token that no query sees reaches a result: equal bits with and without the garbage"""
+    for i, (queries, lengths, heads, window) in enumerate(WINDOWS):
+        p = K.Problem(d + i, lengths, queries=queries, heads=heads, kv=2, d=d, group=group, page=16, dt="bf16" if i % 2 else "f16")
+        want = _check_attention(ascq_gpu, p, causal=causal, window=window)
+        _spoil(p, _unseen(p, causal, window), (2, 3), given_back)
+        args, more = p.args(ascq_gpu)
+        got = ascq_gpu.kv_attention(*args, **more, need_lse=True, causal=causal, window=window)
+        for a, b in zip(got, want):
+            assert torch.isfinite(a[torch.isfinite(b)]).all(), (queries, window)
+            assert torch.equal(a, b), (queries, window)
