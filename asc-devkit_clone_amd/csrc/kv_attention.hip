@@ -1059,8 +1059,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 2 : 3) void kv_weights_ker
             TileRows& x = info[tile - turn];
 #pragma unroll
             for (int i = 0; i < STEPS; ++i) rows_of[((tile - turn) * STEPS + i) * 64 + lane] = q[i];
-            if (j == 0) x.undo[r] = undo, x.lse[r] = lse, x.low[r] = low, x.limit[r] = limit;
+            // (a row that is not there sees nothing; it does not make a step one of an edge, though)
             int any_low = there ? low : v.len, any_limit = there ? limit : 0, all_low = low, all_limit = limit;
+            if (j == 0) x.undo[r] = undo, x.lse[r] = lse, x.low[r] = low, x.limit[r] = any_limit;
 #pragma unroll
             for (int off = 1; off < 16; off <<= 1) {
                 const int y0 = __shfl_xor(any_low, off, 64), y1 = __shfl_xor(any_limit, off, 64);

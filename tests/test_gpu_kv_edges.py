@@ -64,3 +64,28 @@ def test_attention_garbage_before_the_window(ascq_gpu, d, group, causal, given_b
         for a, b in zip(got, want):
             assert torch.isfinite(a[torch.isfinite(b)]).all(), (queries, window)
             assert torch.equal(a, b), (queries, window)
+
+
+@pytest.mark.parametrize("given_back", [False, True])
+@pytest.mark.parametrize("d,group", SHAPES)
+def test_weights_garbage_before_the_window(ascq_gpu, d, group, given_back):
+    """weights of tokens that no query sees are decay times what they were, whatever those tokens' keys are"""
+    for i, (queries, lengths, heads, window) in enumerate(WINDOWS):
+        p = K.Problem(d + i, lengths, queries=queries, heads=heads, kv=2, d=d, group=group, page=16, dt="bf16" if i % 2 else "f16")
+        args, more = p.args(ascq_gpu)
+        _, lse = ascq_gpu.kv_attention(*args, **more, need_lse=True, window=window)
+        unseen = _unseen(p, True, window)
+        cap = unseen.shape[1]
+        before = torch.rand(len(lengths), p.kv, cap, generator=p.g)
+        want = ascq_gpu.kv_weights(args[0], lse, *args[1:], **more, weights=before.cuda(), decay=0.5, window=window)
+        _spoil(p, unseen, (2,), given_back)
+        args, more = p.args(ascq_gpu)
+        got = ascq_gpu.kv_weights(args[0], lse, *args[1:], **more, weights=before.cuda(), decay=0.5, window=window)
+        fresh = ascq_gpu.kv_weights(args[0], lse, *args[1:], **more, window=window)
+        inside = torch.arange(cap)[None, :] < torch.tensor(lengths)[:, None]
+        for h in range(p.kv):
+            kept = got[:, h].cpu()
+            assert torch.equal(kept[unseen & inside], 0.5 * before[:, h][unseen & inside]), (queries, window)
+            assert torch.equal(kept[unseen & ~inside], before[:, h][unseen & ~inside]), (queries, window)
+            assert torch.all(fresh[:, h].cpu()[unseen] == 0), (queries, window)
+        assert torch.equal(got, want), (queries, window)
