@@ -1,4 +1,5 @@
-"""The paged cache where a call's masks end inside its steps: rows that no query sees hold anything."""
+"""The paged cache where a call's masks, tiles and turns end inside its steps: rows that no query sees hold anything, and many
+queries' weights are added up in several turns over the tokens."""
 from __future__ import annotations
 
 import math
@@ -89,3 +90,32 @@ def test_weights_garbage_before_the_window(ascq_gpu, d, group, given_back):
             assert torch.equal(kept[unseen & ~inside], before[:, h][unseen & ~inside]), (queries, window)
             assert torch.all(fresh[:, h].cpu()[unseen] == 0), (queries, window)
         assert torch.equal(got, want), (queries, window)
+
+
+@pytest.mark.parametrize("queries,window", [(70, 0), (150, 0), (150, 2500)])
+@pytest.mark.parametrize("d,group,dt", [(64, 64, "f16"), (128, 32, "bf16"), (256, 64, "f16")])
+def test_weights_in_turns(ascq_gpu, d, group, dt, queries, window):
+    """280 and 600 rows: two or three turns of 256 (d 256: three or five of 128) over ranges of several steps a wave, each adding to what
+    the turn before left.  64 sequences, of which one is long, give ranges of 1536 tokens (d 256: 1280): three steps of the eight
+    waves and more."""
+    p = K.Problem(queries + d, [4401] + [3] * 63, queries=[queries, 1] + [0] * 62, heads=4, kv=1, d=d, group=group, page=64, dt=dt)
+    args, more = p.args(ascq_gpu)
+    kw = dict(window=window)
+    _, lse = ascq_gpu.kv_attention(*args, **more, need_lse=True, **kw)
+    *_, want, tol = K.attention(p, **kw)
+    cap = p.columns * p.page
+    before = torch.rand(64, 1, cap, generator=p.g)
+    fresh = ascq_gpu.kv_weights(args[0], lse, *args[1:], **more, out=torch.full(before.shape, math.nan).cuda(), **kw).cpu()
+    place = before.cuda()
+    for _ in range(3):  # (the same bits from the same inputs)
+        place.copy_(before)
+        ascq_gpu.kv_weights(args[0], lse, *args[1:], **more, weights=place, decay=0.5, out=place, **kw)
+        apart = ascq_gpu.kv_weights(args[0], lse, *args[1:], **more, weights=before.cuda(), decay=0.5, **kw)
+        assert torch.equal(apart, place)
+    for b, n in enumerate(p.lengths):
+        w, e = want[b][:, :n], tol[b][:, :n]
+        assert torch.all((fresh[b, :, :n].double() - w).abs() <= e + 2.0 ** -24)
+        assert torch.all(fresh[b, :, n:] == 0)
+        total = 0.5 * before[b, :, :n].double() + w
+        assert torch.all((place[b, :, :n].cpu().double() - total).abs() <= e + 2.0 ** -23 * total + 2.0 ** -24)
+        assert torch.equal(place[b, :, n:].cpu(), before[b, :, n:])
