@@ -1040,7 +1040,8 @@ def kv_attention_workspace_size(q: torch.Tensor, cache: KvCache, page_table: tor
     c = _cache_arg(what, cache, q)
     if page_table.dim() != 2:
         _refuse(what, "page_table must be [batch, pages]")
-    s = _KvSequences(page_table.data_ptr(), page_table.data_ptr(), _at(starts), 0, *page_table.shape)
+    # (sizes alone are read: any address does for the lengths, and a table without columns has none)
+    s = _KvSequences(page_table.data_ptr(), c.k, _at(starts), 0, *page_table.shape)
     p = _queries_arg(what, q, c, starts, max_queries, None, causal, window)
     need = ctypes.c_size_t(0)
     check(lib().ascq_kv_attention_workspace_size(cache._ref, ctypes.byref(s), ctypes.byref(p), ctypes.byref(need)), what)
@@ -1127,7 +1128,7 @@ def kv_evict_workspace_size(cache: KvCache, page_table: torch.Tensor) -> int:
     c = _cache_arg(what, cache, page_table)
     if page_table.dim() != 2:
         _refuse(what, "page_table must be [batch, pages]")
-    s = _KvSequences(page_table.data_ptr(), page_table.data_ptr(), None, 0, *page_table.shape)
+    s = _KvSequences(page_table.data_ptr(), c.k, None, 0, *page_table.shape)  # (any address, as above)
     need = ctypes.c_size_t(0)
     check(lib().ascq_kv_evict_workspace_size(cache._ref, ctypes.byref(s), ctypes.byref(need)), what)
     return need.value

@@ -119,3 +119,20 @@ def test_weights_in_turns(ascq_gpu, d, group, dt, queries, window):
         total = 0.5 * before[b, :, :n].double() + w
         assert torch.all((place[b, :, :n].cpu().double() - total).abs() <= e + 2.0 ** -23 * total + 2.0 ** -24)
         assert torch.equal(place[b, :, n:].cpu(), before[b, :, n:])
+
+
+def test_an_empty_page_table(ascq_gpu):
+    """sequences that are all empty, the table narrowed to no column: zeros and -inf, zero weights, nothing kept"""
+    a, cache = ascq_gpu, ascq_gpu.kv_cache(4, 2, 16, 128, 32)
+    table, n = torch.zeros(3, 2, dtype=torch.int32, device="cuda")[:, :0], torch.zeros(3, dtype=torch.int32, device="cuda")
+    for starts, most in (([0, 1, 2, 3], 1), ([0, 4, 5, 60], 55)):
+        q = torch.randn(starts[-1], 4, 128, device="cuda").half()
+        kw = {} if most == 1 else dict(starts=torch.tensor(starts).int().cuda(), max_queries=most)
+        out, lse = a.kv_attention(q, cache, table, n, need_lse=True, **kw,
+                                  workspace=torch.empty(a.kv_attention_workspace_size(q, cache, table, **kw), dtype=torch.uint8, device="cuda"))
+        assert torch.all(out == 0) and torch.all(lse == -math.inf)
+        w = a.kv_weights(q, lse, cache, table, n, out=torch.full((3, 2, 7), math.nan, device="cuda"), **kw)
+        assert torch.all(w == 0)
+    room = torch.empty(a.kv_evict_workspace_size(cache, table), dtype=torch.uint8, device="cuda")
+    kept, m, w = a.kv_evict(cache, table, n, torch.ones(3, 2, 7, device="cuda"), 5, 2, workspace=room)
+    assert torch.all(kept == -1) and torch.all(m == 0) and torch.all(w == 0)

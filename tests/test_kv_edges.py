@@ -1,0 +1,19 @@
+"""The paged cache's calls at the ends of what they take, on the CPU: empty page tables, pools without a pitch, numbers past 32 bits."""
+from __future__ import annotations
+
+import torch
+
+import ascq
+
+
+def test_workspace_sizes_of_an_empty_page_table():
+    """a table narrowed to the pages of sequences that are all empty has no columns, and no memory; the calls take it"""
+    cache = ascq.kv_cache(4, 2, 16, 128, 32, device="cpu")
+    q = torch.zeros(3, 4, 128, dtype=torch.bfloat16)
+    table = torch.zeros(3, 2, dtype=torch.int32)
+    for none in (table[:, :0], torch.zeros(3, 0, dtype=torch.int32)):
+        assert ascq.kv_attention_workspace_size(q, cache, none) == 0
+        assert ascq.kv_attention_workspace_size(q, cache, none, starts=torch.zeros(4, dtype=torch.int32), max_queries=2) == 0
+        assert ascq.kv_evict_workspace_size(cache, none) == 0
+    assert ascq.kv_attention_workspace_size(q[:0], cache, table[:0]) == 0
+    assert ascq.kv_evict_workspace_size(cache, table[:0]) == 0
