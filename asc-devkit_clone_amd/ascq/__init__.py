@@ -930,6 +930,8 @@ def _page_pitch(what: str, name: str, t: torch.Tensor, shape, dtype) -> int:
         _refuse(what, f"{name} must be {tuple(shape)} of {dtype}, not {tuple(t.shape)} of {t.dtype}")
     if not t.is_contiguous() and not (t.shape[0] > 0 and t[0].is_contiguous()):
         _refuse(what, f"{name}: the elements of a page must be contiguous")
+    if t.shape[0] > 1 and t.stride(0) == 0:
+        _refuse(what, f"{name}: pages must lie apart")  # (to the library a pitch of 0 is a dense pool's)
     return t.stride(0) if t.shape[0] > 1 else 0
 
 

@@ -4,6 +4,7 @@ from __future__ import annotations
 import torch
 
 import ascq
+from test_block_checks import _refused
 
 
 def test_workspace_sizes_of_an_empty_page_table():
@@ -17,3 +18,14 @@ def test_workspace_sizes_of_an_empty_page_table():
         assert ascq.kv_evict_workspace_size(cache, none) == 0
     assert ascq.kv_attention_workspace_size(q[:0], cache, table[:0]) == 0
     assert ascq.kv_evict_workspace_size(cache, table[:0]) == 0
+
+
+def test_pools_without_a_pitch_are_refused():
+    """pages that all lie in one place (a page expanded to several): the library takes a pitch of 0 as that of dense pools"""
+    one, good = (ascq.kv_cache(n, 2, 16, 128, 32, device="cpu") for n in (1, 8))
+    parts = list(good)
+    for i, t in enumerate(one):
+        _refused(ascq.KvCache, *[t.expand(8, *t.shape[1:]) if i == j else x for j, x in enumerate(parts)])
+    _refused(ascq.KvCache, *[t.expand(8, *t.shape[1:]) for t in one])
+    ascq.KvCache(*one)
+    ascq.KvCache(*[t.expand(1, *t.shape[1:]) for t in one])
