@@ -1093,8 +1093,10 @@ def kv_evict(cache: KvCache, page_table: torch.Tensor, lengths: torch.Tensor, we
     what = "kv_evict"
     c = _cache_arg(what, cache, weights)
     s = _sequences_arg(what, page_table, lengths, None)
-    if weights.dim() != 3 or keep < 1:
-        _refuse(what, "weights must be [batch, kv_heads, cap], keep at least 1")
+    if weights.dim() != 3:
+        _refuse(what, "weights must be [batch, kv_heads, cap]")
+    if not 0 <= recent <= keep or not 1 <= keep < 1 << 31:  # (here: the library's fields would hold the low 32 bits)
+        _refuse(what, "0 <= recent <= keep, and keep at least 1 and below 2^31")
     heads = (s.batch, c.kv_heads)
     _dense(what, "weights", weights, (*heads, weights.shape[2]), torch.float32)
     w = weights if weights_out is None else weights_out

@@ -1,6 +1,7 @@
 """The paged cache's calls at the ends of what they take, on the CPU: empty page tables, pools without a pitch, numbers past 32 bits."""
 from __future__ import annotations
 
+import pytest
 import torch
 
 import ascq
@@ -29,3 +30,12 @@ def test_pools_without_a_pitch_are_refused():
     _refused(ascq.KvCache, *[t.expand(8, *t.shape[1:]) for t in one])
     ascq.KvCache(*one)
     ascq.KvCache(*[t.expand(1, *t.shape[1:]) for t in one])
+
+
+def test_evict_numbers_past_32_bits():
+    """what the library's 32-bit fields cannot hold is refused, not cut to its low bits"""
+    cache = ascq.kv_cache(4, 2, 16, 128, 32, device="cpu")
+    table, n, w = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32), torch.zeros(3, 2, 32)
+    for keep, recent in ((8, (1 << 32) + 1), (8, 1 << 32), (8, -(1 << 32)), (8, 9), (8, -1), ((1 << 32) + 8, 0)):
+        with pytest.raises(ascq.AscqError, match="keep"):
+            ascq.kv_evict(cache, table, n, w, keep, recent)
