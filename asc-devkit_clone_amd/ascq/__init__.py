@@ -1068,6 +1068,9 @@ def kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: KvCache, page_table: t
     shape = (s.batch, c.kv_heads, cap)
     if weights is not None:
         _dense(what, "weights", weights, shape, torch.float32)
+    if out is not None:
+        _dense(what, "out", out, shape, torch.float32)
+    _same_device(what, q, lse, page_table, lengths, starts, weights, out)
     w = out
     if w is None:
         # (positions that the call leaves as they were hold what they held)
@@ -1075,8 +1078,6 @@ def kv_weights(q: torch.Tensor, lse: torch.Tensor, cache: KvCache, page_table: t
         if weights is not None:
             with torch.cuda.stream(torch.cuda.ExternalStream(_stream(stream), q.device)):
                 w.copy_(weights)
-    _dense(what, "out", w, shape, torch.float32)
-    _same_device(what, q, lse, page_table, lengths, starts, weights, w)
     check(lib().ascq_kv_weights(_at(w), _at(weights), cap, decay, _at(q), _at(lse), cache._ref, ctypes.byref(s), ctypes.byref(p),
                                 _stream(stream)), what)
     return w

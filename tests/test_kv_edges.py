@@ -39,3 +39,12 @@ def test_evict_numbers_past_32_bits():
     for keep, recent in ((8, (1 << 32) + 1), (8, 1 << 32), (8, -(1 << 32)), (8, 9), (8, -1), ((1 << 32) + 8, 0)):
         with pytest.raises(ascq.AscqError, match="keep"):
             ascq.kv_evict(cache, table, n, w, keep, recent)
+
+
+def test_weights_on_the_cpu_are_refused():
+    """before anything is copied or a stream is asked for"""
+    cache = ascq.kv_cache(4, 2, 16, 128, 32, device="cpu")
+    q, lse, w = torch.zeros(3, 4, 128).half(), torch.zeros(3, 4), torch.zeros(3, 2, 32)
+    table, n = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    for kw in (dict(), dict(stream=5), dict(out=w)):
+        _refused(ascq.kv_weights, q, lse, cache, table, n, weights=w, **kw)
