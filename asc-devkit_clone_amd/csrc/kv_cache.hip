@@ -589,17 +589,19 @@ void move(const KvEvictArgs& a, int64_t n, hipStream_t st)
 }  // namespace
 
 namespace {
-// parts of a selection: one up to 16 SEL positions (us a launch, 128 rows of 4096 12, and 16 of 131072 by one workgroup each 182)
+// parts of a selection: one up to 16 SEL positions (us a launch, 128 rows of 4096 12, and 16 of 131072 by one workgroup each 182), and
+// where the parts of one sequence are more than a launch has room for (2^34 tokens over all key heads)
+constexpr int64_t PARTS = (int64_t)1 << 21;
 int parts_of(const KvEvictArgs& a)
 {
-    const int64_t cap = (int64_t)a.s.table_pages << a.c.page_shift;
-    return cap <= 16 * SEL ? 1 : (int)((cap + PART - 1) / PART);
+    const int64_t cap = (int64_t)a.s.table_pages << a.c.page_shift, parts = (cap + PART - 1) / PART;
+    return cap <= 16 * SEL || parts * a.c.kv_heads > PARTS ? 1 : (int)parts;
 }
 // sequences of a launch: fewer than 2^16 rows of workgroups, and than 2^32 threads (64 x 256 or 4 x 1024 a row, SEL a part)
 int64_t sequences_of(const KvEvictArgs& a, int parts)
 {
-    const int64_t most = 65535 / a.c.kv_heads, rows = ((int64_t)1 << 21) / parts / a.c.kv_heads;
-    return most < rows ? most : rows < 1 ? 1 : rows;
+    const int64_t most = 65535 / a.c.kv_heads, rows = PARTS / parts / a.c.kv_heads;
+    return most < rows ? most : rows;
 }
 }  // namespace
 

@@ -777,8 +777,8 @@ typedef struct {
  *   weights_out f32 [batch, kv_heads, cap_out]: the weights of what stays, then zeros; may be weights (cap_out = cap)
  * weights f32 [batch, kv_heads, cap], cap >= table_pages * page_size; cap_out >= min(keep, cap).  sequences->starts is not read.  A
  * token on a page that does not exist moves as zeros; nothing is written to a page that does not exist.
- * workspace: optional, 16-byte aligned, ascq_kv_evict_workspace_size bytes (0 for page tables of up to 16384 tokens): counts of
- * long selections; with less, or none, one workgroup selects for a sequence and head, with the same result.
+ * workspace: optional, 16-byte aligned, ascq_kv_evict_workspace_size bytes (0 for page tables of up to 16384 tokens, and of more
+ * than 2^34 over all key heads): counts of long selections; with less, or none, one workgroup selects for a sequence and head, with the same result.
  * (There is no counterpart in the reference.) */
 ascq_status ascq_kv_evict(int32_t* kept, int32_t* new_lengths, float* weights_out, const float* weights, const int32_t* into,
                           const ascq_kv_cache* cache, const ascq_kv_sequences* sequences, const ascq_kv_evict_param* p,

@@ -6,6 +6,7 @@ import torch
 
 import ascq
 from test_block_checks import _refused
+from test_block_launches import _run
 
 
 def test_workspace_sizes_of_an_empty_page_table():
@@ -48,3 +49,8 @@ def test_weights_on_the_cpu_are_refused():
     table, n = torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
     for kw in (dict(), dict(stream=5), dict(out=w)):
         _refused(ascq.kv_weights, q, lse, cache, table, n, weights=w, **kw)
+
+
+def test_evict_of_the_longest_tables(tmp_path):
+    """tables of up to 2^30 tokens over up to 1024 key heads: no grid of 2^32 threads"""
+    _run(tmp_path, "kv_wide")
