@@ -918,7 +918,7 @@ class KvCache:
 
 
 def kv_cache(pages: int, kv_heads: int, page_size: int, d: int, group: int = 32, device="cuda") -> KvCache:
-    """An empty cache (its memory is not set: nothing is read that was not appended)"""
+    """An empty cache (its memory is not set: what no query sees reaches no result)"""
     new = lambda shape, dt: torch.empty(shape, dtype=dt, device=device)  # noqa: E731
     code, scale = (pages, kv_heads, page_size, d // 2), (pages, kv_heads, page_size, d // group, 2)
     return KvCache(new(code, torch.uint8), new(code, torch.uint8), new(scale, torch.float16), new(scale, torch.float16))

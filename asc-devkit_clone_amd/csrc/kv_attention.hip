@@ -12,9 +12,10 @@
 // V's hold 8 channels of a token where a fragment wants 8 tokens of a channel: one v_perm_b32 pairs the halves of two tokens'
 // words, and the same masks then give pairs of tokens.
 //
-// Scores are fp32 sums of exact f16 products (bf16 queries are scaled by a power of two per row into f16's range, which
-// keeps all their bits); P is rounded to f16 after exp2 (2^-12 a weight at most, and independent), sums and statistics are
-// fp32.
+// Scores are fp32 sums of exact f16 products.  Queries are scaled by a power of two per row, the largest into [2^14, 2^15): exact for
+// what lies within 2^31 (bf16) or 2^28 (f16) of it, off by 2^-39 of it at most below.  P is rounded to f16 after exp2, as the matrix
+// instruction takes it: by 2^-11 of a weight at most, or, where f16 has no smaller step, 2^-33 of the row's largest.  Sums and
+// statistics are fp32, of the unrounded weights.
 #include "gemm_core.h"
 
 #include <type_traits>
@@ -274,7 +275,7 @@ __device__ __forceinline__ void add_values(v4f (&acc)[NQ][Shape<D>::TILES], cons
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // Row r of a tile as fragments (8 channels of lane j's quarter a step, in K's order), scaled by a power of two that brings its
-// largest magnitude to [2^14, 2^15): f16 then keeps every bit that matters (39 powers of two below the largest).  The scale's
+// largest magnitude to [2^14, 2^15): f16's rounding is then off by 2^-39 of it at most, and by nothing in what is not far below.  The scale's
 // sign goes into the row too, so that what is returned -- a score to base 2 is that times the product -- is positive, never 0
 // or infinite, and masked products of -inf stay that.  Rows that are not there are zeros.
 template <int D>
@@ -414,7 +415,8 @@ __device__ __forceinline__ void weigh(h8 (&p)[NQ], v4f (&s)[NQ][2], Row (&row)[N
 // each of 32 heads, 8 key heads of 128: 8 sequences of 131072 tokens 205 us, 1090 MB at 5.3 TB/s, the vector units busy 70 %; 32
 // ragged ones up to 8192 40.6 us, 4.0 TB/s, busy 43 %: they end unevenly; 16 x 5 queries (NQ 2) over up to 4099 tokens 26.8 us for
 // 39 MB: some 500 vector instructions a step, at most eight steps a wave and uneven (a second set of registers, which 32 rows have room
-// for: 27.5).  One query over 4096 tokens 7.0 us: the way of a step or two, from table over codes to merge, rather than any rate.
+// for: 27.5), vector units busy 22 % and waiting 36 % of the time: two waves a SIMD do not cover a step's way, and 12 of 32 rows are
+// empty.  One query over 4096 tokens 7.0 us: the way of a step or two, from table over codes to merge, rather than any rate.
 template <int D, int G, int NQ>
 __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 4) void kv_attention_kernel(KvAttentionArgs a, uint32_t groups)
 {
@@ -590,7 +592,9 @@ __global__ __launch_bounds__(256, D == 256 ? 3 - NQ : NQ > 1 ? 2 : 4) void kv_at
 // Bound by the waves' arithmetic beside the matrix products, and the meeting at each step: 2 x 1024 queries of 32 heads over 8192
 // tokens, 258 GFLOP below the diagonal: 292 us (880 TFLOP/s; a plain product of large matrices 1355), matrix cores busy 35 %, vector
 // units 47 %, waiting 28 % of the waves' time, no bank conflicts.  Four waves of 32 rows in 32-token
-// steps: 538; 64 rows a wave do not fit the registers (990).
+// steps: 538; 64 rows a wave do not fit the registers (990).  Causal tiles start in ascending order, the longest last: a prompt's first
+// 8192 queries of 32 heads, 550 GFLOP below the diagonal, 721 us (762 TFLOP/s), 2 x 1024 51 us.  A wave without rows (33 to 64 rows for
+// eight waves) still reads keys and multiplies them.
 template <int D, int G>
 struct Quarter {
     static constexpr int KN = Shape<D>::KW / 2, VN = D == 256 ? 4 : 2;
@@ -962,10 +966,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttentionArgs a, uint32_
 // The weight that cached tokens received: the scores again, exp(score - lse) summed over a tile's rows, tile after tile.  Here S = Q
 // K^T, the operands the other way round, so that a lane's scores belong to one token (its column) and to the rows 4 j .. 4 j + 3: the
 // sum over rows stays in the lane until the end.  A wave takes 64 tokens at a time (d = 256: 32), whose keys stay in registers while
-// the rows, converted once per workgroup, come from LDS, eight tiles at a time; more tiles take another turn over the tokens,
-// adding to what the turn before left in the output.  One query each of 16 ragged sequences up to 8192 (32 heads, 8 key heads of 128):
-// 25 us for 56 MB read and written, waves waiting 44 % of their time: a range is a step or two long.  64 queries of 2 sequences
-// over 16384: 33 us, 17 GFLOP of products, matrix cores busy 17 %, vector units (exp2 of each score) 36 %.
+// the rows, converted once per workgroup, come from LDS, eight tiles at a time (sixteen for eight waves and d below 256); more tiles
+// take another turn over the tokens, adding to what the turn before left in the output.  One query each of 16 ragged sequences up to
+// 8192 (32 heads, 8 key heads of 128): 25 us for 56 MB read and written, no unit busy (vector 16 %) and waves waiting 44 % of their time:
+// a range is three steps a wave at most, behind the rows' way through LDS and a barrier.  64 queries of 2 sequences over 16384:
+// 33 us, 17 GFLOP of products, matrix cores busy 17 %, vector units 36 %, waiting 37 %: a tile's rows are read from LDS when they are used.
 template <int D, int WAVES>
 constexpr int TURN = WAVES == 8 && D < 256 ? 16 : 8;  // tiles of rows in LDS
 struct TileRows {

@@ -52,8 +52,8 @@ __device__ __forceinline__ float of_group(float x, int lanes)
 // A lane takes 8 channels (one word of codes) of a token's keys and values in a head, the group / 8 lanes of a group find its range
 // by exchanges.  fp32 in the order that the header states, every operation IEEE: the same bits as that order anywhere.
 // The two rows' loads are in flight together, and no index needs a division.  8192 tokens x 8 heads of 128, f16, a group a row, to
-// slots in no order: 14.6 us for 42 MB (2.9 TB/s), the vector units busy 55 % of it, and every row's codes and pair are pieces of
-// 64 and 4 bytes at a place of their own.  16 tokens: 3.6 us, launch and latency.
+// slots in no order: 14.6 us for 42 MB (2.9 TB/s), the vector units busy 55 % of it (two IEEE divisions a group, by each of its lanes),
+// and every row's codes and pair are pieces of 64 and 4 bytes at a place of their own.  16 tokens: 3.6 us, launch and latency.
 template <int TYPE>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a, int word_bits, FastDiv heads)
 {
@@ -499,7 +499,9 @@ struct Rows {
 // gridDim.x workgroups.  In place one workgroup takes the tokens of a plane (keys, values, scales, weights: gridDim.z) in order: the
 // token of place i comes from a position >= i, so that a run's reads lie behind all earlier runs' writes.
 // Bound by rows of 64 and 16 bytes read from anywhere: 2 sequences x 8 heads, 16384 kept of 131072, d 128: 28 us for 42 MB kept
-// (108 MB read in whole lines, 48 written: 5.6 TB/s); 16 sequences of up to 4096 cut to 2048 15 us (40 MB read, 33 written).
+// (108 MB read in whole lines, 48 written: 5.6 TB/s); 16 sequences of up to 4096 cut to 2048 15 us (40 MB read, 33 written).  In place
+// the first takes 52 us (16 runs of 1024 tokens one behind the other, on 64 workgroups), the second 12: what keeps its place is not
+// written.
 template <int D, int G, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv_move_kernel(KvEvictArgs a)
 {

@@ -738,7 +738,7 @@ typedef struct {
 /* out [tokens, heads, d] = softmax(scale q k^T over what a query sees) v, query head h on key head h / (heads / kv_heads); lse (f32
  * [tokens, heads], or NULL) the log of the sum of exp of the scaled scores.  A query that sees nothing gives zeros and -inf.
  * Scores and sums are fp32 over the cache's exact values, softmax weights are rounded to f16.  What a query sees has to be finite
- * (as ascq_kv_append leaves it); what lies behind a sequence's length may be anything.
+ * (as ascq_kv_append leaves it); what no query sees -- behind a sequence's length, before every window -- may be anything.
  * workspace: optional, 16-byte aligned, ascq_kv_attention_workspace_size bytes (0 for many calls; it depends on the sizes alone):
  * room for partial sums where several workgroups share a sequence's tokens; with less, or none, they do not.
  * (There is no counterpart in the reference.) */
